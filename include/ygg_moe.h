@@ -339,6 +339,54 @@ int ygg_moe_forward_train(const float* x, int N, int d, int F, int E, int k, int
                           int32_t* topk_idx, float* topk_w, int32_t* counts, int32_t* offsets, float* h_pre,
                           void* workspace, size_t workspace_bytes, ygg_stream_t stream);
 
+/* ---- backward (bf16 rows) ----------------------------------------------------------
+ * ygg_adjoint_weights_f32 prepared in format 3 (E experts, d_in outputs, d_out inputs),
+ * in one pass over W (E, d_out, d_in, 8) fp32; d_out even. */
+int ygg_prepare_adjoint_weights_bf16(const float* W, int E, int d_out, int d_in, void* out, ygg_stream_t stream);
+
+/* The gradient of the input rows of a grouped CliffordLinear (CliffordLinear.backward's
+ * grad_x, clifford_linear.py:125-163) and of the grade-wise activation that made them
+ * (activations.py:135-287): for every expert e's rows,
+ *   dx[r, i] = act'(h_pre[r, i]) applied to sum_j ~W_e[j, i] dy[r, j].
+ * dy: Pauli half-rows (P_max, 2, d_out, 4) bf16; w_adj: ygg_prepare_adjoint_weights_bf16's
+ * output; h_pre: bf16 blade rows (P_max, d_in, 8), the activation's input (not read for
+ * act 0).  dx_layout 0: Pauli half-rows (P_max, 2, d_in, 4) bf16 (d_in even); 1: blade
+ * rows (P_max, d_in, 8) of dx_dtype.  Sums and slopes are fp32, dx is rounded once.  Rows
+ * past offsets[E] are left as they were. */
+int ygg_pauli_grouped_input_grad(const void* dy, int P_max, const void* w_adj, const int32_t* offsets, int E, int d_out,
+                                 int d_in, int act, const void* h_pre, void* dx, int dx_layout, int dx_dtype,
+                                 ygg_stream_t stream);
+
+/* ygg_grouped_weight_grad_pauli_f32 from bf16 Pauli half-rows (the layout of
+ * ygg_pauli_rows_from_blade) of dy (P_max rows, d_out) and a (a_rows rows, d_in; both
+ * widths even), on the bf16 MFMA units: dW (E, d_out, d_in, 8) and db (E, d_out, 8; or
+ * NULL) fp32 blade order, sums in fp32 and in an order that the sizes and offsets alone
+ * fix; zero for an expert without rows.  E <= 64; offsets are clamped into [0, P_max],
+ * and a gather index outside a's rows reads a zero row. */
+size_t ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out);
+int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void* a_pauli, int a_rows, const int32_t* gather,
+                                       const int32_t* offsets, int P_max, int E, int d_in, int d_out, float* dW,
+                                       float* db, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
+
+/* ---- backward of the router ----------------------------------------------------------
+ * The reference's router has no backward (hlm_block.py:202-206); these follow
+ * CliffordRouter.forward (clifford_router.py:54-104).  The choice of the experts is a
+ * constant.  topk_idx and topk_w (N, k) as ygg_route wrote them, dtopk_w (N, k) the
+ * gradient of topk_w (ygg_moe_backward's output); E <= 64, k <= 8.
+ *
+ * dlogits (N, E) = topk_w (dtopk_w - sum_s topk_w dtopk_w) at the chosen experts, zero at
+ * the others (and everywhere for k = 1, whose one weight is constant). */
+int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, int N, int E, int k,
+                       float* dlogits, ygg_stream_t stream);
+
+/* The same through the grade-energy logits: dx (N, d, 8) of x's type (plus dx_add, of the
+ * same type, when not NULL; dx may be dx_add), drouter_w (E, 4) and drouter_b (E), fp32. */
+size_t ygg_route_energy_backward_workspace_bytes(int N, int E);
+int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const float* router_w, int E, int k,
+                              const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, const void* dx_add,
+                              void* dx, float* drouter_w, float* drouter_b, void* workspace, size_t workspace_bytes,
+                              ygg_stream_t stream);
+
 /* ---- weight import: grade-aware quantization -----------------------------------
  * quantize_multivector / dequantize_multivector
  * (bifrost/quantization/grade_quantize.py:86-118,153-238) on T tensors of
@@ -360,6 +408,18 @@ int ygg_grade_quantize(const float* W, int T, size_t mv_per_tensor, const int32_
  * reference's Python float (default 1e-6).  d <= 4096; y must not alias x. */
 int ygg_clifford_layer_norm(const void* x, int x_dtype, int N, int d, const float* gamma, const float* beta,
                             double eps, void* y, int y_dtype, ygg_stream_t stream);
+
+/* The gradients of ygg_clifford_layer_norm: from dy (N, d, 8) of dy_dtype, the gradient of
+ * y, and the forward's x, gamma and eps,
+ *   dx = (gx - x_hat <gx, x_hat> / d) / rms with gx_i = ~gamma_i dy_i (plus residual_grad,
+ *        of x's type, when not NULL), of x's type;
+ *   dgamma_i = sum over the tokens of dy_i ~x_hat_i, dbeta_i = sum of dy_i, fp32 (d, 8),
+ * sums in fp32 and in an order that the sizes alone fix.  dx may be dy or residual_grad
+ * where the types are the same. */
+size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d);
+int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int N, int d,
+                                     const float* gamma, double eps, const void* residual_grad, void* dx, float* dgamma,
+                                     float* dbeta, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
 
 /* Workspace bytes of ygg_moe_block_ffn. */
 size_t ygg_moe_block_ffn_workspace_bytes(int N, int d, int F, int E, int k, int dtype, int w_format);

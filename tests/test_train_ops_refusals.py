@@ -1,0 +1,117 @@
+"""What the training operators refuse, on the CPU: the C entries' checks come before any launch, and the Python
+entries take no CPU tensors."""
+
+import os
+
+import pytest
+import torch
+
+from yggdrasil_amd import _native as N
+from yggdrasil_amd import ops
+
+pytestmark = pytest.mark.skipif(not os.path.exists(N.LIB_PATH), reason="library not built")
+P = 4096  # a pointer that no check may follow
+
+
+def _refused(name, args, word):
+    lib = N.lib()
+    assert getattr(lib, name)(*args) == -1
+    assert word in lib.ygg_last_error().decode(), lib.ygg_last_error()
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, 2, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "dy dtype"),
+    ((P, 0, P, 5, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "x dtype"),
+    ((P, 0, P, 0, -1, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, P, 0, 4, 0, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, P, 0, 4, 4097, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, P, 0, 4, 4, P, -1.0, None, P, P, P, P, 1 << 20, None), "eps"),
+    ((P, 0, P, 0, 4, 4, None, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
+    ((None, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
+    ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 8, None), "workspace"),
+    ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, None, 1 << 20, None), "workspace"),
+])
+def test_norm_backward(args, word):
+    _refused("ygg_clifford_layer_norm_backward", args, word)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, P, 8, None, P, 8, 2, 3, 4, P, P, P, 1 << 30, None), "bad sizes"),
+    ((P, P, 8, None, P, 8, 2, 4, 5, P, P, P, 1 << 30, None), "bad sizes"),
+    ((P, P, 8, None, P, 8, 65, 4, 4, P, P, P, 1 << 30, None), "bad sizes"),
+    ((P, P, 8, None, P, -1, 2, 4, 4, P, P, P, 1 << 30, None), "bad sizes"),
+    ((P, P, 7, None, P, 8, 2, 4, 4, P, P, P, 1 << 30, None), "7 rows"),
+    ((P, P, 8, None, None, 8, 2, 4, 4, P, P, P, 1 << 30, None), "null"),
+    ((P, P, 8, None, P, 8, 2, 4, 4, None, P, P, 1 << 30, None), "null"),
+    ((None, P, 8, None, P, 8, 2, 4, 4, P, P, P, 1 << 30, None), "null"),
+])
+def test_weight_grad(args, word):
+    _refused("ygg_grouped_weight_grad_pauli_bf16", args, word)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, 8, P, P, 2, 4, 4, 1, None, P, 0, 1, None), "null"),        # an activation without its input
+    ((P, 8, P, P, 2, 3, 4, 0, None, P, 0, 1, None), "bad sizes"),   # odd contraction
+    ((P, 8, P, P, 2, 4, 3, 0, None, P, 0, 1, None), "bad sizes"),   # odd Pauli rows out
+    ((P, 8, P, P, 0, 4, 4, 0, None, P, 0, 1, None), "bad sizes"),
+    ((P, 8, P, P, 65, 4, 4, 0, None, P, 0, 1, None), "bad sizes"),
+    ((P, 8, P, P, 2, 4, 4, 4, P, P, 0, 1, None), "activation"),
+    ((P, 8, P, P, 2, 4, 4, 0, None, P, 2, 1, None), "layout"),
+    ((P, 8, P, P, 2, 4, 4, 0, None, P, 0, 0, None), "dtype"),
+    ((P, 8, P, P, 2, 4, 4, 0, None, P, 1, 3, None), "dtype"),
+    ((P, 8, P, P, 2, 1 << 15, 1 << 14, 0, None, P, 0, 1, None), "2 GiB"),
+])
+def test_input_grad(args, word):
+    _refused("ygg_pauli_grouped_input_grad", args, word)
+
+
+def test_adjoint_weights():
+    _refused("ygg_prepare_adjoint_weights_bf16", (P, 2, 3, 4, P, None), "even")
+    _refused("ygg_prepare_adjoint_weights_bf16", (None, 2, 4, 4, P, None), "null")
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, P, P, 4, 65, 2, P, None), "bad sizes"),
+    ((P, P, P, 4, 4, 9, P, None), "bad sizes"),
+    ((P, P, P, 4, 2, 3, P, None), "bad sizes"),
+    ((P, P, P, -1, 4, 2, P, None), "bad sizes"),
+    ((P, None, P, 4, 4, 2, P, None), "null"),
+])
+def test_route_backward(args, word):
+    _refused("ygg_route_backward", args, word)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, 3, 4, 4, P, 4, 2, P, P, P, None, P, P, P, P, 1 << 20, None), "dtype"),
+    ((P, 0, 4, 0, P, 4, 2, P, P, P, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, 4, 4, P, 65, 2, P, P, P, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, 4, 4, P, 4, 5, P, P, P, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, 4, 4, None, 4, 2, P, P, P, None, P, P, P, P, 1 << 20, None), "null"),
+    ((P, 0, 4, 4, P, 4, 2, P, P, P, None, P, None, P, P, 1 << 20, None), "null"),
+    ((P, 0, 4, 4, P, 4, 2, P, P, P, None, P, P, P, None, 0, None), "workspace"),
+])
+def test_route_energy_backward(args, word):
+    _refused("ygg_route_energy_backward", args, word)
+
+
+def test_no_cpu_path():
+    x, w = torch.zeros(3, 4, 8), torch.zeros(3, 2)
+    i, h = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, 4, 4, dtype=torch.bfloat16)
+    o = torch.zeros(3, dtype=torch.int32)
+    adj = ops.PreparedWeights(torch.zeros(1, dtype=torch.uint8), None, "pauli", 2, 4, 4)
+    for f in (lambda: ops.clifford_layer_norm_backward(x, x, torch.zeros(4, 8)),
+              lambda: ops.grouped_weight_grad_pauli(h, h, o, 2),
+              lambda: ops.pauli_grouped_input_grad(h, adj, o),
+              lambda: ops.prepare_adjoint_weights(torch.zeros(2, 4, 4, 8), "pauli"),
+              lambda: ops.route_backward(i, w, w, 4),
+              lambda: ops.route_energy_backward(x, torch.zeros(4, 4), i, w, w)):
+        with pytest.raises(ValueError, match="GPU only"):
+            f()
+
+
+def test_workspace_sizes_of_bad_sizes_are_zero():
+    lib = N.lib()
+    assert lib.ygg_clifford_layer_norm_backward_workspace_bytes(-1, 4) == 0
+    assert lib.ygg_clifford_layer_norm_backward_workspace_bytes(4, 5000) == 0
+    assert lib.ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(-1, 2, 4, 4) == 0
+    assert lib.ygg_route_energy_backward_workspace_bytes(-1, 4) == 0

@@ -70,6 +70,19 @@ SIGNATURES = {
                                   _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
     "ygg_moe_forward_train": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp,
                                        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "ygg_prepare_adjoint_weights_bf16": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp]),
+    "ygg_pauli_grouped_input_grad": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int,
+                                              _c_int, _vp]),
+    "ygg_grouped_weight_grad_pauli_bf16_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
+    "ygg_grouped_weight_grad_pauli_bf16": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
+                                                    _vp, _c_size, _vp]),
+    "ygg_route_backward": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
+    "ygg_route_energy_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "ygg_route_energy_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp,
+                                           _vp, _vp, _c_size, _vp]),
+    "ygg_clifford_layer_norm_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "ygg_clifford_layer_norm_backward": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_double, _vp, _vp, _vp,
+                                                  _vp, _vp, _c_size, _vp]),
     "ygg_grade_quantize": (_c_int, [_vp, _c_int, _c_size, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),
     "ygg_clifford_layer_norm": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_double, _vp, _c_int, _vp]),
     "ygg_moe_block_ffn_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),

@@ -85,7 +85,7 @@ template <int ACT, int IN, int OUT, int OUT_DT, class TL>
 __global__ __launch_bounds__(TL::NT) __attribute__((amdgpu_waves_per_eu(2))) void pauli_gemm_kernel(
     const uint16_t* __restrict__ X, const int32_t* __restrict__ gather, const uint16_t* __restrict__ Wp,
     const float* __restrict__ bias, const int32_t* __restrict__ offsets, int E, int d_in, int d_out,
-    void* __restrict__ Y, int n_xcd, uint32_t x_bytes, uint32_t y_bytes) {
+    void* __restrict__ Y, int n_xcd, uint32_t x_bytes, uint32_t y_bytes, void* Aux, uint32_t aux_bytes) {
   constexpr int NT = TL::NT, T = TL::T, BN = TL::BN, KC = TL::KC, WR = TL::WR, WC = TL::WC, BWT = TL::BWT;
   constexpr int A_PER = TL::A_PER, W_PER = TL::W_PER;
   __shared__ __attribute__((aligned(16))) unsigned char smem[2 * TL::STAGE];
@@ -303,8 +303,9 @@ __global__ __launch_bounds__(TL::NT) __attribute__((amdgpu_waves_per_eu(2))) voi
   };
 
   const __amdgpu_buffer_rsrc_t y_rsrc = __builtin_amdgcn_make_buffer_rsrc(Y, (short)0, y_bytes, kBufferFlags);
+  const __amdgpu_buffer_rsrc_t aux = __builtin_amdgcn_make_buffer_rsrc(Aux, (short)0, aux_bytes, kBufferFlags);
   auto epilogue = [&](const PauliTileInfo& ti) __attribute__((always_inline)) {
-    pauli_tile_epilogue<ACT, OUT, OUT_DT, WR, WC, BWT, false>(acc, bvs, ti, wave, g, l32, d_out, y_rsrc, 0);
+    pauli_tile_epilogue<ACT, OUT, OUT_DT, WR, WC, BWT, false>(acc, bvs, ti, wave, g, l32, d_out, y_rsrc, 0, aux);
   };
 
   // ---- the stream of (tile, chunk) steps ------------------------------------
@@ -429,7 +430,7 @@ template <int ACT, int OUT, int OUT_DT>
 __global__ __launch_bounds__(PauliDmaTile::NT) __attribute__((amdgpu_waves_per_eu(2))) void pauli_gemm_dma_kernel(
     const uint16_t* __restrict__ X, const int32_t* __restrict__ gather, const uint16_t* __restrict__ Wp,
     const float* __restrict__ bias, const int32_t* __restrict__ offsets, int E, int d_in, int d_out,
-    void* __restrict__ Y, int n_xcd, uint64_t x_bytes, uint64_t y_bytes) {
+    void* __restrict__ Y, int n_xcd, uint64_t x_bytes, uint64_t y_bytes, void* Aux, uint64_t aux_bytes) {
   using C = PauliDmaTile;
   constexpr int NT = C::NT, T = C::T, BN = C::BN, KC = C::KC, WR = C::WR, WC = C::WC, BWT = C::BWT;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
@@ -740,7 +741,8 @@ __global__ __launch_bounds__(PauliDmaTile::NT) __attribute__((amdgpu_waves_per_e
   constexpr uint64_t Y_MV_BYTES = (OUT == kOutPauliRows || OUT_DT == kBF16) ? 16 : 32;
   auto epilogue = [&](const PauliTileInfo& ti) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t y_rsrc = rsrc_from(Y, y_bytes, (uint64_t)ti.row0 * d_out * Y_MV_BYTES);
-    pauli_tile_epilogue<ACT, OUT, OUT_DT, WR, WC, BWT, true>(acc, bvs, ti, wave, g, l32, d_out, y_rsrc, ti.row0);
+    const __amdgpu_buffer_rsrc_t aux = rsrc_from(Aux, aux_bytes, (uint64_t)ti.row0 * d_out * 16);
+    pauli_tile_epilogue<ACT, OUT, OUT_DT, WR, WC, BWT, true>(acc, bvs, ti, wave, g, l32, d_out, y_rsrc, ti.row0, aux);
   };
 
   // prologue: the first tile's gather indices; then what steps -4 .. -1 would
@@ -830,6 +832,26 @@ __global__ __launch_bounds__(256) void pauli_prep_weights_kernel(const float* __
   *reinterpret_cast<uint2*>(rec + 8 + (i & 1) * 4) = a1;   // a = 1 half
 }
 
+// The same layout of the adjoint weights (E, d_in, d_out): Wadj_ij = ~W_ji, whose product is the
+// gradient of W's input.  One thread per multivector of the layout.
+__global__ __launch_bounds__(256) void pauli_prep_adjoint_kernel(const float* __restrict__ W, int E, int d_out, int d_in,
+                                                                 uint16_t* __restrict__ out) {
+  const size_t n = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= (size_t)E * d_in * d_out) return;
+  const int j = (int)(n % d_out);
+  const size_t ei = n / d_out;  // e * d_in + i
+  const int i = (int)(ei % d_in);
+  const float* w = W + (((ei / d_in) * d_out + j) * d_in + i) * 8;
+  float x[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) x[c] = (c >= 4 ? -0.5f : 0.5f) * w[c];  // the reverse: grades 2 and 3 change sign
+  float c0[4], c1[4];
+  blade_to_pauli(x, c0, c1);
+  uint16_t* rec = out + ((ei * (d_out >> 1) + (j >> 1)) * 2) * 8;
+  *reinterpret_cast<uint2*>(rec + (j & 1) * 4) = make_uint2(pack2_bf16(c0[0], -c0[1]), pack2_bf16(c1[0], -c1[1]));
+  *reinterpret_cast<uint2*>(rec + 8 + (j & 1) * 4) = make_uint2(pack2_bf16(c0[2], -c0[3]), pack2_bf16(c1[2], -c1[3]));
+}
+
 // blade rows (bf16) -> Pauli half-rows (bf16); one thread per multivector
 __global__ __launch_bounds__(256) void blade_to_pauli_rows_kernel(const uint16_t* __restrict__ x, int rows, int d,
                                                                   uint16_t* __restrict__ out) {
@@ -907,10 +929,12 @@ DeviceShape device_shape() {
 
 template <int ACT, int IN, int OUT, int ODT>
 int launch_pauli(hipStream_t st, const uint16_t* X, uint64_t x_bytes, const int32_t* gather, const uint16_t* Wp,
-                 const float* bias, const int32_t* offsets, int E, int P_max, int d_in, int d_out, void* Y) {
+                 const float* bias, const int32_t* offsets, int E, int P_max, int d_in, int d_out, void* Y,
+                 void* aux = nullptr) {
   const DeviceShape ds = device_shape();
   // the output's size (rows past P_max, from offsets beyond it, are not written)
   const uint64_t y_bytes = (uint64_t)P_max * d_out * ((OUT == kOutPauliRows || ODT == kBF16) ? 16 : 32);
+  const uint64_t aux_bytes = aux ? (uint64_t)P_max * d_out * 16 : 0;  // bf16 blade rows
   // never more workgroups than tiles can exist
   const long long max_tiles =
       ((long long)(P_max + Tile::T - 1) / Tile::T + E) * ((d_out + Tile::BN - 1) / Tile::BN);
@@ -922,10 +946,11 @@ int launch_pauli(hipStream_t st, const uint16_t* X, uint64_t x_bytes, const int3
   }
   if (pauli_uses_dma(IN, d_in))
     pauli_gemm_dma_kernel<ACT, OUT, ODT>
-        <<<grid, PauliDmaTile::NT, 0, st>>>(X, gather, Wp, bias, offsets, E, d_in, d_out, Y, xcds, x_bytes, y_bytes);
+        <<<grid, PauliDmaTile::NT, 0, st>>>(X, gather, Wp, bias, offsets, E, d_in, d_out, Y, xcds, x_bytes, y_bytes,
+                                                aux, aux_bytes);
   else  // the register-staged kernel: whole operands below 2 GiB (checked by the caller)
     pauli_gemm_kernel<ACT, IN, OUT, ODT, Tile><<<grid, Tile::NT, 0, st>>>(
-        X, gather, Wp, bias, offsets, E, d_in, d_out, Y, xcds, (uint32_t)x_bytes, (uint32_t)y_bytes);
+        X, gather, Wp, bias, offsets, E, d_in, d_out, Y, xcds, (uint32_t)x_bytes, (uint32_t)y_bytes, aux, (uint32_t)aux_bytes);
   return check_launch("pauli_gemm");
 }
 
@@ -957,6 +982,18 @@ int ygg::pauli_prepare_weights(const float* W, int E, int d_out, int d_in, void*
   return check_launch("pauli_prep_weights");
 }
 
+YGG_API int ygg_prepare_adjoint_weights_bf16(const float* W, int E, int d_out, int d_in, void* out, hipStream_t stream) {
+  YGG_CHECK_ARG(E >= 0 && d_in >= 1 && d_out >= 2 && d_out % 2 == 0,
+                "ygg_prepare_adjoint_weights_bf16: E=%d d_out=%d d_in=%d (d_out must be even)", E, d_out, d_in);
+  const size_t n = (size_t)E * d_in * d_out;
+  if (n == 0) return 0;
+  YGG_CHECK_ARG(W && out, "ygg_prepare_adjoint_weights_bf16: null pointer");
+  YGG_CHECK_ARG(n <= (size_t)0x7fffffff * 256, "ygg_prepare_adjoint_weights_bf16: %zu multivectors exceed the grid", n);
+  pauli_prep_adjoint_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(W, E, d_out, d_in,
+                                                                              static_cast<uint16_t*>(out));
+  return check_launch("pauli_prep_adjoint");
+}
+
 YGG_API int ygg_pauli_rows_from_blade(const void* x, int rows, int d, void* out, hipStream_t stream) {
   YGG_CHECK_ARG(rows >= 0 && d >= 2 && (d % 2) == 0, "ygg_pauli_rows_from_blade: rows=%d d=%d (d must be even)",
                 rows, d);
@@ -966,6 +1003,44 @@ YGG_API int ygg_pauli_rows_from_blade(const void* x, int rows, int d, void* out,
   blade_to_pauli_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(static_cast<const uint16_t*>(x), rows,
                                                                                d, static_cast<uint16_t*>(out));
   return check_launch("blade_to_pauli_rows");
+}
+
+// The gradient of the input rows: the product with the adjoint weights (contraction d_out, d_in
+// columns), times the activation's slope at h_pre inside its epilogue.
+YGG_API int ygg_pauli_grouped_input_grad(const void* dy, int P_max, const void* w_adj, const int32_t* offsets, int E,
+                                         int d_out, int d_in, int act, const void* h_pre, void* dx, int dx_layout,
+                                         int dx_dtype, hipStream_t stream) {
+  YGG_CHECK_ARG(dx_layout == kOutPauliRows || dx_layout == kOutBlade, "ygg_pauli_grouped_input_grad: dx layout %d",
+                dx_layout);
+  YGG_CHECK_ARG(dx_layout == kOutPauliRows ? dx_dtype == kBF16 : (dx_dtype == kBF16 || dx_dtype == kF32),
+                "ygg_pauli_grouped_input_grad: dx dtype %d invalid for layout %d", dx_dtype, dx_layout);
+  YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_pauli_grouped_input_grad: activation %d", act);
+  YGG_CHECK_ARG(E >= 1 && E <= kPauliMaxExperts && P_max >= 0 && d_out >= 2 && d_out % 2 == 0 && d_in >= 1 &&
+                    (dx_layout != kOutPauliRows || d_in % 2 == 0),
+                "ygg_pauli_grouped_input_grad: bad sizes E=%d P=%d d_out=%d d_in=%d (E <= %d; d_out, and d_in of Pauli "
+                "rows, must be even)", E, P_max, d_out, d_in, kPauliMaxExperts);
+  const char* why = ygg::pauli_size_limit(kInPauliRows, P_max, false, P_max, E, d_out, d_in, dx_layout, dx_dtype);
+  YGG_CHECK_ARG(!why, "ygg_pauli_grouped_input_grad: %s (rows=%d d_out=%d d_in=%d)", why, P_max, d_out, d_in);
+  if (P_max == 0) return 0;
+  YGG_CHECK_ARG(dy && w_adj && offsets && dx && (act == kActNone || h_pre), "ygg_pauli_grouped_input_grad: null pointer");
+  const uint16_t* D = static_cast<const uint16_t*>(dy);
+  const uint16_t* W = static_cast<const uint16_t*>(w_adj);
+  const uint64_t bytes = (uint64_t)P_max * d_out * 16;
+  void* h = const_cast<void*>(h_pre);
+  auto run = [&](auto act_tag) {
+    constexpr int ACT = decltype(act_tag)::value;
+#define YGG_PG(OUT, ODT) \
+  launch_pauli<ACT, kInPauliRows, OUT, ODT>(stream, D, bytes, nullptr, W, nullptr, offsets, E, P_max, d_out, d_in, dx, h)
+    if (dx_layout == kOutPauliRows) return YGG_PG(kOutPauliRows, kBF16);
+    return dx_dtype == kBF16 ? YGG_PG(kOutBlade, kBF16) : YGG_PG(kOutBlade, kF32);
+#undef YGG_PG
+  };
+  switch (act) {
+    case kActNone: return run(std::integral_constant<int, kActNone>{});
+    case kActGelu: return run(std::integral_constant<int, kActGrad + kActGelu>{});
+    case kActRelu: return run(std::integral_constant<int, kActGrad + kActRelu>{});
+    default: return run(std::integral_constant<int, kActGrad + kActSigmoid>{});
+  }
 }
 
 YGG_API int ygg_pauli_grouped_linear(const void* x, int x_layout, int x_rows, const int32_t* gather, int P_max,

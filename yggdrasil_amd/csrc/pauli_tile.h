@@ -10,6 +10,12 @@ namespace ygg {
 enum PauliIn : int { kInBladeGather = 0, kInPauliRows = 1 };
 enum PauliOut : int { kOutPauliRows = 0, kOutBlade = 1 };
 
+// What a tile's epilogue does with its multivectors, the ACT of the functions below: the activations
+// of ygg_common.h (0 to 3); kActGrad + act: the gradient of that activation, at the rows `aux`
+// holds (bf16 blade rows before the activation); kActSave + act: the activation, with the rows
+// before it stored to `aux` (bf16, blade order).
+constexpr int kActGrad = 4, kActSave = 8;
+
 struct PauliTileInfo {
   int e, row0, row_end, col0;
   int half;  // -1: the whole tile; 0 / 1: only row block `half` of every wave
@@ -21,11 +27,12 @@ struct PauliTileInfo {
 
 // One output multivector from its eight sums (a0b0, a0b1, a1b0, a1b1 as re, im pairs): the inverse
 // Pauli map, the bias unless the sums started from it, the activation and the output layout,
-// stored at v_off + s_off of y_rsrc.
+// stored at v_off + s_off of y_rsrc; its blade row in aux, if there is one, at av_off + as_off.
 template <int ACT, int OUT, int OUT_DT, bool BIAS_IN_ACC>
 __device__ __forceinline__ void pauli_store_mv(float a0b0r, float a0b0i, float a0b1r, float a0b1i, float a1b0r, float a1b0i,
                                                float a1b1r, float a1b1i, const float* bv, __amdgpu_buffer_rsrc_t y_rsrc,
-                                               uint32_t v_off, uint32_t s_off, int d_out) {
+                                               uint32_t v_off, uint32_t s_off, int d_out, __amdgpu_buffer_rsrc_t aux,
+                                               uint32_t av_off, uint32_t as_off) {
   typedef unsigned int pu32x2_t __attribute__((ext_vector_type(2)));
   typedef unsigned int pu32x4_t __attribute__((ext_vector_type(4)));
   float y[8];
@@ -34,7 +41,17 @@ __device__ __forceinline__ void pauli_store_mv(float a0b0r, float a0b0i, float a
 #pragma unroll
     for (int c = 0; c < 8; ++c) y[c] += bv[c];
   }
-  activate_blade<ACT>(y);
+  if constexpr (ACT >= kActGrad && ACT < kActSave) {
+    const uint4 q = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(aux, av_off, as_off, 0));
+    const float h[8] = {bf_lo(q.x), bf_hi(q.x), bf_lo(q.y), bf_hi(q.y), bf_lo(q.z), bf_hi(q.z), bf_lo(q.w), bf_hi(q.w)};
+    activate_grad_blade<ACT & 3>(h, y);
+  } else {
+    if constexpr (ACT >= kActSave) {
+      const pu32x4_t o = {pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]), pack2_bf16(y[6], y[7])};
+      __builtin_amdgcn_raw_buffer_store_b128(o, aux, av_off, as_off, 0);
+    }
+    activate_blade<ACT & 3>(y);
+  }
   if constexpr (OUT == kOutPauliRows) {
     float c0[4], c1[4];
     blade_to_pauli(y, c0, c1);
@@ -63,11 +80,12 @@ __device__ __forceinline__ void pauli_store_mv(float a0b0r, float a0b0i, float a
 // BIAS_IN_ACC (the accumulators started from it).  The output is written by
 // buffer stores: y_rsrc starts at output row `row_base` and ends at the output's
 // true end, the row-dependent part of each offset is a scalar, the lane's part a
-// fixed per-lane offset.
+// fixed per-lane offset.  aux (kActGrad, kActSave) starts at row `row_base` too.
 template <int ACT, int OUT, int OUT_DT, int WR, int WC, int BWT, bool BIAS_IN_ACC>
 __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][WC][2][2], const float (&bvs)[WC][8],
                                                     const PauliTileInfo& ti, int wave, int g, int l32, int d_out,
-                                                    __amdgpu_buffer_rsrc_t y_rsrc, int row_base) {
+                                                    __amdgpu_buffer_rsrc_t y_rsrc, int row_base,
+                                                    __amdgpu_buffer_rsrc_t aux) {
   const int wt = wave % BWT, wj = wave / BWT;
   // bytes per output row (Pauli half-row pair, bf16 blade or fp32 blade row)
   constexpr int MV_BYTES = (OUT == kOutPauliRows || OUT_DT == kBF16) ? 16 : 32;
@@ -79,6 +97,7 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
     // lane part of the offset: token 2 g of the group of four, column j
     const uint32_t v_off = OUT == kOutPauliRows ? (uint32_t)((4 * g) * d_out + j) * 8
                                                 : (uint32_t)((2 * g) * d_out + j) * MV_BYTES;
+    const uint32_t av_off = (uint32_t)((2 * g) * d_out + j) * 16;
 #pragma unroll
     for (int rb = 0; rb < WR; ++rb) {
       if (ti.half >= 0 && rb > 0) break;  // a half tile: the first accumulators hold block `half`
@@ -94,7 +113,7 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
           pauli_store_mv<ACT, OUT, OUT_DT, BIAS_IN_ACC>(
               acc[rb][cb][0][0][v0], acc[rb][cb][0][1][v0], acc[rb][cb][0][0][v0 + 1], acc[rb][cb][0][1][v0 + 1],
               acc[rb][cb][1][0][v0], acc[rb][cb][1][1][v0], acc[rb][cb][1][0][v0 + 1], acc[rb][cb][1][1][v0 + 1], bv, y_rsrc,
-              v_off, s_off, d_out);
+              v_off, s_off, d_out, aux, av_off, (uint32_t)(rs - row_base) * d_out * 16);
         }
     }
   }

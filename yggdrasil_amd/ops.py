@@ -640,6 +640,41 @@ def clifford_layer_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor
     return out
 
 
+def clifford_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6,
+                                 residual_grad: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """Gradients of :func:`clifford_layer_norm`: ``(dx like x, dgamma (d, 8), dbeta (d, 8))``, the latter fp32.
+
+    dy: the gradient of its output, of x's shape, float32 or bfloat16.  ``residual_grad`` (like x) is added to
+    dx before it is rounded: the gradient that reaches x past the norm, as in ``x + f(norm(x))``.
+    """
+    dev = _dev(dy, x, gamma, residual_grad)
+    if x.dim() < 2 or x.shape[-1] != 8:
+        raise ValueError(f"clifford_layer_norm_backward: x must be (..., d, 8), got {tuple(x.shape)}")
+    if dy.shape != x.shape:
+        raise ValueError(f"clifford_layer_norm_backward: dy must have x's shape {tuple(x.shape)}, got {tuple(dy.shape)}")
+    d = x.shape[-2]
+    if tuple(gamma.shape) != (d, 8):
+        raise ValueError(f"clifford_layer_norm_backward: gamma must be ({d}, 8)")
+    if residual_grad is not None and (residual_grad.shape != x.shape or residual_grad.dtype != x.dtype):
+        raise ValueError("clifford_layer_norm_backward: residual_grad must have x's shape and dtype")
+    # the kernels load 16 bytes at a time
+    dy, x, residual_grad = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (dy, x, residual_grad))
+    Nt = x.numel() // (8 * d) if d else 0
+    L = lib()
+    need = L.ygg_clifford_layer_norm_backward_workspace_bytes(Nt, d)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    g = gamma.float().contiguous()
+    g = g if g.data_ptr() % 16 == 0 else g.clone()
+    dx = torch.empty_like(x)
+    dgamma = torch.empty((d, 8), device=dev, dtype=torch.float32)
+    dbeta = torch.empty((d, 8), device=dev, dtype=torch.float32)
+    check(L.ygg_clifford_layer_norm_backward(ptr(dy), _dtype_code(dy), ptr(x), _dtype_code(x), Nt, d, ptr(g), float(eps),
+                                             ptr(residual_grad), ptr(dx), ptr(dgamma), ptr(dbeta), ptr(workspace), need,
+                                             stream_handle(dev)), "clifford_layer_norm_backward")
+    return dx, dgamma, dbeta
+
+
 def moe_block_ffn_workspace_bytes(Nt: int, d: int, F: int, E: int, k: int, dtype: torch.dtype, fmt: str) -> int:
     return lib().ygg_moe_block_ffn_workspace_bytes(Nt, d, F, E, k, DTYPE_CODE[dtype], WFORMAT_CODE[fmt])
 
@@ -699,17 +734,22 @@ def adjoint_weights(w: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def prepare_adjoint_weights(w: torch.Tensor) -> PreparedWeights:
-    """``prepare_weights(adjoint_weights(w), "pauli_f32")`` in one pass. w: (E, d_out, d_in, 8) fp32."""
+def prepare_adjoint_weights(w: torch.Tensor, fmt: str = "pauli_f32") -> PreparedWeights:
+    """``prepare_weights(adjoint_weights(w), fmt)`` in one pass. w: (E, d_out, d_in, 8) fp32; fmt 'pauli_f32' or
+    'pauli' (bf16; d_out even)."""
     dev = _dev(w)
     if w.dtype != torch.float32 or w.dim() != 4 or w.shape[-1] != 8:
         raise ValueError("prepare_adjoint_weights: w must be fp32 (E, d_out, d_in, 8)")
+    if fmt not in ("pauli_f32", "pauli"):
+        raise ValueError("prepare_adjoint_weights: fmt must be 'pauli_f32' or 'pauli'")
     E, d_out, d_in = w.shape[:3]
-    data = torch.empty((lib().ygg_prepared_weight_bytes(E, d_in, d_out, WFORMAT_CODE["pauli_f32"]),), device=dev,
+    if fmt == "pauli" and d_out % 2:
+        raise ValueError(f"prepare_adjoint_weights: the 'pauli' format needs an even d_out, got {d_out}")
+    data = torch.empty((lib().ygg_prepared_weight_bytes(E, d_in, d_out, WFORMAT_CODE[fmt]),), device=dev,
                        dtype=torch.uint8)
-    check(lib().ygg_prepare_adjoint_weights_f32(ptr(w), E, d_out, d_in, ptr(data), stream_handle(dev)),
-          "prepare_adjoint_weights")
-    return PreparedWeights(data, None, "pauli_f32", E, d_in, d_out)
+    fn = lib().ygg_prepare_adjoint_weights_f32 if fmt == "pauli_f32" else lib().ygg_prepare_adjoint_weights_bf16
+    check(fn(ptr(w), E, d_out, d_in, ptr(data), stream_handle(dev)), "prepare_adjoint_weights")
+    return PreparedWeights(data, None, fmt, E, d_in, d_out)
 
 
 def grouped_weight_grad(dy: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor, E: int,
@@ -727,12 +767,16 @@ def grouped_weight_grad(dy: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor
 def grouped_weight_grad_pauli(dy_pauli: torch.Tensor, a_pauli: torch.Tensor, offsets: torch.Tensor, E: int,
                               gather: torch.Tensor | None = None, with_bias: bool = True,
                               workspace: torch.Tensor | None = None):
-    """:func:`grouped_weight_grad` on the fp32 MFMA units from fp32 Pauli rows
-    (:func:`pauli_rows_from_blade_f32`) of dy (P, d_out, 2, 2, 2) and a (.., d_in, 2, 2, 2)."""
+    """:func:`grouped_weight_grad` on the MFMA units, from fp32 Pauli rows (:func:`pauli_rows_from_blade_f32`) of
+    dy (P, d_out, 2, 2, 2) and a (.., d_in, 2, 2, 2), or from bf16 Pauli half-rows
+    (:func:`pauli_rows_from_blade`) of dy (P, 2, d_out, 4) and a (.., 2, d_in, 4)."""
     dev = _dev(dy_pauli, a_pauli, offsets, gather)
+    if dy_pauli.dtype == torch.bfloat16 and a_pauli.dtype == torch.bfloat16:
+        return _grouped_weight_grad_bf16(dev, dy_pauli, a_pauli, offsets, E, gather, with_bias, workspace)
     for t in (dy_pauli, a_pauli):
         if t.dtype != torch.float32 or t.dim() != 5 or tuple(t.shape[2:]) != (2, 2, 2):
-            raise ValueError("grouped_weight_grad_pauli: operands must be fp32 Pauli rows (rows, d, 2, 2, 2)")
+            raise ValueError("grouped_weight_grad_pauli: operands must be fp32 Pauli rows (rows, d, 2, 2, 2), or both "
+                             "bf16 Pauli half-rows (rows, 2, d, 4)")
     P, d_out, d_in = dy_pauli.shape[0], dy_pauli.shape[1], a_pauli.shape[1]
     dW = torch.empty((E, d_out, d_in, 8), device=dev, dtype=torch.float32)
     db = torch.empty((E, d_out, 8), device=dev, dtype=torch.float32) if with_bias else None
@@ -743,6 +787,126 @@ def grouped_weight_grad_pauli(dy_pauli: torch.Tensor, a_pauli: torch.Tensor, off
                                                   d_out, ptr(dW), ptr(db), ptr(workspace), workspace.numel(),
                                                   stream_handle(dev)), "grouped_weight_grad_pauli")
     return dW, db
+
+
+def _half_rows(name: str, t: torch.Tensor) -> torch.Tensor:
+    """bf16 Pauli half-rows (rows, 2, d, 4) on 16 bytes, as the kernels load them."""
+    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[1] != 2 or t.shape[3] != 4:
+        raise ValueError(f"{name} must be bf16 Pauli half-rows (rows, 2, d, 4), got {t.dtype} {tuple(t.shape)}")
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_bounds(offsets: torch.Tensor, E: int, dev) -> None:
+    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or offsets.device != dev:
+        raise ValueError(f"offsets must be int32 ({E + 1},) on {dev}, got {offsets.dtype} {tuple(offsets.shape)}")
+
+
+def _grouped_weight_grad_bf16(dev, dy, a, offsets, E, gather, with_bias, workspace):
+    dy, a = _half_rows("dy_pauli", dy), _half_rows("a_pauli", a)
+    P, d_out, d_in = dy.shape[0], dy.shape[2], a.shape[2]
+    _check_bounds(offsets, E, dev)
+    if gather is not None and (gather.dtype != torch.int32 or tuple(gather.shape) != (P,)):
+        raise ValueError(f"gather must be int32 ({P},), got {gather.dtype} {tuple(gather.shape)}")
+    L = lib()
+    need = L.ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(P, E, d_in, d_out)
+    if workspace is None:
+        workspace = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    dW = torch.empty((E, d_out, d_in, 8), device=dev, dtype=torch.float32)
+    db = torch.empty((E, d_out, 8), device=dev, dtype=torch.float32) if with_bias else None
+    check(L.ygg_grouped_weight_grad_pauli_bf16(ptr(dy), ptr(a), a.shape[0], ptr(gather), ptr(offsets), P, E, d_in, d_out,
+                                               ptr(dW), ptr(db), ptr(workspace),
+                                               workspace.numel() * workspace.element_size(), stream_handle(dev)),
+          "grouped_weight_grad_pauli")
+    return dW, db
+
+
+def pauli_grouped_input_grad(dy_pauli: torch.Tensor, pw_adj: PreparedWeights, offsets: torch.Tensor,
+                             h_pre: torch.Tensor | None = None, act: str = "none", y_layout: str = "blade",
+                             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The gradient of a grouped CliffordLinear's input rows, and of the activation that made them.
+
+    dy_pauli: the gradient of the product's rows, grouped by expert, as bf16 Pauli half-rows (P, 2, d_out, 4).
+    pw_adj: ``prepare_adjoint_weights(w, "pauli")`` of the weights (E, d_out, d_in, 8).
+    h_pre (P, d_in, 8) bf16 blade rows: the input of the activation ``act`` whose output the product read.
+    y_layout 'blade' returns (P, d_in, 8) of out_dtype, 'pauli' (P, 2, d_in, 4) bf16.  Rows past
+    ``offsets[E]`` are not written.
+    """
+    if pw_adj.fmt != "pauli":
+        raise ValueError("pauli_grouped_input_grad needs adjoint weights prepared with fmt='pauli'")
+    if act not in ACT_CODE:
+        raise ValueError(f"act must be one of {tuple(ACT_CODE)}")
+    if y_layout not in Y_LAYOUT:
+        raise ValueError("y_layout must be 'blade' or 'pauli'")
+    dev = _dev(dy_pauli, offsets, h_pre)
+    dy_pauli = _half_rows("dy_pauli", dy_pauli)
+    P, d_out, d_in, E = dy_pauli.shape[0], dy_pauli.shape[2], pw_adj.d_out, pw_adj.E
+    if d_out != pw_adj.d_in:
+        raise ValueError(f"dy_pauli has d_out={d_out}, the adjoint weights expect {pw_adj.d_in}")
+    _check_bounds(offsets, E, dev)
+    if act != "none":
+        if h_pre is None or h_pre.dtype != torch.bfloat16 or tuple(h_pre.shape) != (P, d_in, 8):
+            raise ValueError(f"act={act!r} needs h_pre, bf16 ({P}, {d_in}, 8)")
+        if h_pre.data_ptr() % 16:
+            h_pre = h_pre.clone()
+    if y_layout == "pauli":
+        dx = torch.empty((P, 2, d_in, 4), device=dev, dtype=torch.bfloat16)
+    else:
+        dx = torch.empty((P, d_in, 8), device=dev, dtype=out_dtype)
+    check(lib().ygg_pauli_grouped_input_grad(ptr(dy_pauli), P, ptr(pw_adj.data), ptr(offsets), E, d_out, d_in,
+                                             ACT_CODE[act], ptr(h_pre) if act != "none" else None, ptr(dx),
+                                             Y_LAYOUT[y_layout], _dtype_code(dx), stream_handle(dev)),
+          "pauli_grouped_input_grad")
+    return dx
+
+
+def _check_slots(topk_idx, topk_w, dtopk_w):
+    if topk_idx.dtype != torch.int32 or topk_idx.dim() != 2:
+        raise ValueError(f"topk_idx must be int32 (N, k), got {topk_idx.dtype} {tuple(topk_idx.shape)}")
+    for name, t in (("topk_w", topk_w), ("dtopk_w", dtopk_w)):
+        if t.dtype != torch.float32 or t.shape != topk_idx.shape:
+            raise ValueError(f"{name} must be float32 {tuple(topk_idx.shape)}, got {t.dtype} {tuple(t.shape)}")
+    return topk_idx.shape
+
+
+def route_backward(topk_idx: torch.Tensor, topk_w: torch.Tensor, dtopk_w: torch.Tensor, E: int) -> torch.Tensor:
+    """Gradient of the logits (N, E) from that of the routing weights of :func:`route`, all (N, k): the
+    chosen experts' softmax weights are functions of their own logits alone, the choice is a constant."""
+    dev = _dev(topk_idx, topk_w, dtopk_w)
+    Nt, k = _check_slots(topk_idx, topk_w, dtopk_w)
+    dlogits = torch.empty((Nt, E), device=dev, dtype=torch.float32)
+    check(lib().ygg_route_backward(ptr(topk_idx), ptr(topk_w), ptr(dtopk_w), Nt, E, k, ptr(dlogits), stream_handle(dev)),
+          "route_backward")
+    return dlogits
+
+
+def route_energy_backward(x: torch.Tensor, router_weight: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
+                          dtopk_w: torch.Tensor, dx_add: torch.Tensor | None = None):
+    """Gradients of :func:`route_energy`: ``(dx like x, drouter_weight (E, 4), drouter_bias (E,))`` from that of its
+    routing weights (N, k).  ``dx_add`` (like x) is added to dx before it is rounded."""
+    dev = _dev(x, router_weight, topk_idx, topk_w, dtopk_w, dx_add)
+    if x.dim() != 3 or x.shape[2] != 8:
+        raise ValueError(f"route_energy_backward: x must be (N, d, 8), got {tuple(x.shape)}")
+    Nt, d = x.shape[:2]
+    E = router_weight.shape[0]
+    if tuple(router_weight.shape) != (E, 4):
+        raise ValueError(f"route_energy_backward: router_weight must be (E, 4), got {tuple(router_weight.shape)}")
+    if _check_slots(topk_idx, topk_w, dtopk_w)[0] != Nt:
+        raise ValueError(f"route_energy_backward: {topk_idx.shape[0]} tokens' routing for {Nt} tokens")
+    if dx_add is not None and (dx_add.shape != x.shape or dx_add.dtype != x.dtype):
+        raise ValueError("route_energy_backward: dx_add must have x's shape and dtype")
+    x = x if x.data_ptr() % 16 == 0 else x.clone()
+    dx_add = dx_add if dx_add is None or dx_add.data_ptr() % 16 == 0 else dx_add.clone()
+    L = lib()
+    need = L.ygg_route_energy_backward_workspace_bytes(Nt, E)
+    ws = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    rw = router_weight.float().contiguous()
+    dx = torch.empty_like(x)
+    drw = torch.empty((E, 4), device=dev, dtype=torch.float32)
+    drb = torch.empty((E,), device=dev, dtype=torch.float32)
+    check(L.ygg_route_energy_backward(ptr(x), _dtype_code(x), Nt, d, ptr(rw), E, topk_idx.shape[1], ptr(topk_idx),
+                                      ptr(topk_w), ptr(dtopk_w), ptr(dx_add), ptr(dx), ptr(drw), ptr(drb), ptr(ws),
+                                      need, stream_handle(dev)), "route_energy_backward")
+    return dx, drw, drb
 
 
 def activation_backward(h: torch.Tensor, grad_out: torch.Tensor, act: str) -> torch.Tensor:
