@@ -62,6 +62,8 @@ WEIGHT_CASES = [
     ([7, 200, 0, 190, 3], 100, 36, False, True),
     ([400], 24, 72, True, True),
     ([1] * 64, 16, 20, True, True),
+    ([1300, 0, 513, 512], 6, 10, True, True),  # experts of several chunks of rows
+    ([0, 1025], 70, 66, False, True),
 ]
 
 

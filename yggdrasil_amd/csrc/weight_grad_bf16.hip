@@ -11,115 +11,269 @@
 
 #include <hip/hip_runtime.h>
 
-#include "pauli_common.h"
+#include <algorithm>
+
+#include "pauli_split.h"
 #include "ygg_common.h"
 
 namespace ygg {
 namespace {
 
-constexpr int kRows = 8;   // rows staged at a time
-constexpr int kTile = 32;  // columns j and i of a workgroup
+constexpr int kWbTile = 64;     // output columns j and input columns i of a workgroup
+constexpr int kWbRows = 8;      // rows of a stage
+constexpr int kWbStages = 4;    // stages in LDS: three in flight while one is read
+constexpr int kWbChunk = 512;   // rows of a workgroup at most
+constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
+constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
+constexpr int kWbStage = 2 * kWbOperand;
 
-// An expert's rows, whatever `offsets` holds: inside [0, P] and not negative
-__device__ inline void expert_rows(const int32_t* __restrict__ offsets, int e, int P, int& r0, int& r1) {
-  r0 = min(max(offsets[e], 0), P);
-  r1 = max(min(offsets[e + 1], P), r0);
+// Lane e: the rows of expert e and their chunks, n = ceil(rows / kWbChunk) of equal length (a multiple of a
+// stage's rows).  Whatever `offsets` holds, the ranges are inside [0, P] and disjoint: every bound is
+// clamped and at least the one before it.
+struct WbExpert {
+  int beg, end, n, len;
+};
+__device__ __forceinline__ WbExpert wb_experts(const int32_t* __restrict__ offsets, int E, int P, int lane) {
+  int beg = min(max(offsets[min(lane, E)], 0), P);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(beg, o);
+    if (lane >= o) beg = max(beg, u);
+  }
+  WbExpert x = {beg, max(beg, min(offsets[min(lane + 1, E)], P)), 0, 0};
+  if (lane >= E) x.end = x.beg;
+  x.n = (x.end - x.beg + kWbChunk - 1) / kWbChunk;
+  x.len = x.n > 0 ? ((x.end - x.beg + x.n - 1) / x.n + kWbRows - 1) / kWbRows * kWbRows : 0;
+  return x;
+}
+__device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
 }
 
-// Workgroup: a 32 (j) x 32 (i) tile of one expert; thread (tj, ti) the pairs (tj + 16 p, ti + 16 q).
-__global__ __launch_bounds__(256) void weight_grad_bf16_kernel(const uint16_t* __restrict__ D,
-                                                               const uint16_t* __restrict__ A, int a_rows,
-                                                               const int32_t* __restrict__ gather,
-                                                               const int32_t* __restrict__ offsets, int P, int d_in,
-                                                               int d_out, float* __restrict__ dW,
-                                                               float* __restrict__ db) {
-  __shared__ float4 sd[kRows][kTile][2], sa[kRows][kTile][2];  // columns b = 0, 1: re, im of entries 0 and 1
-  const int e = blockIdx.z, j0 = blockIdx.x * kTile, i0 = blockIdx.y * kTile;
-  const int tid = threadIdx.x, tj = tid & 15, ti = tid >> 4;
-  int r0, r1;
-  expert_rows(offsets, e, P, r0, r1);
-  float acc[2][2][8] = {}, bsum[8] = {};  // [p][q][a c re/im]; this thread's staged rows of dy
-  const int sr = tid >> 5, sc = tid & 31;
-  auto stage = [&](const uint16_t* rows, long long row, int d, int col, float4 (&to)[kRows][kTile][2]) {
+__device__ __forceinline__ float swap_pair(float v) {  // the value of the neighbouring lane (lane ^ 1)
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true));
+}
+// From this lane's half of a summed matrix -- lane parity c: entries (0, c) and (1, c), re and im -- and its
+// neighbour's, four values of half its blades: blades 0 to 3 for c = 0, 4 to 7 for c = 1.
+__device__ __forceinline__ float4 half_blades(float r0, float i0, float r1, float i1, int c) {
+  const float x = swap_pair(c ? r1 : i0), y = swap_pair(c ? r0 : r1), z = swap_pair(c ? i0 : i1);
+  return c ? make_float4(0.5f * (x - i1), 0.5f * (y - r0), 0.5f * (z + i0), 0.5f * (x + i1))
+           : make_float4(0.5f * (r0 + x), 0.5f * (r1 + y), 0.5f * (i1 - z), 0.5f * (r0 - x));
+}
+
+// One workgroup: 64 (j) x 64 (i) of one chunk's sum, a wave 32 x 32 of it.
+//
+// v_mfma_f32_32x32x16_bf16 with the operand rows (j, a) and columns (i, c), 16 of each index: the dword
+// (re, im) of entry a of column b of D_rj is one (r, b) term of the contraction, and four such dwords (two
+// rows, b = 0, 1) are a lane's operand.  D . A sums re re + im im, the real part of D conj(A); with A rotated
+// to (im, -re) the sum is minus the imaginary part.  The dwords of 32 operand rows are neighbours in a
+// half-row, so the LDS reads, four times 4 bytes per operand, are free of bank conflicts without padding.
+//
+// The rows come by direct-to-LDS loads, 16 bytes a lane, one row of 64 columns an instruction, from buffer
+// descriptors based at the row (so the operands may have any size); a row past the chunk, or outside a,
+// has an empty descriptor and reads zeros.
+__global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
+    const uint16_t* __restrict__ D, const uint16_t* __restrict__ A, int a_rows, const int32_t* __restrict__ gather,
+    const int32_t* __restrict__ offsets, int P, int E, int d_in, int d_out, int n_xcd, float* __restrict__ part,
+    float* __restrict__ dbpart, float* __restrict__ dW, float* __restrict__ db) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kWbStages * kWbStage];
+  __shared__ int s_src[kWbChunk + kWbRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int nj = (d_out + kWbTile - 1) / kWbTile, ni = (d_in + kWbTile - 1) / kWbTile, nt = nj * ni;
+  // all tiles of a chunk on one XCD (workgroup b runs on XCD b mod 8): its rows are read into one L2
+  const int bq = blockIdx.x / n_xcd, chunk = bq / nt * n_xcd + (blockIdx.x - bq * n_xcd), tile = bq % nt;
+  const WbExpert x = wb_experts(offsets, E, P, lane);
+  const int incl = wave_inclusive_sum(x.n, lane), planes = wave_inclusive_sum(x.n > 1 ? x.n : 0, lane);
+  const uint64_t after = __ballot(incl > chunk);
+  if (after == 0) return;
+  const int e = (int)__builtin_ctzll(after);
+  const int n = __builtin_amdgcn_readlane(x.n, e), c = chunk - (__builtin_amdgcn_readlane(incl, e) - n);
+  const int len = __builtin_amdgcn_readlane(x.len, e);
+  const int r0 = __builtin_amdgcn_readlane(x.beg, e) + c * len;
+  const int rows = max(0, min(len, __builtin_amdgcn_readlane(x.end, e) - r0));
+  const int plane = __builtin_amdgcn_readlane(planes, e) - n + c;  // of an expert of several chunks
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j0 = (tile % nj) * kWbTile, i0 = (tile / nj) * kWbTile;
+
+  if (gather != nullptr)
+    for (int i = tid; i < rows; i += 256) s_src[i] = gather[r0 + i];
+  __syncthreads();
+
+  // this lane's piece of a row: half lane / 32, columns 2 (lane % 32) and the next
+  const int col = 2 * (lane & 31);
+  const uint32_t d_off = j0 + col < d_out ? (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 : kBufferOff;
+  const uint32_t a_off = i0 + col < d_in ? (uint32_t)((lane >> 5) * d_in + i0 + col) * 8 : kBufferOff;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem;
+  auto row_of = [](const uint16_t* base, long long row, bool live, int d) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base) + (live ? row : 0) * d * 8, (short)0,
+                                             live ? (uint32_t)d * 16 : 0u, kBufferFlags);
+  };
+  auto issue = [&](int f) __attribute__((always_inline)) {  // stage f's rows: two of each operand a wave
+    const uint32_t st = lds0 + (f % kWbStages) * kWbStage + 2 * wave * 2 * kWbHalf;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row >= 0 && col < d) {
-        const uint2 q = *reinterpret_cast<const uint2*>(rows + (((size_t)row * 2 + b) * d + col) * 4);
-        v = make_float4(bf_lo(q.x), bf_hi(q.x), bf_lo(q.y), bf_hi(q.y));
-      }
-      to[sr][sc][b] = v;
+    for (int u = 0; u < 2; ++u) {
+      const int r = f * kWbRows + 2 * wave + u;
+      const bool live = r < rows;
+      int src = r0 + r;
+      if (gather != nullptr) src = __builtin_amdgcn_readfirstlane(s_src[min(r, kWbChunk - 1)]);
+      split_dma(row_of(D, r0 + r, live, d_out), st + u * 2 * kWbHalf, d_off, 0);
+      split_dma(row_of(A, src, live && src >= 0 && src < a_rows, d_in), st + kWbOperand + u * 2 * kWbHalf, a_off, 0);
     }
   };
-  for (int base = r0; base < r1; base += kRows) {
-    const int r = base + sr;
-    const int src = r < r1 ? (gather ? gather[r] : r) : -1;
-    stage(D, r < r1 ? r : -1, d_out, j0 + sc, sd);
-    stage(A, src >= 0 && src < a_rows ? src : -1, d_in, i0 + sc, sa);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const float4 v = sd[sr][sc][b];
-      bsum[4 * b] += v.x; bsum[4 * b + 1] += v.y; bsum[4 * b + 2] += v.z; bsum[4 * b + 3] += v.w;
-    }
-    __syncthreads();
-    for (int rr = 0; rr < min(kRows, r1 - base); ++rr)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 u = sd[rr][tj + 16 * p][b], v = sa[rr][ti + 16 * q][b];
-            float* s = acc[p][q];
-            s[0] += u.x * v.x + u.y * v.y;  s[1] += u.y * v.x - u.x * v.y;  // a = 0, c = 0
-            s[2] += u.x * v.z + u.y * v.w;  s[3] += u.y * v.z - u.x * v.w;  // a = 0, c = 1
-            s[4] += u.z * v.x + u.w * v.y;  s[5] += u.w * v.x - u.z * v.y;  // a = 1, c = 0
-            s[6] += u.z * v.z + u.w * v.w;  s[7] += u.w * v.z - u.z * v.w;  // a = 1, c = 1
-          }
-    __syncthreads();
-  }
-  auto store = [](float* dst, const float* s) {  // half the blades of the summed matrix
-    float o[8];
-    pauli_to_blade(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], o);
-    float4* q = reinterpret_cast<float4*>(dst);
-    q[0] = make_float4(0.5f * o[0], 0.5f * o[1], 0.5f * o[2], 0.5f * o[3]);
-    q[1] = make_float4(0.5f * o[4], 0.5f * o[5], 0.5f * o[6], 0.5f * o[7]);
-  };
+  const int wj = wave & 1, wi = wave >> 1, l32 = lane & 31, g = lane >> 5;
+  const uint32_t d_rd = 4 * g * kWbHalf + wj * 256 + l32 * 4, a_rd = kWbOperand + 4 * g * kWbHalf + wi * 256 + l32 * 4;
+
+  pf32x16_t acc[2][2][2];  // [16 j][16 i][real, minus imaginary]
 #pragma unroll
   for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int j = j0 + tj + 16 * p, i = i0 + ti + 16 * q;
-      if (j < d_out && i < d_in) store(dW + (((size_t)e * d_out + j) * d_in + i) * 8, acc[p][q]);
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[p][q][h][v] = 0.f;
+  const bool bias_wave = db != nullptr && i0 == 0 && wi == 0;
+  float bs[2][2][2] = {};  // [16 j][b][re, im] of D's entry l32 % 2
+
+  const int nf = (rows + kWbRows - 1) / kWbRows;
+#pragma unroll
+  for (int f = 0; f < kWbStages - 1; ++f) issue(f);
+  for (int f = 0; f < nf; ++f) {
+    // four loads a stage: those of the two newer stages may stay outstanding
+    asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+    issue(f + kWbStages - 1);  // over the stage read before the barrier
+    const unsigned char* st = smem + (f % kWbStages) * kWbStage;
+#pragma unroll
+    for (int s = 0; s < kWbRows / 4; ++s) {
+      uint32_t d[2][4], a[2][4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          d[p][q] = *reinterpret_cast<const uint32_t*>(st + d_rd + (8 * s + q) * kWbHalf + p * 128);
+          a[p][q] = *reinterpret_cast<const uint32_t*>(st + a_rd + (8 * s + q) * kWbHalf + p * 128);
+        }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const pbf16x8_t X = __builtin_bit_cast(pbf16x8_t, make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]));
+        const pbf16x8_t R = __builtin_bit_cast(
+            pbf16x8_t, make_uint4(rot_conj(a[q][0]), rot_conj(a[q][1]), rot_conj(a[q][2]), rot_conj(a[q][3])));
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const pbf16x8_t Y = __builtin_bit_cast(pbf16x8_t, make_uint4(d[p][0], d[p][1], d[p][2], d[p][3]));
+          acc[p][q][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, X, acc[p][q][0], 0, 0, 0);
+          acc[p][q][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, R, acc[p][q][1], 0, 0, 0);
+        }
+      }
+      if (bias_wave) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            bs[p][q & 1][0] += bf_lo(d[p][q]);
+            bs[p][q & 1][1] += bf_hi(d[p][q]);
+          }
+      }
     }
-  if (db != nullptr && blockIdx.y == 0) {
-    float* red = reinterpret_cast<float*>(&sd[0][0][0]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the last stage write LDS too
+
+  // lane: column i0 + 32 wi + 16 q + l32 / 2, its entry c = l32 % 2; rows j0 + 32 wj + 16 p + 4 v + 2 g + h
+  const int c01 = l32 & 1;
+  float* const out = n == 1 ? dW + (size_t)e * d_out * d_in * 8 : part + (size_t)plane * d_out * d_in * 8;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) red[(sr * kTile + sc) * 8 + c] = bsum[c];
-    __syncthreads();
-    if (sr == 0 && j0 + sc < d_out) {
-      float s[8] = {};
-      for (int q = 0; q < kRows; ++q)
+  for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) s[c] += red[(q * kTile + sc) * 8 + c];
-      // columns (entry 0, entry 1) b = 0, 1 -> M00, M01, M10, M11
-      const float m[8] = {s[0], s[1], s[4], s[5], s[2], s[3], s[6], s[7]};
-      store(db + ((size_t)e * d_out + j0 + sc) * 8, m);
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = j0 + 32 * wj + 16 * p + 4 * v + 2 * g + h, i = i0 + 32 * wi + 16 * q + (l32 >> 1);
+          const int k = 4 * v + 2 * h;
+          const float4 o = half_blades(acc[p][q][0][k], -acc[p][q][1][k], acc[p][q][0][k + 1], -acc[p][q][1][k + 1], c01);
+          if (j < d_out && i < d_in) *reinterpret_cast<float4*>(out + ((size_t)j * d_in + i) * 8 + 4 * c01) = o;
+        }
+  if (bias_wave) {
+    float* const ob = n == 1 ? db + (size_t)e * d_out * 8 : dbpart + (size_t)plane * d_out * 8;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bs[p][b][h] += __shfl_xor(bs[p][b][h], 32);
+      // this lane has row a = l32 % 2 of the matrix: its columns are the transposed matrix's entries, so
+      // half_blades of the transpose: entries (0, a) and (1, a) there are (a, 0) and (a, 1) here
+      const float4 t = half_blades(bs[p][0][0], bs[p][0][1], bs[p][1][0], bs[p][1][1], c01);
+      const int j = j0 + 32 * wj + 16 * p + (l32 >> 1);
+      // transposing keeps every blade but v2 and b13 (the antisymmetric ones), which change sign
+      const float4 o = c01 ? make_float4(t.x, -t.y, t.z, t.w) : make_float4(t.x, t.y, -t.z, t.w);
+      if (g == 0 && j < d_out) *reinterpret_cast<float4*>(ob + (size_t)j * 8 + 4 * c01) = o;
     }
   }
 }
 
+// dW and db of the experts whose rows are several chunks, their planes added in order, or none: zero.
+// A thread per four values, blockIdx.y the expert.
+__global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const float* __restrict__ part,
+                                                                      const float* __restrict__ dbpart,
+                                                                      const int32_t* __restrict__ offsets, int P, int E,
+                                                                      int d_in, int d_out, float* __restrict__ dW,
+                                                                      float* __restrict__ db) {
+  const int e = blockIdx.y, lane = threadIdx.x & 63;
+  const WbExpert x = wb_experts(offsets, E, P, lane);
+  const int n = __builtin_amdgcn_readlane(x.n, e);
+  if (n == 1) return;
+  const int first = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), e) - n;
+  const size_t nw = (size_t)d_out * d_in * 2, nb = db != nullptr ? (size_t)d_out * 2 : 0;
+  size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= nw + nb) return;
+  const bool bias = u >= nw;
+  const size_t stride = bias ? nb : nw;
+  if (bias) u -= nw;
+  const float4* p = reinterpret_cast<const float4*>(bias ? dbpart : part) + (size_t)first * stride + u;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int q = 0; q < n; ++q) {
+    const float4 v = p[(size_t)q * stride];
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  (reinterpret_cast<float4*>(bias ? db : dW) + (size_t)e * stride)[u] = s;
+}
+
+// chunks there can be, and planes of the experts that have several: such an expert has more than kWbChunk rows
+long long wb_chunks(long long P, int E) { return P / kWbChunk + std::min<long long>(E, P); }
+long long wb_planes(long long P, int E) { return P / kWbChunk + std::min<long long>(E, P / (kWbChunk + 1)); }
+
 }  // namespace
 
-size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out) { return 0; }
+size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out) {
+  return (size_t)wb_planes(P_max, E) * d_out * (d_in + 1) * 8 * sizeof(float);
+}
 
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream) {
   if (E == 0) return 0;
-  hipLaunchKernelGGL(weight_grad_bf16_kernel, dim3((d_out + kTile - 1) / kTile, (d_in + kTile - 1) / kTile, E), dim3(256),
-                     0, stream, static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(a), a_rows, gather,
-                     offsets, P_max, d_in, d_out, dW, db);
-  return check_launch("weight gradient (bf16)");
+  const long long planes = wb_planes(P_max, E), chunks = wb_chunks(P_max, E);
+  float* part = static_cast<float*>(workspace);
+  float* dbpart = part + (size_t)planes * d_out * d_in * 8;
+  const int n_xcd = 8;  // workgroups go to the XCDs round robin (8 on MI355X)
+  const long long nt = (long long)((d_out + kWbTile - 1) / kWbTile) * ((d_in + kWbTile - 1) / kWbTile);
+  if (chunks > 0) {
+    hipLaunchKernelGGL(weight_grad_bf16_kernel, dim3((unsigned)((chunks + n_xcd - 1) / n_xcd * n_xcd * nt)), dim3(256), 0,
+                       stream, static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(a), a_rows, gather, offsets,
+                       P_max, E, d_in, d_out, n_xcd, part, dbpart, dW, db);
+    if (check_launch("weight gradient (bf16)")) return -1;
+  }
+  const size_t n4 = (size_t)d_out * (d_in + (db ? 1 : 0)) * 2;
+  hipLaunchKernelGGL(weight_grad_bf16_reduce_kernel, dim3((unsigned)((n4 + 255) / 256), E), dim3(256), 0, stream, part,
+                     dbpart, offsets, P_max, E, d_in, d_out, dW, db);
+  return check_launch("weight gradient (bf16, reduction)");
 }
 
 }  // namespace ygg
@@ -140,6 +294,9 @@ YGG_API int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void*
                 "d_out)", P_max, E, d_in, d_out);
   YGG_CHECK_ARG(a_rows >= 0 && (gather != nullptr || a_rows >= P_max),
                 "ygg_grouped_weight_grad_pauli_bf16: a has %d rows, %d are read without a gather", a_rows, P_max);
+  YGG_CHECK_ARG((long long)(wb_chunks(P_max, E) + 8) * ((d_out + kWbTile - 1) / kWbTile) *
+                        ((d_in + kWbTile - 1) / kWbTile) <= 0x7fffffffLL && (long long)std::max(d_in, d_out) * 16 < 1LL << 31,
+                "ygg_grouped_weight_grad_pauli_bf16: P_max=%d d_in=%d d_out=%d exceed a launch", P_max, d_in, d_out);
   if (E == 0) return 0;
   YGG_CHECK_ARG(offsets && dW && (P_max == 0 || (dy_pauli && a_pauli)),
                 "ygg_grouped_weight_grad_pauli_bf16: null pointer argument");
