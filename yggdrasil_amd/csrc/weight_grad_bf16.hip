@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pauli_split.h"
 #include "ygg_common.h"
@@ -22,18 +23,19 @@ namespace {
 constexpr int kWbTile = 64;     // output columns j and input columns i of a workgroup
 constexpr int kWbRows = 8;      // rows of a stage
 constexpr int kWbStages = 4;    // stages in LDS: three in flight while one is read
-constexpr int kWbChunk = 512;   // rows of a workgroup at most
+constexpr int kWbMaxChunk = 1024, kWbMinChunk = 128;  // rows of a workgroup at most, see chunk_rows
 constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
 
-// Lane e: the rows of expert e and their chunks, n = ceil(rows / kWbChunk) of equal length (a multiple of a
+// Lane e: the rows of expert e and their chunks, n = ceil(rows / limit) of equal length (a multiple of a
 // stage's rows).  Whatever `offsets` holds, the ranges are inside [0, P] and disjoint: every bound is
 // clamped and at least the one before it.
 struct WbExpert {
   int beg, end, n, len;
 };
-__device__ __forceinline__ WbExpert wb_experts(const int32_t* __restrict__ offsets, int E, int P, int lane) {
+__device__ __forceinline__ WbExpert wb_experts(const int32_t* __restrict__ offsets, int E, int P, int limit,
+                                               int lane) {
   int beg = min(max(offsets[min(lane, E)], 0), P);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -42,7 +44,7 @@ __device__ __forceinline__ WbExpert wb_experts(const int32_t* __restrict__ offse
   }
   WbExpert x = {beg, max(beg, min(offsets[min(lane + 1, E)], P)), 0, 0};
   if (lane >= E) x.end = x.beg;
-  x.n = (x.end - x.beg + kWbChunk - 1) / kWbChunk;
+  x.n = (x.end - x.beg + limit - 1) / limit;
   x.len = x.n > 0 ? ((x.end - x.beg + x.n - 1) / x.n + kWbRows - 1) / kWbRows * kWbRows : 0;
   return x;
 }
@@ -74,25 +76,33 @@ __device__ __forceinline__ float4 half_blades(float r0, float i0, float r1, floa
 // to (im, -re) the sum is minus the imaginary part.  The dwords of 32 operand rows are neighbours in a
 // half-row, so the LDS reads, four times 4 bytes per operand, are free of bank conflicts without padding.
 //
-// The rows come by direct-to-LDS loads, 16 bytes a lane, one row of 64 columns an instruction, from buffer
-// descriptors based at the row (so the operands may have any size); a row past the chunk, or outside a,
-// has an empty descriptor and reads zeros.
+// The rows come by direct-to-LDS loads, 16 bytes a lane, one row of 64 columns an instruction.  Rows in place
+// are addressed from the chunk's first one (64-bit base: operands of any size); gathered rows over the whole
+// of A, which the host keeps below 2 GiB.
+template <bool GATHER>
 __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
-    const uint16_t* __restrict__ D, const uint16_t* __restrict__ A, int a_rows, const int32_t* __restrict__ gather,
-    const int32_t* __restrict__ offsets, int P, int E, int d_in, int d_out, int n_xcd, float* __restrict__ part,
+    const uint16_t* __restrict__ D, const uint16_t* __restrict__ A, int a_rows, const int32_t* __restrict__ gather_rows,
+    const int32_t* __restrict__ offsets, int P, int limit, int E, int d_in, int d_out, int n_xcd, float* __restrict__ part,
     float* __restrict__ dbpart, float* __restrict__ dW, float* __restrict__ db) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kWbStages * kWbStage];
-  __shared__ int s_src[kWbChunk + kWbRows];
+  __shared__ uint32_t s_src[GATHER ? kWbMaxChunk + kWbRows * kWbStages : 1];
+  const int32_t* const gather = GATHER ? gather_rows : nullptr;
   const int tid = threadIdx.x, lane = tid & 63;
   const int nj = (d_out + kWbTile - 1) / kWbTile, ni = (d_in + kWbTile - 1) / kWbTile, nt = nj * ni;
   // all tiles of a chunk on one XCD (workgroup b runs on XCD b mod 8): its rows are read into one L2
   const int bq = blockIdx.x / n_xcd, chunk = bq / nt * n_xcd + (blockIdx.x - bq * n_xcd), tile = bq % nt;
-  const WbExpert x = wb_experts(offsets, E, P, lane);
-  const int incl = wave_inclusive_sum(x.n, lane), planes = wave_inclusive_sum(x.n > 1 ? x.n : 0, lane);
-  const uint64_t after = __ballot(incl > chunk);
-  if (after == 0) return;
-  const int e = (int)__builtin_ctzll(after);
-  const int n = __builtin_amdgcn_readlane(x.n, e), c = chunk - (__builtin_amdgcn_readlane(incl, e) - n);
+  const WbExpert x = wb_experts(offsets, E, P, limit, lane);
+  // the chunks in order of falling length, so that the last to start are short: this lane's expert's first one
+  const int planes = wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), key = x.len * 64 + 63 - lane;
+  int first = 0;
+  for (int i = 0; i < E; ++i) {
+    const int k = __builtin_amdgcn_readlane(key, i), m = __builtin_amdgcn_readlane(x.n, i);
+    first += k > key ? m : 0;
+  }
+  const uint64_t mine = __ballot(lane < E && chunk >= first && chunk < first + x.n);
+  if (mine == 0) return;
+  const int e = (int)__builtin_ctzll(mine);
+  const int n = __builtin_amdgcn_readlane(x.n, e), c = chunk - __builtin_amdgcn_readlane(first, e);
   const int len = __builtin_amdgcn_readlane(x.len, e);
   const int r0 = __builtin_amdgcn_readlane(x.beg, e) + c * len;
   const int rows = max(0, min(len, __builtin_amdgcn_readlane(x.end, e) - r0));
@@ -100,33 +110,56 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j0 = (tile % nj) * kWbTile, i0 = (tile / nj) * kWbTile;
 
+  // the byte offset of every row's A from a_rsrc's base, or one past any range
+  const uint32_t a_row = (uint32_t)d_in * 16;
   if (gather != nullptr)
-    for (int i = tid; i < rows; i += 256) s_src[i] = gather[r0 + i];
+    for (int i = tid; i < limit + kWbRows * kWbStages; i += 256) {
+      const int src = i < rows ? gather[r0 + i] : -1;
+      s_src[i] = src >= 0 && src < a_rows ? (uint32_t)src * a_row : kBufferOff;
+    }
   __syncthreads();
 
-  // this lane's piece of a row: half lane / 32, columns 2 (lane % 32) and the next
+  // A row past the chunk lies past its descriptor's range and reads zeros.  This lane's piece of a row:
+  // half lane / 32, columns 2 (lane % 32) and the next; columns past the width get an offset past any range.
+  const __amdgpu_buffer_rsrc_t d_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(D) + (size_t)r0 * d_out * 8, (short)0, (uint32_t)rows * d_out * 16, kBufferFlags);
+  const __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(A) + (gather ? 0 : (size_t)r0 * d_in * 8), (short)0, (uint32_t)(gather ? a_rows : rows) * a_row,
+      kBufferFlags);
   const int col = 2 * (lane & 31);
-  const uint32_t d_off = j0 + col < d_out ? (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 : kBufferOff;
-  const uint32_t a_off = i0 + col < d_in ? (uint32_t)((lane >> 5) * d_in + i0 + col) * 8 : kBufferOff;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem;
-  auto row_of = [](const uint16_t* base, long long row, bool live, int d) __attribute__((always_inline)) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base) + (live ? row : 0) * d * 8, (short)0,
-                                             live ? (uint32_t)d * 16 : 0u, kBufferFlags);
-  };
-  auto issue = [&](int f) __attribute__((always_inline)) {  // stage f's rows: two of each operand a wave
-    const uint32_t st = lds0 + (f % kWbStages) * kWbStage + 2 * wave * 2 * kWbHalf;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = f * kWbRows + 2 * wave + u;
-      const bool live = r < rows;
-      int src = r0 + r;
-      if (gather != nullptr) src = __builtin_amdgcn_readfirstlane(s_src[min(r, kWbChunk - 1)]);
-      split_dma(row_of(D, r0 + r, live, d_out), st + u * 2 * kWbHalf, d_off, 0);
-      split_dma(row_of(A, src, live && src >= 0 && src < a_rows, d_in), st + kWbOperand + u * 2 * kWbHalf, a_off, 0);
+  const uint32_t d_bad = j0 + col < d_out ? 0u : kBufferOff, a_bad = i0 + col < d_in ? 0u : kBufferOff;
+  const uint32_t a_lane = (uint32_t)((lane >> 5) * d_in + i0 + col) * 8;
+  uint32_t d_next = (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 + (uint32_t)(2 * wave) * d_out * 16;
+  uint32_t a_next = a_lane + (uint32_t)(2 * wave) * a_row;  // (rows in place)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem + 2 * wave * 2 * kWbHalf;
+  uint32_t src[2] = {0, 0};  // gathered: the offsets of the next stage's two rows
+  auto next_src = [&](int f) __attribute__((always_inline)) {
+    if constexpr (GATHER) {
+      src[0] = s_src[f * kWbRows + 2 * wave];
+      src[1] = s_src[f * kWbRows + 2 * wave + 1];
     }
   };
+  auto issue = [&](int f) __attribute__((always_inline)) {  // stage f's rows: two of each operand a wave
+    const uint32_t st = lds0 + (f % kWbStages) * kWbStage;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      split_dma(d_rsrc, st + u * 2 * kWbHalf, (d_next + u * (uint32_t)d_out * 16) | d_bad, 0);
+      split_dma(a_rsrc, st + kWbOperand + u * 2 * kWbHalf, (GATHER ? src[u] + a_lane : a_next + u * a_row) | a_bad, 0);
+    }
+    d_next += (uint32_t)kWbRows * d_out * 16;
+    a_next += (uint32_t)kWbRows * a_row;
+  };
   const int wj = wave & 1, wi = wave >> 1, l32 = lane & 31, g = lane >> 5;
-  const uint32_t d_rd = 4 * g * kWbHalf + wj * 256 + l32 * 4, a_rd = kWbOperand + 4 * g * kWbHalf + wi * 256 + l32 * 4;
+  // (bases that the compiler cannot relate, so that it pairs the reads of two half-rows, whose values are
+  // neighbours in an operand, and not those of two blocks)
+  uint32_t d_rd[2], a_rd[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    d_rd[p] = 4 * g * kWbHalf + wj * 256 + p * 128 + l32 * 4;
+    a_rd[p] = kWbOperand + 4 * g * kWbHalf + wi * 256 + p * 128 + l32 * 4;
+    asm("" : "+v"(d_rd[p]));
+    asm("" : "+v"(a_rd[p]));
+  }
 
   pf32x16_t acc[2][2][2];  // [16 j][16 i][real, minus imaginary]
 #pragma unroll
@@ -142,45 +175,58 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
 
   const int nf = (rows + kWbRows - 1) / kWbRows;
 #pragma unroll
-  for (int f = 0; f < kWbStages - 1; ++f) issue(f);
-  for (int f = 0; f < nf; ++f) {
-    // four loads a stage: those of the two newer stages may stay outstanding
-    asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
-    issue(f + kWbStages - 1);  // over the stage read before the barrier
-    const unsigned char* st = smem + (f % kWbStages) * kWbStage;
+  for (int f = 0; f < kWbStages - 1; ++f) {
+    next_src(f);
+    issue(f);
+  }
+  next_src(kWbStages - 1);
+  auto loop = [&](auto bias_tag) __attribute__((always_inline)) {
+    constexpr bool BIAS = decltype(bias_tag)::value;
+    for (int f = 0; f < nf; ++f) {
+      // four loads a stage: those of the two newer stages may stay outstanding
+      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+      const unsigned char* st = smem + (f % kWbStages) * kWbStage;
+      uint32_t d[2][2][4], a[2][2][4];  // [four rows][block][half-row]
 #pragma unroll
-    for (int s = 0; s < kWbRows / 4; ++s) {
-      uint32_t d[2][4], a[2][4];
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          d[p][q] = *reinterpret_cast<const uint32_t*>(st + d_rd + (8 * s + q) * kWbHalf + p * 128);
-          a[p][q] = *reinterpret_cast<const uint32_t*>(st + a_rd + (8 * s + q) * kWbHalf + p * 128);
-        }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const pbf16x8_t X = __builtin_bit_cast(pbf16x8_t, make_uint4(a[q][0], a[q][1], a[q][2], a[q][3]));
-        const pbf16x8_t R = __builtin_bit_cast(
-            pbf16x8_t, make_uint4(rot_conj(a[q][0]), rot_conj(a[q][1]), rot_conj(a[q][2]), rot_conj(a[q][3])));
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const pbf16x8_t Y = __builtin_bit_cast(pbf16x8_t, make_uint4(d[p][0], d[p][1], d[p][2], d[p][3]));
-          acc[p][q][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, X, acc[p][q][0], 0, 0, 0);
-          acc[p][q][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, R, acc[p][q][1], 0, 0, 0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) d[s][p][q] = *reinterpret_cast<const uint32_t*>(st + d_rd[p] + (8 * s + q) * kWbHalf);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) a[s][p][q] = *reinterpret_cast<const uint32_t*>(st + a_rd[p] + (8 * s + q) * kWbHalf);
+        }
+      issue(f + kWbStages - 1);  // over the stage read before the barrier
+      next_src(f + kWbStages);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t* w = a[s][q];
+          const pbf16x8_t X = __builtin_bit_cast(pbf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+          const pbf16x8_t R = __builtin_bit_cast(
+              pbf16x8_t, make_uint4(rot_conj(w[0]), rot_conj(w[1]), rot_conj(w[2]), rot_conj(w[3])));
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const pbf16x8_t Y = __builtin_bit_cast(pbf16x8_t, make_uint4(d[s][p][0], d[s][p][1], d[s][p][2], d[s][p][3]));
+            acc[p][q][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, X, acc[p][q][0], 0, 0, 0);
+            acc[p][q][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Y, R, acc[p][q][1], 0, 0, 0);
+          }
+        }
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              bs[p][q & 1][0] += bf_lo(d[s][p][q]);
+              bs[p][q & 1][1] += bf_hi(d[s][p][q]);
+            }
         }
       }
-      if (bias_wave) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            bs[p][q & 1][0] += bf_lo(d[p][q]);
-            bs[p][q & 1][1] += bf_hi(d[p][q]);
-          }
-      }
     }
-  }
+  };
+  if (bias_wave) loop(std::true_type{});
+  else loop(std::false_type{});
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads past the last stage write LDS too
 
   // lane: column i0 + 32 wi + 16 q + l32 / 2, its entry c = l32 % 2; rows j0 + 32 wj + 16 p + 4 v + 2 g + h
@@ -222,11 +268,11 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
 // A thread per four values, blockIdx.y the expert.
 __global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const float* __restrict__ part,
                                                                       const float* __restrict__ dbpart,
-                                                                      const int32_t* __restrict__ offsets, int P, int E,
-                                                                      int d_in, int d_out, float* __restrict__ dW,
-                                                                      float* __restrict__ db) {
+                                                                      const int32_t* __restrict__ offsets, int P, int limit,
+                                                                      int E, int d_in, int d_out,
+                                                                      float* __restrict__ dW, float* __restrict__ db) {
   const int e = blockIdx.y, lane = threadIdx.x & 63;
-  const WbExpert x = wb_experts(offsets, E, P, lane);
+  const WbExpert x = wb_experts(offsets, E, P, limit, lane);
   const int n = __builtin_amdgcn_readlane(x.n, e);
   if (n == 1) return;
   const int first = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), e) - n;
@@ -246,33 +292,49 @@ __global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const floa
   (reinterpret_cast<float4*>(bias ? db : dW) + (size_t)e * stride)[u] = s;
 }
 
-// chunks there can be, and planes of the experts that have several: such an expert has more than kWbChunk rows
-long long wb_chunks(long long P, int E) { return P / kWbChunk + std::min<long long>(E, P); }
-long long wb_planes(long long P, int E) { return P / kWbChunk + std::min<long long>(E, P / (kWbChunk + 1)); }
+long long wb_tiles(int d_in, int d_out) {
+  return (long long)((d_out + kWbTile - 1) / kWbTile) * ((d_in + kWbTile - 1) / kWbTile);
+}
+// The rows of a chunk at most: what each of the 512 workgroups that the chip holds would have of all rows' tiles,
+// within limits -- below 128 rows a workgroup's start and its plane cost more than its products (CHUNKTEXT)
+int chunk_rows(int P, int d_in, int d_out) {
+  const long long even = (long long)P * wb_tiles(d_in, d_out) / 512;
+  return (int)std::min<long long>(kWbMaxChunk, std::max<long long>(kWbMinChunk, even)) / kWbRows * kWbRows;
+}
+// chunks there can be, and planes of the experts that have several: such an expert has more than `limit` rows
+long long wb_chunks(long long P, int E, int limit) { return P / limit + std::min<long long>(E, P); }
+long long wb_planes(long long P, int E, int limit) { return P / limit + std::min<long long>(E, P / (limit + 1)); }
 
 }  // namespace
 
 size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out) {
-  return (size_t)wb_planes(P_max, E) * d_out * (d_in + 1) * 8 * sizeof(float);
+  return (size_t)wb_planes(P_max, E, chunk_rows(P_max, d_in, d_out)) * d_out * (d_in + 1) * 8 * sizeof(float);
 }
 
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream) {
   if (E == 0) return 0;
-  const long long planes = wb_planes(P_max, E), chunks = wb_chunks(P_max, E);
+  const int limit = chunk_rows(P_max, d_in, d_out);
+  const long long planes = wb_planes(P_max, E, limit), chunks = wb_chunks(P_max, E, limit);
   float* part = static_cast<float*>(workspace);
   float* dbpart = part + (size_t)planes * d_out * d_in * 8;
   const int n_xcd = 8;  // workgroups go to the XCDs round robin (8 on MI355X)
-  const long long nt = (long long)((d_out + kWbTile - 1) / kWbTile) * ((d_in + kWbTile - 1) / kWbTile);
+  const long long nt = wb_tiles(d_in, d_out);
   if (chunks > 0) {
-    hipLaunchKernelGGL(weight_grad_bf16_kernel, dim3((unsigned)((chunks + n_xcd - 1) / n_xcd * n_xcd * nt)), dim3(256), 0,
-                       stream, static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(a), a_rows, gather, offsets,
-                       P_max, E, d_in, d_out, n_xcd, part, dbpart, dW, db);
+    const dim3 grid((unsigned)((chunks + n_xcd - 1) / n_xcd * n_xcd * nt));
+    if (gather)
+      hipLaunchKernelGGL(weight_grad_bf16_kernel<true>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(dy),
+                         static_cast<const uint16_t*>(a), a_rows, gather, offsets, P_max, limit, E, d_in, d_out, n_xcd, part,
+                         dbpart, dW, db);
+    else
+      hipLaunchKernelGGL(weight_grad_bf16_kernel<false>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(dy),
+                         static_cast<const uint16_t*>(a), a_rows, gather, offsets, P_max, limit, E, d_in, d_out, n_xcd, part,
+                         dbpart, dW, db);
     if (check_launch("weight gradient (bf16)")) return -1;
   }
   const size_t n4 = (size_t)d_out * (d_in + (db ? 1 : 0)) * 2;
   hipLaunchKernelGGL(weight_grad_bf16_reduce_kernel, dim3((unsigned)((n4 + 255) / 256), E), dim3(256), 0, stream, part,
-                     dbpart, offsets, P_max, E, d_in, d_out, dW, db);
+                     dbpart, offsets, P_max, limit, E, d_in, d_out, dW, db);
   return check_launch("weight gradient (bf16, reduction)");
 }
 
@@ -294,9 +356,10 @@ YGG_API int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void*
                 "d_out)", P_max, E, d_in, d_out);
   YGG_CHECK_ARG(a_rows >= 0 && (gather != nullptr || a_rows >= P_max),
                 "ygg_grouped_weight_grad_pauli_bf16: a has %d rows, %d are read without a gather", a_rows, P_max);
-  YGG_CHECK_ARG((long long)(wb_chunks(P_max, E) + 8) * ((d_out + kWbTile - 1) / kWbTile) *
-                        ((d_in + kWbTile - 1) / kWbTile) <= 0x7fffffffLL && (long long)std::max(d_in, d_out) * 16 < 1LL << 31,
+  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) <= 0x7fffffffLL && (long long)(kWbMaxChunk + kWbRows * kWbStages) * std::max(d_in, d_out) * 16 < 1LL << 31,
                 "ygg_grouped_weight_grad_pauli_bf16: P_max=%d d_in=%d d_out=%d exceed a launch", P_max, d_in, d_out);
+  YGG_CHECK_ARG(gather == nullptr || (long long)a_rows * d_in * 16 < 1LL << 31,
+                "ygg_grouped_weight_grad_pauli_bf16: gathered rows span 2 GiB or more (a_rows=%d d_in=%d)", a_rows, d_in);
   if (E == 0) return 0;
   YGG_CHECK_ARG(offsets && dW && (P_max == 0 || (dy_pauli && a_pauli)),
                 "ygg_grouped_weight_grad_pauli_bf16: null pointer argument");
