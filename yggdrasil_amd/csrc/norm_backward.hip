@@ -15,7 +15,9 @@
 
 #include <hip/hip_runtime.h>
 
-#include "pauli_common.h"
+#include <algorithm>
+
+#include "rows.h"
 #include "ygg_common.h"
 
 namespace ygg {
@@ -24,26 +26,6 @@ namespace {
 constexpr int kNbMaxD = 4096;     // the forward's limit
 constexpr int kNbPlaneTokens = 64;  // tokens per partial plane
 
-__device__ inline void load_mv(const float* p, size_t n, float v[8]) {
-  const float4* q = reinterpret_cast<const float4*>(p + n * 8);
-  const float4 a = q[0], b = q[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ inline void load_mv(const uint16_t* p, size_t n, float v[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p + n * 8);
-  v[0] = bf_lo(q.x); v[1] = bf_hi(q.x); v[2] = bf_lo(q.y); v[3] = bf_hi(q.y);
-  v[4] = bf_lo(q.z); v[5] = bf_hi(q.z); v[6] = bf_lo(q.w); v[7] = bf_hi(q.w);
-}
-__device__ inline void store_mv(float* p, size_t n, const float v[8]) {
-  float4* q = reinterpret_cast<float4*>(p + n * 8);
-  q[0] = make_float4(v[0], v[1], v[2], v[3]);
-  q[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ inline void store_mv(uint16_t* p, size_t n, const float v[8]) {
-  *reinterpret_cast<uint4*>(p + n * 8) =
-      make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
-}
 __device__ constexpr float rev(int c) { return c >= 4 ? -1.f : 1.f; }  // grades 2 and 3 change sign
 
 // o = (~)a b or a ~b, over the blades
@@ -139,36 +121,227 @@ __global__ __launch_bounds__(64) void norm_param_kernel(const GT* __restrict__ d
   store_mv(p, 1, sb);
 }
 
-// The planes added in order: a thread per value.
-__global__ __launch_bounds__(256) void norm_param_reduce_kernel(const float* __restrict__ part, int planes, int d,
-                                                                float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= d * 16) return;
-  float s = 0.f;
-  for (int p = 0; p < planes; ++p) s += part[(size_t)p * d * 16 + n];
-  const int i = n >> 4, c = n & 15;
-  (c < 8 ? dgamma : dbeta)[(size_t)i * 8 + (c & 7)] = s;
+// ---- rows of at most 1024 multivectors: one pass -------------------------------------------------
+// A workgroup of four waves takes U tokens at a time: CS waves share a row (a lane holds NQ of its multivectors),
+// the 4 / CS groups of them different tokens.  With M the Pauli matrices of pauli_common.h, where reversion is
+// the conjugate transpose, gx = M(gamma)^H M(dy) and the gradient of gamma is M(dy) M(xh)^H: 32 multiply-adds
+// each, and <gx, x> is half the sum of the matrices' entries' products.  Every row is read once; the sums over
+// the tokens stay in registers until the workgroup's last token, and are a plane of the workgroup's own then.
+//
+// Bound by memory: FUSEDTEXT
+constexpr int kNbFusedMaxD = 1024, kNbMaxPlanes = 512;  // planes: two workgroups on each of 256 CUs
+
+template <typename XT, typename GT, int CS, int NQ, int U>
+__global__ __launch_bounds__(256) void norm_backward_kernel(const GT* __restrict__ dy, const XT* __restrict__ x, int N,
+                                                            int d, const float* __restrict__ gamma, float two_eps,
+                                                            const XT* residual, XT* dx, float* __restrict__ part) {
+  constexpr int TS = 4 / CS;
+  __shared__ float red[2][4][2 * U];  // [parity][wave][token of the batch: |x|^2, <gx, x>]
+  __shared__ float4 sums[TS > 1 ? TS - 1 : 1][64 * CS][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int cw = wave % CS, tw = wave / CS;
+  int col[NQ];
+  bool live[NQ];
+  float ga[NQ][2][4];  // the columns of gamma's matrix: (re, im) of entries 0 and 1
+  float sg[NQ][8], sb[NQ][8];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int i = (q * CS + cw) * 64 + lane;
+    live[q] = i < d;
+    col[q] = live[q] ? i : 0;
+    float v[8];
+    load_mv(gamma, col[q], v);
+    blade_to_pauli(v, ga[q][0], ga[q][1]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) sg[q][c] = sb[q][c] = 0.f;
+  }
+  int parity = 0;
+  for (int t0 = (blockIdx.x * TS + tw) * U, round = 0; round * gridDim.x * TS * U < N; ++round, t0 += gridDim.x * TS * U) {
+    // (a token past the last repeats it, adds nothing and is not stored)
+    RawMv<XT> rx[U][NQ], rr[U][NQ];
+    RawMv<GT> rg[U][NQ];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const size_t n = (size_t)min(t0 + u, N - 1) * d + col[q];
+        rx[u][q] = load_raw(x, n);
+        rg[u][q] = load_raw(dy, n);
+      }
+    if (residual != nullptr) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) rr[u][q] = load_raw(residual, (size_t)min(t0 + u, N - 1) * d + col[q]);
+    }
+    float gx[U][NQ][2][4], own[2 * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float n2 = 0.f, dot = 0.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float v[8], xp[2][4], gp[2][4];
+        unpack(rx[u][q], v);
+        if (!live[q])
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) n2 = __builtin_fmaf(v[c], v[c], n2);
+        blade_to_pauli(v, xp[0], xp[1]);
+        unpack(rg[u][q], v);
+        if (!live[q])
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = 0.f;
+        blade_to_pauli(v, gp[0], gp[1]);
+        // gx[r][b] = sum_a conj(gamma[a][r]) dy[a][b]
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float* h = ga[q][r];
+            const float* y = gp[b];
+            const float re = __builtin_fmaf(h[3], y[3], __builtin_fmaf(h[2], y[2], __builtin_fmaf(h[1], y[1], h[0] * y[0])));
+            const float im = __builtin_fmaf(-h[3], y[2], __builtin_fmaf(h[2], y[3], __builtin_fmaf(-h[1], y[0], h[0] * y[1])));
+            gx[u][q][b][2 * r] = re;
+            gx[u][q][b][2 * r + 1] = im;
+            dot = __builtin_fmaf(re, xp[b][2 * r], __builtin_fmaf(im, xp[b][2 * r + 1], dot));
+          }
+      }
+      own[2 * u] = n2;
+      own[2 * u + 1] = dot;
+    }
+    const float s = wave_sums<2 * U>(own, lane);
+    if ((lane & (64 / (2 * U) - 1)) == 0) red[parity][wave][wave_sums_of<2 * U>(lane)] = s;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float n2 = 0.f, dot = 0.f;
+#pragma unroll
+      for (int w = 0; w < CS; ++w) {
+        n2 += red[parity][tw * CS + w][2 * u];
+        dot += red[parity][tw * CS + w][2 * u + 1];
+      }
+      if (t0 + u >= N) continue;
+      const float r = 1.0f / sqrtf(n2 / (float)d + two_eps);
+      const float hr = 0.5f * r, w = -hr * (0.5f * dot) * r * r / (float)d;  // dx = (gx - x <gx, x> / (rms^2 d)) / rms
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float v[8], g[8], xp[2][4], gp[2][4], o[8], e[8];
+        unpack(rx[u][q], v);
+        unpack(rg[u][q], g);
+        blade_to_pauli(v, xp[0], xp[1]);
+        blade_to_pauli(g, gp[0], gp[1]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) e[4 * b + c] = __builtin_fmaf(hr, gx[u][q][b][c], w * xp[b][c]);
+        pauli_to_blade(e[0], e[1], e[4], e[5], e[2], e[3], e[6], e[7], o);
+        if (residual != nullptr) {
+          float f[8];
+          unpack(rr[u][q], f);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) o[c] += f[c];
+        }
+        if (live[q]) {
+          store_mv(dx, (size_t)(t0 + u) * d + col[q], o);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) sb[q][c] += g[c];
+        }
+        // M(dy) M(xh)^H, entry (a, c) = sum_b dy[a][b] conj(xh[c][b])
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) xp[b][c] *= r;
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float yr = gp[b][2 * a], yi = gp[b][2 * a + 1], xr = xp[b][2 * c], xi = xp[b][2 * c + 1];
+              float* to = sg[q] + 4 * a + 2 * c;
+              to[0] = __builtin_fmaf(yi, xi, __builtin_fmaf(yr, xr, to[0]));
+              to[1] = __builtin_fmaf(-yr, xi, __builtin_fmaf(yi, xr, to[1]));
+            }
+        }
+      }
+    }
+    parity ^= 1;  // the sums just read are written again after the next barrier
+  }
+  // the token groups' sums added in order
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    float o[16];
+    pauli_to_blade(sg[q][0], sg[q][1], sg[q][2], sg[q][3], sg[q][4], sg[q][5], sg[q][6], sg[q][7], o);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      o[c] *= 0.5f;
+      o[8 + c] = sb[q][c];
+    }
+    if constexpr (TS > 1) {
+      __syncthreads();
+      if (tw > 0)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sums[tw - 1][cw * 64 + lane][c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      __syncthreads();
+      if (tw == 0)
+#pragma unroll
+        for (int k = 0; k < TS - 1; ++k)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float4 m = sums[k][cw * 64 + lane][c];
+            o[4 * c] += m.x; o[4 * c + 1] += m.y; o[4 * c + 2] += m.z; o[4 * c + 3] += m.w;
+          }
+    }
+    if (tw == 0 && live[q]) {
+      float* to = part + ((size_t)blockIdx.x * d + col[q]) * 16;
+      store_mv(to, 0, o);
+      store_mv(to, 1, o + 8);
+    }
+  }
 }
 
-int planes_of(int N) { return (N + kNbPlaneTokens - 1) / kNbPlaneTokens; }
-size_t rrms_bytes(int N) { return ((size_t)N * 4 + 255) / 256 * 256; }
+__global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int planes, int d,
+                                                                 float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  add_planes(part, planes, d * 16, [&](int n, float v) { ((n & 15) < 8 ? dgamma : dbeta)[(size_t)(n >> 4) * 8 + (n & 7)] = v; });
+}
+
+// The tokens of a workgroup's batch and the planes of the one-pass kernel
+int fused_batch(int d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 256 ? 4 : d <= 512 ? 2 : 1; }
+int planes_of(int N, int d) {
+  if (d > kNbFusedMaxD) return (N + kNbPlaneTokens - 1) / kNbPlaneTokens;
+  return std::min((N + fused_batch(d) - 1) / fused_batch(d), kNbMaxPlanes);
+}
+size_t rrms_bytes(int N, int d) { return d <= kNbFusedMaxD ? 0 : ((size_t)N * 4 + 255) / 256 * 256; }
 
 template <typename XT, typename GT>
 int launch(const void* dy, const void* x, int N, int d, const float* gamma, float two_eps, const void* residual,
            void* dx, float* dgamma, float* dbeta, void* workspace, hipStream_t stream) {
   float* rrms = static_cast<float*>(workspace);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + rrms_bytes(N));
-  if (N > 0) {
+  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + rrms_bytes(N, d));
+  const int planes = planes_of(N, d);
+  if (N > 0 && d <= kNbFusedMaxD) {
+#define YGG_NB(CS, NQ, U)                                                                                              \
+  hipLaunchKernelGGL((norm_backward_kernel<XT, GT, CS, NQ, U>), dim3(planes), dim3(256), 0, stream,                    \
+                     static_cast<const GT*>(dy), static_cast<const XT*>(x), N, d, gamma, two_eps,                      \
+                     static_cast<const XT*>(residual), static_cast<XT*>(dx), part)
+    if (d <= 64) YGG_NB(1, 1, 4);
+    else if (d <= 128) YGG_NB(2, 1, 4);
+    else if (d <= 256) YGG_NB(4, 1, 4);
+    else if (d <= 512) YGG_NB(4, 2, 2);
+    else YGG_NB(4, 4, 1);
+#undef YGG_NB
+    if (check_launch("norm backward")) return -1;
+  } else if (N > 0) {
     hipLaunchKernelGGL((norm_dx_kernel<XT, GT>), dim3((N + 3) / 4), dim3(256), 0, stream, static_cast<const GT*>(dy),
                        static_cast<const XT*>(x), N, d, gamma, two_eps, static_cast<const XT*>(residual),
                        static_cast<XT*>(dx), rrms);
     if (check_launch("norm backward")) return -1;
-    hipLaunchKernelGGL((norm_param_kernel<XT, GT>), dim3(planes_of(N), (d + 63) / 64), dim3(64), 0, stream,
+    hipLaunchKernelGGL((norm_param_kernel<XT, GT>), dim3(planes, (d + 63) / 64), dim3(64), 0, stream,
                        static_cast<const GT*>(dy), static_cast<const XT*>(x), N, d, rrms, part);
     if (check_launch("norm backward (gamma and beta)")) return -1;
   }
-  hipLaunchKernelGGL(norm_param_reduce_kernel, dim3((d * 16 + 255) / 256), dim3(256), 0, stream, part, planes_of(N), d,
-                     dgamma, dbeta);
+  hipLaunchKernelGGL(norm_param_reduce_kernel, dim3((d * 16 + 31) / 32), dim3(1024), 0, stream, part, planes, d, dgamma,
+                     dbeta);
   return check_launch("norm backward (reduction)");
 }
 
@@ -179,7 +352,7 @@ using namespace ygg;
 
 YGG_API size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d) {
   if (N < 0 || d < 1 || d > kNbMaxD) return 0;
-  return rrms_bytes(N) + (size_t)planes_of(N) * d * 16 * sizeof(float);
+  return rrms_bytes(N, d) + (size_t)planes_of(N, d) * d * 16 * sizeof(float);
 }
 
 YGG_API int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int N, int d,

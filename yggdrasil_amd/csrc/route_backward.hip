@@ -17,7 +17,10 @@
 
 #include <hip/hip_runtime.h>
 
-#include "pauli_common.h"
+#include <algorithm>
+#include <type_traits>
+
+#include "rows.h"
 #include "ygg_common.h"
 
 namespace ygg {
@@ -52,119 +55,145 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const int32_t* __re
   dlogits[n] = v;
 }
 
-__device__ inline void load8(const float* p, size_t n, float v[8]) {
-  const float4* q = reinterpret_cast<const float4*>(p + n * 8);
-  const float4 a = q[0], b = q[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ inline void load8(const uint16_t* p, size_t n, float v[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p + n * 8);
-  v[0] = bf_lo(q.x); v[1] = bf_hi(q.x); v[2] = bf_lo(q.y); v[3] = bf_hi(q.y);
-  v[4] = bf_lo(q.z); v[5] = bf_hi(q.z); v[6] = bf_lo(q.w); v[7] = bf_hi(q.w);
-}
-__device__ inline void store8(float* p, size_t n, const float v[8]) {
-  float4* q = reinterpret_cast<float4*>(p + n * 8);
-  q[0] = make_float4(v[0], v[1], v[2], v[3]);
-  q[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ inline void store8(uint16_t* p, size_t n, const float v[8]) {
-  *reinterpret_cast<uint4*>(p + n * 8) =
-      make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
-}
+// A workgroup takes tokens_per tokens, a wave one at a time (a row of up to 64 NQ multivectors in registers, the
+// rest read again from L2): the energies, dx (plus add), and for the parameters the token's shares and slot
+// gradients, which stay in LDS.  Then lane e of every wave adds what expert e has of the wave's share of the
+// slots, the waves' sums are added in order, and the workgroup writes them as a plane of its own.
+//
+// Bound by memory: ROUTETEXT
+constexpr int kRbTokens = 32;  // tokens of a workgroup at most
 
-// One wave per token: dx (plus add), and the token's energy shares for the parameters' sums.
-template <typename T>
+template <typename T, int NQ>
 __global__ __launch_bounds__(256) void energy_backward_kernel(const T* __restrict__ x, int N, int d,
                                                               const float* __restrict__ W, int E, int k,
                                                               const int32_t* __restrict__ idx,
                                                               const float* __restrict__ w, const float* __restrict__ g,
-                                                              const T* __restrict__ add, T* __restrict__ dx,
-                                                              float* __restrict__ shares) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= N) return;
-  const size_t row = (size_t)t * d;
-  float en[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = lane; i < d; i += 64) {
-    float v[8];
-    load8(x, row + i, v);
-    en[0] = __builtin_fmaf(v[0], v[0], en[0]);
-    en[3] = __builtin_fmaf(v[7], v[7], en[3]);
+                                                              const T* add, T* dx, int tokens_per,
+                                                              float* __restrict__ part) {
+  __shared__ float4 s_share[kRbTokens];
+  __shared__ float s_dl[kRbTokens * kRbMaxK];
+  __shared__ int s_idx[kRbTokens * kRbMaxK];
+  __shared__ float s_red[4][5][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = blockIdx.x * tokens_per, tokens = min(tokens_per, N - t0);
+  for (int u = wave; u < tokens; u += 4) {
+    const int t = t0 + u;
+    const size_t row = (size_t)t * d;
+    RawMv<T> rx[NQ], ra[NQ];
 #pragma unroll
-    for (int c = 0; c < 3; ++c) {
-      en[1] = __builtin_fmaf(v[1 + c], v[1 + c], en[1]);
-      en[2] = __builtin_fmaf(v[4 + c], v[4 + c], en[2]);
+    for (int q = 0; q < NQ; ++q)
+      if (lane + 64 * q < d) rx[q] = load_raw(x, row + lane + 64 * q);
+    if (add != nullptr) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+        if (lane + 64 * q < d) ra[q] = load_raw(add, row + lane + 64 * q);
     }
-  }
-#pragma unroll
-  for (int h = 0; h < 4; ++h)
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) en[h] += __shfl_xor(en[h], o);
-  const float total = ((en[0] + en[1]) + (en[2] + en[3])) + 1e-12f;
-  float dl[kRbMaxK], ds[4] = {0.f, 0.f, 0.f, 0.f}, sh[4], dot = 0.f;
-  slot_gradients(w, g, t, k, dl);
-#pragma unroll
-  for (int s = 0; s < kRbMaxK; ++s) {
-    const int e = s < k ? idx[(size_t)t * k + s] : 0;
-    if (s < k && e >= 0 && e < E)
-#pragma unroll
-      for (int h = 0; h < 4; ++h) ds[h] = __builtin_fmaf(dl[s], W[e * 4 + h], ds[h]);
-  }
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    sh[h] = en[h] / total;
-    dot = __builtin_fmaf(ds[h], sh[h], dot);
-  }
-  if (lane < 4) shares[(size_t)t * 4 + lane] = lane == 0 ? sh[0] : lane == 1 ? sh[1] : lane == 2 ? sh[2] : sh[3];
-  float de[4];
-#pragma unroll
-  for (int h = 0; h < 4; ++h) de[h] = 2.f * (ds[h] - dot) / total;
-  for (int i = lane; i < d; i += 64) {
-    float v[8], o[8] = {};
-    load8(x, row + i, v);
-    if (add != nullptr) load8(add, row + i, o);
-#pragma unroll
-    for (int c = 0; c < 8; ++c) o[c] = __builtin_fmaf(v[c], de[c == 0 ? 0 : c < 4 ? 1 : c < 7 ? 2 : 3], o[c]);
-    store8(dx, row + i, o);
-  }
-}
-
-// One workgroup per expert: its slots of all tokens, added per thread and then over the threads.
-__global__ __launch_bounds__(256) void router_param_kernel(const int32_t* __restrict__ idx, const float* __restrict__ w,
-                                                           const float* __restrict__ g,
-                                                           const float* __restrict__ shares, int N, int k,
-                                                           float* __restrict__ dW, float* __restrict__ db) {
-  const int e = blockIdx.x;
-  float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int t = threadIdx.x; t < N; t += 256) {
-    float v = 0.f;
-    bool mine = false;
-    for (int s = 0; s < k; ++s) mine |= idx[(size_t)t * k + s] == e;
-    if (!mine) continue;
-    float dl[kRbMaxK];
+    // the slots' gradients and those of the shares (the same in every lane)
+    float dl[kRbMaxK], ds[4] = {0.f, 0.f, 0.f, 0.f};
     slot_gradients(w, g, t, k, dl);
 #pragma unroll
     for (int s = 0; s < kRbMaxK; ++s)
-      if (s < k && idx[(size_t)t * k + s] == e) v += dl[s];
+      if (s < k) {
+        const int e = idx[(size_t)t * k + s];
+        const bool known = e >= 0 && e < E;
+        if (known)
 #pragma unroll
-    for (int h = 0; h < 4; ++h) s5[h] = __builtin_fmaf(v, shares[(size_t)t * 4 + h], s5[h]);
-    s5[4] += v;
-  }
-  __shared__ float red[4][5];
+          for (int h = 0; h < 4; ++h) ds[h] = __builtin_fmaf(dl[s], W[e * 4 + h], ds[h]);
+        if (lane == 0) {
+          s_dl[u * kRbMaxK + s] = dl[s];
+          s_idx[u * kRbMaxK + s] = e;
+        }
+      }
+    float en[4] = {0.f, 0.f, 0.f, 0.f};
+    auto energies = [&](const float v[8]) __attribute__((always_inline)) {
+      en[0] = __builtin_fmaf(v[0], v[0], en[0]);
+      en[3] = __builtin_fmaf(v[7], v[7], en[3]);
 #pragma unroll
-  for (int h = 0; h < 5; ++h) {
+      for (int c = 0; c < 3; ++c) {
+        en[1] = __builtin_fmaf(v[1 + c], v[1 + c], en[1]);
+        en[2] = __builtin_fmaf(v[4 + c], v[4 + c], en[2]);
+      }
+    };
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s5[h] += __shfl_xor(s5[h], o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][h] = s5[h];
+    for (int q = 0; q < NQ; ++q)
+      if (lane + 64 * q < d) {
+        float v[8];
+        unpack(rx[q], v);
+        energies(v);
+      }
+    for (int i = lane + 64 * NQ; i < d; i += 64) {
+      float v[8];
+      load_mv(x, row + i, v);
+      energies(v);
+    }
+    const float sum = wave_sums<4>(en, lane);
+    float sh[4], dot = 0.f;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) en[h] = __shfl(sum, 16 * h);
+    const float total = ((en[0] + en[1]) + (en[2] + en[3])) + 1e-12f;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      sh[h] = en[h] / total;
+      dot = __builtin_fmaf(ds[h], sh[h], dot);
+    }
+    if (lane == 0) s_share[u] = make_float4(sh[0], sh[1], sh[2], sh[3]);
+    float de[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) de[h] = 2.f * (ds[h] - dot) / total;
+    auto out = [&](float v[8], float o[8], int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) o[c] = __builtin_fmaf(v[c], de[c == 0 ? 0 : c < 4 ? 1 : c < 7 ? 2 : 3], o[c]);
+      store_mv(dx, row + i, o);
+    };
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+      if (lane + 64 * q < d) {
+        float v[8], o[8] = {};
+        unpack(rx[q], v);
+        if (add != nullptr) unpack(ra[q], o);
+        out(v, o, lane + 64 * q);
+      }
+    for (int i = lane + 64 * NQ; i < d; i += 64) {
+      float v[8], o[8] = {};
+      load_mv(x, row + i, v);
+      if (add != nullptr) load_mv(add, row + i, o);
+      out(v, o, i);
+    }
   }
   __syncthreads();
-  if (threadIdx.x < 5) {
-    const float v = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    if (threadIdx.x < 4) dW[e * 4 + threadIdx.x] = v;
-    else db[e] = v;
+  float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int u = wave; u < tokens; u += 4) {
+    const float4 share = s_share[u];
+    for (int s = 0; s < k; ++s) {
+      const float v = s_idx[u * kRbMaxK + s] == lane ? s_dl[u * kRbMaxK + s] : 0.f;
+      s5[0] = __builtin_fmaf(v, share.x, s5[0]);
+      s5[1] = __builtin_fmaf(v, share.y, s5[1]);
+      s5[2] = __builtin_fmaf(v, share.z, s5[2]);
+      s5[3] = __builtin_fmaf(v, share.w, s5[3]);
+      s5[4] += v;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 5; ++h) s_red[wave][h][lane] = s5[h];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 5 * E; i += 256) {  // plane: [5][E], the last row the bias
+    const int h = i / E, e = i - h * E;
+    part[(size_t)blockIdx.x * 5 * E + i] = (s_red[0][h][e] + s_red[1][h][e]) + (s_red[2][h][e] + s_red[3][h][e]);
   }
 }
+
+__global__ __launch_bounds__(1024) void router_param_kernel(const float* __restrict__ part, int planes, int E,
+                                                            float* __restrict__ dW, float* __restrict__ db) {
+  add_planes(part, planes, 5 * E, [&](int n, float v) {
+    const int h = n / E, e = n - h * E;
+    if (h < 4) dW[e * 4 + h] = v;
+    else db[e] = v;
+  });
+}
+
+// Tokens of a workgroup: enough workgroups to fill the chip first (eight on each of 256 CUs), then fewer planes
+int tokens_per_group(int N) { return std::min(kRbTokens, std::max(4, (N / 2048 + 3) / 4 * 4)); }
+int route_planes(int N) { return (N + tokens_per_group(N) - 1) / tokens_per_group(N); }
 
 }  // namespace
 }  // namespace ygg
@@ -185,7 +214,7 @@ YGG_API int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, con
 
 YGG_API size_t ygg_route_energy_backward_workspace_bytes(int N, int E) {
   if (N < 0 || E < 1) return 0;
-  return (size_t)N * 16;
+  return (size_t)route_planes(N) * 5 * E * sizeof(float);
 }
 
 YGG_API int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const float* router_w, int E, int k,
@@ -201,20 +230,24 @@ YGG_API int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, 
   const size_t need = ygg_route_energy_backward_workspace_bytes(N, E);
   YGG_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                 "ygg_route_energy_backward: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0, need);
-  float* shares = static_cast<float*>(workspace);
+  float* part = static_cast<float*>(workspace);
   if (N > 0) {
-    const dim3 grid((N + 3) / 4);
-    if (x_dtype == kF32)
-      hipLaunchKernelGGL(energy_backward_kernel<float>, grid, dim3(256), 0, stream, static_cast<const float*>(x), N, d,
-                         router_w, E, k, topk_idx, topk_w, dtopk_w, static_cast<const float*>(dx_add),
-                         static_cast<float*>(dx), shares);
-    else
-      hipLaunchKernelGGL(energy_backward_kernel<uint16_t>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(x), N,
-                         d, router_w, E, k, topk_idx, topk_w, dtopk_w, static_cast<const uint16_t*>(dx_add),
-                         static_cast<uint16_t*>(dx), shares);
+    auto run = [&](auto* xt, auto nq) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(xt)>>;
+      hipLaunchKernelGGL((energy_backward_kernel<T, decltype(nq)::value>), dim3(route_planes(N)), dim3(256), 0, stream, xt,
+                         N, d, router_w, E, k, topk_idx, topk_w, dtopk_w, static_cast<const T*>(dx_add),
+                         static_cast<T*>(dx), tokens_per_group(N), part);
+    };
+    auto by_width = [&](auto* xt) {
+      if (d <= 64) run(xt, std::integral_constant<int, 1>{});
+      else if (d <= 128) run(xt, std::integral_constant<int, 2>{});
+      else run(xt, std::integral_constant<int, 4>{});
+    };
+    if (x_dtype == kF32) by_width(static_cast<const float*>(x));
+    else by_width(static_cast<const uint16_t*>(x));
     if (check_launch("ygg_route_energy_backward")) return -1;
   }
-  hipLaunchKernelGGL(router_param_kernel, dim3(E), dim3(256), 0, stream, topk_idx, topk_w, dtopk_w, shares, N, k,
-                     drouter_w, drouter_b);
+  hipLaunchKernelGGL(router_param_kernel, dim3((5 * E + 31) / 32), dim3(1024), 0, stream, part, N > 0 ? route_planes(N) : 0, E, drouter_w,
+                     drouter_b);
   return check_launch("ygg_route_energy_backward (parameters)");
 }
