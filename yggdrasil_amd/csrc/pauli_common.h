@@ -81,27 +81,27 @@ __device__ inline void activate_blade(float* y) {
 }
 
 // The activation's gradient at the input h, from the gradient g of its output, into g (blade order).
-// s (1 - s) of a sigmoid s is e r^2 with e = 2^-|z log2 e|, r = 1 / (1 + e): no cancellation at either end.
-__device__ inline float sigmoid_slope(float z2) {  // z2 = z log2(e)
-  const float e = __builtin_amdgcn_exp2f(-fabsf(z2)), r = __builtin_amdgcn_rcpf(1.0f + e);
-  return e * r * r;
+// A sigmoid and its slope from one exponential: with e = 2^-|z log2 e| and r = 1 / (1 + e), s' = e r^2 and s is
+// r or e r, so that neither end cancels.
+__device__ inline float sigmoid_and_slope(float z2, float& slope) {  // z2 = z log2(e)
+  const float e = __builtin_amdgcn_exp2f(-fabsf(z2)), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
+  slope = er * r;
+  return z2 >= 0.f ? r : er;
 }
 // grades 1 and 2: out = (f(m) / m) g + (f'(m) - f(m) / m) (c . g) c / m^2, m the length of c
 template <int ACT>
 __device__ inline void gate_grad(const float* c, float* g) {
   constexpr float kL = 1.4426950408889634f, k2 = 2.0f * 0.7978845608028654f;
   const float m2 = __builtin_fmaf(c[2], c[2], __builtin_fmaf(c[1], c[1], __builtin_fmaf(c[0], c[0], 1e-12f)));
-  const float m = __builtin_amdgcn_sqrtf(m2);
+  const float rm = __builtin_amdgcn_rsqf(m2), m = m2 * rm;
   const float dot = __builtin_fmaf(c[2], g[2], __builtin_fmaf(c[1], g[1], c[0] * g[0]));
-  float a, b;
+  float a, b, slope;
   if constexpr (ACT == kActGelu) {  // f(m) / m = s(z), z = k2 (m + 0.044715 m^3): f' - f / m = m s' z'
-    a = gelu_gate(m);
-    b = sigmoid_slope(kL * k2 * m * __builtin_fmaf(0.044715f, m2, 1.0f)) * (k2 * __builtin_fmaf(3.0f * 0.044715f, m2, 1.0f)) *
-        __builtin_amdgcn_rcpf(m);
+    a = sigmoid_and_slope(m * __builtin_fmaf(kL * k2 * 0.044715f, m2, kL * k2), slope);
+    b = slope * __builtin_fmaf(3.0f * 0.044715f * k2, m2, k2) * rm;
   } else {  // f = s
-    const float rm = __builtin_amdgcn_rcpf(m);
-    a = fsigmoid(m) * rm;
-    b = (sigmoid_slope(kL * m) - a) * (rm * rm);
+    a = sigmoid_and_slope(kL * m, slope) * rm;
+    b = (slope - a) * (rm * rm);
   }
   b *= dot;
 #pragma unroll
@@ -114,15 +114,19 @@ __device__ inline void activate_grad_blade(const float* h, float* g) {
     g[7] = h[7] != 0.f ? g[7] : 0.f;
   } else if constexpr (ACT == kActGelu || ACT == kActSigmoid) {
     constexpr float kL = 1.4426950408889634f, k2 = 2.0f * 0.7978845608028654f;
-    const float v = h[0];
-    if constexpr (ACT == kActGelu)  // (v s(z))' = s + v s' z'
-      g[0] *= __builtin_fmaf(v * (k2 * __builtin_fmaf(3.0f * 0.044715f, v * v, 1.0f)),
-                             sigmoid_slope(kL * k2 * v * __builtin_fmaf(0.044715f, v * v, 1.0f)), gelu_gate(v));
-    else
-      g[0] *= sigmoid_slope(kL * v);
+    const float v = h[0], v2 = v * v;
+    float slope;
+    if constexpr (ACT == kActGelu) {  // (v s(z))' = s + v s' z'
+      const float s = sigmoid_and_slope(v * __builtin_fmaf(kL * k2 * 0.044715f, v2, kL * k2), slope);
+      g[0] *= __builtin_fmaf(v * __builtin_fmaf(3.0f * 0.044715f * k2, v2, k2), slope, s);
+    } else {
+      sigmoid_and_slope(kL * v, slope);
+      g[0] *= slope;
+    }
     gate_grad<ACT>(h + 1, g + 1);
     gate_grad<ACT>(h + 4, g + 4);
-    g[7] *= 4.0f * sigmoid_slope(2.0f * kL * h[7]);  // 1 - tanh^2
+    sigmoid_and_slope(2.0f * kL * h[7], slope);
+    g[7] *= 4.0f * slope;  // 1 - tanh^2
   }
 }
 

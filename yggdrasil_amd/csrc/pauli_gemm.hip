@@ -833,23 +833,46 @@ __global__ __launch_bounds__(256) void pauli_prep_weights_kernel(const float* __
 }
 
 // The same layout of the adjoint weights (E, d_in, d_out): Wadj_ij = ~W_ji, whose product is the
-// gradient of W's input.  One thread per multivector of the layout.
-__global__ __launch_bounds__(256) void pauli_prep_adjoint_kernel(const float* __restrict__ W, int E, int d_out, int d_in,
+// gradient of W's input.  A workgroup transposes 32 (j) x 32 (i) of an expert through LDS, so that
+// it reads runs of 32 multivectors and writes runs of 16 records (a thread per multivector of the
+// layout, which read single ones, took 200 us for 64 x 1024 x 256 and this PREPTEXT).
+constexpr int kPrepT = 32;
+__global__ __launch_bounds__(256) void pauli_prep_adjoint_kernel(const float* __restrict__ W, int d_out, int d_in,
                                                                  uint16_t* __restrict__ out) {
-  const size_t n = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= (size_t)E * d_in * d_out) return;
-  const int j = (int)(n % d_out);
-  const size_t ei = n / d_out;  // e * d_in + i
-  const int i = (int)(ei % d_in);
-  const float* w = W + (((ei / d_in) * d_out + j) * d_in + i) * 8;
-  float x[8];
+  // [i][pair of j][a][j of the pair], 8 bytes each; a row of i is 8 bytes longer, against bank conflicts
+  __shared__ uint2 tile[kPrepT][kPrepT * 2 + 1];
+  const size_t e = blockIdx.z;
+  const int j0 = blockIdx.y * kPrepT, i0 = blockIdx.x * kPrepT;
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  float4 v[4][2];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) x[c] = (c >= 4 ? -0.5f : 0.5f) * w[c];  // the reverse: grades 2 and 3 change sign
-  float c0[4], c1[4];
-  blade_to_pauli(x, c0, c1);
-  uint16_t* rec = out + ((ei * (d_out >> 1) + (j >> 1)) * 2) * 8;
-  *reinterpret_cast<uint2*>(rec + (j & 1) * 4) = make_uint2(pack2_bf16(c0[0], -c0[1]), pack2_bf16(c1[0], -c1[1]));
-  *reinterpret_cast<uint2*>(rec + 8 + (j & 1) * 4) = make_uint2(pack2_bf16(c0[2], -c0[3]), pack2_bf16(c1[2], -c1[3]));
+  for (int u = 0; u < 4; ++u) {
+    const int j = min(j0 + r + 8 * u, d_out - 1), i = min(i0 + c, d_in - 1);
+    const float* w = W + ((e * d_out + j) * d_in + i) * 8;
+    __builtin_memcpy(&v[u][0], w, 16);  // (any aligned floats)
+    __builtin_memcpy(&v[u][1], w + 4, 16);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float4 p = v[u][0], q = v[u][1];
+    // half the reverse: grades 2 and 3 change sign
+    const float x[8] = {0.5f * p.x, 0.5f * p.y, 0.5f * p.z, 0.5f * p.w, -0.5f * q.x, -0.5f * q.y, -0.5f * q.z, -0.5f * q.w};
+    float c0[4], c1[4];
+    blade_to_pauli(x, c0, c1);
+    const int j = r + 8 * u;
+    uint2* rec = &tile[c][(j >> 1) * 4 + (j & 1)];
+    rec[0] = make_uint2(pack2_bf16(c0[0], -c0[1]), pack2_bf16(c1[0], -c1[1]));
+    rec[2] = make_uint2(pack2_bf16(c0[2], -c0[3]), pack2_bf16(c1[2], -c1[3]));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {  // 16 bytes a thread: half c of row r + 8 u
+    const int i = i0 + r + 8 * u, j = j0 + (c >> 1) * 2;
+    if (i >= d_in || j >= d_out) continue;
+    const uint2 lo = tile[r + 8 * u][2 * c], hi = tile[r + 8 * u][2 * c + 1];
+    *reinterpret_cast<uint4*>(out + (((e * d_in + i) * (d_out >> 1) + (j >> 1)) * 2 + (c & 1)) * 8) =
+        make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
 }
 
 // blade rows (bf16) -> Pauli half-rows (bf16); one thread per multivector
@@ -988,9 +1011,10 @@ YGG_API int ygg_prepare_adjoint_weights_bf16(const float* W, int E, int d_out, i
   const size_t n = (size_t)E * d_in * d_out;
   if (n == 0) return 0;
   YGG_CHECK_ARG(W && out, "ygg_prepare_adjoint_weights_bf16: null pointer");
-  YGG_CHECK_ARG(n <= (size_t)0x7fffffff * 256, "ygg_prepare_adjoint_weights_bf16: %zu multivectors exceed the grid", n);
-  pauli_prep_adjoint_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(W, E, d_out, d_in,
-                                                                              static_cast<uint16_t*>(out));
+  YGG_CHECK_ARG(E <= 65535 && (d_out + kPrepT - 1) / kPrepT <= 65535,
+                "ygg_prepare_adjoint_weights_bf16: E=%d d_out=%d exceed a launch", E, d_out);
+  pauli_prep_adjoint_kernel<<<dim3((d_in + kPrepT - 1) / kPrepT, (d_out + kPrepT - 1) / kPrepT, E), 256, 0, stream>>>(
+      W, d_out, d_in, static_cast<uint16_t*>(out));
   return check_launch("pauli_prep_adjoint");
 }
 

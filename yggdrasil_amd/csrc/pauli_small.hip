@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64) void pauli_small_kernel(
         const uint32_t off = OUT == kOutPauliRows ? ((uint32_t)rl * 2 * d_out + j) * 8 : ((uint32_t)rl * d_out + j) * 16;
         pauli_store_mv<ACT, OUT, kBF16, BIAS_FIRST>(s[0][0][2 * h], s[0][1][2 * h], s[0][0][2 * h + 1], s[0][1][2 * h + 1],
                                                     s[1][0][2 * h], s[1][1][2 * h], s[1][0][2 * h + 1], s[1][1][2 * h + 1],
-                                                    bvs[cb], y_rsrc, off, 0, d_out, y_rsrc, 0, 0);
+                                                    bvs[cb], y_rsrc, off, 0, d_out, y_rsrc, 0, 0, uint4{});
       }
   }
 }

@@ -27,12 +27,13 @@ struct PauliTileInfo {
 
 // One output multivector from its eight sums (a0b0, a0b1, a1b0, a1b1 as re, im pairs): the inverse
 // Pauli map, the bias unless the sums started from it, the activation and the output layout,
-// stored at v_off + s_off of y_rsrc; its blade row in aux, if there is one, at av_off + as_off.
+// stored at v_off + s_off of y_rsrc.  kActSave stores its blade row to aux at av_off + as_off; kActGrad takes the
+// blade row before the activation as h_pre.
 template <int ACT, int OUT, int OUT_DT, bool BIAS_IN_ACC>
 __device__ __forceinline__ void pauli_store_mv(float a0b0r, float a0b0i, float a0b1r, float a0b1i, float a1b0r, float a1b0i,
                                                float a1b1r, float a1b1i, const float* bv, __amdgpu_buffer_rsrc_t y_rsrc,
                                                uint32_t v_off, uint32_t s_off, int d_out, __amdgpu_buffer_rsrc_t aux,
-                                               uint32_t av_off, uint32_t as_off) {
+                                               uint32_t av_off, uint32_t as_off, const uint4& h_pre) {
   typedef unsigned int pu32x2_t __attribute__((ext_vector_type(2)));
   typedef unsigned int pu32x4_t __attribute__((ext_vector_type(4)));
   float y[8];
@@ -42,7 +43,7 @@ __device__ __forceinline__ void pauli_store_mv(float a0b0r, float a0b0i, float a
     for (int c = 0; c < 8; ++c) y[c] += bv[c];
   }
   if constexpr (ACT >= kActGrad && ACT < kActSave) {
-    const uint4 q = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(aux, av_off, as_off, 0));
+    const uint4 q = h_pre;
     const float h[8] = {bf_lo(q.x), bf_hi(q.x), bf_lo(q.y), bf_hi(q.y), bf_lo(q.z), bf_hi(q.z), bf_lo(q.w), bf_hi(q.w)};
     activate_grad_blade<ACT & 3>(h, y);
   } else {
@@ -98,10 +99,25 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
     const uint32_t v_off = OUT == kOutPauliRows ? (uint32_t)((4 * g) * d_out + j) * 8
                                                 : (uint32_t)((2 * g) * d_out + j) * MV_BYTES;
     const uint32_t av_off = (uint32_t)((2 * g) * d_out + j) * 16;
+    // kActGrad: the eight rows before the activation of a row block, asked for together.  Rows past the tile's
+    // last repeat it.
+    uint4 hq[8] = {};
+    auto load_h = [&](int rb) __attribute__((always_inline)) {
+      if constexpr (ACT >= kActGrad && ACT < kActSave) {
+        const int rbr = ti.half >= 0 ? ti.half : rb;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int r = ti.row0 + (ti.compact ? wt * 16 : (wt * WR + rbr) * 16) + 4 * (n >> 1) + (n & 1) + 2 * g;
+          const uint32_t off = (uint32_t)((min(r, ti.row_end - 1) - row_base) * d_out + j) * 16;
+          hq[n] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(aux, off, 0, 0));
+        }
+      }
+    };
 #pragma unroll
     for (int rb = 0; rb < WR; ++rb) {
       if (ti.half >= 0 && rb > 0) break;  // a half tile: the first accumulators hold block `half`
       const int rbr = ti.half >= 0 ? ti.half : rb;
+      load_h(rb);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -113,7 +129,8 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
           pauli_store_mv<ACT, OUT, OUT_DT, BIAS_IN_ACC>(
               acc[rb][cb][0][0][v0], acc[rb][cb][0][1][v0], acc[rb][cb][0][0][v0 + 1], acc[rb][cb][0][1][v0 + 1],
               acc[rb][cb][1][0][v0], acc[rb][cb][1][1][v0], acc[rb][cb][1][0][v0 + 1], acc[rb][cb][1][1][v0 + 1], bv, y_rsrc,
-              v_off, s_off, d_out, aux, av_off, (uint32_t)(rs - row_base) * d_out * 16);
+              v_off, s_off, d_out, aux, av_off, (uint32_t)(rs - row_base) * d_out * 16,
+              hq[2 * q + h]);
         }
     }
   }
