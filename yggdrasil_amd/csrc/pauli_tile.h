@@ -122,15 +122,19 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
       for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int rs = ti.row0 + (ti.compact ? wt * 16 : (wt * WR + rbr) * 16) + 4 * q + h;  // row of lanes with g = 0
-          if (rs + 2 * g >= ti.row_end) continue;
+          const int rs0 = ti.row0 + (ti.compact ? wt * 16 : (wt * WR + rbr) * 16) + 4 * q + h;  // row of lanes with g = 0
+          // kActGrad: no branch, so that the long chains of several multivectors run side by side; a row past the
+          // tile's last has an offset past the output, where a store does nothing
+          constexpr bool NO_BRANCH = ACT >= kActGrad && ACT < kActSave;
+          if (!NO_BRANCH && rs0 + 2 * g >= ti.row_end) continue;
+          const int rs = NO_BRANCH ? min(rs0, ti.row_end - 1) : rs0;
+          const uint32_t v_at = NO_BRANCH && rs0 + 2 * g >= ti.row_end ? kBufferOff : v_off;
           const uint32_t s_off = (uint32_t)(rs - row_base) * d_out * MV_BYTES;
           const int v0 = 4 * q + 2 * h;  // b = 0 at v0, b = 1 at v0 + 1
           pauli_store_mv<ACT, OUT, OUT_DT, BIAS_IN_ACC>(
               acc[rb][cb][0][0][v0], acc[rb][cb][0][1][v0], acc[rb][cb][0][0][v0 + 1], acc[rb][cb][0][1][v0 + 1],
               acc[rb][cb][1][0][v0], acc[rb][cb][1][1][v0], acc[rb][cb][1][0][v0 + 1], acc[rb][cb][1][1][v0 + 1], bv, y_rsrc,
-              v_off, s_off, d_out, aux, av_off, (uint32_t)(rs - row_base) * d_out * 16,
-              hq[2 * q + h]);
+              v_at, s_off, d_out, aux, av_off, (uint32_t)(rs - row_base) * d_out * 16, hq[2 * q + h]);
         }
     }
   }
