@@ -368,6 +368,29 @@ int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void* a_pauli
                                        const int32_t* offsets, int P_max, int E, int d_in, int d_out, float* dW,
                                        float* db, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
 
+/* A training step of the bf16 layer with bf16 Pauli weights (format 3; even d and F).  The
+ * forward is ygg_moe_forward's, output and routing arrays bit for bit; it writes into `saved`
+ * (ygg_moe_train_bf16_saved_bytes, its layout the library's own) the rows that the backward
+ * reads: x's Pauli rows, the hidden rows before and after the activation, the experts' outputs
+ * and the rows' tokens and places.  The backward takes those with the forward's topk_w and
+ * offsets, the adjoint weights (ygg_prepare_adjoint_weights_bf16 of W_up and W_down) and dout
+ * (N, d, 8) bf16, and writes dx (N, d, 8) bf16 (with dout added when `residual`, i.e. when the
+ * forward added x to its output), dw_up (E, F, d, 8), db_up (E, F, 8), dw_down (E, d, F, 8),
+ * db_down (E, d, 8) fp32, and dtopk_w (N, k) when not NULL.  Rows between two operators are
+ * bf16, sums inside one fp32.  `saved` is only read by the backward. */
+size_t ygg_moe_train_bf16_saved_bytes(int N, int d, int F, int E, int k);
+size_t ygg_moe_forward_train_bf16_workspace_bytes(int N, int d, int F, int E, int k);
+int ygg_moe_forward_train_bf16(const void* x, int N, int d, int F, int E, int k, int act, const float* logits,
+                               const float* router_w, const float* router_b, const void* w_up, const float* b_up,
+                               const void* w_down, const float* b_down, const void* residual, void* out,
+                               int32_t* topk_idx, float* topk_w, int32_t* counts, int32_t* offsets, void* saved,
+                               size_t saved_bytes, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
+size_t ygg_moe_backward_bf16_workspace_bytes(int N, int d, int F, int E, int k);
+int ygg_moe_backward_bf16(int N, int d, int F, int E, int k, int act, const void* w_up_adj, const void* w_down_adj,
+                          int residual, const void* dout, const void* saved, size_t saved_bytes, const float* topk_w,
+                          const int32_t* offsets, void* dx, float* dw_up, float* db_up, float* dw_down, float* db_down,
+                          float* dtopk_w, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
+
 /* ---- backward of the router ----------------------------------------------------------
  * The reference's router has no backward (hlm_block.py:202-206); these follow
  * CliffordRouter.forward (clifford_router.py:54-104).  The choice of the experts is a

@@ -94,6 +94,44 @@ def test_route_energy_backward(args, word):
     _refused("ygg_route_energy_backward", args, word)
 
 
+_FWD = [P, 4, 8, 8, 4, 2, 1, P, None, None, P, None, P, None, None, P, P, P, P, P, P, 1 << 30, P, 1 << 30, None]
+
+
+@pytest.mark.parametrize("at,value,word", [
+    (1, -1, "bad sizes"), (2, 7, "bad sizes"), (3, 7, "bad sizes"), (4, 65, "bad sizes"), (5, 5, "bad sizes"),
+    (5, 9, "bad sizes"), (6, 4, "activation"), (0, None, "null"), (7, None, "need logits"), (10, None, "null"),
+    (18, None, "null"), (20, None, "null"), (21, 64, "keep rows"), (23, 8, "workspace"), (1, 1 << 30, "2^31")])
+def test_forward_train_bf16(at, value, word):
+    args = list(_FWD)
+    args[at] = value
+    _refused("ygg_moe_forward_train_bf16", args, word)
+
+
+_BWD = [4, 8, 8, 4, 2, 1, P, P, 0, P, P, 1 << 30, P, P, P, P, P, P, P, None, P, 1 << 30, None]
+
+
+@pytest.mark.parametrize("at,value,word", [
+    (0, -1, "bad sizes"), (1, 7, "bad sizes"), (2, 0, "bad sizes"), (3, 0, "bad sizes"), (4, 5, "bad sizes"),
+    (5, -1, "activation"), (6, None, "null"), (9, None, "null"), (10, None, "null"), (11, 64, "kept rows"),
+    (14, None, "null"), (16, None, "null"), (21, 8, "workspace")])
+def test_backward_bf16(at, value, word):
+    args = list(_BWD)
+    args[at] = value
+    _refused("ygg_moe_backward_bf16", args, word)
+
+
+def test_config():
+    import yggdrasil_amd as y
+
+    for kw in (dict(bf16_grad=True), dict(dtype=torch.bfloat16, weight_format="int8", bf16_grad=True),
+               dict(dtype=torch.bfloat16, router_grad=True), dict(router="clifford_head", router_grad=True)):
+        with pytest.raises(ValueError):
+            y.MoEHLMConfig(d_model=8, d_ff=16, **kw)
+    with pytest.raises(ValueError, match="grad"):
+        y.CliffordMoEBlockFFN(y.MoEHLMConfig(d_model=8, d_ff=16, dtype=torch.bfloat16), grad=True)
+    assert not y.MoEHLMConfig(d_model=8, d_ff=16).router_grad
+
+
 def test_no_cpu_path():
     x, w = torch.zeros(3, 4, 8), torch.zeros(3, 2)
     i, h = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2, 4, 4, dtype=torch.bfloat16)

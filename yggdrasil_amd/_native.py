@@ -76,6 +76,13 @@ SIGNATURES = {
     "ygg_grouped_weight_grad_pauli_bf16_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
     "ygg_grouped_weight_grad_pauli_bf16": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
                                                     _vp, _c_size, _vp]),
+    "ygg_moe_train_bf16_saved_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ygg_moe_forward_train_bf16_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ygg_moe_forward_train_bf16": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp,
+                                            _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp, _c_size, _vp]),
+    "ygg_moe_backward_bf16_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ygg_moe_backward_bf16": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_size,
+                                       _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
     "ygg_route_backward": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "ygg_route_energy_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "ygg_route_energy_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp,

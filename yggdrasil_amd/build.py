@@ -19,7 +19,8 @@ CSRC = os.path.join(PKG, "csrc")
 OUT_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(OUT_DIR, "libygg_moe.so")
 SOURCES = ["capi.hip", "route.hip", "dispatch.hip", "clifford_gemm.hip", "decode.hip", "decode_pauli.hip", "pauli_gemm.hip", "pauli_f32.hip", "pauli_split.hip", "pauli_small.hip",
-           "norm.hip", "quantize.hip", "backward.hip", "norm_backward.hip", "route_backward.hip", "weight_grad_bf16.hip"]
+           "norm.hip", "quantize.hip", "backward.hip", "norm_backward.hip", "route_backward.hip", "weight_grad_bf16.hip",
+           "train_bf16.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1029,6 +1029,23 @@ YGG_API int ygg_pauli_rows_from_blade(const void* x, int rows, int d, void* out,
   return check_launch("blade_to_pauli_rows");
 }
 
+// The up product of a training step: Pauli half-rows of h, and in h_pre the bf16 blade rows before the activation.
+int ygg::pauli_linear_save_pre(const void* x, int x_rows, const int32_t* gather, int P, const void* w, const float* bias,
+                               const int32_t* offsets, int E, int d_in, int d_out, int act, void* h, void* h_pre,
+                               hipStream_t stream) {
+  auto run = [&](auto act_tag) {
+    return launch_pauli<decltype(act_tag)::value, kInPauliRows, kOutPauliRows, kBF16>(
+        stream, static_cast<const uint16_t*>(x), (uint64_t)x_rows * d_in * 16, gather, static_cast<const uint16_t*>(w),
+        bias, offsets, E, P, d_in, d_out, h, h_pre);
+  };
+  switch (act) {
+    case kActNone: return run(std::integral_constant<int, kActNone>{});
+    case kActGelu: return run(std::integral_constant<int, kActSave + kActGelu>{});
+    case kActRelu: return run(std::integral_constant<int, kActSave + kActRelu>{});
+    default: return run(std::integral_constant<int, kActSave + kActSigmoid>{});
+  }
+}
+
 // The gradient of the input rows: the product with the adjoint weights (contraction d_out, d_in
 // columns), times the activation's slope at h_pre inside its epilogue.
 YGG_API int ygg_pauli_grouped_input_grad(const void* dy, int P_max, const void* w_adj, const int32_t* offsets, int E,

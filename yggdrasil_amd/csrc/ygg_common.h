@@ -283,6 +283,17 @@ int combine_backward(const float* dout, const float* y_sorted, int N, int k, int
 int dispatch_backward(const float* dxs, int N, int k, int d, const int32_t* slot_pos, const float* residual_grad,
                       float* dx, hipStream_t stream);
 
+// The bf16 layer's training pieces.  pauli_gemm.hip: the up product (Pauli half-rows gathered, h as
+// Pauli half-rows) that also keeps its blade rows before the activation (act 0: h alone).
+// weight_grad_bf16.hip: ygg_grouped_weight_grad_pauli_bf16 without its checks.  train_bf16.hip: the
+// combine's backward (dy as Pauli half-rows; dtopk_w when not NULL) and the dispatch's, on bf16 rows.
+int pauli_linear_save_pre(const void* x, int x_rows, const int32_t* gather, int P, const void* w, const float* bias,
+                          const int32_t* offsets, int E, int d_in, int d_out, int act, void* h, void* h_pre,
+                          hipStream_t stream);
+size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out);
+int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
+                     int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream);
+
 inline int dtype_size(int dt) { return dt == kF32 ? 4 : dt == kBF16 ? 2 : dt == kI8 ? 1 : 0; }
 
 }  // namespace ygg

@@ -21,6 +21,7 @@ from dataclasses import dataclass
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -48,6 +49,11 @@ class MoEHLMConfig:
     router      'energy' -- CliffordRouter's grade-energy logits (default, the reference);
                 'clifford_head' -- CliffordLinear(d -> E) then the scalar part;
                 'logits' -- the caller passes logits to forward()
+    bf16_grad   bf16 'pauli' layers: their outputs carry a graph, and gradients reach x, the residual and the experts'
+                weights and biases, as those of fp32 'pauli_f32' layers always do
+    router_grad gradients also reach the router -- its weight, its bias and, through the grade energies, x
+                (router 'energy'), or the caller's logits.  The reference's router has no backward
+                (hlm_block.py:202-206); without this the routing is a constant of the backward
     """
 
     d_model: int
@@ -58,6 +64,8 @@ class MoEHLMConfig:
     dtype: torch.dtype = torch.float32
     weight_format: str | None = None
     router: str = "energy"
+    bf16_grad: bool = False
+    router_grad: bool = False
 
     def __post_init__(self):
         if self.activation not in ACTIVATIONS:
@@ -78,6 +86,12 @@ class MoEHLMConfig:
             raise ValueError("the 'int8_pauli' weight format serves d_model <= 128")
         if self.weight_format == "pauli" and not even:
             raise ValueError("the 'pauli' weight format needs even d_model and d_ff")
+        if self.bf16_grad and self.weight_format != "pauli":
+            raise ValueError("bf16_grad is for bf16 layers with 'pauli' weights")
+        if self.router_grad and self.router == "clifford_head":
+            raise ValueError("router_grad serves the routers 'energy' and 'logits'")
+        if self.router_grad and not (self.weight_format == "pauli_f32" or self.bf16_grad):
+            raise ValueError("router_grad needs a layer with gradients: 'pauli_f32' weights, or bf16_grad")
         if not 1 <= self.n_experts <= 64 or not 1 <= self.top_k <= min(8, self.n_experts):
             raise ValueError("need 1 <= n_experts <= 64 and 1 <= top_k <= min(8, n_experts)")
 
@@ -162,6 +176,10 @@ class CliffordMoELayer(nn.Module):
     @torch.no_grad()
     def prepare(self):
         """Build the device weight layouts (done lazily; redone when parameters change)."""
+        self._prepared = self._layouts()
+        return self._prepared
+
+    def _layouts(self) -> dict:
         fmt = self.cfg.weight_format
         head = None
         if self.head_weight is not None:
@@ -175,8 +193,7 @@ class CliffordMoELayer(nn.Module):
                                 ("b_down", b_down.shape, (E, d, 8))):
             if got != want:
                 raise ValueError(f"{name} must be of shape {want}, got {tuple(got)}")
-        self._prepared = dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head)
-        return self._prepared
+        return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head)
 
     def _get_prepared(self):
         if self._prepared is None or self._prepared["key"] != self._param_versions():
@@ -218,11 +235,12 @@ class CliffordMoELayer(nn.Module):
         ws = self.__dict__["_workspace"]
         if ws is None or ws.numel() < ws_bytes or ws.device != x.device:
             ws = self.__dict__["_workspace"] = torch.empty((max(ws_bytes, 1),), device=x.device, dtype=torch.uint8)
-        if self._needs_grad(x, residual):
+        if self._needs_grad(x, residual, logits):
             flat = x.reshape(N, d, 8)
             res = residual.reshape(N, d, 8) if residual is not None else None
             lg = logits.reshape(N, E) if logits is not None else None
-            return _MoEFunction.apply(flat, res, self.w_up, self.b_up, self.w_down, self.b_down, self, lg).reshape(B, T, d, 8)
+            return _MoEFunction.apply(flat, res, self.w_up, self.b_up, self.w_down, self.b_down, self.router_weight,
+                                      self.router_bias, self, lg).reshape(B, T, d, 8)
         rw = rb = None
         if logits is None:
             rw, rb = self.router_weight.detach(), self.router_bias.detach()
@@ -240,22 +258,27 @@ class CliffordMoELayer(nn.Module):
         self.__dict__["_last_routing"] = routing
         return out
 
-    def _needs_grad(self, x, residual) -> bool:
-        """Autograd runs for fp32 layers with 'pauli_f32' weights (the backward's format);
-        other formats compute the forward only and their output carries no graph."""
-        if self.cfg.weight_format != "pauli_f32" or not torch.is_grad_enabled():
+    def _needs_grad(self, x, residual, logits=None) -> bool:
+        """Autograd runs for fp32 layers with 'pauli_f32' weights, and for bf16 layers with 'pauli' ones that ask for
+        it (``bf16_grad``); other formats compute the forward only and their output carries no graph."""
+        if not (self.cfg.weight_format == "pauli_f32" or self.cfg.bf16_grad) or not torch.is_grad_enabled():
             return False
+        more = ((self.router_weight, self.router_bias) if logits is None else (logits,)) if self.cfg.router_grad else ()
         return x.requires_grad or (residual is not None and residual.requires_grad) or any(
-            p.requires_grad for p in (self.w_up, self.b_up, self.w_down, self.b_down))
+            p.requires_grad for p in (self.w_up, self.b_up, self.w_down, self.b_down, *more))
 
     @torch.no_grad()
     def _get_adjoint(self):
-        """Adjoint expert weights (reverse, channel axes exchanged) in the 'pauli_f32' layout."""
+        """Adjoint expert weights (reverse, channel axes exchanged) in the layout of the layer's products."""
         key = self._param_versions()
         if getattr(self, "_adjoint", None) is None or self._adjoint["key"] != key:
-            self._adjoint = dict(key=key, w_up=ops.prepare_adjoint_weights(self.w_up.detach().contiguous()),
-                                 w_down=ops.prepare_adjoint_weights(self.w_down.detach().contiguous()))
+            self._adjoint = dict(key=key, **self._adjoint_layouts())
         return self._adjoint
+
+    def _adjoint_layouts(self) -> dict:
+        fmt = self.cfg.weight_format
+        return dict(w_up=ops.prepare_adjoint_weights(self.w_up.detach().contiguous(), fmt),
+                    w_down=ops.prepare_adjoint_weights(self.w_down.detach().contiguous(), fmt))
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor | None = None):
         """geoformer interface: (B, T, 8 d) or (B, T, d, 8) -> (same shape, aux_loss)."""
@@ -296,41 +319,85 @@ class CliffordMoELayer(nn.Module):
         return ((f - 1.0 / self.cfg.n_experts) ** 2).sum()
 
 
-class _MoEFunction(torch.autograd.Function):
-    """The layer as one autograd node: forward ``ygg_moe_forward``, backward ``ygg_moe_backward``.
+def _in_capture(layer, block: bool) -> bool:
+    """Whether a training step lays the weights out anew in a graph that is being captured, where its replays find
+    them updated by an optimizer step of the same graph.  (The fp32 layer alone replays the layouts of the capture.)"""
+    return (block or layer.cfg.bf16_grad) and torch.cuda.is_current_stream_capturing()
 
-    Gradients reach x, the residual and the expert weights and biases.  The
-    routing is a constant of the backward, as in the reference, whose router
-    has no backward (``hlm_block.py:202-206``).
+
+def _train_forward(layer, flat, res, logits, workspace=None, block=False):
+    """The layer's forward for a training step: ``(out, kept)``, what the backward reads in ``kept``."""
+    cfg, prep = layer.cfg, layer._layouts() if _in_capture(layer, block) else layer._get_prepared()
+    rw = layer.router_weight.detach() if logits is None else None
+    rb = layer.router_bias.detach() if logits is None else None
+    if cfg.weight_format == "pauli_f32":
+        out, routing, rows = ops.moe_forward_train(flat, cfg.top_k, prep["w_up"], prep["w_down"], prep["b_up"],
+                                                   prep["b_down"], cfg.activation, logits=logits, router_weight=rw,
+                                                   router_bias=rb, residual=res, workspace=workspace)
+    else:
+        out, routing, rows = ops.moe_forward_train_bf16(flat, cfg.top_k, prep["w_up"], prep["w_down"], prep["b_up"],
+                                                        prep["b_down"], cfg.activation, logits=logits, router_weight=rw,
+                                                        router_bias=rb, residual=res)
+    layer.last_routing = routing
+    return out, (rows, routing["topk_idx"], routing["topk_w"], routing["offsets"])
+
+
+def _check_versions(layer, versions) -> None:
+    """The backward lays the weights out anew: they have to be those of the forward (None: not looked at)."""
+    if versions is not None and versions != layer._param_versions():
+        raise RuntimeError("the layer's parameters were modified in place between its forward and its backward")
+
+
+def _train_backward(layer, flat, logits, kept, dout, residual: bool, block=False):
+    """Gradients of :func:`_train_forward`: ``(dx, dW_up, db_up, dW_down, db_down, drouter_weight, drouter_bias,
+    dlogits)``, the last three None where the router gets none.  ``residual``: dx includes dout (bf16 layers)."""
+    rows, idx, w, offsets = kept
+    cfg = layer.cfg
+    capture = _in_capture(layer, block)
+    adj = layer._adjoint_layouts() if capture else layer._get_adjoint()
+    dout = dout.contiguous()
+    if cfg.weight_format == "pauli_f32":
+        prep = layer._layouts() if capture else layer._get_prepared()
+        dx, *grads, dtw = ops.moe_backward(
+            flat, cfg.top_k, prep["w_up"], adj["w_up"], prep["w_down"], adj["w_down"], dout, prep["b_up"], prep["b_down"],
+            cfg.activation, logits=logits, router_weight=None if logits is not None else layer.router_weight.detach(),
+            router_bias=None if logits is not None else layer.router_bias.detach(), routing_grad=cfg.router_grad,
+            h_pre=rows, residual=residual)
+    else:
+        dx, *grads, dtw = ops.moe_backward_bf16(dout, rows, dict(topk_w=w, offsets=offsets), adj["w_up"], adj["w_down"],
+                                                cfg.activation, residual=residual, routing_grad=cfg.router_grad)
+    drw = drb = dlogits = None
+    if cfg.router_grad and logits is not None:
+        dlogits = ops.route_backward(idx, w, dtw, cfg.n_experts)
+    elif cfg.router_grad:
+        dx, drw, drb = ops.route_energy_backward(flat, layer.router_weight.detach(), idx, w, dtw, dx_add=dx)
+    return (dx, *grads, drw, drb, dlogits)
+
+
+class _MoEFunction(torch.autograd.Function):
+    """The layer as one autograd node: forward ``ygg_moe_forward``, backward ``ygg_moe_backward`` (bf16 layers:
+    ``ygg_moe_forward_train_bf16`` and ``ygg_moe_backward_bf16``).
+
+    Gradients reach x, the residual and the expert weights and biases; the router's parameters or the
+    logits too when the layer asks for it (``router_grad``).  Otherwise the routing is a constant of the
+    backward, as in the reference, whose router has no backward (``hlm_block.py:202-206``).
     """
 
     @staticmethod
-    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, layer, logits):
-        ctx.layer, ctx.has_res = layer, res is not None
-        cfg, prep = layer.cfg, layer._get_prepared()
-        out, routing, h_pre = ops.moe_forward_train(
-            flat, cfg.top_k, prep["w_up"], prep["w_down"], prep["b_up"], prep["b_down"], cfg.activation,
-            logits=logits, router_weight=layer.router_weight.detach() if logits is None else None,
-            router_bias=layer.router_bias.detach() if logits is None else None, residual=res,
-            workspace=layer._workspace)
-        layer.last_routing = routing
-        ctx.save_for_backward(flat, logits if logits is not None else flat.new_empty(0), h_pre)
-        ctx.has_logits = logits is not None
+    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, logits):
+        ctx.layer, ctx.has_res, ctx.has_logits = layer, res is not None, logits is not None
+        out, kept = _train_forward(layer, flat, res, logits, workspace=layer._workspace)
+        ctx.versions = layer._param_versions() if layer.cfg.bf16_grad else None
+        ctx.save_for_backward(flat, logits if logits is not None else flat.new_empty(0), *kept)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        flat, logits, h_pre = ctx.saved_tensors
-        layer = ctx.layer
-        cfg = layer.cfg
-        prep, adj = layer._get_prepared(), layer._get_adjoint()
-        use_logits = ctx.has_logits
-        dx, dWu, dbu, dWd, dbd, _ = ops.moe_backward(
-            flat, cfg.top_k, prep["w_up"], adj["w_up"], prep["w_down"], adj["w_down"], dout.contiguous(),
-            prep["b_up"], prep["b_down"], cfg.activation, logits=logits if use_logits else None,
-            router_weight=None if use_logits else layer.router_weight.detach(),
-            router_bias=None if use_logits else layer.router_bias.detach(), routing_grad=False, h_pre=h_pre)
-        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, None, None
+        flat, logits, *kept = ctx.saved_tensors
+        _check_versions(ctx.layer, ctx.versions)
+        dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
+            ctx.layer, flat, logits if ctx.has_logits else None, kept, dout, residual=False)
+        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, dlogits
 
 
 class CliffordLinear(nn.Module):
@@ -364,12 +431,13 @@ class CliffordLayerNorm(nn.Module):
     """CliffordLayerNorm (``normalization.py:19-67``): y = gamma x_hat + beta (geometric product).
 
     gamma starts as the scalar 1 and beta at zero, as in the reference
-    (``normalization.py:33-41``).  x: (..., d, 8), fp32 or bf16.
+    (``normalization.py:33-41``).  x: (..., d, 8), fp32 or bf16.  With ``grad`` the output
+    carries a graph: gradients reach x, gamma and beta.
     """
 
-    def __init__(self, d_model: int, eps: float = 1e-6, device=None):
+    def __init__(self, d_model: int, eps: float = 1e-6, device=None, grad: bool = False):
         super().__init__()
-        self.d_model, self.eps = d_model, eps
+        self.d_model, self.eps, self.grad = d_model, eps, grad
         gamma = torch.zeros(d_model, 8)
         gamma[:, 0] = 1.0
         self.gamma = nn.Parameter(gamma)
@@ -378,8 +446,30 @@ class CliffordLayerNorm(nn.Module):
             self.to(device)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        # (a norm saved before it could have a graph has no `grad`)
+        if self.__dict__.get("grad", False) and torch.is_grad_enabled() and any(
+                t.requires_grad for t in (x, self.gamma, self.beta)):
+            return _NormFunction.apply(x, self.gamma, self.beta, self.eps, out_dtype)
         return ops.clifford_layer_norm(x.contiguous(), self.gamma.detach(), self.beta.detach(), self.eps,
                                        out_dtype=out_dtype)
+
+
+class _NormFunction(torch.autograd.Function):
+    """CliffordLayerNorm as one autograd node."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps, out_dtype):
+        x = x.contiguous()
+        ctx.save_for_backward(x, gamma)
+        ctx.eps, ctx.beta_dtype = eps, beta.dtype
+        return ops.clifford_layer_norm(x, gamma, beta, eps, out_dtype=out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gamma = ctx.saved_tensors
+        dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dy.contiguous(), x, gamma, ctx.eps)
+        return dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), None, None
 
 
 class CliffordMoEBlockFFN(nn.Module):
@@ -387,14 +477,20 @@ class CliffordMoEBlockFFN(nn.Module):
 
     With the energy router or caller logits the whole sub-layer is one library
     call (``ygg_moe_block_ffn``): the norm, then the MoE layer on the normed
-    tokens with x added back in its combine.  Inference only: its output
-    carries no autograd graph.
+    tokens with x added back in its combine.
+
+    With ``grad`` (fp32 'pauli_f32' layers, and bf16 ones with ``bf16_grad``) the output carries a
+    graph where autograd is on: gradients reach x, the norm's gamma and beta, the experts, and the
+    router when the layer asks for it (``router_grad``).  Without it the block computes the
+    forward only.
     """
 
     def __init__(self, cfg: MoEHLMConfig, device=None, generator: torch.Generator | None = None,
-                 norm_eps: float = 1e-6):
+                 norm_eps: float = 1e-6, grad: bool = False):
         super().__init__()
-        self.cfg = cfg
+        if grad and not (cfg.weight_format == "pauli_f32" or cfg.bf16_grad):
+            raise ValueError("a block with grad needs a layer with gradients: 'pauli_f32' weights, or bf16_grad")
+        self.cfg, self.grad = cfg, grad
         self.ffn_norm = CliffordLayerNorm(cfg.d_model, norm_eps, device=device)
         self.moe = CliffordMoELayer(cfg, device=device, generator=generator)
         self._workspace = None
@@ -427,8 +523,12 @@ class CliffordMoEBlockFFN(nn.Module):
             raise ValueError(f"expected (B, T, {cfg.d_model}, 8), got {tuple(x.shape)}")
         if x.dtype != cfg.dtype:
             raise ValueError(f"layer dtype is {cfg.dtype}, input is {x.dtype}")
+        if self.__dict__.get("grad", False) and torch.is_grad_enabled() and (
+                any(t.requires_grad for t in (x, self.ffn_norm.gamma, self.ffn_norm.beta)) or
+                moe._needs_grad(x, None, logits)):
+            return self._forward_with_graph(x, logits)
         if cfg.router == "clifford_head" and logits is None:
-            with torch.no_grad():  # the block is inference-only (the norm has no backward here)
+            with torch.no_grad():  # no graph: the whole call is the forward alone
                 x_norm = self.ffn_norm(x)
                 return moe.moe_forward(x_norm, logits=moe._head_logits(
                     x_norm.reshape(-1, cfg.d_model, 8), moe._get_prepared()), residual=x)
@@ -451,3 +551,43 @@ class CliffordMoEBlockFFN(nn.Module):
             workspace=self._workspace)
         moe.last_routing = routing
         return out.reshape(B, T, cfg.d_model, 8)
+
+    def _forward_with_graph(self, x: torch.Tensor, logits: torch.Tensor | None) -> torch.Tensor:
+        cfg, moe = self.cfg, self.moe
+        if cfg.router == "logits" and logits is None:
+            raise ValueError("router='logits' needs logits")
+        B, T, d = x.shape[:3]
+        if logits is not None:
+            logits = logits.reshape(B * T, cfg.n_experts).float().contiguous()
+        flat = x.reshape(B * T, d, 8).contiguous()
+        return _BlockFunction.apply(flat, self.ffn_norm.gamma, self.ffn_norm.beta, moe.w_up, moe.b_up, moe.w_down,
+                                    moe.b_down, moe.router_weight, moe.router_bias, self, logits).reshape(B, T, d, 8)
+
+
+class _BlockFunction(torch.autograd.Function):
+    """``x + moe(norm(x))`` as one autograd node: the norm's backward adds the residual's gradient as it writes dx."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, w_up, b_up, w_down, b_down, router_weight, router_bias, block, logits):
+        moe = block.moe
+        xn = ops.clifford_layer_norm(x, gamma, beta, block.ffn_norm.eps)
+        ctx.block, ctx.from_caller, ctx.beta_dtype = block, logits is not None, beta.dtype
+        if logits is None and block.cfg.router == "clifford_head":  # (a constant of the backward)
+            logits = moe._head_logits(xn, moe._get_prepared())
+        ctx.has_logits = logits is not None
+        out, kept = _train_forward(moe, xn, x, logits, block=True)
+        ctx.versions = moe._param_versions()
+        ctx.save_for_backward(x, gamma, xn, logits if logits is not None else x.new_empty(0), *kept)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, gamma, xn, logits, *kept = ctx.saved_tensors
+        _check_versions(ctx.block.moe, ctx.versions)
+        dout = dout.contiguous()
+        dxn, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
+            ctx.block.moe, xn, logits if ctx.has_logits else None, kept, dout, residual=False, block=True)
+        dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.block.ffn_norm.eps, residual_grad=dout)
+        return (dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), dWu, dbu, dWd, dbd, drw, drb, None,
+                dlogits if ctx.from_caller else None)

@@ -995,6 +995,74 @@ def moe_forward_train(x: torch.Tensor, k: int, w_up: PreparedWeights, w_down: Pr
     return out, dict(topk_idx=topk_idx, topk_w=topk_w, counts=counts, offsets=offsets), h_pre
 
 
+def moe_forward_train_bf16(x: torch.Tensor, k: int, w_up: PreparedWeights, w_down: PreparedWeights,
+                           b_up: torch.Tensor | None = None, b_down: torch.Tensor | None = None, act: str = "gelu",
+                           logits: torch.Tensor | None = None, router_weight: torch.Tensor | None = None,
+                           router_bias: torch.Tensor | None = None, residual: torch.Tensor | None = None):
+    """:func:`moe_forward` for a training step of a bf16 layer ('pauli' weights): ``(out, routing, saved)`` with the
+    rows that :func:`moe_backward_bf16` reads in ``saved`` (uint8)."""
+    dev = _dev(x, logits, residual, router_weight, router_bias, b_up, b_down)
+    if w_up.fmt != "pauli" or w_down.fmt != "pauli" or x.dtype != torch.bfloat16:
+        raise ValueError("moe_forward_train_bf16: bf16 layers with 'pauli' weights")
+    if x.dim() != 3 or x.shape[2] != 8:
+        raise ValueError(f"x must be (N, d, 8), got {tuple(x.shape)}")
+    Nt, d = x.shape[0], x.shape[1]
+    E, F = w_up.E, w_up.d_out
+    if w_down.d_in != F or w_down.d_out != d or w_up.d_in != d or w_down.E != E:
+        raise ValueError("expert weight shapes do not chain d -> F -> d")
+    _check_layer_args(x, k, E, F, logits, residual, router_weight, router_bias, b_up, b_down)
+    L = lib()
+    x = x if x.data_ptr() % 16 == 0 else x.clone()
+    out = torch.empty_like(x)
+    saved = torch.empty((max(L.ygg_moe_train_bf16_saved_bytes(Nt, d, F, E, k), 1),), device=dev, dtype=torch.uint8)
+    ws_bytes = L.ygg_moe_forward_train_bf16_workspace_bytes(Nt, d, F, E, k)
+    ws = torch.empty((max(ws_bytes, 1),), device=dev, dtype=torch.uint8)
+    r = LayerRouting(Nt, k, E, dev)
+    idx, w, counts, offsets = r.pointers()
+    rw = router_weight.float().contiguous() if router_weight is not None else None
+    rb = router_bias.float().contiguous() if router_bias is not None else None
+    check(L.ygg_moe_forward_train_bf16(ptr(x), Nt, d, F, E, k, ACT_CODE[act], ptr(logits), ptr(rw), ptr(rb),
+                                       ptr(w_up.data), ptr(b_up), ptr(w_down.data), ptr(b_down), ptr(residual), ptr(out),
+                                       idx, w, counts, offsets, ptr(saved), saved.numel(), ptr(ws), ws_bytes,
+                                       stream_handle(dev)), "moe_forward_train_bf16")
+    return out, r.arrays(), saved
+
+
+def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_up_adj: PreparedWeights,
+                      w_down_adj: PreparedWeights, act: str = "gelu", residual: bool = False, routing_grad: bool = False):
+    """Backward of :func:`moe_forward_train_bf16`: ``(dx, dW_up, db_up, dW_down, db_down, dtopk_w or None)``.
+
+    ``saved`` and ``routing`` as the forward returned them, the adjoint weights from
+    ``prepare_adjoint_weights(w, "pauli")``; dout and dx (N, d, 8) bf16, the weights' gradients fp32."""
+    topk_w, offsets = routing["topk_w"], routing["offsets"]
+    dev = _dev(dout, saved, topk_w, offsets)
+    if w_up_adj.fmt != "pauli" or w_down_adj.fmt != "pauli" or dout.dtype != torch.bfloat16:
+        raise ValueError("moe_backward_bf16: bf16 dout and adjoint weights prepared as 'pauli'")
+    E, d, F = w_up_adj.E, w_up_adj.d_out, w_up_adj.d_in
+    if (w_down_adj.E, w_down_adj.d_out, w_down_adj.d_in) != (E, F, d):
+        raise ValueError("moe_backward_bf16: adjoint weight shapes do not chain F -> d -> F")
+    if dout.dim() != 3 or tuple(dout.shape[1:]) != (d, 8):
+        raise ValueError(f"dout must be (N, {d}, 8), got {tuple(dout.shape)}")
+    Nt, k = dout.shape[0], topk_w.shape[-1]
+    if topk_w.dtype != torch.float32 or tuple(topk_w.shape) != (Nt, k) or saved.dtype != torch.uint8:
+        raise ValueError(f"moe_backward_bf16: the routing and the saved rows are not those of {Nt} tokens")
+    _check_bounds(offsets, E, dev)
+    L = lib()
+    dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
+    ws_bytes = L.ygg_moe_backward_bf16_workspace_bytes(Nt, d, F, E, k)
+    ws = torch.empty((max(ws_bytes, 1),), device=dev, dtype=torch.uint8)
+    f32 = dict(device=dev, dtype=torch.float32)
+    dx = torch.empty_like(dout)
+    dWu, dbu = torch.empty((E, F, d, 8), **f32), torch.empty((E, F, 8), **f32)
+    dWd, dbd = torch.empty((E, d, F, 8), **f32), torch.empty((E, d, 8), **f32)
+    dtw = torch.empty((Nt, k), **f32) if routing_grad else None
+    check(L.ygg_moe_backward_bf16(Nt, d, F, E, k, ACT_CODE[act], ptr(w_up_adj.data), ptr(w_down_adj.data), int(residual),
+                                  ptr(dout), ptr(saved), saved.numel(), ptr(topk_w), ptr(offsets), ptr(dx), ptr(dWu),
+                                  ptr(dbu), ptr(dWd), ptr(dbd), ptr(dtw), ptr(ws), ws_bytes, stream_handle(dev)),
+          "moe_backward_bf16")
+    return dx, dWu, dbu, dWd, dbd, dtw
+
+
 def grade_quantize(w: torch.Tensor, grade_bits=(8, 6, 6, 4), symmetric: bool = True, codes: bool = True):
     """Grade-aware quantization per leading index (``grade_quantize.py:153-238``).
 
