@@ -23,7 +23,8 @@ namespace {
 constexpr int kWbTile = 64;     // output columns j and input columns i of a workgroup
 constexpr int kWbRows = 8;      // rows of a stage
 constexpr int kWbStages = 4;    // stages in LDS: three in flight while one is read
-constexpr int kWbMaxChunk = 1024, kWbMinChunk = 128;  // rows of a workgroup at most, see chunk_rows
+constexpr int kWbMaxChunk = 1024, kWbMinChunk = 256;  // rows of a workgroup at most, see chunk_rows
+constexpr int kWbMaxRows1 = 512;
 constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
@@ -68,6 +69,18 @@ __device__ __forceinline__ float4 half_blades(float r0, float i0, float r1, floa
            : make_float4(0.5f * (r0 + x), 0.5f * (r1 + y), 0.5f * (i1 - z), 0.5f * (r0 - x));
 }
 
+// A tile of the gradient of expert e, which has no rows
+__device__ __forceinline__ void zero_tile(int jt, int it, int e, int d_in, int d_out, float* __restrict__ dW,
+                                          float* __restrict__ db, int tid) {
+  const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int n = tid; n < kWbTile * kWbTile * 2; n += 256) {
+    const int j = jt * kWbTile + n / (kWbTile * 2), i2 = it * kWbTile * 2 + n % (kWbTile * 2);
+    if (j < d_out && i2 < d_in * 2) reinterpret_cast<float4*>(dW)[((size_t)e * d_out + j) * d_in * 2 + i2] = z;
+  }
+  if (db != nullptr && it == 0 && tid < kWbTile * 2 && jt * kWbTile * 2 + tid < d_out * 2)
+    reinterpret_cast<float4*>(db)[(size_t)e * d_out * 2 + jt * kWbTile * 2 + tid] = z;
+}
+
 // One workgroup: 64 (j) x 64 (i) of one chunk's sum, a wave 32 x 32 of it.
 //
 // v_mfma_f32_32x32x16_bf16 with the operand rows (j, a) and columns (i, c), 16 of each index: the dword
@@ -100,7 +113,14 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
     first += k > key ? m : 0;
   }
   const uint64_t mine = __ballot(lane < E && chunk >= first && chunk < first + x.n);
-  if (mine == 0) return;
+  if (mine == 0) {  // behind the chunks: the experts without rows, whose gradient is zero
+    const uint64_t none = __ballot(lane < E && x.n == 0);
+    const int total = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n, lane), 63);
+    const int nth = __popcll(none & ((1ull << lane) - 1));  // this lane's place among them
+    const uint64_t here = __ballot(lane < E && x.n == 0 && nth == chunk - total);
+    if (here != 0) zero_tile(tile % nj, tile / nj, (int)__builtin_ctzll(here), d_in, d_out, dW, db, tid);
+    return;
+  }
   const int e = (int)__builtin_ctzll(mine);
   const int n = __builtin_amdgcn_readlane(x.n, e), c = chunk - __builtin_amdgcn_readlane(first, e);
   const int len = __builtin_amdgcn_readlane(x.len, e);
@@ -264,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   }
 }
 
-// dW and db of the experts whose rows are several chunks, their planes added in order, or none: zero.
+// dW and db of the experts whose rows are several chunks, their planes added in order.
 // A thread per four values, blockIdx.y the expert.
 __global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const float* __restrict__ part,
                                                                       const float* __restrict__ dbpart,
@@ -274,7 +294,7 @@ __global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const floa
   const int e = blockIdx.y, lane = threadIdx.x & 63;
   const WbExpert x = wb_experts(offsets, E, P, limit, lane);
   const int n = __builtin_amdgcn_readlane(x.n, e);
-  if (n == 1) return;
+  if (n <= 1) return;
   const int first = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), e) - n;
   const size_t nw = (size_t)d_out * d_in * 2, nb = db != nullptr ? (size_t)d_out * 2 : 0;
   size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -298,12 +318,16 @@ long long wb_tiles(int d_in, int d_out) {
 // The rows of a chunk at most: what each of the 512 workgroups that the chip holds would have of all rows' tiles,
 // within limits -- below 128 rows a workgroup's start and its plane cost more than its products (CHUNKTEXT)
 int chunk_rows(int P, int d_in, int d_out) {
+  if (P <= kWbMaxRows1) return kWbMaxRows1;  // one chunk an expert: no planes and no second launch
   const long long even = (long long)P * wb_tiles(d_in, d_out) / 512;
   return (int)std::min<long long>(kWbMaxChunk, std::max<long long>(kWbMinChunk, even)) / kWbRows * kWbRows;
 }
-// chunks there can be, and planes of the experts that have several: such an expert has more than `limit` rows
-long long wb_chunks(long long P, int E, int limit) { return P / limit + std::min<long long>(E, P); }
-long long wb_planes(long long P, int E, int limit) { return P / limit + std::min<long long>(E, P / (limit + 1)); }
+// chunks there can be with the experts without any, and planes of the experts that have several: such an expert
+// has more than `limit` rows
+long long wb_chunks(long long P, int E, int limit) { return P / limit + E; }
+long long wb_planes(long long P, int E, int limit) {
+  return P > limit ? P / limit + std::min<long long>(E, P / (limit + 1)) : 0;
+}
 
 }  // namespace
 
@@ -320,18 +344,12 @@ int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* g
   float* dbpart = part + (size_t)planes * d_out * d_in * 8;
   const int n_xcd = 8;  // workgroups go to the XCDs round robin (8 on MI355X)
   const long long nt = wb_tiles(d_in, d_out);
-  if (chunks > 0) {
-    const dim3 grid((unsigned)((chunks + n_xcd - 1) / n_xcd * n_xcd * nt));
-    if (gather)
-      hipLaunchKernelGGL(weight_grad_bf16_kernel<true>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(dy),
-                         static_cast<const uint16_t*>(a), a_rows, gather, offsets, P_max, limit, E, d_in, d_out, n_xcd, part,
-                         dbpart, dW, db);
-    else
-      hipLaunchKernelGGL(weight_grad_bf16_kernel<false>, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(dy),
-                         static_cast<const uint16_t*>(a), a_rows, gather, offsets, P_max, limit, E, d_in, d_out, n_xcd, part,
-                         dbpart, dW, db);
-    if (check_launch("weight gradient (bf16)")) return -1;
-  }
+  const dim3 grid((unsigned)((chunks + n_xcd - 1) / n_xcd * n_xcd * nt));
+  auto* kernel = gather ? weight_grad_bf16_kernel<true> : weight_grad_bf16_kernel<false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, static_cast<const uint16_t*>(dy), static_cast<const uint16_t*>(a),
+                     a_rows, gather, offsets, P_max, limit, E, d_in, d_out, n_xcd, part, dbpart, dW, db);
+  if (check_launch("weight gradient (bf16)")) return -1;
+  if (planes == 0) return 0;
   const size_t n4 = (size_t)d_out * (d_in + (db ? 1 : 0)) * 2;
   hipLaunchKernelGGL(weight_grad_bf16_reduce_kernel, dim3((unsigned)((n4 + 255) / 256), E), dim3(256), 0, stream, part,
                      dbpart, offsets, P_max, limit, E, d_in, d_out, dW, db);

@@ -41,6 +41,22 @@ def _dtype_code(t: torch.Tensor) -> int:
         raise ValueError(f"unsupported dtype {t.dtype}; use float32 or bfloat16") from None
 
 
+def _aligned(t):
+    """t itself, or a copy of it on 16 bytes: the kernels load 16 bytes at a time."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _fp32(t):
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def _workspace(given, need: int, dev) -> torch.Tensor:
+    """The caller's workspace if it is large enough, else one of `need` bytes."""
+    if given is not None and given.numel() * given.element_size() >= need:
+        return given
+    return torch.empty(need, device=dev, dtype=torch.uint8)
+
+
 def _check_layer_args(x, k, E, F, logits=None, residual=None, router_weight=None, router_bias=None, b_up=None,
                       b_down=None):
     """Shapes and dtypes of a layer call's tensors, checked before their pointers reach the kernels."""
@@ -648,30 +664,26 @@ def clifford_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch
     dx before it is rounded: the gradient that reaches x past the norm, as in ``x + f(norm(x))``.
     """
     dev = _dev(dy, x, gamma, residual_grad)
-    if x.dim() < 2 or x.shape[-1] != 8:
-        raise ValueError(f"clifford_layer_norm_backward: x must be (..., d, 8), got {tuple(x.shape)}")
-    if dy.shape != x.shape:
-        raise ValueError(f"clifford_layer_norm_backward: dy must have x's shape {tuple(x.shape)}, got {tuple(dy.shape)}")
-    d = x.shape[-2]
-    if tuple(gamma.shape) != (d, 8):
+    shape = x.shape
+    if len(shape) < 2 or shape[-1] != 8:
+        raise ValueError(f"clifford_layer_norm_backward: x must be (..., d, 8), got {tuple(shape)}")
+    if dy.shape != shape:
+        raise ValueError(f"clifford_layer_norm_backward: dy must have x's shape {tuple(shape)}, got {tuple(dy.shape)}")
+    d = shape[-2]
+    if gamma.shape != (d, 8):
         raise ValueError(f"clifford_layer_norm_backward: gamma must be ({d}, 8)")
-    if residual_grad is not None and (residual_grad.shape != x.shape or residual_grad.dtype != x.dtype):
+    if residual_grad is not None and (residual_grad.shape != shape or residual_grad.dtype != x.dtype):
         raise ValueError("clifford_layer_norm_backward: residual_grad must have x's shape and dtype")
-    # the kernels load 16 bytes at a time
-    dy, x, residual_grad = (t if t is None or t.data_ptr() % 16 == 0 else t.clone() for t in (dy, x, residual_grad))
+    dy, x, residual_grad, g = _aligned(dy), _aligned(x), _aligned(residual_grad), _aligned(_fp32(gamma))
     Nt = x.numel() // (8 * d) if d else 0
     L = lib()
     need = L.ygg_clifford_layer_norm_backward_workspace_bytes(Nt, d)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
-    g = gamma.float().contiguous()
-    g = g if g.data_ptr() % 16 == 0 else g.clone()
-    dx = torch.empty_like(x)
-    dgamma = torch.empty((d, 8), device=dev, dtype=torch.float32)
-    dbeta = torch.empty((d, 8), device=dev, dtype=torch.float32)
-    check(L.ygg_clifford_layer_norm_backward(ptr(dy), _dtype_code(dy), ptr(x), _dtype_code(x), Nt, d, ptr(g), float(eps),
-                                             ptr(residual_grad), ptr(dx), ptr(dgamma), ptr(dbeta), ptr(workspace), need,
-                                             stream_handle(dev)), "clifford_layer_norm_backward")
+    workspace = _workspace(workspace, need, dev)
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(g), torch.empty_like(g)
+    check(L.ygg_clifford_layer_norm_backward(dy.data_ptr(), _dtype_code(dy), x.data_ptr(), _dtype_code(x), Nt, d,
+                                             g.data_ptr(), eps, ptr(residual_grad), dx.data_ptr(), dgamma.data_ptr(),
+                                             dbeta.data_ptr(), workspace.data_ptr(), need, stream_handle(dev)),
+          "clifford_layer_norm_backward")
     return dx, dgamma, dbeta
 
 
@@ -791,13 +803,14 @@ def grouped_weight_grad_pauli(dy_pauli: torch.Tensor, a_pauli: torch.Tensor, off
 
 def _half_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     """bf16 Pauli half-rows (rows, 2, d, 4) on 16 bytes, as the kernels load them."""
-    if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[1] != 2 or t.shape[3] != 4:
-        raise ValueError(f"{name} must be bf16 Pauli half-rows (rows, 2, d, 4), got {t.dtype} {tuple(t.shape)}")
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    shape = t.shape
+    if t.dtype != torch.bfloat16 or len(shape) != 4 or shape[1] != 2 or shape[3] != 4:
+        raise ValueError(f"{name} must be bf16 Pauli half-rows (rows, 2, d, 4), got {t.dtype} {tuple(shape)}")
+    return _aligned(t)
 
 
 def _check_bounds(offsets: torch.Tensor, E: int, dev) -> None:
-    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,) or offsets.device != dev:
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or offsets.device != dev:
         raise ValueError(f"offsets must be int32 ({E + 1},) on {dev}, got {offsets.dtype} {tuple(offsets.shape)}")
 
 
@@ -805,18 +818,16 @@ def _grouped_weight_grad_bf16(dev, dy, a, offsets, E, gather, with_bias, workspa
     dy, a = _half_rows("dy_pauli", dy), _half_rows("a_pauli", a)
     P, d_out, d_in = dy.shape[0], dy.shape[2], a.shape[2]
     _check_bounds(offsets, E, dev)
-    if gather is not None and (gather.dtype != torch.int32 or tuple(gather.shape) != (P,)):
+    if gather is not None and (gather.dtype != torch.int32 or gather.shape != (P,)):
         raise ValueError(f"gather must be int32 ({P},), got {gather.dtype} {tuple(gather.shape)}")
     L = lib()
     need = L.ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(P, E, d_in, d_out)
-    if workspace is None:
-        workspace = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    workspace = _workspace(workspace, need, dev) if need else None
     dW = torch.empty((E, d_out, d_in, 8), device=dev, dtype=torch.float32)
     db = torch.empty((E, d_out, 8), device=dev, dtype=torch.float32) if with_bias else None
-    check(L.ygg_grouped_weight_grad_pauli_bf16(ptr(dy), ptr(a), a.shape[0], ptr(gather), ptr(offsets), P, E, d_in, d_out,
-                                               ptr(dW), ptr(db), ptr(workspace),
-                                               workspace.numel() * workspace.element_size(), stream_handle(dev)),
-          "grouped_weight_grad_pauli")
+    check(L.ygg_grouped_weight_grad_pauli_bf16(dy.data_ptr(), a.data_ptr(), a.shape[0], ptr(gather), offsets.data_ptr(), P,
+                                               E, d_in, d_out, dW.data_ptr(), ptr(db), ptr(workspace), need,
+                                               stream_handle(dev)), "grouped_weight_grad_pauli")
     return dW, db
 
 
@@ -844,16 +855,15 @@ def pauli_grouped_input_grad(dy_pauli: torch.Tensor, pw_adj: PreparedWeights, of
         raise ValueError(f"dy_pauli has d_out={d_out}, the adjoint weights expect {pw_adj.d_in}")
     _check_bounds(offsets, E, dev)
     if act != "none":
-        if h_pre is None or h_pre.dtype != torch.bfloat16 or tuple(h_pre.shape) != (P, d_in, 8):
+        if h_pre is None or h_pre.dtype != torch.bfloat16 or h_pre.shape != (P, d_in, 8):
             raise ValueError(f"act={act!r} needs h_pre, bf16 ({P}, {d_in}, 8)")
-        if h_pre.data_ptr() % 16:
-            h_pre = h_pre.clone()
+        h_pre = _aligned(h_pre)
     if y_layout == "pauli":
         dx = torch.empty((P, 2, d_in, 4), device=dev, dtype=torch.bfloat16)
     else:
         dx = torch.empty((P, d_in, 8), device=dev, dtype=out_dtype)
-    check(lib().ygg_pauli_grouped_input_grad(ptr(dy_pauli), P, ptr(pw_adj.data), ptr(offsets), E, d_out, d_in,
-                                             ACT_CODE[act], ptr(h_pre) if act != "none" else None, ptr(dx),
+    check(lib().ygg_pauli_grouped_input_grad(dy_pauli.data_ptr(), P, pw_adj.data.data_ptr(), offsets.data_ptr(), E, d_out,
+                                             d_in, ACT_CODE[act], ptr(h_pre) if act != "none" else None, dx.data_ptr(),
                                              Y_LAYOUT[y_layout], _dtype_code(dx), stream_handle(dev)),
           "pauli_grouped_input_grad")
     return dx
@@ -874,8 +884,8 @@ def route_backward(topk_idx: torch.Tensor, topk_w: torch.Tensor, dtopk_w: torch.
     dev = _dev(topk_idx, topk_w, dtopk_w)
     Nt, k = _check_slots(topk_idx, topk_w, dtopk_w)
     dlogits = torch.empty((Nt, E), device=dev, dtype=torch.float32)
-    check(lib().ygg_route_backward(ptr(topk_idx), ptr(topk_w), ptr(dtopk_w), Nt, E, k, ptr(dlogits), stream_handle(dev)),
-          "route_backward")
+    check(lib().ygg_route_backward(topk_idx.data_ptr(), topk_w.data_ptr(), dtopk_w.data_ptr(), Nt, E, k,
+                                   dlogits.data_ptr(), stream_handle(dev)), "route_backward")
     return dlogits
 
 
@@ -888,24 +898,22 @@ def route_energy_backward(x: torch.Tensor, router_weight: torch.Tensor, topk_idx
         raise ValueError(f"route_energy_backward: x must be (N, d, 8), got {tuple(x.shape)}")
     Nt, d = x.shape[:2]
     E = router_weight.shape[0]
-    if tuple(router_weight.shape) != (E, 4):
+    if router_weight.shape != (E, 4):
         raise ValueError(f"route_energy_backward: router_weight must be (E, 4), got {tuple(router_weight.shape)}")
     if _check_slots(topk_idx, topk_w, dtopk_w)[0] != Nt:
         raise ValueError(f"route_energy_backward: {topk_idx.shape[0]} tokens' routing for {Nt} tokens")
     if dx_add is not None and (dx_add.shape != x.shape or dx_add.dtype != x.dtype):
         raise ValueError("route_energy_backward: dx_add must have x's shape and dtype")
-    x = x if x.data_ptr() % 16 == 0 else x.clone()
-    dx_add = dx_add if dx_add is None or dx_add.data_ptr() % 16 == 0 else dx_add.clone()
+    x, dx_add, rw = _aligned(x), _aligned(dx_add), _fp32(router_weight)
     L = lib()
     need = L.ygg_route_energy_backward_workspace_bytes(Nt, E)
-    ws = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
-    rw = router_weight.float().contiguous()
-    dx = torch.empty_like(x)
-    drw = torch.empty((E, 4), device=dev, dtype=torch.float32)
-    drb = torch.empty((E,), device=dev, dtype=torch.float32)
-    check(L.ygg_route_energy_backward(ptr(x), _dtype_code(x), Nt, d, ptr(rw), E, topk_idx.shape[1], ptr(topk_idx),
-                                      ptr(topk_w), ptr(dtopk_w), ptr(dx_add), ptr(dx), ptr(drw), ptr(drb), ptr(ws),
-                                      need, stream_handle(dev)), "route_energy_backward")
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    dx, drw = torch.empty_like(x), torch.empty_like(rw)
+    drb = torch.empty(E, device=dev, dtype=torch.float32)
+    check(L.ygg_route_energy_backward(x.data_ptr(), _dtype_code(x), Nt, d, rw.data_ptr(), E, topk_idx.shape[1],
+                                      topk_idx.data_ptr(), topk_w.data_ptr(), dtopk_w.data_ptr(), ptr(dx_add),
+                                      dx.data_ptr(), drw.data_ptr(), drb.data_ptr(), ws.data_ptr(), need,
+                                      stream_handle(dev)), "route_energy_backward")
     return dx, drw, drb
 
 
