@@ -21,10 +21,11 @@ namespace ygg {
 namespace {
 
 constexpr int kWbTile = 64;     // output columns j and input columns i of a workgroup
-constexpr int kWbRows = 8;      // rows of a stage
-constexpr int kWbStages = 4;    // stages in LDS: three in flight while one is read
+constexpr int kWbRows = 12;      // rows of a stage
+constexpr int kWbStages = 3;    // stages in LDS: two in flight while one is read
+constexpr int kWbWaveRows = kWbRows / 4;  // rows that a wave loads per stage
 constexpr int kWbMaxChunk = 1024, kWbMinChunk = 256;  // rows of a workgroup at most, see chunk_rows
-constexpr int kWbMaxRows1 = 512;
+constexpr int kWbMaxRows1 = 516;
 constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
     const int32_t* __restrict__ offsets, int P, int limit, int E, int d_in, int d_out, int n_xcd, float* __restrict__ part,
     float* __restrict__ dbpart, float* __restrict__ dW, float* __restrict__ db) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kWbStages * kWbStage];
-  __shared__ uint32_t s_src[GATHER ? kWbMaxChunk + kWbRows * kWbStages : 1];
+  __shared__ uint32_t s_src[GATHER ? kWbMaxChunk + kWbRows * (kWbStages + 1) : 1];
   const int32_t* const gather = GATHER ? gather_rows : nullptr;
   const int tid = threadIdx.x, lane = tid & 63;
   const int nj = (d_out + kWbTile - 1) / kWbTile, ni = (d_in + kWbTile - 1) / kWbTile, nt = nj * ni;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   // the byte offset of every row's A from a_rsrc's base, or one past any range
   const uint32_t a_row = (uint32_t)d_in * 16;
   if (gather != nullptr)
-    for (int i = tid; i < limit + kWbRows * kWbStages; i += 256) {
+    for (int i = tid; i < limit + kWbRows * (kWbStages + 1); i += 256) {
       const int src = i < rows ? gather[r0 + i] : -1;
       s_src[i] = src >= 0 && src < a_rows ? (uint32_t)src * a_row : kBufferOff;
     }
@@ -149,20 +150,20 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   const int col = 2 * (lane & 31);
   const uint32_t d_bad = j0 + col < d_out ? 0u : kBufferOff, a_bad = i0 + col < d_in ? 0u : kBufferOff;
   const uint32_t a_lane = (uint32_t)((lane >> 5) * d_in + i0 + col) * 8;
-  uint32_t d_next = (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 + (uint32_t)(2 * wave) * d_out * 16;
-  uint32_t a_next = a_lane + (uint32_t)(2 * wave) * a_row;  // (rows in place)
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem + 2 * wave * 2 * kWbHalf;
-  uint32_t src[2] = {0, 0};  // gathered: the offsets of the next stage's two rows
+  uint32_t d_next = (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 + (uint32_t)(kWbWaveRows * wave) * d_out * 16;
+  uint32_t a_next = a_lane + (uint32_t)(kWbWaveRows * wave) * a_row;  // (rows in place)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem + kWbWaveRows * wave * 2 * kWbHalf;
+  uint32_t src[kWbWaveRows] = {};  // gathered: the offsets of the next stage's two rows
   auto next_src = [&](int f) __attribute__((always_inline)) {
     if constexpr (GATHER) {
-      src[0] = s_src[f * kWbRows + 2 * wave];
-      src[1] = s_src[f * kWbRows + 2 * wave + 1];
+#pragma unroll
+      for (int u = 0; u < kWbWaveRows; ++u) src[u] = s_src[f * kWbRows + kWbWaveRows * wave + u];
     }
   };
-  auto issue = [&](int f) __attribute__((always_inline)) {  // stage f's rows: two of each operand a wave
+  auto issue = [&](int f) __attribute__((always_inline)) {  // stage f's rows, three of each operand a wave
     const uint32_t st = lds0 + (f % kWbStages) * kWbStage;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kWbWaveRows; ++u) {
       split_dma(d_rsrc, st + u * 2 * kWbHalf, (d_next + u * (uint32_t)d_out * 16) | d_bad, 0);
       split_dma(a_rsrc, st + kWbOperand + u * 2 * kWbHalf, (GATHER ? src[u] + a_lane : a_next + u * a_row) | a_bad, 0);
     }
@@ -203,12 +204,12 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   auto loop = [&](auto bias_tag) __attribute__((always_inline)) {
     constexpr bool BIAS = decltype(bias_tag)::value;
     for (int f = 0; f < nf; ++f) {
-      // four loads a stage: those of the two newer stages may stay outstanding
-      asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+      // the loads of the newer stage may stay outstanding
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kWbStages - 2) * 2 * kWbWaveRows) : "memory");
       const unsigned char* st = smem + (f % kWbStages) * kWbStage;
-      uint32_t d[2][2][4], a[2][2][4];  // [four rows][block][half-row]
+      uint32_t d[kWbRows / 4][2][4], a[kWbRows / 4][2][4];  // [four rows][block][half-row]
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < kWbRows / 4; ++s)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
 #pragma unroll
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
       issue(f + kWbStages - 1);  // over the stage read before the barrier
       next_src(f + kWbStages);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < kWbRows / 4; ++s) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint32_t* w = a[s][q];
@@ -374,7 +375,7 @@ YGG_API int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void*
                 "d_out)", P_max, E, d_in, d_out);
   YGG_CHECK_ARG(a_rows >= 0 && (gather != nullptr || a_rows >= P_max),
                 "ygg_grouped_weight_grad_pauli_bf16: a has %d rows, %d are read without a gather", a_rows, P_max);
-  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) <= 0x7fffffffLL && (long long)(kWbMaxChunk + kWbRows * kWbStages) * std::max(d_in, d_out) * 16 < 1LL << 31,
+  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) <= 0x7fffffffLL && (long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 < 1LL << 31,
                 "ygg_grouped_weight_grad_pauli_bf16: P_max=%d d_in=%d d_out=%d exceed a launch", P_max, d_in, d_out);
   YGG_CHECK_ARG(gather == nullptr || (long long)a_rows * d_in * 16 < 1LL << 31,
                 "ygg_grouped_weight_grad_pauli_bf16: gathered rows span 2 GiB or more (a_rows=%d d_in=%d)", a_rows, d_in);
