@@ -251,7 +251,8 @@ def test_norm_backward_of_no_tokens():
 @pytest.mark.parametrize("N,d,E,k,dt,add", [
     (1, 1, 1, 1, "f32", False), (5, 3, 4, 2, "f32", True), (257, 64, 8, 2, "f32", False), (70, 100, 12, 3, "bf16", True),
     (33, 7, 64, 8, "bf16", False), (1000, 16, 64, 2, "bf16", True), (19, 300, 16, 4, "f32", True), (300, 8, 3, 3, "bf16", False),
-    (40, 20, 6, 1, "f32", True), (3000, 2, 5, 2, "f32", False)])
+    (40, 20, 6, 1, "f32", True), (3000, 2, 5, 2, "f32", False),
+    (40003, 3, 6, 2, "f32", True)])  # (the last: more than a batch a workgroup)
 def test_router_backward(N, d, E, k, dt, add):
     ops = _ops()
     g = np.random.default_rng(N + d * 3 + E)

@@ -25,6 +25,7 @@ def _refused(name, args, word):
     ((P, 0, P, 0, -1, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
     ((P, 0, P, 0, 4, 0, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
     ((P, 0, P, 0, 4, 4097, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
+    ((P, 0, P, 0, 0x7fff0001, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "bad sizes"),
     ((P, 0, P, 0, 4, 4, P, -1.0, None, P, P, P, P, 1 << 20, None), "eps"),
     ((P, 0, P, 0, 4, 4, None, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
     ((None, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
@@ -153,3 +154,49 @@ def test_workspace_sizes_of_bad_sizes_are_zero():
     assert lib.ygg_clifford_layer_norm_backward_workspace_bytes(4, 5000) == 0
     assert lib.ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(-1, 2, 4, 4) == 0
     assert lib.ygg_route_energy_backward_workspace_bytes(-1, 4) == 0
+
+
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    """An operator called while another device is current runs with its tensors' device current."""
+    seen, current = [], [0]
+
+    class Device:
+        def __init__(self, d):
+            self.d = d
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.d.index
+
+        def __exit__(self, *exc):
+            current[0] = self.was
+
+    class Tensor:
+        is_cuda, device = True, torch.device("cuda", 3)
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+
+    @ops._on_its_device
+    def op(t, more, key=None):
+        seen.append((current[0], more, key))
+        return "done"
+
+    assert op(Tensor(), 5, key=6) == "done" and seen == [(3, 5, 6)] and current == [0]
+    current[0] = 3
+    assert op(Tensor(), 7) == "done" and seen[1] == (3, 7, None)
+
+
+def test_tensors_of_two_devices_are_refused():
+    class Tensor:
+        is_cuda = True
+
+        def __init__(self, n):
+            self.device = torch.device("cuda", n)
+
+        def is_contiguous(self):
+            return True
+
+    a, b = Tensor(0), Tensor(1)
+    assert ops._one_device(a, None, a) == a.device
+    with pytest.raises(ValueError, match="one device"):
+        ops._one_device(a, b)

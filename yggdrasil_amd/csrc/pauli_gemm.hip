@@ -835,7 +835,7 @@ __global__ __launch_bounds__(256) void pauli_prep_weights_kernel(const float* __
 // The same layout of the adjoint weights (E, d_in, d_out): Wadj_ij = ~W_ji, whose product is the
 // gradient of W's input.  A workgroup transposes 32 (j) x 32 (i) of an expert through LDS, so that
 // it reads runs of 32 multivectors and writes runs of 16 records (a thread per multivector of the
-// layout, which read single ones, took 200 us for 64 x 1024 x 256 and this PREPTEXT).
+// layout, which read single ones, took 200 us for 64 x 1024 x 256; this takes 134, 6.0 TB/s).
 constexpr int kPrepT = 32;
 __global__ __launch_bounds__(256) void pauli_prep_adjoint_kernel(const float* __restrict__ W, int d_out, int d_in,
                                                                  uint16_t* __restrict__ out) {

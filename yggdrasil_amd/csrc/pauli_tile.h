@@ -100,7 +100,9 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
                                                 : (uint32_t)((2 * g) * d_out + j) * MV_BYTES;
     const uint32_t av_off = (uint32_t)((2 * g) * d_out + j) * 16;
     // kActGrad: the eight rows before the activation of a row block, asked for together.  Rows past the tile's
-    // last repeat it.
+    // last repeat it.  (Input gradient of 8192 tokens, d = 128, F = 512, E = 32, k = 4 through gelu: the product takes
+    // 191 us, 178 without these loads, 177 without the slopes, 180 without the stores and about
+    // 165 without all three.)
     uint4 hq[8] = {};
     auto load_h = [&](int rb) __attribute__((always_inline)) {
       if constexpr (ACT >= kActGrad && ACT < kActSave) {
@@ -123,8 +125,8 @@ __device__ __forceinline__ void pauli_tile_epilogue(const pf32x16_t (&acc)[WR][W
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int rs0 = ti.row0 + (ti.compact ? wt * 16 : (wt * WR + rbr) * 16) + 4 * q + h;  // row of lanes with g = 0
-          // kActGrad: no branch, so that the long chains of several multivectors run side by side; a row past the
-          // tile's last has an offset past the output, where a store does nothing
+          // kActGrad: no branch, so that the long chains of several multivectors run side by side (with one for each
+          // multivector 220 us); a row past the tile's last has an offset past the output, where a store does nothing
           constexpr bool NO_BRANCH = ACT >= kActGrad && ACT < kActSave;
           if (!NO_BRANCH && rs0 + 2 * g >= ti.row_end) continue;
           const int rs = NO_BRANCH ? min(rs0, ti.row_end - 1) : rs0;

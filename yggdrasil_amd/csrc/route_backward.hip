@@ -43,25 +43,27 @@ __device__ inline void slot_gradients(const float* __restrict__ w, const float* 
 __global__ __launch_bounds__(256) void route_backward_kernel(const int32_t* __restrict__ idx, const float* __restrict__ w,
                                                              const float* __restrict__ g, int N, int E, int k,
                                                              float* __restrict__ dlogits) {
-  const size_t n = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= (size_t)N * E) return;
-  const size_t t = n / E;
-  const int e = (int)(n - t * E);
-  float dl[kRbMaxK], v = 0.f;
-  slot_gradients(w, g, t, k, dl);
+  for (size_t n = (size_t)blockIdx.x * 256 + threadIdx.x; n < (size_t)N * E; n += (size_t)gridDim.x * 256) {
+    const size_t t = n / E;
+    const int e = (int)(n - t * E);
+    float dl[kRbMaxK], v = 0.f;
+    slot_gradients(w, g, t, k, dl);
 #pragma unroll
-  for (int s = 0; s < kRbMaxK; ++s)
-    if (s < k && idx[t * k + s] == e) v += dl[s];
-  dlogits[n] = v;
+    for (int s = 0; s < kRbMaxK; ++s)
+      if (s < k && idx[t * k + s] == e) v += dl[s];
+    dlogits[n] = v;
+  }
 }
 
-// A workgroup takes tokens_per tokens, a wave one at a time (a row of up to 64 NQ multivectors in registers, the
-// rest read again from L2): the energies, dx (plus add), and for the parameters the token's shares and slot
-// gradients, which stay in LDS.  Then lane e of every wave adds what expert e has of the wave's share of the
-// slots, the waves' sums are added in order, and the workgroup writes them as a plane of its own.
+// A workgroup takes batches of up to 16 tokens, a wave one token at a time (a row of up to 64 NQ multivectors in
+// registers, the rest read again from L2): the energies, dx (plus add), and for the parameters the token's shares
+// and slot gradients, which stay in LDS.  Then lane e of every wave adds what expert e has of the wave's share of
+// the slots.  The waves' sums are added in order at the end, and are a plane of the workgroup's own.
 //
-// Bound by memory: ROUTETEXT
-constexpr int kRbTokens = 32;  // tokens of a workgroup at most
+// Bound by memory: 32768 tokens of 256 multivectors, bf16, E = 64, k = 2 take 59 us in all, 47 of them here (268 MB
+// read and written: 5.7 TB/s; a copy of 1 GiB runs at 5.1) and 5 in the planes' sum.  As three passes -- dx, then one
+// workgroup per expert over all tokens -- the same took 244 us.
+constexpr int kRbTokens = 16, kRbMaxPlanes = 2048;  // planes: eight workgroups on each of 256 CUs
 
 template <typename T, int NQ>
 __global__ __launch_bounds__(256) void energy_backward_kernel(const T* __restrict__ x, int N, int d,
@@ -75,103 +77,106 @@ __global__ __launch_bounds__(256) void energy_backward_kernel(const T* __restric
   __shared__ int s_idx[kRbTokens * kRbMaxK];
   __shared__ float s_red[4][5][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t0 = blockIdx.x * tokens_per, tokens = min(tokens_per, N - t0);
-  for (int u = wave; u < tokens; u += 4) {
-    const int t = t0 + u;
-    const size_t row = (size_t)t * d;
-    RawMv<T> rx[NQ], ra[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (lane + 64 * q < d) rx[q] = load_raw(x, row + lane + 64 * q);
-    if (add != nullptr) {
+  float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  for (long long t0 = (long long)blockIdx.x * tokens_per; t0 < N; t0 += (long long)gridDim.x * tokens_per) {
+    const int tokens = (int)min((long long)tokens_per, N - t0);
+    for (int u = wave; u < tokens; u += 4) {
+      const size_t t = (size_t)t0 + u;
+      const size_t row = t * d;
+      RawMv<T> rx[NQ], ra[NQ];
 #pragma unroll
       for (int q = 0; q < NQ; ++q)
-        if (lane + 64 * q < d) ra[q] = load_raw(add, row + lane + 64 * q);
-    }
-    // the slots' gradients and those of the shares (the same in every lane)
-    float dl[kRbMaxK], ds[4] = {0.f, 0.f, 0.f, 0.f};
-    slot_gradients(w, g, t, k, dl);
+        if (lane + 64 * q < d) rx[q] = load_raw(x, row + lane + 64 * q);
+      if (add != nullptr) {
 #pragma unroll
-    for (int s = 0; s < kRbMaxK; ++s)
-      if (s < k) {
-        const int e = idx[(size_t)t * k + s];
-        const bool known = e >= 0 && e < E;
-        if (known)
+        for (int q = 0; q < NQ; ++q)
+          if (lane + 64 * q < d) ra[q] = load_raw(add, row + lane + 64 * q);
+      }
+      // the slots' gradients and those of the shares (the same in every lane)
+      float dl[kRbMaxK], ds[4] = {0.f, 0.f, 0.f, 0.f};
+      slot_gradients(w, g, t, k, dl);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) ds[h] = __builtin_fmaf(dl[s], W[e * 4 + h], ds[h]);
-        if (lane == 0) {
-          s_dl[u * kRbMaxK + s] = dl[s];
-          s_idx[u * kRbMaxK + s] = e;
+      for (int s = 0; s < kRbMaxK; ++s)
+        if (s < k) {
+          const int e = idx[t * k + s];
+          const bool known = e >= 0 && e < E;
+          if (known)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) ds[h] = __builtin_fmaf(dl[s], W[e * 4 + h], ds[h]);
+          if (lane == 0) {
+            s_dl[u * kRbMaxK + s] = dl[s];
+            s_idx[u * kRbMaxK + s] = e;
+          }
         }
-      }
-    float en[4] = {0.f, 0.f, 0.f, 0.f};
-    auto energies = [&](const float v[8]) __attribute__((always_inline)) {
-      en[0] = __builtin_fmaf(v[0], v[0], en[0]);
-      en[3] = __builtin_fmaf(v[7], v[7], en[3]);
+      float en[4] = {0.f, 0.f, 0.f, 0.f};
+      auto energies = [&](const float v[8]) __attribute__((always_inline)) {
+        en[0] = __builtin_fmaf(v[0], v[0], en[0]);
+        en[3] = __builtin_fmaf(v[7], v[7], en[3]);
 #pragma unroll
-      for (int c = 0; c < 3; ++c) {
-        en[1] = __builtin_fmaf(v[1 + c], v[1 + c], en[1]);
-        en[2] = __builtin_fmaf(v[4 + c], v[4 + c], en[2]);
-      }
-    };
+        for (int c = 0; c < 3; ++c) {
+          en[1] = __builtin_fmaf(v[1 + c], v[1 + c], en[1]);
+          en[2] = __builtin_fmaf(v[4 + c], v[4 + c], en[2]);
+        }
+      };
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (lane + 64 * q < d) {
+      for (int q = 0; q < NQ; ++q)
+        if (lane + 64 * q < d) {
+          float v[8];
+          unpack(rx[q], v);
+          energies(v);
+        }
+      for (int i = lane + 64 * NQ; i < d; i += 64) {
         float v[8];
-        unpack(rx[q], v);
+        load_mv(x, row + i, v);
         energies(v);
       }
-    for (int i = lane + 64 * NQ; i < d; i += 64) {
-      float v[8];
-      load_mv(x, row + i, v);
-      energies(v);
-    }
-    const float sum = wave_sums<4>(en, lane);
-    float sh[4], dot = 0.f;
+      const float sum = wave_sums<4>(en, lane);
+      float sh[4], dot = 0.f;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) en[h] = __shfl(sum, 16 * h);
-    const float total = ((en[0] + en[1]) + (en[2] + en[3])) + 1e-12f;
+      for (int h = 0; h < 4; ++h) en[h] = __shfl(sum, 16 * h);
+      const float total = ((en[0] + en[1]) + (en[2] + en[3])) + 1e-12f;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      sh[h] = en[h] / total;
-      dot = __builtin_fmaf(ds[h], sh[h], dot);
-    }
-    if (lane == 0) s_share[u] = make_float4(sh[0], sh[1], sh[2], sh[3]);
-    float de[4];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) de[h] = 2.f * (ds[h] - dot) / total;
-    auto out = [&](float v[8], float o[8], int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) o[c] = __builtin_fmaf(v[c], de[c == 0 ? 0 : c < 4 ? 1 : c < 7 ? 2 : 3], o[c]);
-      store_mv(dx, row + i, o);
-    };
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (lane + 64 * q < d) {
-        float v[8], o[8] = {};
-        unpack(rx[q], v);
-        if (add != nullptr) unpack(ra[q], o);
-        out(v, o, lane + 64 * q);
+      for (int h = 0; h < 4; ++h) {
+        sh[h] = en[h] / total;
+        dot = __builtin_fmaf(ds[h], sh[h], dot);
       }
-    for (int i = lane + 64 * NQ; i < d; i += 64) {
-      float v[8], o[8] = {};
-      load_mv(x, row + i, v);
-      if (add != nullptr) load_mv(add, row + i, o);
-      out(v, o, i);
+      if (lane == 0) s_share[u] = make_float4(sh[0], sh[1], sh[2], sh[3]);
+      float de[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) de[h] = 2.f * (ds[h] - dot) / total;
+      auto out = [&](float v[8], float o[8], int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[c] = __builtin_fmaf(v[c], de[c == 0 ? 0 : c < 4 ? 1 : c < 7 ? 2 : 3], o[c]);
+        store_mv(dx, row + i, o);
+      };
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+        if (lane + 64 * q < d) {
+          float v[8], o[8] = {};
+          unpack(rx[q], v);
+          if (add != nullptr) unpack(ra[q], o);
+          out(v, o, lane + 64 * q);
+        }
+      for (int i = lane + 64 * NQ; i < d; i += 64) {
+        float v[8], o[8] = {};
+        load_mv(x, row + i, v);
+        if (add != nullptr) load_mv(add, row + i, o);
+        out(v, o, i);
+      }
     }
-  }
-  __syncthreads();
-  float s5[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int u = wave; u < tokens; u += 4) {
-    const float4 share = s_share[u];
-    for (int s = 0; s < k; ++s) {
-      const float v = s_idx[u * kRbMaxK + s] == lane ? s_dl[u * kRbMaxK + s] : 0.f;
-      s5[0] = __builtin_fmaf(v, share.x, s5[0]);
-      s5[1] = __builtin_fmaf(v, share.y, s5[1]);
-      s5[2] = __builtin_fmaf(v, share.z, s5[2]);
-      s5[3] = __builtin_fmaf(v, share.w, s5[3]);
-      s5[4] += v;
+    __syncthreads();
+    for (int u = wave; u < tokens; u += 4) {
+      const float4 share = s_share[u];
+      for (int s = 0; s < k; ++s) {
+        const float v = s_idx[u * kRbMaxK + s] == lane ? s_dl[u * kRbMaxK + s] : 0.f;
+        s5[0] = __builtin_fmaf(v, share.x, s5[0]);
+        s5[1] = __builtin_fmaf(v, share.y, s5[1]);
+        s5[2] = __builtin_fmaf(v, share.z, s5[2]);
+        s5[3] = __builtin_fmaf(v, share.w, s5[3]);
+        s5[4] += v;
+      }
     }
+    __syncthreads();  // the next batch's slots
   }
 #pragma unroll
   for (int h = 0; h < 5; ++h) s_red[wave][h][lane] = s5[h];
@@ -191,9 +196,12 @@ __global__ __launch_bounds__(1024) void router_param_kernel(const float* __restr
   });
 }
 
-// Tokens of a workgroup: enough workgroups to fill the chip first (eight on each of 256 CUs), then fewer planes
-int tokens_per_group(int N) { return std::min(kRbTokens, std::max(4, (N / 2048 + 3) / 4 * 4)); }
-int route_planes(int N) { return (N + tokens_per_group(N) - 1) / tokens_per_group(N); }
+// Tokens of a batch: enough workgroups to fill the chip first, then larger batches, then several a workgroup
+int batch_tokens(int N) { return std::min(kRbTokens, std::max(4, (N / kRbMaxPlanes + 3) / 4 * 4)); }
+int route_planes(int N) {
+  const int per = batch_tokens(N);
+  return std::min(kRbMaxPlanes, N / per + (N % per != 0));
+}
 
 }  // namespace
 }  // namespace ygg
@@ -207,8 +215,9 @@ YGG_API int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, con
   if (N == 0) return 0;
   YGG_CHECK_ARG(topk_idx && topk_w && dtopk_w && dlogits, "ygg_route_backward: null pointer argument");
   const size_t n = (size_t)N * E;
-  hipLaunchKernelGGL(route_backward_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, topk_idx, topk_w,
-                     dtopk_w, N, E, k, dlogits);
+  const unsigned groups = (unsigned)std::min<size_t>((n + 255) / 256, 1u << 23);  // a launch holds below 2^32 threads
+  hipLaunchKernelGGL(route_backward_kernel, dim3(groups), dim3(256), 0, stream, topk_idx, topk_w, dtopk_w, N, E, k,
+                     dlogits);
   return check_launch("ygg_route_backward");
 }
 
@@ -236,7 +245,7 @@ YGG_API int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, 
       using T = std::remove_const_t<std::remove_pointer_t<decltype(xt)>>;
       hipLaunchKernelGGL((energy_backward_kernel<T, decltype(nq)::value>), dim3(route_planes(N)), dim3(256), 0, stream, xt,
                          N, d, router_w, E, k, topk_idx, topk_w, dtopk_w, static_cast<const T*>(dx_add),
-                         static_cast<T*>(dx), tokens_per_group(N), part);
+                         static_cast<T*>(dx), batch_tokens(N), part);
     };
     auto by_width = [&](auto* xt) {
       if (d <= 64) run(xt, std::integral_constant<int, 1>{});

@@ -25,7 +25,7 @@ constexpr int kWbRows = 12;      // rows of a stage
 constexpr int kWbStages = 3;    // stages in LDS: two in flight while one is read
 constexpr int kWbWaveRows = kWbRows / 4;  // rows that a wave loads per stage
 constexpr int kWbMaxChunk = 1024, kWbMinChunk = 256;  // rows of a workgroup at most, see chunk_rows
-constexpr int kWbMaxRows1 = 516;
+constexpr int kWbMaxRows1 = 516;  // rows up to which every expert is one chunk
 constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
@@ -83,6 +83,12 @@ __device__ __forceinline__ void zero_tile(int jt, int it, int e, int d_in, int d
 }
 
 // One workgroup: 64 (j) x 64 (i) of one chunk's sum, a wave 32 x 32 of it.
+//
+// Bound by the matrix units and the loads into LDS together: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's
+// law take 163 us in all, 145 here and 18 in the planes' sum: 137 GFLOP at 0.95 PFLOP/s here, where a large bf16
+// product reaches 1.37.  Without the loads (data in LDS as it was) the whole took 137 us, without the products 133.
+// Larger tiles did not pay: 128 x 64 with eight waves 160 us, with four waves of 64 x 32, one a SIMD, 179; nor did
+// reading the next stage's operands into registers ahead (160) or raising the waves' priority (174).
 //
 // v_mfma_f32_32x32x16_bf16 with the operand rows (j, a) and columns (i, c), 16 of each index: the dword
 // (re, im) of entry a of column b of D_rj is one (r, b) term of the contraction, and four such dwords (two
@@ -317,7 +323,11 @@ long long wb_tiles(int d_in, int d_out) {
   return (long long)((d_out + kWbTile - 1) / kWbTile) * ((d_in + kWbTile - 1) / kWbTile);
 }
 // The rows of a chunk at most: what each of the 512 workgroups that the chip holds would have of all rows' tiles,
-// within limits -- below 128 rows a workgroup's start and its plane cost more than its products (CHUNKTEXT)
+// within limits.  More rows leave CUs idle at the end, fewer make more planes, which the reduction reads at the
+// rate of memory: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's law took 180 us with 512 rows, 170 with 768,
+// 161 with this rule's 1024 (and the longest chunks first), 276 with 2048; 1500 tokens, d = 100, F = 300, E = 12,
+// k = 3 took 35 us with 512, 28 with 256, 29 with 128.  Few rows take one chunk an expert, no planes and no second
+// launch (256 tokens, d = 64, F = 256, E = 8, k = 2: 16 us a call with planes, 11 without).
 int chunk_rows(int P, int d_in, int d_out) {
   if (P <= kWbMaxRows1) return kWbMaxRows1;  // one chunk an expert: no planes and no second launch
   const long long even = (long long)P * wb_tiles(d_in, d_out) / 512;

@@ -8,6 +8,7 @@ There is no CPU path: CPU tensors are rejected.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -41,6 +42,28 @@ def _dtype_code(t: torch.Tensor) -> int:
         raise ValueError(f"unsupported dtype {t.dtype}; use float32 or bfloat16") from None
 
 
+def _on_its_device(fn):
+    """An operator whose launches go to the device of its first tensor, whichever is current."""
+
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        if first.is_cuda and torch._C._cuda_getDevice() != first.device.index:
+            with torch.cuda.device(first.device):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
+
+    return call
+
+
+def _one_device(*tensors):
+    """:func:`_dev`, with every tensor on the first one's device."""
+    dev = _dev(*tensors)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: an operator takes them on one device")
+    return dev
+
+
 def _aligned(t):
     """t itself, or a copy of it on 16 bytes: the kernels load 16 bytes at a time."""
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
@@ -52,7 +75,7 @@ def _fp32(t):
 
 def _workspace(given, need: int, dev) -> torch.Tensor:
     """The caller's workspace if it is large enough, else one of `need` bytes."""
-    if given is not None and given.numel() * given.element_size() >= need:
+    if given is not None and given.device == dev and given.numel() * given.element_size() >= need:
         return given
     return torch.empty(need, device=dev, dtype=torch.uint8)
 
@@ -656,6 +679,7 @@ def clifford_layer_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor
     return out
 
 
+@_on_its_device
 def clifford_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6,
                                  residual_grad: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """Gradients of :func:`clifford_layer_norm`: ``(dx like x, dgamma (d, 8), dbeta (d, 8))``, the latter fp32.
@@ -663,7 +687,7 @@ def clifford_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch
     dy: the gradient of its output, of x's shape, float32 or bfloat16.  ``residual_grad`` (like x) is added to
     dx before it is rounded: the gradient that reaches x past the norm, as in ``x + f(norm(x))``.
     """
-    dev = _dev(dy, x, gamma, residual_grad)
+    dev = _one_device(dy, x, gamma, residual_grad)
     shape = x.shape
     if len(shape) < 2 or shape[-1] != 8:
         raise ValueError(f"clifford_layer_norm_backward: x must be (..., d, 8), got {tuple(shape)}")
@@ -746,6 +770,7 @@ def adjoint_weights(w: torch.Tensor) -> torch.Tensor:
     return out
 
 
+@_on_its_device
 def prepare_adjoint_weights(w: torch.Tensor, fmt: str = "pauli_f32") -> PreparedWeights:
     """``prepare_weights(adjoint_weights(w), fmt)`` in one pass. w: (E, d_out, d_in, 8) fp32; fmt 'pauli_f32' or
     'pauli' (bf16; d_out even)."""
@@ -776,13 +801,14 @@ def grouped_weight_grad(dy: torch.Tensor, a: torch.Tensor, offsets: torch.Tensor
     return dW, db
 
 
+@_on_its_device
 def grouped_weight_grad_pauli(dy_pauli: torch.Tensor, a_pauli: torch.Tensor, offsets: torch.Tensor, E: int,
                               gather: torch.Tensor | None = None, with_bias: bool = True,
                               workspace: torch.Tensor | None = None):
     """:func:`grouped_weight_grad` on the MFMA units, from fp32 Pauli rows (:func:`pauli_rows_from_blade_f32`) of
     dy (P, d_out, 2, 2, 2) and a (.., d_in, 2, 2, 2), or from bf16 Pauli half-rows
     (:func:`pauli_rows_from_blade`) of dy (P, 2, d_out, 4) and a (.., 2, d_in, 4)."""
-    dev = _dev(dy_pauli, a_pauli, offsets, gather)
+    dev = _one_device(dy_pauli, a_pauli, offsets, gather)
     if dy_pauli.dtype == torch.bfloat16 and a_pauli.dtype == torch.bfloat16:
         return _grouped_weight_grad_bf16(dev, dy_pauli, a_pauli, offsets, E, gather, with_bias, workspace)
     for t in (dy_pauli, a_pauli):
@@ -831,6 +857,7 @@ def _grouped_weight_grad_bf16(dev, dy, a, offsets, E, gather, with_bias, workspa
     return dW, db
 
 
+@_on_its_device
 def pauli_grouped_input_grad(dy_pauli: torch.Tensor, pw_adj: PreparedWeights, offsets: torch.Tensor,
                              h_pre: torch.Tensor | None = None, act: str = "none", y_layout: str = "blade",
                              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -848,7 +875,7 @@ def pauli_grouped_input_grad(dy_pauli: torch.Tensor, pw_adj: PreparedWeights, of
         raise ValueError(f"act must be one of {tuple(ACT_CODE)}")
     if y_layout not in Y_LAYOUT:
         raise ValueError("y_layout must be 'blade' or 'pauli'")
-    dev = _dev(dy_pauli, offsets, h_pre)
+    dev = _one_device(dy_pauli, offsets, h_pre)
     dy_pauli = _half_rows("dy_pauli", dy_pauli)
     P, d_out, d_in, E = dy_pauli.shape[0], dy_pauli.shape[2], pw_adj.d_out, pw_adj.E
     if d_out != pw_adj.d_in:
@@ -878,10 +905,11 @@ def _check_slots(topk_idx, topk_w, dtopk_w):
     return topk_idx.shape
 
 
+@_on_its_device
 def route_backward(topk_idx: torch.Tensor, topk_w: torch.Tensor, dtopk_w: torch.Tensor, E: int) -> torch.Tensor:
     """Gradient of the logits (N, E) from that of the routing weights of :func:`route`, all (N, k): the
     chosen experts' softmax weights are functions of their own logits alone, the choice is a constant."""
-    dev = _dev(topk_idx, topk_w, dtopk_w)
+    dev = _one_device(topk_idx, topk_w, dtopk_w)
     Nt, k = _check_slots(topk_idx, topk_w, dtopk_w)
     dlogits = torch.empty((Nt, E), device=dev, dtype=torch.float32)
     check(lib().ygg_route_backward(topk_idx.data_ptr(), topk_w.data_ptr(), dtopk_w.data_ptr(), Nt, E, k,
@@ -889,11 +917,12 @@ def route_backward(topk_idx: torch.Tensor, topk_w: torch.Tensor, dtopk_w: torch.
     return dlogits
 
 
+@_on_its_device
 def route_energy_backward(x: torch.Tensor, router_weight: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
                           dtopk_w: torch.Tensor, dx_add: torch.Tensor | None = None):
     """Gradients of :func:`route_energy`: ``(dx like x, drouter_weight (E, 4), drouter_bias (E,))`` from that of its
     routing weights (N, k).  ``dx_add`` (like x) is added to dx before it is rounded."""
-    dev = _dev(x, router_weight, topk_idx, topk_w, dtopk_w, dx_add)
+    dev = _one_device(x, router_weight, topk_idx, topk_w, dtopk_w, dx_add)
     if x.dim() != 3 or x.shape[2] != 8:
         raise ValueError(f"route_energy_backward: x must be (N, d, 8), got {tuple(x.shape)}")
     Nt, d = x.shape[:2]
@@ -1003,13 +1032,14 @@ def moe_forward_train(x: torch.Tensor, k: int, w_up: PreparedWeights, w_down: Pr
     return out, dict(topk_idx=topk_idx, topk_w=topk_w, counts=counts, offsets=offsets), h_pre
 
 
+@_on_its_device
 def moe_forward_train_bf16(x: torch.Tensor, k: int, w_up: PreparedWeights, w_down: PreparedWeights,
                            b_up: torch.Tensor | None = None, b_down: torch.Tensor | None = None, act: str = "gelu",
                            logits: torch.Tensor | None = None, router_weight: torch.Tensor | None = None,
                            router_bias: torch.Tensor | None = None, residual: torch.Tensor | None = None):
     """:func:`moe_forward` for a training step of a bf16 layer ('pauli' weights): ``(out, routing, saved)`` with the
     rows that :func:`moe_backward_bf16` reads in ``saved`` (uint8)."""
-    dev = _dev(x, logits, residual, router_weight, router_bias, b_up, b_down)
+    dev = _one_device(x, logits, residual, router_weight, router_bias, b_up, b_down)
     if w_up.fmt != "pauli" or w_down.fmt != "pauli" or x.dtype != torch.bfloat16:
         raise ValueError("moe_forward_train_bf16: bf16 layers with 'pauli' weights")
     if x.dim() != 3 or x.shape[2] != 8:
@@ -1036,6 +1066,7 @@ def moe_forward_train_bf16(x: torch.Tensor, k: int, w_up: PreparedWeights, w_dow
     return out, r.arrays(), saved
 
 
+@_on_its_device
 def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_up_adj: PreparedWeights,
                       w_down_adj: PreparedWeights, act: str = "gelu", residual: bool = False, routing_grad: bool = False):
     """Backward of :func:`moe_forward_train_bf16`: ``(dx, dW_up, db_up, dW_down, db_down, dtopk_w or None)``.
@@ -1043,7 +1074,7 @@ def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_
     ``saved`` and ``routing`` as the forward returned them, the adjoint weights from
     ``prepare_adjoint_weights(w, "pauli")``; dout and dx (N, d, 8) bf16, the weights' gradients fp32."""
     topk_w, offsets = routing["topk_w"], routing["offsets"]
-    dev = _dev(dout, saved, topk_w, offsets)
+    dev = _one_device(dout, saved, topk_w, offsets)
     if w_up_adj.fmt != "pauli" or w_down_adj.fmt != "pauli" or dout.dtype != torch.bfloat16:
         raise ValueError("moe_backward_bf16: bf16 dout and adjoint weights prepared as 'pauli'")
     E, d, F = w_up_adj.E, w_up_adj.d_out, w_up_adj.d_in
