@@ -437,8 +437,8 @@ int ygg_clifford_layer_norm(const void* x, int x_dtype, int N, int d, const floa
  *   dx = (gx - x_hat <gx, x_hat> / d) / rms with gx_i = ~gamma_i dy_i (plus residual_grad,
  *        of x's type, when not NULL), of x's type;
  *   dgamma_i = sum over the tokens of dy_i ~x_hat_i, dbeta_i = sum of dy_i, fp32 (d, 8),
- * sums in fp32 and in an order that the sizes alone fix.  dx may be dy or residual_grad
- * where the types are the same. */
+ * sums in fp32 and in an order that the sizes alone fix.  Where the types are the same dx may
+ * be residual_grad, and up to d = 1024 dy. */
 size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d);
 int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int N, int d,
                                      const float* gamma, double eps, const void* residual_grad, void* dx, float* dgamma,

@@ -386,3 +386,58 @@ def test_two_steps_at_once():
     for i in (0, 1):
         got = torch.autograd.grad(outs[i].float().sum(), [xs[i], m.moe.w_up, m.ffn_norm.gamma, m.moe.router_weight])
         assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+
+
+@pytest.mark.parametrize("block", [False, True])
+def test_layouts_of_a_capture_stay_in_its_graph(block):
+    """Weights first laid out in a capture: an eager call before any replay lays them out for itself."""
+    g = np.random.default_rng(13)
+    m = _layer(g, 16, 24, 4, 2, torch.bfloat16, block=block)
+    x = _tokens(g, 1, 20, 16, torch.bfloat16)
+    run = (lambda: m(x)) if block else (lambda: m.moe_forward(x))
+    say(f"weights first laid out in a capture, block={block}")
+    run()
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(1.25)
+    other = _layer(np.random.default_rng(13), 16, 24, 4, 2, torch.bfloat16, block=block)
+    other.load_state_dict(m.state_dict())
+    want = other(x) if block else other.moe_forward(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run().detach()
+    assert torch.equal(run(), want)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(run(), want)
+
+
+@pytest.mark.parametrize("which", ["layer", "block", "norm"])
+def test_capture_refused_while_an_eager_graph_lives(which):
+    """Refused on the host; without the eager graph the same step is captured."""
+    y = _pkg()
+    g = np.random.default_rng(14)
+    x = _tokens(g, 1, 20, 16, torch.bfloat16)
+    if which == "norm":
+        m = y.CliffordLayerNorm(16, device="cuda", grad=True)
+    else:
+        m = _layer(g, 16, 24, 4, 2, torch.bfloat16, block=which == "block")
+    run = (lambda: m.moe_forward(x)) if which == "layer" else (lambda: m(x))
+    say(f"a capture beside an eager graph of the {which}")
+    alive = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            run()
+    want = alive.detach().clone()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run().detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -380,3 +380,33 @@ def test_operands_off_their_alignment():
               lambda s: ops.clifford_layer_norm_backward(s(x), s(x), s(gamma), residual_grad=s(x)),
               lambda s: ops.route_energy_backward(s(x), s(rw), r.topk_idx, r.topk_w, gw, dx_add=s(x))):
         assert all(torch.equal(p, q) for p, q in zip(f(shifted), f(lambda t: t)))
+
+
+@pytest.mark.parametrize("d", [36, 300, 1024, 1100])
+def test_outputs_in_place(d):
+    """dx in the place of dy or of the gradient that it adds."""
+    from yggdrasil_amd import _native as N
+
+    ops, L = _ops(), N.lib()
+    g = np.random.default_rng(d)
+    x, dy, res = (_dev(g.standard_normal((9, d, 8)).astype(np.float32)) for _ in range(3))
+    gamma = _dev(g.standard_normal((d, 8)).astype(np.float32))
+    say(f"outputs in place of inputs d={d}")
+    want = ops.clifford_layer_norm_backward(dy, x, gamma, residual_grad=res)
+    ws = torch.empty(L.ygg_clifford_layer_norm_backward_workspace_bytes(9, d), device="cuda", dtype=torch.uint8)
+    for which in ("res", "dy")[:2 if d <= 1024 else 1]:
+        a, r, dg, db = dy.clone(), res.clone(), torch.empty_like(gamma), torch.empty_like(gamma)
+        dx = r if which == "res" else a
+        N.check(L.ygg_clifford_layer_norm_backward(a.data_ptr(), 0, x.data_ptr(), 0, 9, d, gamma.data_ptr(), 1e-6,
+                                                   r.data_ptr(), dx.data_ptr(), dg.data_ptr(), db.data_ptr(),
+                                                   ws.data_ptr(), ws.numel(), N.stream_handle(x.device)), "norm")
+        assert all(torch.equal(p, q) for p, q in zip((dx, dg, db), want))
+    rw, gw = _dev(g.standard_normal((5, 4)).astype(np.float32)), _dev(g.standard_normal((9, 2)).astype(np.float32))
+    r = ops.route(_dev(g.standard_normal((9, 5)).astype(np.float32)), 2)
+    want = ops.route_energy_backward(x, rw, r.topk_idx, r.topk_w, gw, dx_add=res)
+    dx, dw, db = res.clone(), torch.empty_like(rw), torch.empty(5, device="cuda")
+    ws = torch.empty(L.ygg_route_energy_backward_workspace_bytes(9, 5), device="cuda", dtype=torch.uint8)
+    N.check(L.ygg_route_energy_backward(x.data_ptr(), 0, 9, d, rw.data_ptr(), 5, 2, r.topk_idx.data_ptr(),
+                                        r.topk_w.data_ptr(), gw.data_ptr(), dx.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+                                        db.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_handle(x.device)), "router")
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), want))

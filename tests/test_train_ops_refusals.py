@@ -29,6 +29,7 @@ def _refused(name, args, word):
     ((P, 0, P, 0, 4, 4, P, -1.0, None, P, P, P, P, 1 << 20, None), "eps"),
     ((P, 0, P, 0, 4, 4, None, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
     ((None, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
+    ((P, 0, P, 0, 4, 1025, P, 1e-6, None, P, P, P, P, 1 << 20, None), "dx is dy"),
     ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 8, None), "workspace"),
     ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, None, 1 << 20, None), "workspace"),
 ])
@@ -165,13 +166,14 @@ def test_launches_go_to_the_tensors_device(monkeypatch):
             self.d = d
 
         def __enter__(self):
-            self.was, current[0] = current[0], self.d.index
+            self.was, current[0] = current[0], self.d
 
         def __exit__(self, *exc):
             current[0] = self.was
 
     class Tensor:
-        is_cuda, device = True, torch.device("cuda", 3)
+        def get_device(self):
+            return 3
 
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch.cuda, "device", Device)
@@ -193,6 +195,9 @@ def test_tensors_of_two_devices_are_refused():
         def __init__(self, n):
             self.device = torch.device("cuda", n)
 
+        def get_device(self):
+            return self.device.index
+
         def is_contiguous(self):
             return True
 
@@ -200,3 +205,56 @@ def test_tensors_of_two_devices_are_refused():
     assert ops._one_device(a, None, a) == a.device
     with pytest.raises(ValueError, match="one device"):
         ops._one_device(a, b)
+
+
+def test_operators_take_their_arguments_by_name():
+    w = torch.zeros(1, 4, 4, 8)
+    with pytest.raises(ValueError, match="GPU only"):
+        ops.prepare_adjoint_weights(w=w)
+    with pytest.raises(ValueError, match="GPU only"):
+        ops.grouped_weight_grad_pauli(E=1, dy_pauli=w, a_pauli=w, offsets=w)
+    with pytest.raises(TypeError):
+        ops.prepare_adjoint_weights()
+
+
+def test_a_workspace_that_does_not_hold_its_bytes_is_not_used():
+    dev = torch.device("cpu")
+    one = torch.empty(256, dtype=torch.uint8)
+    assert ops._workspace(one, 256, dev) is one
+    assert ops._workspace(one, 257, dev).numel() == 257
+    assert ops._workspace(torch.empty(1, dtype=torch.uint8).expand(256), 256, dev).is_contiguous()
+    assert ops._workspace(one[4:], 64, dev).data_ptr() != one[4:].data_ptr()
+    assert ops._workspace(one, 64, torch.device("cuda", 0) if torch.cuda.is_available() else torch.device("meta")) is not one
+
+
+def test_a_capture_is_refused_while_an_eager_graph_lives(monkeypatch):
+    """The graphs are found by their autograd nodes, which live as long as any output does."""
+    from yggdrasil_amd import layers
+
+    capturing, stream = [False], [0]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: stream[0])
+
+    class Node(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, w, module):
+            layers._note_graph(ctx, None, module)
+            return 2 * w
+
+        @staticmethod
+        def backward(ctx, g):
+            return 2 * g, None
+
+    a, b = torch.nn.Linear(2, 2), torch.nn.Linear(2, 2)
+    loss = Node.apply(a.weight, a).sum()
+    loss.backward()
+    capturing[0] = True
+    Node.apply(b.weight, b)
+    with pytest.raises(RuntimeError, match="still alive"):
+        Node.apply(a.weight, a)
+    del loss
+    Node.apply(a.weight, a)
+    capturing[0], stream[0] = False, 7  # a graph of another stream can join a capture
+    loss = Node.apply(a.weight, a).sum()
+    capturing[0] = True
+    Node.apply(a.weight, a)

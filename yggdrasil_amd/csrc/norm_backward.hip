@@ -372,6 +372,8 @@ YGG_API int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const
   YGG_CHECK_ARG(eps >= 0.0, "ygg_clifford_layer_norm_backward: eps must be non-negative");
   YGG_CHECK_ARG(gamma && dgamma && dbeta && (N == 0 || (dy && x && dx)),
                 "ygg_clifford_layer_norm_backward: null pointer argument");
+  YGG_CHECK_ARG(N == 0 || d <= kNbFusedMaxD || dx != dy,
+                "ygg_clifford_layer_norm_backward: dx is dy, which d=%d reads again (d <= %d)", d, kNbFusedMaxD);
   const size_t need = ygg_clifford_layer_norm_backward_workspace_bytes(N, d);
   YGG_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                 "ygg_clifford_layer_norm_backward: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0,

@@ -17,6 +17,7 @@ There is no CPU path.
 from __future__ import annotations
 
 import math
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -217,7 +218,8 @@ class CliffordMoELayer(nn.Module):
         N, E = B * T, cfg.n_experts
         if not x.is_contiguous():
             x = x.contiguous()
-        prep = self._get_prepared()
+        graph = self._needs_grad(x, residual, logits)
+        prep = _step_layouts(self) if graph else self._get_prepared()
         if cfg.router == "logits":
             if logits is None:
                 raise ValueError("router='logits' needs logits")
@@ -235,12 +237,12 @@ class CliffordMoELayer(nn.Module):
         ws = self.__dict__["_workspace"]
         if ws is None or ws.numel() < ws_bytes or ws.device != x.device:
             ws = self.__dict__["_workspace"] = torch.empty((max(ws_bytes, 1),), device=x.device, dtype=torch.uint8)
-        if self._needs_grad(x, residual, logits):
+        if graph:
             flat = x.reshape(N, d, 8)
             res = residual.reshape(N, d, 8) if residual is not None else None
             lg = logits.reshape(N, E) if logits is not None else None
             return _MoEFunction.apply(flat, res, self.w_up, self.b_up, self.w_down, self.b_down, self.router_weight,
-                                      self.router_bias, self, lg).reshape(B, T, d, 8)
+                                      self.router_bias, self, prep, lg).reshape(B, T, d, 8)
         rw = rb = None
         if logits is None:
             rw, rb = self.router_weight.detach(), self.router_bias.detach()
@@ -325,9 +327,34 @@ def _in_capture(layer, block: bool) -> bool:
     return (block or layer.cfg.bf16_grad) and torch.cuda.is_current_stream_capturing()
 
 
-def _train_forward(layer, flat, res, logits, workspace=None, block=False):
+@torch.no_grad()
+def _step_layouts(layer, block: bool = False) -> dict:
+    """The weight layouts of a training step's forward.  Those of a capture are the graph's own: nothing else finds
+    them, since they hold values only after a replay."""
+    return layer._layouts() if _in_capture(layer, block) else layer._get_prepared()
+
+
+# The eager graphs of each module that gets gradients through a node of its own, made on the default stream and
+# still alive
+_eager_graphs = weakref.WeakKeyDictionary()
+
+
+def _note_graph(ctx, dev, *modules) -> None:
+    """Refuses to capture a training step while an eager graph of the same parameters lives.  autograd then adds the
+    captured gradients on the stream of the eager graph; on the default stream, which no capture may use, that ends
+    the process."""
+    if torch.cuda.is_current_stream_capturing():
+        if any(_eager_graphs.get(m) for m in modules):
+            raise RuntimeError("a graph of this module made outside the capture is still alive: delete its outputs (and "
+                               "losses made of them) before capturing a training step")
+    elif ops.stream_handle(dev) == 0:
+        for m in modules:
+            _eager_graphs.setdefault(m, weakref.WeakSet()).add(ctx)
+
+
+def _train_forward(layer, flat, res, logits, prep, workspace=None):
     """The layer's forward for a training step: ``(out, kept)``, what the backward reads in ``kept``."""
-    cfg, prep = layer.cfg, layer._layouts() if _in_capture(layer, block) else layer._get_prepared()
+    cfg = layer.cfg
     rw = layer.router_weight.detach() if logits is None else None
     rb = layer.router_bias.detach() if logits is None else None
     if cfg.weight_format == "pauli_f32":
@@ -384,9 +411,11 @@ class _MoEFunction(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, logits):
+    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, prep, logits):
         ctx.layer, ctx.has_res, ctx.has_logits = layer, res is not None, logits is not None
-        out, kept = _train_forward(layer, flat, res, logits, workspace=layer._workspace)
+        if layer.cfg.bf16_grad:
+            _note_graph(ctx, flat.device, layer)
+        out, kept = _train_forward(layer, flat, res, logits, prep, workspace=layer._workspace)
         ctx.versions = layer._param_versions() if layer.cfg.bf16_grad else None
         ctx.save_for_backward(flat, logits if logits is not None else flat.new_empty(0), *kept)
         return out
@@ -397,7 +426,7 @@ class _MoEFunction(torch.autograd.Function):
         _check_versions(ctx.layer, ctx.versions)
         dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
             ctx.layer, flat, logits if ctx.has_logits else None, kept, dout, residual=False)
-        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, dlogits
+        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, dlogits
 
 
 class CliffordLinear(nn.Module):
@@ -449,7 +478,7 @@ class CliffordLayerNorm(nn.Module):
         # (a norm saved before it could have a graph has no `grad`)
         if self.__dict__.get("grad", False) and torch.is_grad_enabled() and any(
                 t.requires_grad for t in (x, self.gamma, self.beta)):
-            return _NormFunction.apply(x, self.gamma, self.beta, self.eps, out_dtype)
+            return _NormFunction.apply(x, self.gamma, self.beta, self, out_dtype)
         return ops.clifford_layer_norm(x.contiguous(), self.gamma.detach(), self.beta.detach(), self.eps,
                                        out_dtype=out_dtype)
 
@@ -458,11 +487,12 @@ class _NormFunction(torch.autograd.Function):
     """CliffordLayerNorm as one autograd node."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, eps, out_dtype):
+    def forward(ctx, x, gamma, beta, norm, out_dtype):
         x = x.contiguous()
+        _note_graph(ctx, x.device, norm)
         ctx.save_for_backward(x, gamma)
-        ctx.eps, ctx.beta_dtype = eps, beta.dtype
-        return ops.clifford_layer_norm(x, gamma, beta, eps, out_dtype=out_dtype)
+        ctx.eps, ctx.beta_dtype = norm.eps, beta.dtype
+        return ops.clifford_layer_norm(x, gamma, beta, norm.eps, out_dtype=out_dtype)
 
     @staticmethod
     @once_differentiable
@@ -570,12 +600,14 @@ class _BlockFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, w_up, b_up, w_down, b_down, router_weight, router_bias, block, logits):
         moe = block.moe
+        _note_graph(ctx, x.device, moe, block.ffn_norm)
+        prep = _step_layouts(moe, block=True)
         xn = ops.clifford_layer_norm(x, gamma, beta, block.ffn_norm.eps)
-        ctx.block, ctx.from_caller, ctx.beta_dtype = block, logits is not None, beta.dtype
+        ctx.block, ctx.from_caller, ctx.beta_dtype, ctx.eps = block, logits is not None, beta.dtype, block.ffn_norm.eps
         if logits is None and block.cfg.router == "clifford_head":  # (a constant of the backward)
-            logits = moe._head_logits(xn, moe._get_prepared())
+            logits = moe._head_logits(xn, prep)
         ctx.has_logits = logits is not None
-        out, kept = _train_forward(moe, xn, x, logits, block=True)
+        out, kept = _train_forward(moe, xn, x, logits, prep)
         ctx.versions = moe._param_versions()
         ctx.save_for_backward(x, gamma, xn, logits if logits is not None else x.new_empty(0), *kept)
         return out
@@ -588,6 +620,6 @@ class _BlockFunction(torch.autograd.Function):
         dout = dout.contiguous()
         dxn, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
             ctx.block.moe, xn, logits if ctx.has_logits else None, kept, dout, residual=False, block=True)
-        dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.block.ffn_norm.eps, residual_grad=dout)
+        dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.eps, residual_grad=dout)
         return (dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), dWu, dbu, dWd, dbd, drw, drb, None,
                 dlogits if ctx.from_caller else None)

@@ -46,22 +46,28 @@ def _on_its_device(fn):
     """An operator whose launches go to the device of its first tensor, whichever is current."""
 
     @functools.wraps(fn)
-    def call(first, *args, **kwargs):
-        if first.is_cuda and torch._C._cuda_getDevice() != first.device.index:
-            with torch.cuda.device(first.device):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
+    def call(*args, **kwargs):
+        first = args[0] if args else next((v for v in kwargs.values() if hasattr(v, "get_device")), None)
+        try:
+            at = first.get_device()
+        except AttributeError:  # no tensor: the operator says what it needs
+            at = -1
+        if at >= 0 and torch._C._cuda_getDevice() != at:
+            with torch.cuda.device(at):
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
 
     return call
 
 
 def _one_device(*tensors):
     """:func:`_dev`, with every tensor on the first one's device."""
-    dev = _dev(*tensors)
+    at = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
+        if t is not None and (t.get_device() != at or at < 0 or not t.is_contiguous()):
+            dev = _dev(*tensors)
             raise ValueError(f"tensors on {dev} and {t.device}: an operator takes them on one device")
-    return dev
+    return tensors[0].device
 
 
 def _aligned(t):
@@ -74,8 +80,9 @@ def _fp32(t):
 
 
 def _workspace(given, need: int, dev) -> torch.Tensor:
-    """The caller's workspace if it is large enough, else one of `need` bytes."""
-    if given is not None and given.device == dev and given.numel() * given.element_size() >= need:
+    """The caller's workspace if it is one piece, on 16 bytes and large enough, else one of `need` bytes."""
+    if (given is not None and given.device == dev and given.is_contiguous() and given.data_ptr() % 16 == 0 and
+            given.numel() * given.element_size() >= need):
         return given
     return torch.empty(need, device=dev, dtype=torch.uint8)
 
