@@ -85,8 +85,9 @@ __device__ __forceinline__ void zero_tile(int jt, int it, int e, int d_in, int d
 // One workgroup: 64 (j) x 64 (i) of one chunk's sum, a wave 32 x 32 of it.
 //
 // Bound by the matrix units and the loads into LDS together: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's
-// law take 163 us in all, 145 here and 18 in the planes' sum: 137 GFLOP at 0.95 PFLOP/s here, where a large bf16
-// product reaches 1.37.  Without the loads (data in LDS as it was) the whole took 137 us, without the products 133.
+// law take 159 us in all, 140 here and 18 in the planes' sum: 137 GFLOP at 0.98 PFLOP/s here, where a large bf16
+// product reaches 1.37.  The matrix units are busy 48 % of the time: of the two waves that a SIMD holds 1.4 are there
+// on average, as the chunks of uneven experts do not end together.  Without the loads (data in LDS as it was) the whole took 137 us, without the products 133.
 // Larger tiles did not pay: 128 x 64 with eight waves 160 us, with four waves of 64 x 32, one a SIMD, 179; nor did
 // reading the next stage's operands into registers ahead (160) or raising the waves' priority (174).
 //
@@ -109,8 +110,10 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   const int32_t* const gather = GATHER ? gather_rows : nullptr;
   const int tid = threadIdx.x, lane = tid & 63;
   const int nj = (d_out + kWbTile - 1) / kWbTile, ni = (d_in + kWbTile - 1) / kWbTile, nt = nj * ni;
-  // all tiles of a chunk on one XCD (workgroup b runs on XCD b mod 8): its rows are read into one L2
-  const int bq = blockIdx.x / n_xcd, chunk = bq / nt * n_xcd + (blockIdx.x - bq * n_xcd), tile = bq % nt;
+  // all tiles of a chunk on one XCD (workgroup b runs on XCD b mod 8): its rows are read into one L2.  The chunks
+  // fall in length, so every second round of them goes over the XCDs backwards (Zipf's law as above: 162 -> 159 us).
+  const int bq = blockIdx.x / n_xcd, round = bq / nt, tile = bq - round * nt, xcd = blockIdx.x - bq * n_xcd;
+  const int chunk = round * n_xcd + ((round & 1) ? n_xcd - 1 - xcd : xcd);
   const WbExpert x = wb_experts(offsets, E, P, limit, lane);
   // the chunks in order of falling length, so that the last to start are short: this lane's expert's first one
   const int planes = wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), key = x.len * 64 + 63 - lane;
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   uint32_t d_next = (uint32_t)((lane >> 5) * d_out + j0 + col) * 8 + (uint32_t)(kWbWaveRows * wave) * d_out * 16;
   uint32_t a_next = a_lane + (uint32_t)(kWbWaveRows * wave) * a_row;  // (rows in place)
   const uint32_t lds0 = (uint32_t)(uintptr_t)(sp_lds_t*)smem + kWbWaveRows * wave * 2 * kWbHalf;
-  uint32_t src[kWbWaveRows] = {};  // gathered: the offsets of the next stage's two rows
+  uint32_t src[kWbWaveRows] = {};  // gathered: the offsets of the next stage's rows
   auto next_src = [&](int f) __attribute__((always_inline)) {
     if constexpr (GATHER) {
 #pragma unroll
@@ -385,7 +388,8 @@ YGG_API int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void*
                 "d_out)", P_max, E, d_in, d_out);
   YGG_CHECK_ARG(a_rows >= 0 && (gather != nullptr || a_rows >= P_max),
                 "ygg_grouped_weight_grad_pauli_bf16: a has %d rows, %d are read without a gather", a_rows, P_max);
-  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) <= 0x7fffffffLL && (long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 < 1LL << 31,
+  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) < 1LL << 24 &&
+                    (long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 < 1LL << 31,
                 "ygg_grouped_weight_grad_pauli_bf16: P_max=%d d_in=%d d_out=%d exceed a launch", P_max, d_in, d_out);
   YGG_CHECK_ARG(gather == nullptr || (long long)a_rows * d_in * 16 < 1LL << 31,
                 "ygg_grouped_weight_grad_pauli_bf16: gathered rows span 2 GiB or more (a_rows=%d d_in=%d)", a_rows, d_in);
