@@ -6,6 +6,8 @@ token dispatch, grouped CliffordLinear expert products with the grade-wise
 activation fused, and the weighted combine, behind the C ABI declared in
 ``include/ygg_moe.h`` and the torch module ``CliffordMoELayer``; the pre-norm
 and residual around it (``hlm_block.py:144-151``) as ``CliffordMoEBlockFFN``.
+fp32 layers train through autograd; bf16 layers, the router, the norm and the
+block do so on request (``bf16_grad``, ``router_grad``, ``grad``).
 """
 
 from .layers import (CliffordLayerNorm, CliffordLinear, CliffordMoEBlockFFN, CliffordMoELayer,  # noqa: F401
