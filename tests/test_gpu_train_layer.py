@@ -441,3 +441,22 @@ def test_capture_refused_while_an_eager_graph_lives(which):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_tokens_changed_before_the_backward():
+    """A bf16 layer's backward reads its tokens for the router's gradient alone: elsewhere they may be overwritten."""
+    g = np.random.default_rng(15)
+    x = _tokens(g, 1, 20, 16, torch.bfloat16)
+    dout = _tokens(g, 1, 20, 16, torch.bfloat16)
+    for more in (dict(), dict(router_grad=True)):
+        m = _layer(g, 16, 24, 4, 2, torch.bfloat16, **more)
+        say(f"tokens overwritten after the forward {more}")
+        want = torch.autograd.grad(m.moe_forward(x.clone()), [m.w_up, m.w_down], dout)
+        y = x.clone()
+        out = m.moe_forward(y)
+        y.zero_()
+        if more:
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad(out, [m.w_up, m.w_down], dout)
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [m.w_up, m.w_down], dout), want))

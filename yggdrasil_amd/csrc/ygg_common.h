@@ -285,8 +285,7 @@ int dispatch_backward(const float* dxs, int N, int k, int d, const int32_t* slot
 
 // The bf16 layer's training pieces.  pauli_gemm.hip: the up product (Pauli half-rows gathered, h as
 // Pauli half-rows) that also keeps its blade rows before the activation (act 0: h alone).
-// weight_grad_bf16.hip: ygg_grouped_weight_grad_pauli_bf16 without its checks.  train_bf16.hip: the
-// combine's backward (dy as Pauli half-rows; dtopk_w when not NULL) and the dispatch's, on bf16 rows.
+// weight_grad_bf16.hip: ygg_grouped_weight_grad_pauli_bf16 without its checks.
 int pauli_linear_save_pre(const void* x, int x_rows, const int32_t* gather, int P, const void* w, const float* bias,
                           const int32_t* offsets, int E, int d_in, int d_out, int act, void* h, void* h_pre,
                           hipStream_t stream);

@@ -375,6 +375,14 @@ def _check_versions(layer, versions) -> None:
         raise RuntimeError("the layer's parameters were modified in place between its forward and its backward")
 
 
+def _for_backward(layer, flat, logits):
+    """The tokens and the caller's logits where the backward reads them, and empty tensors where it does not (a bf16
+    layer keeps rows of its own; its tokens are read for the router's gradient alone)."""
+    fp32 = layer.cfg.weight_format == "pauli_f32"
+    return (flat if fp32 or (layer.cfg.router_grad and logits is None) else flat.new_empty(0),
+            logits if fp32 and logits is not None else flat.new_empty(0))
+
+
 def _train_backward(layer, flat, logits, kept, dout, residual: bool, block=False):
     """Gradients of :func:`_train_forward`: ``(dx, dW_up, db_up, dW_down, db_down, drouter_weight, drouter_bias,
     dlogits)``, the last three None where the router gets none.  ``residual``: dx includes dout (bf16 layers)."""
@@ -417,7 +425,7 @@ class _MoEFunction(torch.autograd.Function):
             _note_graph(ctx, flat.device, layer)
         out, kept = _train_forward(layer, flat, res, logits, prep, workspace=layer._workspace)
         ctx.versions = layer._param_versions() if layer.cfg.bf16_grad else None
-        ctx.save_for_backward(flat, logits if logits is not None else flat.new_empty(0), *kept)
+        ctx.save_for_backward(*_for_backward(layer, flat, logits), *kept)
         return out
 
     @staticmethod
@@ -609,7 +617,7 @@ class _BlockFunction(torch.autograd.Function):
         ctx.has_logits = logits is not None
         out, kept = _train_forward(moe, xn, x, logits, prep)
         ctx.versions = moe._param_versions()
-        ctx.save_for_backward(x, gamma, xn, logits if logits is not None else x.new_empty(0), *kept)
+        ctx.save_for_backward(x, gamma, *_for_backward(moe, xn, logits), *kept)
         return out
 
     @staticmethod
