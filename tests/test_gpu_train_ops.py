@@ -64,6 +64,7 @@ WEIGHT_CASES = [
     ([1] * 64, 16, 20, True, True),
     ([1300, 0, 513, 512], 6, 10, True, True),  # experts of several chunks of rows
     ([0, 1025], 70, 66, False, True),
+    ([0 if e % 5 == 0 else e * 37 % 90 for e in range(62)] + [700, 1100], 10, 6, True, True),
 ]
 
 

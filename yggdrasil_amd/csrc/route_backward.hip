@@ -256,7 +256,7 @@ YGG_API int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, 
     else by_width(static_cast<const uint16_t*>(x));
     if (check_launch("ygg_route_energy_backward")) return -1;
   }
-  hipLaunchKernelGGL(router_param_kernel, dim3((5 * E + 31) / 32), dim3(1024), 0, stream, part, N > 0 ? route_planes(N) : 0, E, drouter_w,
-                     drouter_b);
+  hipLaunchKernelGGL(router_param_kernel, dim3((5 * E + 31) / 32), dim3(1024), 0, stream, part,
+                     N > 0 ? route_planes(N) : 0, E, drouter_w, drouter_b);
   return check_launch("ygg_route_energy_backward (parameters)");
 }

@@ -30,6 +30,24 @@ constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a s
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
 
+// Inclusive scans over the wave by DPP moves (rows of 16 lanes, then each row's last lane to the next rows): a
+// quarter of the latency of six exchanges through LDS, of which a workgroup waits for three one after another.
+template <bool MAX>
+__device__ __forceinline__ int wave_scan(int v) {
+  auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    const int u = __builtin_amdgcn_update_dpp(MAX ? v : 0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v = MAX ? max(v, u) : v + u;
+  };
+  typedef std::integral_constant<int, 0xf> all;
+  step(std::integral_constant<int, 0x111>{}, all{});  // row_shr:1, 2, 4, 8
+  step(std::integral_constant<int, 0x112>{}, all{});
+  step(std::integral_constant<int, 0x114>{}, all{});
+  step(std::integral_constant<int, 0x118>{}, all{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 into rows 1 and 3
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // Lane e: the rows of expert e and their chunks, n = ceil(rows / limit) of equal length (a multiple of a
 // stage's rows).  Whatever `offsets` holds, the ranges are inside [0, P] and disjoint: every bound is
 // clamped and at least the one before it.
@@ -38,25 +56,12 @@ struct WbExpert {
 };
 __device__ __forceinline__ WbExpert wb_experts(const int32_t* __restrict__ offsets, int E, int P, int limit,
                                                int lane) {
-  int beg = min(max(offsets[min(lane, E)], 0), P);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(beg, o);
-    if (lane >= o) beg = max(beg, u);
-  }
+  const int beg = wave_scan<true>(min(max(offsets[min(lane, E)], 0), P));
   WbExpert x = {beg, max(beg, min(offsets[min(lane + 1, E)], P)), 0, 0};
   if (lane >= E) x.end = x.beg;
   x.n = (x.end - x.beg + limit - 1) / limit;
   x.len = x.n > 0 ? ((x.end - x.beg + x.n - 1) / x.n + kWbRows - 1) / kWbRows * kWbRows : 0;
   return x;
-}
-__device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
 }
 
 __device__ __forceinline__ float swap_pair(float v) {  // the value of the neighbouring lane (lane ^ 1)
@@ -87,9 +92,11 @@ __device__ __forceinline__ void zero_tile(int jt, int it, int e, int d_in, int d
 // Bound by the matrix units and the loads into LDS together: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's
 // law take 159 us in all, 140 here and 18 in the planes' sum: 137 GFLOP at 0.98 PFLOP/s here, where a large bf16
 // product reaches 1.37.  The matrix units are busy 48 % of the time: of the two waves that a SIMD holds 1.4 are there
-// on average, as the chunks of uneven experts do not end together.  Without the loads (data in LDS as it was) the whole took 137 us, without the products 133.
-// Larger tiles did not pay: 128 x 64 with eight waves 160 us, with four waves of 64 x 32, one a SIMD, 179; nor did
-// reading the next stage's operands into registers ahead (160) or raising the waves' priority (174).
+// on average, as the chunks of uneven experts do not end together.  Without the loads (data in LDS as it was) the
+// whole took 137 us, without the products 133.  Larger tiles did not pay: 128 x 64 with eight waves 160 us, with four
+// waves of 64 x 32, one a SIMD, 179; nor did eight waves on one tile, half of a chunk's rows each (157, and half the
+// planes, but one tile a CU: 1500 ragged tokens as below 26-30 us against 27), reading the next stage's operands
+// into registers ahead (160) or raising the waves' priority (174).
 //
 // v_mfma_f32_32x32x16_bf16 with the operand rows (j, a) and columns (i, c), 16 of each index: the dword
 // (re, im) of entry a of column b of D_rj is one (r, b) term of the contraction, and four such dwords (two
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   const int chunk = round * n_xcd + ((round & 1) ? n_xcd - 1 - xcd : xcd);
   const WbExpert x = wb_experts(offsets, E, P, limit, lane);
   // the chunks in order of falling length, so that the last to start are short: this lane's expert's first one
-  const int planes = wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), key = x.len * 64 + 63 - lane;
+  const int planes = wave_scan<false>(x.n > 1 ? x.n : 0), key = x.len * 64 + 63 - lane;
   int first = 0;
   for (int i = 0; i < E; ++i) {
     const int k = __builtin_amdgcn_readlane(key, i), m = __builtin_amdgcn_readlane(x.n, i);
@@ -125,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   const uint64_t mine = __ballot(lane < E && chunk >= first && chunk < first + x.n);
   if (mine == 0) {  // behind the chunks: the experts without rows, whose gradient is zero
     const uint64_t none = __ballot(lane < E && x.n == 0);
-    const int total = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n, lane), 63);
+    const int total = __builtin_amdgcn_readlane(wave_scan<false>(x.n), 63);
     const int nth = __popcll(none & ((1ull << lane) - 1));  // this lane's place among them
     const uint64_t here = __ballot(lane < E && x.n == 0 && nth == chunk - total);
     if (here != 0) zero_tile(tile % nj, tile / nj, (int)__builtin_ctzll(here), d_in, d_out, dW, db, tid);
@@ -305,7 +312,7 @@ __global__ __launch_bounds__(256) void weight_grad_bf16_reduce_kernel(const floa
   const WbExpert x = wb_experts(offsets, E, P, limit, lane);
   const int n = __builtin_amdgcn_readlane(x.n, e);
   if (n <= 1) return;
-  const int first = __builtin_amdgcn_readlane(wave_inclusive_sum(x.n > 1 ? x.n : 0, lane), e) - n;
+  const int first = __builtin_amdgcn_readlane(wave_scan<false>(x.n > 1 ? x.n : 0), e) - n;
   const size_t nw = (size_t)d_out * d_in * 2, nb = db != nullptr ? (size_t)d_out * 2 : 0;
   size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= nw + nb) return;
