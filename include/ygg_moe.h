@@ -404,7 +404,7 @@ int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, const float
 
 /* The same through the grade-energy logits: dx (N, d, 8) of x's type (plus dx_add, of the
  * same type, when not NULL; dx may be dx_add), drouter_w (E, 4) and drouter_b (E), fp32. */
-size_t ygg_route_energy_backward_workspace_bytes(int N, int E);
+size_t ygg_route_energy_backward_workspace_bytes(int N, int d, int E, int k);
 int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const float* router_w, int E, int k,
                               const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, const void* dx_add,
                               void* dx, float* drouter_w, float* drouter_b, void* workspace, size_t workspace_bytes,
@@ -437,8 +437,7 @@ int ygg_clifford_layer_norm(const void* x, int x_dtype, int N, int d, const floa
  *   dx = (gx - x_hat <gx, x_hat> / d) / rms with gx_i = ~gamma_i dy_i (plus residual_grad,
  *        of x's type, when not NULL), of x's type;
  *   dgamma_i = sum over the tokens of dy_i ~x_hat_i, dbeta_i = sum of dy_i, fp32 (d, 8),
- * sums in fp32 and in an order that the sizes alone fix.  Where the types are the same dx may
- * be residual_grad, and up to d = 1024 dy. */
+ * sums in fp32 and in an order that the sizes alone fix.  dx may be residual_grad, not dy. */
 size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d);
 int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int N, int d,
                                      const float* gamma, double eps, const void* residual_grad, void* dx, float* dgamma,

@@ -214,7 +214,9 @@ def test_input_grad_leaves_the_rows_past_the_last_expert():
     (200, 100, "bf16", "bf16", True), (130, 33, "bf16", "f32", False), (31, 129, "f32", "bf16", True),
     (40, 256, "bf16", "bf16", False), (19, 300, "f32", "f32", True), (5, 1000, "bf16", "bf16", True),
     (3, 1025, "bf16", "bf16", False), (2, 4096, "f32", "f32", True), (700, 8, "bf16", "bf16", False),
-    (2500, 16, "f32", "f32", False)])
+    (2500, 16, "f32", "f32", False), (600, 64, "bf16", "bf16", True), (515, 100, "f32", "bf16", False),
+    (300, 256, "bf16", "bf16", True), (150, 300, "f32", "f32", True), (50, 1000, "bf16", "f32", False),
+    (512, 64, "f32", "f32", True), (513, 8, "f32", "f32", False), (32, 1024, "bf16", "bf16", True)])
 @pytest.mark.parametrize("eps", [1e-6, 0.25])
 def test_norm_backward(N, d, dt, gdt, residual, eps):
     ops = _ops()
@@ -253,6 +255,8 @@ def test_norm_backward_of_no_tokens():
     (1, 1, 1, 1, "f32", False), (5, 3, 4, 2, "f32", True), (257, 64, 8, 2, "f32", False), (70, 100, 12, 3, "bf16", True),
     (33, 7, 64, 8, "bf16", False), (1000, 16, 64, 2, "bf16", True), (19, 300, 16, 4, "f32", True), (300, 8, 3, 3, "bf16", False),
     (40, 20, 6, 1, "f32", True), (3000, 2, 5, 2, "f32", False),
+    (400, 100, 64, 8, "bf16", True), (300, 200, 16, 2, "f32", False), (120, 300, 9, 3, "bf16", True),
+    (512, 64, 64, 8, "f32", True), (513, 5, 3, 2, "bf16", False), (2, 2000, 4, 4, "f32", True),
     (40003, 3, 6, 2, "f32", True)])  # (the last: more than a batch a workgroup)
 def test_router_backward(N, d, E, k, dt, add):
     ops = _ops()
@@ -383,31 +387,29 @@ def test_operands_off_their_alignment():
         assert all(torch.equal(p, q) for p, q in zip(f(shifted), f(lambda t: t)))
 
 
-@pytest.mark.parametrize("d", [36, 300, 1024, 1100])
-def test_outputs_in_place(d):
-    """dx in the place of dy or of the gradient that it adds."""
+@pytest.mark.parametrize("n,d", [(9, 36), (700, 36), (9, 300), (300, 300), (9, 1024), (9, 1100)])
+def test_outputs_in_place(n, d):
+    """dx in the place of the gradient that it adds."""
     from yggdrasil_amd import _native as N
 
     ops, L = _ops(), N.lib()
     g = np.random.default_rng(d)
-    x, dy, res = (_dev(g.standard_normal((9, d, 8)).astype(np.float32)) for _ in range(3))
+    x, dy, res = (_dev(g.standard_normal((n, d, 8)).astype(np.float32)) for _ in range(3))
     gamma = _dev(g.standard_normal((d, 8)).astype(np.float32))
-    say(f"outputs in place of inputs d={d}")
+    say(f"outputs in place of inputs n={n} d={d}")
     want = ops.clifford_layer_norm_backward(dy, x, gamma, residual_grad=res)
-    ws = torch.empty(L.ygg_clifford_layer_norm_backward_workspace_bytes(9, d), device="cuda", dtype=torch.uint8)
-    for which in ("res", "dy")[:2 if d <= 1024 else 1]:
-        a, r, dg, db = dy.clone(), res.clone(), torch.empty_like(gamma), torch.empty_like(gamma)
-        dx = r if which == "res" else a
-        N.check(L.ygg_clifford_layer_norm_backward(a.data_ptr(), 0, x.data_ptr(), 0, 9, d, gamma.data_ptr(), 1e-6,
-                                                   r.data_ptr(), dx.data_ptr(), dg.data_ptr(), db.data_ptr(),
-                                                   ws.data_ptr(), ws.numel(), N.stream_handle(x.device)), "norm")
-        assert all(torch.equal(p, q) for p, q in zip((dx, dg, db), want))
-    rw, gw = _dev(g.standard_normal((5, 4)).astype(np.float32)), _dev(g.standard_normal((9, 2)).astype(np.float32))
-    r = ops.route(_dev(g.standard_normal((9, 5)).astype(np.float32)), 2)
+    ws = torch.empty(L.ygg_clifford_layer_norm_backward_workspace_bytes(n, d) + 1, device="cuda", dtype=torch.uint8)
+    dx, dg, db = res.clone(), torch.empty_like(gamma), torch.empty_like(gamma)
+    N.check(L.ygg_clifford_layer_norm_backward(dy.data_ptr(), 0, x.data_ptr(), 0, n, d, gamma.data_ptr(), 1e-6,
+                                               dx.data_ptr(), dx.data_ptr(), dg.data_ptr(), db.data_ptr(), ws.data_ptr(),
+                                               ws.numel(), N.stream_handle(x.device)), "norm")
+    assert all(torch.equal(p, q) for p, q in zip((dx, dg, db), want))
+    rw, gw = _dev(g.standard_normal((5, 4)).astype(np.float32)), _dev(g.standard_normal((n, 2)).astype(np.float32))
+    r = ops.route(_dev(g.standard_normal((n, 5)).astype(np.float32)), 2)
     want = ops.route_energy_backward(x, rw, r.topk_idx, r.topk_w, gw, dx_add=res)
     dx, dw, db = res.clone(), torch.empty_like(rw), torch.empty(5, device="cuda")
-    ws = torch.empty(L.ygg_route_energy_backward_workspace_bytes(9, 5), device="cuda", dtype=torch.uint8)
-    N.check(L.ygg_route_energy_backward(x.data_ptr(), 0, 9, d, rw.data_ptr(), 5, 2, r.topk_idx.data_ptr(),
+    ws = torch.empty(L.ygg_route_energy_backward_workspace_bytes(n, d, 5, 2) + 1, device="cuda", dtype=torch.uint8)
+    N.check(L.ygg_route_energy_backward(x.data_ptr(), 0, n, d, rw.data_ptr(), 5, 2, r.topk_idx.data_ptr(),
                                         r.topk_w.data_ptr(), gw.data_ptr(), dx.data_ptr(), dx.data_ptr(), dw.data_ptr(),
                                         db.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_handle(x.device)), "router")
     assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), want))

@@ -29,9 +29,9 @@ def _refused(name, args, word):
     ((P, 0, P, 0, 4, 4, P, -1.0, None, P, P, P, P, 1 << 20, None), "eps"),
     ((P, 0, P, 0, 4, 4, None, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
     ((None, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "null"),
-    ((P, 0, P, 0, 4, 1025, P, 1e-6, None, P, P, P, P, 1 << 20, None), "dx is dy"),
-    ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 8, None), "workspace"),
-    ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, None, 1 << 20, None), "workspace"),
+    ((P, 0, P, 0, 4, 4, P, 1e-6, None, P, P, P, P, 1 << 20, None), "dx is dy"),
+    ((P, 0, P, 0, 4000, 4, P, 1e-6, None, P, P, P, P, 8, None), "workspace"),
+    ((P, 0, P, 0, 4000, 4, P, 1e-6, None, P, P, P, None, 1 << 20, None), "workspace"),
 ])
 def test_norm_backward(args, word):
     _refused("ygg_clifford_layer_norm_backward", args, word)
@@ -90,7 +90,7 @@ def test_route_backward(args, word):
     ((P, 0, 4, 4, P, 4, 5, P, P, P, None, P, P, P, P, 1 << 20, None), "bad sizes"),
     ((P, 0, 4, 4, None, 4, 2, P, P, P, None, P, P, P, P, 1 << 20, None), "null"),
     ((P, 0, 4, 4, P, 4, 2, P, P, P, None, P, None, P, P, 1 << 20, None), "null"),
-    ((P, 0, 4, 4, P, 4, 2, P, P, P, None, P, P, P, None, 0, None), "workspace"),
+    ((P, 0, 4000, 4, P, 4, 2, P, P, P, None, P, P, P, None, 0, None), "workspace"),
 ])
 def test_route_energy_backward(args, word):
     _refused("ygg_route_energy_backward", args, word)
@@ -154,7 +154,7 @@ def test_workspace_sizes_of_bad_sizes_are_zero():
     assert lib.ygg_clifford_layer_norm_backward_workspace_bytes(-1, 4) == 0
     assert lib.ygg_clifford_layer_norm_backward_workspace_bytes(4, 5000) == 0
     assert lib.ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(-1, 2, 4, 4) == 0
-    assert lib.ygg_route_energy_backward_workspace_bytes(-1, 4) == 0
+    assert lib.ygg_route_energy_backward_workspace_bytes(-1, 4, 4, 2) == 0
 
 
 def test_launches_go_to_the_tensors_device(monkeypatch):

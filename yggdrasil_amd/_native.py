@@ -84,7 +84,7 @@ SIGNATURES = {
     "ygg_moe_backward_bf16": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_size,
                                        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
     "ygg_route_backward": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
-    "ygg_route_energy_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "ygg_route_energy_backward_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
     "ygg_route_energy_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp,
                                            _vp, _vp, _c_size, _vp]),
     "ygg_clifford_layer_norm_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),

@@ -46,16 +46,10 @@ __device__ inline void product(const float a[8], const float b[8], float o[8]) {
   }
 }
 
-// One wave per token: 1 / rms and dx.
+// dx of one token by a wave, which reads its row twice; returns 1 / rms.
 template <typename XT, typename GT>
-__global__ __launch_bounds__(256) void norm_dx_kernel(const GT* __restrict__ dy, const XT* __restrict__ x, int N, int d,
-                                                      const float* __restrict__ gamma, float two_eps,
-                                                      const XT* __restrict__ residual, XT* __restrict__ dx,
-                                                      float* __restrict__ rrms) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= N) return;
-  const size_t row = (size_t)t * d;
+__device__ __forceinline__ float norm_dx_row(const GT* dy, const XT* x, size_t row, int d, const float* gamma,
+                                             float two_eps, const XT* residual, XT* dx, int lane) {
   float n2 = 0.f, dot = 0.f;
   for (int i = lane; i < d; i += 64) {
     float v[8], u[8], g[8], gx[8];
@@ -76,7 +70,6 @@ __global__ __launch_bounds__(256) void norm_dx_kernel(const GT* __restrict__ dy,
   }
   const float r = 1.0f / sqrtf(n2 / (float)d + two_eps);
   const float w = dot * r * r / (float)d;  // <gx, x> / (rms^2 d): dx = (gx - x w) / rms
-  if (lane == 0) rrms[t] = r;
   for (int i = lane; i < d; i += 64) {
     float v[8], u[8], g[8], gx[8], o[8];
     load_mv(x, row + i, v);
@@ -93,6 +86,19 @@ __global__ __launch_bounds__(256) void norm_dx_kernel(const GT* __restrict__ dy,
     }
     store_mv(dx, row + i, o);
   }
+  return r;
+}
+
+// One wave per token: 1 / rms and dx.
+template <typename XT, typename GT>
+__global__ __launch_bounds__(256) void norm_dx_kernel(const GT* __restrict__ dy, const XT* __restrict__ x, int N, int d,
+                                                      const float* __restrict__ gamma, float two_eps, const XT* residual,
+                                                      XT* dx, float* __restrict__ rrms) {
+  const int lane = threadIdx.x & 63;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= N) return;
+  const float r = norm_dx_row(dy, x, (size_t)t * d, d, gamma, two_eps, residual, dx, lane);
+  if (lane == 0) rrms[t] = r;
 }
 
 // Partial sums of dgamma and dbeta over kNbPlaneTokens tokens: a thread per multivector.
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(64) void norm_param_kernel(const GT* __restrict__ d
 // them here (537 MB: 5.1 TB/s, the rate of a copy of 1 GiB) and 6 in the planes' sum.  As two passes over the rows --
 // dx, then gamma and beta -- the same took 291 us.  181 registers for four tokens at a time allow two workgroups on a
 // CU; two tokens at a time and four workgroups took 112 us against 108 on one box, three workgroups with
-// spilled registers 119.
+// spilled registers 119.  Wider rows (d > 1024) would need more registers than a wave has, and take two passes.
 constexpr int kNbFusedMaxD = 1024, kNbMaxPlanes = 512;  // planes: two workgroups on each of 256 CUs
 
 template <typename XT, typename GT, int CS, int NQ, int U>
@@ -305,9 +311,113 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const GT* __restrict
   }
 }
 
+// ---- few rows: one launch -------------------------------------------------------------------------
+// The first workgroups take 16 multivectors each of gamma and beta, over all tokens: their waves find every token's
+// rms, a row at a time, and then a thread adds every 64th token of its multivector; the sums meet by exchanges and in
+// LDS, in an order that the sizes fix.  The other workgroups write dx, a wave a token.
+//
+// A second launch and a workspace are most of what a small call takes: 256 tokens of 64 multivectors, fp32, 10.5 us a
+// call here, 15.2 with planes; 384 tokens 13.3 and 15.3, 512 tokens 15.6 and 15.2; 64 tokens of 512 multivectors,
+// fp32, 19.5 and 15.
+constexpr int kNbSmallTokens = 384, kNbSmallD = 256;
+constexpr int kNbSmallUnits = 512;  // tokens times wave loads a row: the most that the first workgroups read through
+constexpr int kNbCols = 16;
+
+template <typename XT, typename GT>
+__global__ __launch_bounds__(1024) void norm_backward_small_kernel(const GT* __restrict__ dy, const XT* __restrict__ x,
+                                                                   int N, int d, const float* __restrict__ gamma,
+                                                                   float two_eps, const XT* residual, XT* dx,
+                                                                   float* __restrict__ dgamma, float* __restrict__ dbeta) {
+  constexpr int U = 8;  // rows' pieces that a wave asks for together
+  __shared__ float s_r[kNbSmallTokens];
+  __shared__ float s_sum[16][16][kNbCols + 1];  // [wave][value][column]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = (d + kNbCols - 1) / kNbCols;
+  if ((int)blockIdx.x >= blocks) {
+    const int t = ((int)blockIdx.x - blocks) * 16 + wave;
+    if (t < N) norm_dx_row(dy, x, (size_t)t * d, d, gamma, two_eps, residual, dx, lane);
+    return;
+  }
+  const int col = blockIdx.x * kNbCols + (lane & 15), slot = wave * 4 + (lane >> 4);  // of 64 slots for tokens
+  for (int t0 = wave; t0 < N; t0 += 16 * U) {
+    float n2[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) n2[u] = 0.f;
+    for (int i = lane; i < d; i += 64) {
+      RawMv<XT> m[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) m[u] = load_raw(x, (size_t)min(t0 + 16 * u, N - 1) * d + i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[8];
+        unpack(m[u], v);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) n2[u] = __builtin_fmaf(v[c], v[c], n2[u]);
+      }
+    }
+    const float s = wave_sums<U>(n2, lane);
+    const int t = t0 + 16 * wave_sums_of<U>(lane);
+    if ((lane & (64 / U - 1)) == 0 && t < N) s_r[t] = 1.0f / sqrtf(s / (float)d + two_eps);
+  }
+  __syncthreads();
+  float o[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c) o[c] = 0.f;
+  if (col < d)
+    for (int t0 = slot; t0 < N; t0 += 64 * 2) {
+      RawMv<XT> mx[2];
+      RawMv<GT> mg[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const size_t n = (size_t)min(t0 + 64 * u, N - 1) * d + col;
+        mx[u] = load_raw(x, n);
+        mg[u] = load_raw(dy, n);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (t0 + 64 * u >= N) break;
+        float v[8], g[8], p[8];
+        unpack(mx[u], v);
+        unpack(mg[u], g);
+        const float r = s_r[t0 + 64 * u];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] *= r;
+        product<false, true>(g, v, p);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          o[c] += p[c];
+          o[8 + c] += g[c];
+        }
+      }
+    }
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    o[c] += __shfl_xor(o[c], 16);
+    o[c] += __shfl_xor(o[c], 32);
+    if (lane < 16) s_sum[wave][c][lane] = o[c];
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 * kNbCols) {
+    const int c = threadIdx.x & 15, k = threadIdx.x >> 4, i = blockIdx.x * kNbCols + k;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += s_sum[w][c][k];
+    if (i < d && c < 8) dgamma[(size_t)i * 8 + c] = s;
+    if (i < d && c >= 8) dbeta[(size_t)i * 8 + c - 8] = s;
+  }
+}
+
 __global__ __launch_bounds__(1024) void norm_param_reduce_kernel(const float* __restrict__ part, int planes, int d,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  add_planes(part, planes, d * 16, [&](int n, float v) { ((n & 15) < 8 ? dgamma : dbeta)[(size_t)(n >> 4) * 8 + (n & 7)] = v; });
+  add_planes(part, planes, d * 16, [&](int n, float v) {
+    const size_t at = (size_t)(n >> 4) * 8 + (n & 7);
+    if ((n & 15) < 8) dgamma[at] = v;  // (a choice between the two pointers would put them into scratch memory)
+    else dbeta[at] = v;
+  });
+}
+
+bool few_rows(int N, int d) {
+  return d <= kNbSmallD && N <= kNbSmallTokens && (long long)N * ((d + 63) / 64) <= kNbSmallUnits;
 }
 
 // The tokens of a workgroup's batch and the planes of the one-pass kernel
@@ -321,6 +431,12 @@ size_t rrms_bytes(int N, int d) { return d <= kNbFusedMaxD ? 0 : ((size_t)N * 4 
 template <typename XT, typename GT>
 int launch(const void* dy, const void* x, int N, int d, const float* gamma, float two_eps, const void* residual,
            void* dx, float* dgamma, float* dbeta, void* workspace, hipStream_t stream) {
+  if (few_rows(N, d)) {
+    hipLaunchKernelGGL((norm_backward_small_kernel<XT, GT>), dim3((d + kNbCols - 1) / kNbCols + (N + 15) / 16), dim3(1024), 0,
+                       stream, static_cast<const GT*>(dy), static_cast<const XT*>(x), N, d, gamma, two_eps,
+                       static_cast<const XT*>(residual), static_cast<XT*>(dx), dgamma, dbeta);
+    return check_launch("norm backward (few rows)");
+  }
   float* rrms = static_cast<float*>(workspace);
   float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + rrms_bytes(N, d));
   const int planes = planes_of(N, d);
@@ -356,7 +472,7 @@ int launch(const void* dy, const void* x, int N, int d, const float* gamma, floa
 using namespace ygg;
 
 YGG_API size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d) {
-  if (N < 0 || d < 1 || d > kNbMaxD) return 0;
+  if (N < 0 || d < 1 || d > kNbMaxD || few_rows(N, d)) return 0;
   return rrms_bytes(N, d) + (size_t)planes_of(N, d) * d * 16 * sizeof(float);
 }
 
@@ -372,12 +488,11 @@ YGG_API int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const
   YGG_CHECK_ARG(eps >= 0.0, "ygg_clifford_layer_norm_backward: eps must be non-negative");
   YGG_CHECK_ARG(gamma && dgamma && dbeta && (N == 0 || (dy && x && dx)),
                 "ygg_clifford_layer_norm_backward: null pointer argument");
-  YGG_CHECK_ARG(N == 0 || d <= kNbFusedMaxD || dx != dy,
-                "ygg_clifford_layer_norm_backward: dx is dy, which d=%d reads again (d <= %d)", d, kNbFusedMaxD);
   const size_t need = ygg_clifford_layer_norm_backward_workspace_bytes(N, d);
   YGG_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                 "ygg_clifford_layer_norm_backward: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0,
                 need);
+  YGG_CHECK_ARG(N == 0 || dx != dy, "ygg_clifford_layer_norm_backward: dx is dy, which other workgroups read");
   const float two_eps = (float)(2.0 * eps);  // as the forward adds it
   if (x_dtype == kF32)
     return dy_dtype == kF32

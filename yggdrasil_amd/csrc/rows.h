@@ -48,20 +48,21 @@ __device__ __forceinline__ void store_mv(uint16_t* p, size_t n, const float v[8]
 
 // V values (a power of two) summed over the wave with V + log2(64 / V) - 1 exchanges in the place of 6 V: each
 // of the first steps halves the values that a lane carries on.  Returns the sum of value wave_sums_of(lane).
-template <int V>
+// (By recursion: as loops over n and o, 16 values were indexed at run time.)
+template <int V, int N = V / 2, int O = 32>
 __device__ __forceinline__ float wave_sums(float (&v)[V], int lane) {
-  int o = 32;
+  if constexpr (N > 0) {
+    const bool up = (lane & O) != 0;
 #pragma unroll
-  for (int n = V / 2; n > 0; n /= 2, o /= 2) {
-    const bool up = (lane & o) != 0;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
-      v[i] = keep + __shfl_xor(give, o);
+    for (int i = 0; i < N; ++i) {
+      const float keep = up ? v[i + N] : v[i], give = up ? v[i] : v[i + N];
+      v[i] = keep + __shfl_xor(give, O);
     }
+    return wave_sums<V, N / 2, O / 2>(v, lane);
+  } else if constexpr (O > 0) {
+    v[0] += __shfl_xor(v[0], O);
+    return wave_sums<V, 0, O / 2>(v, lane);
   }
-#pragma unroll
-  for (; o > 0; o /= 2) v[0] += __shfl_xor(v[0], o);
   return v[0];
 }
 // the value whose sum the lane holds: bit 5 of the lane chose between the halves, bit 4 between their halves, ...

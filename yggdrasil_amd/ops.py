@@ -709,11 +709,11 @@ def clifford_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, gamma: torch
     Nt = x.numel() // (8 * d) if d else 0
     L = lib()
     need = L.ygg_clifford_layer_norm_backward_workspace_bytes(Nt, d)
-    workspace = _workspace(workspace, need, dev)
+    workspace = _workspace(workspace, need, dev) if need else None
     dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(g), torch.empty_like(g)
     check(L.ygg_clifford_layer_norm_backward(dy.data_ptr(), _dtype_code(dy), x.data_ptr(), _dtype_code(x), Nt, d,
                                              g.data_ptr(), eps, ptr(residual_grad), dx.data_ptr(), dgamma.data_ptr(),
-                                             dbeta.data_ptr(), workspace.data_ptr(), need, stream_handle(dev)),
+                                             dbeta.data_ptr(), ptr(workspace), need, stream_handle(dev)),
           "clifford_layer_norm_backward")
     return dx, dgamma, dbeta
 
@@ -942,13 +942,13 @@ def route_energy_backward(x: torch.Tensor, router_weight: torch.Tensor, topk_idx
         raise ValueError("route_energy_backward: dx_add must have x's shape and dtype")
     x, dx_add, rw = _aligned(x), _aligned(dx_add), _fp32(router_weight)
     L = lib()
-    need = L.ygg_route_energy_backward_workspace_bytes(Nt, E)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    need = L.ygg_route_energy_backward_workspace_bytes(Nt, d, E, topk_idx.shape[1])
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
     dx, drw = torch.empty_like(x), torch.empty_like(rw)
     drb = torch.empty(E, device=dev, dtype=torch.float32)
     check(L.ygg_route_energy_backward(x.data_ptr(), _dtype_code(x), Nt, d, rw.data_ptr(), E, topk_idx.shape[1],
                                       topk_idx.data_ptr(), topk_w.data_ptr(), dtopk_w.data_ptr(), ptr(dx_add),
-                                      dx.data_ptr(), drw.data_ptr(), drb.data_ptr(), ws.data_ptr(), need,
+                                      dx.data_ptr(), drw.data_ptr(), drb.data_ptr(), ptr(ws), need,
                                       stream_handle(dev)), "route_energy_backward")
     return dx, drw, drb
 
