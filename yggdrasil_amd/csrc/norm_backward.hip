@@ -135,11 +135,11 @@ __global__ __launch_bounds__(64) void norm_param_kernel(const GT* __restrict__ d
 // each, and <gx, x> is half the sum of the matrices' entries' products.  Every row is read once; the sums over
 // the tokens stay in registers until the workgroup's last token, and are a plane of the workgroup's own then.
 //
-// Bound by memory: 32768 tokens of 256 multivectors with the residual's gradient, bf16, take 115 us in all, 106 of
-// them here (537 MB: 5.1 TB/s, the rate of a copy of 1 GiB) and 6 in the planes' sum.  As two passes over the rows --
+// Bound by memory: 32768 tokens of 256 multivectors with the residual's gradient, bf16, take 107 us in all, 102 of
+// them here (537 MB: 5.2 TB/s, the rate of a copy of 1 GiB) and 4 in the planes' sum.  As two passes over the rows --
 // dx, then gamma and beta -- the same took 291 us.  181 registers for four tokens at a time allow two workgroups on a
-// CU; two tokens at a time and four workgroups took 112 us against 108 on one box, three workgroups with
-// spilled registers 119.  Wider rows (d > 1024) would need more registers than a wave has, and take two passes.
+// CU; two tokens at a time and four workgroups took 4 us more, three workgroups with
+// spilled registers 11 more.  Wider rows (d > 1024) would need more registers than a wave has, and take two passes.
 constexpr int kNbFusedMaxD = 1024, kNbMaxPlanes = 512;  // planes: two workgroups on each of 256 CUs
 
 template <typename XT, typename GT, int CS, int NQ, int U>

@@ -175,8 +175,8 @@ __device__ __forceinline__ void add_slots(float4 share, const float* dl, const i
 // and slot gradients stay in LDS.  Then lane e of every wave adds what expert e has of the wave's share of
 // the slots.  The waves' sums are added in order at the end, and are a plane of the workgroup's own.
 //
-// Bound by memory: 32768 tokens of 256 multivectors, bf16, E = 64, k = 2 take 59 us in all, 47 of them here (268 MB
-// read and written: 5.7 TB/s; a copy of 1 GiB runs at 5.1) and 5 in the planes' sum.  As three passes -- dx, then one
+// Bound by memory: 32768 tokens of 256 multivectors, bf16, E = 64, k = 2 take 60 us in all, 49 of them here (268 MB
+// read and written: 5.4 TB/s; a copy of 1 GiB runs at 5.1) and 5 in the planes' sum.  As three passes -- dx, then one
 // workgroup per expert over all tokens -- the same took 244 us.
 constexpr int kRbTokens = 16, kRbMaxPlanes = 2048;  // planes: eight workgroups on each of 256 CUs
 
