@@ -413,3 +413,35 @@ def test_outputs_in_place(n, d):
                                         r.topk_w.data_ptr(), gw.data_ptr(), dx.data_ptr(), dx.data_ptr(), dw.data_ptr(),
                                         db.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_handle(x.device)), "router")
     assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), want))
+
+
+@pytest.mark.parametrize("d", [6, 600])
+def test_router_backward_of_no_tokens(d):
+    ops = _ops()
+    say(f"router backward of no tokens d={d}")
+    i, f = torch.empty(0, 2, device="cuda", dtype=torch.int32), torch.empty(0, 2, device="cuda")
+    dx, dW, db = ops.route_energy_backward(torch.empty(0, d, 8, device="cuda"), torch.ones(5, 4, device="cuda"), i, f, f)
+    assert dx.shape == (0, d, 8) and dW.shape == (5, 4) and not bool(dW.any()) and not bool(db.any())
+    assert ops.route_backward(i, f, f, 5).shape == (0, 5)
+
+
+@pytest.mark.parametrize("n", [384, 385])
+def test_few_rows_and_more_agree(n):
+    """The tokens of one launch and of two: dx is a token's own, the parameters' sums differ by their order.
+
+    dx: two orders of sums of 8 d = 320 terms, whose roundings add up to less than 2^8 half steps of the largest value;
+    parameters: sums of n tokens' terms, each of at most 8 products, a half step an addition."""
+    ops = _ops()
+    g = np.random.default_rng(21)
+    say(f"norm and router backward around the last call in one launch n={n}")
+    x, dy = (_dev(g.standard_normal((n, 40, 8)).astype(np.float32)) for _ in range(2))
+    gamma, rw = _dev(g.standard_normal((40, 8)).astype(np.float32)), _dev(g.standard_normal((7, 4)).astype(np.float32))
+    r = ops.route(_dev(g.standard_normal((n, 7)).astype(np.float32)), 3)
+    gw = _dev(g.standard_normal((n, 3)).astype(np.float32))
+    for call in (lambda s: ops.clifford_layer_norm_backward(dy[s], x[s], gamma),
+                 lambda s: ops.route_energy_backward(x[s], rw, r.topk_idx[s], r.topk_w[s], gw[s])):
+        whole, parts = call(slice(0, n)), [call(slice(0, 200)), call(slice(200, n))]
+        scale = [float(t.abs().max()) for t in whole]
+        assert float((whole[0] - torch.cat([p[0] for p in parts])).abs().max()) < 2.0 ** -16 * scale[0]
+        for i in (1, 2):
+            assert float((whole[i] - parts[0][i] - parts[1][i]).abs().max()) < 2.0 ** -24 * n * 8 * scale[i]
