@@ -174,6 +174,13 @@ class CliffordMoELayer(nn.Module):
             return [v._version for v in self.parameters()] + [self.w_up.device]
         return [v._version for v in p.values() if v is not None] + [p["w_up"].device]
 
+    # Whether a training step of this layer was captured.  The replays of such a graph may update the parameters, which
+    # their version counters do not show: from then on no layout outlives the call that made it.
+    _replayed = False
+
+    def __getstate__(self):
+        return {n: v for n, v in self.__dict__.items() if n != "_replayed"}  # (no graph updates a copy's parameters)
+
     @torch.no_grad()
     def prepare(self):
         """Build the device weight layouts (done lazily; redone when parameters change)."""
@@ -197,7 +204,7 @@ class CliffordMoELayer(nn.Module):
         return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head)
 
     def _get_prepared(self):
-        if self._prepared is None or self._prepared["key"] != self._param_versions():
+        if self._replayed or self._prepared is None or self._prepared["key"] != self._param_versions():
             self.prepare()
         return self._prepared
 
@@ -273,7 +280,7 @@ class CliffordMoELayer(nn.Module):
     def _get_adjoint(self):
         """Adjoint expert weights (reverse, channel axes exchanged) in the layout of the layer's products."""
         key = self._param_versions()
-        if getattr(self, "_adjoint", None) is None or self._adjoint["key"] != key:
+        if self._replayed or getattr(self, "_adjoint", None) is None or self._adjoint["key"] != key:
             self._adjoint = dict(key=key, **self._adjoint_layouts())
         return self._adjoint
 
@@ -331,7 +338,10 @@ def _in_capture(layer, block: bool) -> bool:
 def _step_layouts(layer, block: bool = False) -> dict:
     """The weight layouts of a training step's forward.  Those of a capture are the graph's own: nothing else finds
     them, since they hold values only after a replay."""
-    return layer._layouts() if _in_capture(layer, block) else layer._get_prepared()
+    if not _in_capture(layer, block):
+        return layer._get_prepared()
+    layer.__dict__["_replayed"] = True
+    return layer._layouts()
 
 
 # The eager graphs of each module that gets gradients through a node of its own, made on the default stream and
