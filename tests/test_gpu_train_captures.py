@@ -1,4 +1,4 @@
-"""GPU: captured training steps beside eager calls of the same module.
+"""GPU: captured training steps beside eager calls of the same module, and parameters changed before a backward.
 
 A captured step with its update changes the weights at every replay.  Eager calls between the replays -- with a
 graph and without -- have to see them, which a module of its own with the same state shows.  Both run the same kernels
@@ -65,3 +65,17 @@ def test_eager_calls_between_replays_with_updates(block, dtype):
         assert all(same), same
         seen.append(got[0])
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_parameters_changed_between_forward_and_backward():
+    """An fp32 layer's backward lays out and routes anew: it refuses parameters that its forward did not see."""
+    m = _layer(np.random.default_rng(23), 16, 24, 4, 2, torch.float32, router_grad=True)
+    x = _tokens(np.random.default_rng(24), 1, 30, 16, torch.float32)
+    say("fp32 layer, parameters changed before the backward")
+    for p in (m.router_weight, m.w_down):
+        out = m.moe_forward(x)
+        with torch.no_grad():
+            p.mul_(1.5)
+        with pytest.raises(RuntimeError, match="modified in place"):
+            out.sum().backward()
+    m.moe_forward(x).sum().backward()

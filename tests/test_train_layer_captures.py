@@ -1,6 +1,6 @@
-"""Which weight layouts a layer's calls use around a captured training step, on the CPU: the layouts are copies of the
-weights here, a capture is one that says so, and a replay changes values without the version counters, as the replays
-of a graph do."""
+"""Which parameters a layer's calls and its backward use, around a captured training step and otherwise, on the CPU:
+the layouts are copies of the weights here, a capture is one that says so, and a replay changes values without the
+version counters, as the replays of a graph do."""
 
 import copy
 
@@ -56,3 +56,33 @@ def test_eager_calls_between_replays_use_the_present_weights(capturing, block):
     assert _fresh(layer)
     other = copy.deepcopy(layer)  # parameters of its own, which no graph updates
     assert _fresh(other) and other._get_prepared() is other._get_prepared()
+
+
+def _autograd(monkeypatch):
+    """The layer's node around a forward and a backward that only hand x and dout on."""
+    none = torch.zeros(0)
+    monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
+                        (2 * flat, (none, none, none, none)))
+    monkeypatch.setattr(layers, "_train_backward", lambda layer, flat, logits, kept, dout, residual, block=False:
+                        (2 * dout, *(torch.zeros_like(getattr(layer, n)) for n in ("w_up", "b_up", "w_down", "b_down")),
+                         None, None, None))
+    monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
+    return lambda layer, x, logits=None: layers._MoEFunction.apply(
+        x, None, layer.w_up, layer.b_up, layer.w_down, layer.b_down, layer.router_weight, layer.router_bias, layer, None,
+        logits)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parameters_changed_between_forward_and_backward(capturing, monkeypatch, dtype):
+    run = _autograd(monkeypatch)
+    layer, x = _layer(dtype), torch.ones(5, 4, 8)
+    for name in ("w_up", "b_up", "w_down", "b_down", "router_weight", "router_bias"):
+        out = run(layer, x)
+        with torch.no_grad():
+            getattr(layer, name).add_(1.0)
+        with pytest.raises(RuntimeError, match="modified in place"):
+            out.sum().backward()
+    out = run(layer, x, torch.zeros(5, 3))  # with the caller's logits the router's parameters are not read
+    with torch.no_grad():
+        layer.router_weight.add_(1.0)
+    out.sum().backward()

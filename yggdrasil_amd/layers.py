@@ -379,9 +379,19 @@ def _train_forward(layer, flat, res, logits, prep, workspace=None):
     return out, (rows, routing["topk_idx"], routing["topk_w"], routing["offsets"])
 
 
-def _check_versions(layer, versions) -> None:
-    """The backward lays the weights out anew: they have to be those of the forward (None: not looked at)."""
-    if versions is not None and versions != layer._param_versions():
+def _read_versions(layer, logits) -> list:
+    """The versions of the parameters that a backward reads beside what its forward kept: the experts', and the router's
+    unless the caller gave the logits."""
+    p = layer._parameters
+    if layer._modules or "w_up" not in p:  # parametrized or pruned
+        return layer._param_versions()
+    names = ("w_up", "b_up", "w_down", "b_down") + (("router_weight", "router_bias") if logits is None else ())
+    return [p[n]._version for n in names]
+
+
+def _check_versions(layer, versions, logits) -> None:
+    """The backward lays the weights out anew, and an fp32 layer routes anew: all have to be those of the forward."""
+    if versions != _read_versions(layer, logits):
         raise RuntimeError("the layer's parameters were modified in place between its forward and its backward")
 
 
@@ -434,16 +444,16 @@ class _MoEFunction(torch.autograd.Function):
         if layer.cfg.bf16_grad:
             _note_graph(ctx, flat.device, layer)
         out, kept = _train_forward(layer, flat, res, logits, prep, workspace=layer._workspace)
-        ctx.versions = layer._param_versions() if layer.cfg.bf16_grad else None
+        ctx.versions = _read_versions(layer, logits)
         ctx.save_for_backward(*_for_backward(layer, flat, logits), *kept)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         flat, logits, *kept = ctx.saved_tensors
-        _check_versions(ctx.layer, ctx.versions)
-        dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
-            ctx.layer, flat, logits if ctx.has_logits else None, kept, dout, residual=False)
+        logits = logits if ctx.has_logits else None
+        _check_versions(ctx.layer, ctx.versions, logits)
+        dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(ctx.layer, flat, logits, kept, dout, residual=False)
         return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, dlogits
 
 
@@ -626,7 +636,7 @@ class _BlockFunction(torch.autograd.Function):
             logits = moe._head_logits(xn, prep)
         ctx.has_logits = logits is not None
         out, kept = _train_forward(moe, xn, x, logits, prep)
-        ctx.versions = moe._param_versions()
+        ctx.versions = _read_versions(moe, logits)
         ctx.save_for_backward(x, gamma, *_for_backward(moe, xn, logits), *kept)
         return out
 
@@ -634,10 +644,11 @@ class _BlockFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         x, gamma, xn, logits, *kept = ctx.saved_tensors
-        _check_versions(ctx.block.moe, ctx.versions)
+        logits = logits if ctx.has_logits else None
+        _check_versions(ctx.block.moe, ctx.versions, logits)
         dout = dout.contiguous()
         dxn, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
-            ctx.block.moe, xn, logits if ctx.has_logits else None, kept, dout, residual=False, block=True)
+            ctx.block.moe, xn, logits, kept, dout, residual=False, block=True)
         dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.eps, residual_grad=dout)
         return (dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), dWu, dbu, dWd, dbd, drw, drb, None,
                 dlogits if ctx.from_caller else None)
