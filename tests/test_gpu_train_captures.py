@@ -29,7 +29,8 @@ def _eager(m, x, grad, block):
     return [plain, out.detach(), *(g for g in grads if g is not None)]
 
 
-@pytest.mark.parametrize("block,dtype", [(False, torch.bfloat16), (True, torch.bfloat16), (True, torch.float32)])
+@pytest.mark.parametrize("block,dtype", [(False, torch.bfloat16), (True, torch.bfloat16), (True, torch.float32),
+                                         (False, torch.float32)])
 def test_eager_calls_between_replays_with_updates(block, dtype):
     make = lambda: _layer(np.random.default_rng(20), 16, 24, 4, 2, dtype, block=block, router_grad=True)
     m = make()
@@ -79,3 +80,100 @@ def test_parameters_changed_between_forward_and_backward():
         with pytest.raises(RuntimeError, match="modified in place"):
             out.sum().backward()
     m.moe_forward(x).sum().backward()
+
+
+def test_captured_step_of_an_fp32_layer_with_its_update():
+    """Every replay trains the weights of the replay before, also where the layouts were fresh at the capture."""
+    m = _layer(np.random.default_rng(25), 16, 24, 4, 2, torch.float32, router_grad=True)
+    params = list(m.parameters())
+    x, grad = (_tokens(np.random.default_rng(i), 1, 40, 16, torch.float32) for i in (26, 27))
+
+    def step():
+        out = m.moe_forward(x)
+        grads = torch.autograd.grad(out, params, grad)
+        with torch.no_grad():
+            for p, g in zip(params, grads):
+                p.add_(g.sign(), alpha=-0.02)
+        return out.detach()
+
+    say("captured training steps of an fp32 layer with updates")
+    start = [p.detach().clone() for p in params]
+
+    def restart():
+        with torch.no_grad():
+            for p, s in zip(params, start):
+                p.copy_(s)
+
+    want = [(step().clone(), [p.detach().clone() for p in params]) for _ in range(4)]
+    assert not torch.equal(want[0][0], want[1][0])
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    restart()
+    with torch.no_grad():
+        m.moe_forward(x)  # the layouts of these weights are there now
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    restart()
+    for o, ps in want:
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, o) and all(torch.equal(p.detach(), q) for p, q in zip(params, ps))
+
+
+@pytest.mark.parametrize("graph_of", ["training", "inference"])
+def test_weights_first_laid_out_in_a_capture(graph_of):
+    """An eager call before any replay lays the weights out for itself."""
+    m, other = (_layer(np.random.default_rng(28), 16, 24, 4, 2, torch.float32) for _ in range(2))
+    x = _tokens(np.random.default_rng(29), 1, 20, 16, torch.float32)
+
+    def run(layer):
+        with torch.set_grad_enabled(graph_of == "training"):
+            return layer.moe_forward(x).detach()
+
+    say(f"fp32 weights first laid out in a capture ({graph_of})")
+    run(m)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(1.25)
+    other.load_state_dict(m.state_dict())
+    want = run(other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(m)
+    assert torch.equal(run(m), want)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(run(m), want)
+
+
+@pytest.mark.parametrize("block,dtype", [(False, torch.float32), (True, torch.bfloat16)])
+def test_an_inference_graph_keeps_the_layouts_of_its_capture(block, dtype):
+    """New weights are laid out beside those that a graph reads."""
+    m = _layer(np.random.default_rng(30), 16, 24, 4, 2, dtype, block=block)
+    x = _tokens(np.random.default_rng(31), 1, 20, 16, dtype)
+    say(f"an inference graph beside new weights, block={block} {dtype}")
+    with torch.no_grad():
+        _run(m, x, block)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _run(m, x, block)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = got.clone()
+        moe = m.moe if block else m
+        for _ in range(3):
+            moe.w_up.mul_(1.5)
+            assert not torch.equal(_run(m, x, block), want)
+            other = [torch.full((n,), 255, device="cuda", dtype=torch.uint8) for n in (4096, 65536, 1 << 20) for _ in range(8)]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            del other

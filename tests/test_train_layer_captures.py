@@ -3,6 +3,7 @@ the layouts are copies of the weights here, a capture is one that says so, and a
 version counters, as the replays of a graph do."""
 
 import copy
+import weakref
 
 import pytest
 import torch
@@ -21,6 +22,7 @@ def capturing(monkeypatch):
     monkeypatch.setattr(layers.ops, "prepare_weights", lay_out)
     monkeypatch.setattr(layers.ops, "prepare_adjoint_weights", lay_out)
     monkeypatch.setattr(layers.ops, "prepare_bias", lambda b: b.detach().clone())
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0])
     return now
 
@@ -43,12 +45,12 @@ def _fresh(layer):
             torch.equal(layer._get_adjoint()["w_up"].data, layer.w_up))
 
 
-@pytest.mark.parametrize("block", [False, True])
-def test_eager_calls_between_replays_use_the_present_weights(capturing, block):
-    layer = _layer()
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_eager_calls_between_replays_use_the_present_weights(capturing, dtype):
+    layer = _layer(dtype)
     assert _fresh(layer) and layer._get_prepared() is layer._get_prepared()
     capturing[0] = True
-    layers._step_layouts(layer, block)
+    layers._step_layouts(layer)
     capturing[0] = False
     for _ in range(3):
         assert _fresh(layer)
@@ -63,7 +65,7 @@ def _autograd(monkeypatch):
     none = torch.zeros(0)
     monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
                         (2 * flat, (none, none, none, none)))
-    monkeypatch.setattr(layers, "_train_backward", lambda layer, flat, logits, kept, dout, residual, block=False:
+    monkeypatch.setattr(layers, "_train_backward", lambda layer, prep, flat, logits, kept, dout, residual:
                         (2 * dout, *(torch.zeros_like(getattr(layer, n)) for n in ("w_up", "b_up", "w_down", "b_down")),
                          None, None, None))
     monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
@@ -86,3 +88,57 @@ def test_parameters_changed_between_forward_and_backward(capturing, monkeypatch,
     with torch.no_grad():
         layer.router_weight.add_(1.0)
     out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layouts_of_a_capture_are_found_by_nothing_else(capturing, dtype):
+    layer = _layer(dtype)
+    before = layer._get_prepared(), layer._get_adjoint()
+    with torch.no_grad():
+        layer.w_up.add_(1.0)
+    capturing[0] = True
+    inference = layer._get_prepared()  # stale: laid out in the capture
+    capturing[0] = False
+    after = layer._get_prepared()
+    assert after is not inference and after is not before[0] and after is layer._get_prepared()
+    capturing[0] = True
+    step = layers._step_layouts(layer)
+    capturing[0] = False
+    assert step is not after and layer._get_prepared() is not step
+
+
+def test_layouts_that_a_capture_reads_stay(capturing):
+    """An inference graph reads the layouts that it found at every replay: new ones do not free them."""
+    layer = _layer(torch.float32)
+    layer._get_prepared()
+    capturing[0] = True
+    read = layer._get_prepared()
+    assert layer._get_prepared() is read
+    capturing[0] = False
+    alive = weakref.ref(read["w_up"])
+    with torch.no_grad():
+        layer.w_up.add_(1.0)
+    new = layer._get_prepared()
+    del read
+    assert new["w_up"] is not alive() and alive() is not None
+    assert "_kept" in layer.__dict__ and "_kept" not in copy.deepcopy(layer).__dict__
+
+
+def test_a_captured_backward_reads_layouts_of_its_own(capturing, monkeypatch):
+    """The forward's layouts reach an fp32 backward, and the adjoint ones are the graph's."""
+    layer, seen = _layer(torch.float32), []
+    layer._get_adjoint()
+    monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
+                        (2 * flat, (torch.zeros(0),) * 4))
+    monkeypatch.setattr(layers.ops, "moe_backward", lambda x, k, up, up_adj, down, down_adj, dout, *a, **kw:
+                        seen.append((up, up_adj)) or (dout, *(torch.zeros_like(p) for p in (
+                            layer.w_up, layer.b_up, layer.w_down, layer.b_down)), None))
+    monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 7)
+    for now in (True, False):
+        capturing[0] = now
+        prep = layers._step_layouts(layer)
+        out = layers._MoEFunction.apply(torch.ones(5, 4, 8), None, layer.w_up, layer.b_up, layer.w_down, layer.b_down,
+                                        layer.router_weight, layer.router_bias, layer, prep, None)
+        out.sum().backward()
+        assert seen[-1][0] is prep["w_up"] and (seen[-1][1] is layer._adjoint["w_up"]) == (not now)
+    del out

@@ -179,13 +179,16 @@ class CliffordMoELayer(nn.Module):
     _replayed = False
 
     def __getstate__(self):
-        return {n: v for n, v in self.__dict__.items() if n != "_replayed"}  # (no graph updates a copy's parameters)
+        return {n: v for n, v in self.__dict__.items() if n not in ("_replayed", "_kept")}  # (no graph knows a copy)
 
     @torch.no_grad()
     def prepare(self):
-        """Build the device weight layouts (done lazily; redone when parameters change)."""
-        self._prepared = self._layouts()
-        return self._prepared
+        """Build the device weight layouts (done lazily; redone when parameters change).  In a capture they are the
+        graph's own, which lays the weights out anew at every replay: no other call finds them."""
+        prep = self._layouts()
+        if not _capturing():
+            self._prepared = prep
+        return prep
 
     def _layouts(self) -> dict:
         fmt = self.cfg.weight_format
@@ -204,9 +207,14 @@ class CliffordMoELayer(nn.Module):
         return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head)
 
     def _get_prepared(self):
-        if self._replayed or self._prepared is None or self._prepared["key"] != self._param_versions():
-            self.prepare()
-        return self._prepared
+        prep = self._prepared
+        if self._replayed or prep is None or prep["key"] != self._param_versions():
+            return self.prepare()
+        if _capturing():  # the graph reads these layouts at every replay: they outlive the next ones
+            kept = self.__dict__.setdefault("_kept", [])
+            if not any(k is prep for k in kept):
+                kept.append(prep)
+        return prep
 
     # -- forward ---------------------------------------------------------------
     def _head_logits(self, flat_x: torch.Tensor, prep) -> torch.Tensor:
@@ -328,17 +336,16 @@ class CliffordMoELayer(nn.Module):
         return ((f - 1.0 / self.cfg.n_experts) ** 2).sum()
 
 
-def _in_capture(layer, block: bool) -> bool:
-    """Whether a training step lays the weights out anew in a graph that is being captured, where its replays find
-    them updated by an optimizer step of the same graph.  (The fp32 layer alone replays the layouts of the capture.)"""
-    return (block or layer.cfg.bf16_grad) and torch.cuda.is_current_stream_capturing()
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 @torch.no_grad()
-def _step_layouts(layer, block: bool = False) -> dict:
-    """The weight layouts of a training step's forward.  Those of a capture are the graph's own: nothing else finds
-    them, since they hold values only after a replay."""
-    if not _in_capture(layer, block):
+def _step_layouts(layer) -> dict:
+    """The weight layouts of a training step's forward.  A capture lays the weights out anew, so that its replays find
+    them updated by an optimizer step of the same graph, and nothing else finds those layouts: they hold values only
+    after a replay."""
+    if not _capturing():
         return layer._get_prepared()
     layer.__dict__["_replayed"] = True
     return layer._layouts()
@@ -403,16 +410,15 @@ def _for_backward(layer, flat, logits):
             logits if fp32 and logits is not None else flat.new_empty(0))
 
 
-def _train_backward(layer, flat, logits, kept, dout, residual: bool, block=False):
+def _train_backward(layer, prep, flat, logits, kept, dout, residual: bool):
     """Gradients of :func:`_train_forward`: ``(dx, dW_up, db_up, dW_down, db_down, drouter_weight, drouter_bias,
-    dlogits)``, the last three None where the router gets none.  ``residual``: dx includes dout (bf16 layers)."""
+    dlogits)``, the last three None where the router gets none.  prep: the forward's layouts (fp32 layers).
+    ``residual``: dx includes dout (bf16 layers)."""
     rows, idx, w, offsets = kept
     cfg = layer.cfg
-    capture = _in_capture(layer, block)
-    adj = layer._adjoint_layouts() if capture else layer._get_adjoint()
+    adj = layer._adjoint_layouts() if _capturing() else layer._get_adjoint()
     dout = dout.contiguous()
     if cfg.weight_format == "pauli_f32":
-        prep = layer._layouts() if capture else layer._get_prepared()
         dx, *grads, dtw = ops.moe_backward(
             flat, cfg.top_k, prep["w_up"], adj["w_up"], prep["w_down"], adj["w_down"], dout, prep["b_up"], prep["b_down"],
             cfg.activation, logits=logits, router_weight=None if logits is not None else layer.router_weight.detach(),
@@ -441,6 +447,7 @@ class _MoEFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, prep, logits):
         ctx.layer, ctx.has_res, ctx.has_logits = layer, res is not None, logits is not None
+        ctx.prep = prep if layer.cfg.weight_format == "pauli_f32" else None
         if layer.cfg.bf16_grad:
             _note_graph(ctx, flat.device, layer)
         out, kept = _train_forward(layer, flat, res, logits, prep, workspace=layer._workspace)
@@ -453,7 +460,8 @@ class _MoEFunction(torch.autograd.Function):
         flat, logits, *kept = ctx.saved_tensors
         logits = logits if ctx.has_logits else None
         _check_versions(ctx.layer, ctx.versions, logits)
-        dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(ctx.layer, flat, logits, kept, dout, residual=False)
+        dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
+            ctx.layer, ctx.prep, flat, logits, kept, dout, residual=False)
         return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, dlogits
 
 
@@ -629,7 +637,8 @@ class _BlockFunction(torch.autograd.Function):
     def forward(ctx, x, gamma, beta, w_up, b_up, w_down, b_down, router_weight, router_bias, block, logits):
         moe = block.moe
         _note_graph(ctx, x.device, moe, block.ffn_norm)
-        prep = _step_layouts(moe, block=True)
+        prep = _step_layouts(moe)
+        ctx.prep = prep if block.cfg.weight_format == "pauli_f32" else None
         xn = ops.clifford_layer_norm(x, gamma, beta, block.ffn_norm.eps)
         ctx.block, ctx.from_caller, ctx.beta_dtype, ctx.eps = block, logits is not None, beta.dtype, block.ffn_norm.eps
         if logits is None and block.cfg.router == "clifford_head":  # (a constant of the backward)
@@ -648,7 +657,7 @@ class _BlockFunction(torch.autograd.Function):
         _check_versions(ctx.block.moe, ctx.versions, logits)
         dout = dout.contiguous()
         dxn, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
-            ctx.block.moe, xn, logits, kept, dout, residual=False, block=True)
+            ctx.block.moe, ctx.prep, xn, logits, kept, dout, residual=False)
         dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.eps, residual_grad=dout)
         return (dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), dWu, dbu, dWd, dbd, drw, drb, None,
                 dlogits if ctx.from_caller else None)
