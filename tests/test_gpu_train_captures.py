@@ -177,3 +177,25 @@ def test_an_inference_graph_keeps_the_layouts_of_its_capture(block, dtype):
             torch.cuda.synchronize()
             assert torch.equal(got, want)
             del other
+
+
+@pytest.mark.parametrize("block,dtype", [(False, torch.float32), (False, torch.bfloat16), (True, torch.bfloat16)])
+def test_a_graph_writes_no_memory_that_eager_calls_free(block, dtype):
+    """After an eager call of more tokens, whose workspace takes the place of the module's, replays leave every other
+    tensor as it is."""
+    m = _layer(np.random.default_rng(32), 16, 24, 4, 2, dtype, block=block)
+    x, more = (_tokens(np.random.default_rng(33 + i), 1, n, 16, dtype) for i, n in enumerate((20, 2000)))
+    say(f"a graph beside an eager call of more tokens, block={block} {dtype}")
+    with torch.no_grad():
+        want = _run(m, x, block).clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _run(m, x, block)
+        _run(m, more, block)
+        others = [torch.full((n,), 7, device="cuda", dtype=torch.uint8)
+                  for n in (512, 4096, 20000, 65536, 200000, 1 << 20) for _ in range(8)]
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and all(bool((t == 7).all()) for t in others)

@@ -71,7 +71,7 @@ def _autograd(monkeypatch):
     monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
     return lambda layer, x, logits=None: layers._MoEFunction.apply(
         x, None, layer.w_up, layer.b_up, layer.w_down, layer.b_down, layer.router_weight, layer.router_bias, layer, None,
-        logits)
+        None, logits)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -138,7 +138,20 @@ def test_a_captured_backward_reads_layouts_of_its_own(capturing, monkeypatch):
         capturing[0] = now
         prep = layers._step_layouts(layer)
         out = layers._MoEFunction.apply(torch.ones(5, 4, 8), None, layer.w_up, layer.b_up, layer.w_down, layer.b_down,
-                                        layer.router_weight, layer.router_bias, layer, prep, None)
+                                        layer.router_weight, layer.router_bias, layer, prep, None,
+                                        None)
         out.sum().backward()
         assert seen[-1][0] is prep["w_up"] and (seen[-1][1] is layer._adjoint["w_up"]) == (not now)
     del out
+
+
+def test_a_graph_has_a_workspace_of_its_own(capturing):
+    """What a graph writes is no tensor that a later eager call may free."""
+    layer, dev = _layer(torch.float32), torch.device("cpu")
+    ws = layers._call_workspace(layer, 100, dev)
+    assert ws.numel() == 100 and layers._call_workspace(layer, 50, dev) is ws
+    capturing[0] = True
+    own = layers._call_workspace(layer, 50, dev), layers._call_workspace(layer, 500, dev)
+    assert own[0] is not ws and own[1].numel() == 500 and layer._workspace is ws
+    capturing[0] = False
+    assert layers._call_workspace(layer, 100, dev) is ws and layers._call_workspace(layer, 101, dev) is not ws

@@ -249,15 +249,13 @@ class CliffordMoELayer(nn.Module):
             if residual.dtype != x.dtype:
                 raise ValueError("residual must have x's shape and dtype")
         ws_bytes = ops.moe_workspace_bytes(N, d, cfg.d_ff, E, cfg.top_k, cfg.dtype, cfg.weight_format)
-        ws = self.__dict__["_workspace"]
-        if ws is None or ws.numel() < ws_bytes or ws.device != x.device:
-            ws = self.__dict__["_workspace"] = torch.empty((max(ws_bytes, 1),), device=x.device, dtype=torch.uint8)
+        ws = _call_workspace(self, ws_bytes, x.device)
         if graph:
             flat = x.reshape(N, d, 8)
             res = residual.reshape(N, d, 8) if residual is not None else None
             lg = logits.reshape(N, E) if logits is not None else None
             return _MoEFunction.apply(flat, res, self.w_up, self.b_up, self.w_down, self.b_down, self.router_weight,
-                                      self.router_bias, self, prep, lg).reshape(B, T, d, 8)
+                                      self.router_bias, self, prep, ws, lg).reshape(B, T, d, 8)
         rw = rb = None
         if logits is None:
             rw, rb = self.router_weight.detach(), self.router_bias.detach()
@@ -338,6 +336,17 @@ class CliffordMoELayer(nn.Module):
 
 def _capturing() -> bool:
     return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _call_workspace(module, need: int, dev) -> torch.Tensor:
+    """The workspace of a call: kept by the module for its next one, except in a capture.  A graph's is its own, since
+    an eager call of more tokens would free the module's while the graph still writes it."""
+    ws = module.__dict__["_workspace"]
+    if _capturing():
+        return torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    if ws is None or ws.numel() < need or ws.device != dev:
+        ws = module.__dict__["_workspace"] = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
+    return ws
 
 
 @torch.no_grad()
@@ -445,12 +454,12 @@ class _MoEFunction(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, prep, logits):
+    def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, prep, workspace, logits):
         ctx.layer, ctx.has_res, ctx.has_logits = layer, res is not None, logits is not None
         ctx.prep = prep if layer.cfg.weight_format == "pauli_f32" else None
         if layer.cfg.bf16_grad:
             _note_graph(ctx, flat.device, layer)
-        out, kept = _train_forward(layer, flat, res, logits, prep, workspace=layer._workspace)
+        out, kept = _train_forward(layer, flat, res, logits, prep, workspace=workspace)
         ctx.versions = _read_versions(layer, logits)
         ctx.save_for_backward(*_for_backward(layer, flat, logits), *kept)
         return out
@@ -462,7 +471,7 @@ class _MoEFunction(torch.autograd.Function):
         _check_versions(ctx.layer, ctx.versions, logits)
         dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
             ctx.layer, ctx.prep, flat, logits, kept, dout, residual=False)
-        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, dlogits
+        return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, None, dlogits
 
 
 class CliffordLinear(nn.Module):
@@ -607,14 +616,12 @@ class CliffordMoEBlockFFN(nn.Module):
             logits = logits.reshape(B * T, cfg.n_experts).float().contiguous()
         ws_bytes = ops.moe_block_ffn_workspace_bytes(B * T, cfg.d_model, cfg.d_ff, cfg.n_experts, cfg.top_k,
                                                      cfg.dtype, cfg.weight_format)
-        if self._workspace is None or self._workspace.numel() < ws_bytes or self._workspace.device != x.device:
-            self._workspace = torch.empty((max(ws_bytes, 1),), device=x.device, dtype=torch.uint8)
         out, routing = ops.moe_block_ffn(
             flat, cfg.top_k, self.ffn_norm.gamma.detach(), self.ffn_norm.beta.detach(), prep["w_up"],
             prep["w_down"], prep["b_up"], prep["b_down"], cfg.activation, logits=logits,
             router_weight=moe.router_weight.detach() if logits is None else None,
             router_bias=moe.router_bias.detach() if logits is None else None, norm_eps=self.ffn_norm.eps,
-            workspace=self._workspace)
+            workspace=_call_workspace(self, ws_bytes, x.device))
         moe.last_routing = routing
         return out.reshape(B, T, cfg.d_model, 8)
 
