@@ -199,3 +199,35 @@ def test_a_graph_writes_no_memory_that_eager_calls_free(block, dtype):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want) and all(bool((t == 7).all()) for t in others)
+
+
+def test_a_captured_fp32_step_is_refused_beside_an_eager_graph():
+    """Refused on the host, before any gradient is added; the forward alone is captured, and without the eager graph
+    the whole step."""
+    m = _layer(np.random.default_rng(35), 16, 24, 4, 2, torch.float32)
+    x, grad = (_tokens(np.random.default_rng(i), 1, 20, 16, torch.float32) for i in (36, 37))
+    experts = [m.w_up, m.b_up, m.w_down, m.b_down]
+    say("an fp32 step captured beside an eager graph")
+    alive = m.moe_forward(x)
+    want = [alive.detach().clone(), *(t.clone() for t in torch.autograd.grad(alive, experts, grad, retain_graph=True))]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = m.moe_forward(x).detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want[0])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(m.moe_forward(x), experts, grad)
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.moe_forward(x)
+        got = [out.detach(), *torch.autograd.grad(out, experts, grad)]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -155,3 +155,26 @@ def test_a_graph_has_a_workspace_of_its_own(capturing):
     assert own[0] is not ws and own[1].numel() == 500 and layer._workspace is ws
     capturing[0] = False
     assert layers._call_workspace(layer, 100, dev) is ws and layers._call_workspace(layer, 101, dev) is not ws
+
+
+def test_a_captured_fp32_backward_is_refused_while_an_eager_graph_lives(capturing, monkeypatch):
+    """Its forward may be captured beside one: it carries a graph that nobody asked for."""
+    run, x = _autograd(monkeypatch), torch.ones(5, 4, 8)
+    layer, other = _layer(torch.float32), _layer(torch.float32)
+    alive = run(layer, x)
+    alive.sum().backward()
+    capturing[0] = True
+    run(other, x).sum().backward()
+    out = run(layer, x)
+    with pytest.raises(RuntimeError, match="still alive"):
+        out.sum().backward()
+    del alive
+    run(layer, x).sum().backward()
+    # parameters without gradients have none to add
+    capturing[0] = False
+    for p in layer.parameters():
+        p.requires_grad_(False)
+    alive = run(layer, x.requires_grad_(True))
+    capturing[0] = True
+    run(layer, x).sum().backward()
+    del alive

@@ -365,14 +365,20 @@ def _step_layouts(layer) -> dict:
 _eager_graphs = weakref.WeakKeyDictionary()
 
 
-def _note_graph(ctx, dev, *modules) -> None:
+def _refuse_beside_eager(*modules) -> None:
     """Refuses to capture a training step while an eager graph of the same parameters lives.  autograd then adds the
     captured gradients on the stream of the eager graph; on the default stream, which no capture may use, that ends
     the process."""
+    if any(_eager_graphs.get(m) for m in modules):
+        raise RuntimeError("a graph of this module made outside the capture is still alive: delete its outputs (and "
+                           "losses made of them) before capturing a training step")
+
+
+def _note_graph(ctx, dev, *modules, forward_alone=False) -> None:
+    """Notes an eager graph; in a capture, refuses beside one -- with `forward_alone` only the backward does so."""
     if torch.cuda.is_current_stream_capturing():
-        if any(_eager_graphs.get(m) for m in modules):
-            raise RuntimeError("a graph of this module made outside the capture is still alive: delete its outputs (and "
-                               "losses made of them) before capturing a training step")
+        if not forward_alone:
+            _refuse_beside_eager(*modules)
     elif ops.stream_handle(dev) == 0:
         for m in modules:
             _eager_graphs.setdefault(m, weakref.WeakSet()).add(ctx)
@@ -457,8 +463,8 @@ class _MoEFunction(torch.autograd.Function):
     def forward(ctx, flat, res, w_up, b_up, w_down, b_down, router_weight, router_bias, layer, prep, workspace, logits):
         ctx.layer, ctx.has_res, ctx.has_logits = layer, res is not None, logits is not None
         ctx.prep = prep if layer.cfg.weight_format == "pauli_f32" else None
-        if layer.cfg.bf16_grad:
-            _note_graph(ctx, flat.device, layer)
+        # (an fp32 layer carries a graph without being asked for one: its forward may be captured for itself)
+        _note_graph(ctx, flat.device, layer, forward_alone=not layer.cfg.bf16_grad)
         out, kept = _train_forward(layer, flat, res, logits, prep, workspace=workspace)
         ctx.versions = _read_versions(layer, logits)
         ctx.save_for_backward(*_for_backward(layer, flat, logits), *kept)
@@ -468,6 +474,8 @@ class _MoEFunction(torch.autograd.Function):
     def backward(ctx, dout):
         flat, logits, *kept = ctx.saved_tensors
         logits = logits if ctx.has_logits else None
+        if _capturing() and any(ctx.needs_input_grad[2:8 if ctx.layer.cfg.router_grad else 6]):
+            _refuse_beside_eager(ctx.layer)
         _check_versions(ctx.layer, ctx.versions, logits)
         dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
             ctx.layer, ctx.prep, flat, logits, kept, dout, residual=False)
