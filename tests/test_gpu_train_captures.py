@@ -231,3 +231,24 @@ def test_a_captured_fp32_step_is_refused_beside_an_eager_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("which", ["layer", "block", "norm"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_are_not_differentiated_again(which, dtype):
+    import yggdrasil_amd as y
+
+    g = np.random.default_rng(38)
+    m = (y.CliffordLayerNorm(16, device="cuda", grad=True) if which == "norm" else
+         _layer(g, 16, 24, 4, 2, dtype, block=which == "block", router_grad=True))
+    x = _tokens(g, 1, 20, 16, dtype).requires_grad_(True)
+    params = list(m.parameters())
+    say(f"gradients with create_graph, {which} {dtype}")
+    out = m.moe_forward(x) if which == "layer" else m(x)
+    dout = torch.ones_like(out)
+    want = torch.autograd.grad(out, [x, *params], dout, retain_graph=True)
+    got = torch.autograd.grad(out, [x, *params], dout, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for t in got:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (t.sum() + x.float().sum()).backward(retain_graph=True)

@@ -178,3 +178,35 @@ def test_a_captured_fp32_backward_is_refused_while_an_eager_graph_lives(capturin
     capturing[0] = True
     run(layer, x).sum().backward()
     del alive
+
+
+def _first_order_only(out, inputs):
+    """The gradients of `out` for an incoming one that is a constant, and for one that is not: each equal to the plain
+    gradients, and each refusing to be differentiated."""
+    want = torch.autograd.grad(out, inputs, torch.ones_like(out), retain_graph=True)
+    assert not any(t.requires_grad for t in want)
+    for dout in (torch.ones_like(out), torch.ones_like(out, requires_grad=True)):
+        got = torch.autograd.grad(out, inputs, dout, retain_graph=True, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for t in got:
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                (t.sum() + inputs[0].sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_are_not_differentiated_again(capturing, monkeypatch, dtype):
+    run = _autograd(monkeypatch)
+    layer, x = _layer(dtype), torch.ones(5, 4, 8, requires_grad=True)
+    _first_order_only(run(layer, x), [x, layer.w_up, layer.b_down])
+    monkeypatch.setattr(layers.ops, "clifford_layer_norm", lambda x, gamma, beta, eps, out_dtype=None: 2 * x)
+    monkeypatch.setattr(layers.ops, "clifford_layer_norm_backward", lambda dy, x, gamma, eps, residual_grad=None:
+                        (2 * dy, torch.zeros_like(gamma), torch.zeros_like(gamma)))
+    norm = layers.CliffordLayerNorm(4, grad=True)
+    _first_order_only(norm(x), [x, norm.gamma, norm.beta])
+    # a residual's gradient is the incoming one, with its graph
+    res = torch.ones(5, 4, 8, requires_grad=True)
+    out = layers._MoEFunction.apply(x, res, layer.w_up, layer.b_up, layer.w_down, layer.b_down, layer.router_weight,
+                                    layer.router_bias, layer, None, None, None)
+    a = torch.tensor(3.0, requires_grad=True)
+    dres, = torch.autograd.grad(out, [res], a * torch.ones_like(out), create_graph=True)
+    assert torch.autograd.grad(dres.sum(), [a])[0] == dres.numel()

@@ -16,13 +16,13 @@ There is no CPU path.
 
 from __future__ import annotations
 
+import functools
 import math
 import weakref
 from dataclasses import dataclass
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -360,6 +360,36 @@ def _step_layouts(layer) -> dict:
     return layer._layouts()
 
 
+class _Differentiated(torch.autograd.Function):
+    """Gradients as they are, which refuse to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, token, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradients of these modules cannot be differentiated again: their backward has none")
+
+
+def _first_order(backward):
+    """A node's backward that has no backward itself.  Where autograd asks for a graph of it (create_graph), its gradients
+    refuse to be differentiated instead of being constants there, whether or not the incoming one has a graph; an
+    incoming gradient that is handed on keeps its own."""
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        mine = [t for t in out if t is not None and not any(t is g for g in grads)]
+        refusing = iter(_Differentiated.apply(torch.empty(0, requires_grad=True), *mine))
+        return tuple(next(refusing) if any(t is m for m in mine) else t for t in out)
+
+    return call
+
+
 # The eager graphs of each module that gets gradients through a node of its own, made on the default stream and
 # still alive
 _eager_graphs = weakref.WeakKeyDictionary()
@@ -471,6 +501,7 @@ class _MoEFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order
     def backward(ctx, dout):
         flat, logits, *kept = ctx.saved_tensors
         logits = logits if ctx.has_logits else None
@@ -548,7 +579,7 @@ class _NormFunction(torch.autograd.Function):
         return ops.clifford_layer_norm(x, gamma, beta, norm.eps, out_dtype=out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, gamma = ctx.saved_tensors
         dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dy.contiguous(), x, gamma, ctx.eps)
@@ -665,7 +696,7 @@ class _BlockFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         x, gamma, xn, logits, *kept = ctx.saved_tensors
         logits = logits if ctx.has_logits else None
