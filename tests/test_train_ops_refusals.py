@@ -258,3 +258,22 @@ def test_a_capture_is_refused_while_an_eager_graph_lives(monkeypatch):
     loss = Node.apply(a.weight, a).sum()
     capturing[0] = True
     Node.apply(a.weight, a)
+
+
+@pytest.mark.parametrize("N,d,F", [(2000, 18, 300000), (2000, 300000, 18), (1 << 20, 32, 125204)])
+def test_a_training_step_has_the_weight_gradients_limits(N, d, F):
+    """A chunk of 1024 rows of 300000 multivectors passes 2^32 bytes: refused before the forward, as by the operator."""
+    big = 1 << 62
+    for at, name, args in ((1, "ygg_moe_forward_train_bf16", _FWD), (0, "ygg_moe_backward_bf16", _BWD)):
+        args = list(args)
+        args[at:at + 3] = N, d, F
+        for i, v in enumerate(args):
+            if v == 1 << 30:
+                args[i] = big
+        _refused(name, args, "2 GiB")
+    _refused("ygg_grouped_weight_grad_pauli_bf16", (P, P, 2 * N, None, P, 2 * N, 4, F, d, P, P, P, big, None), "2 GiB")
+
+
+def test_a_weight_gradient_beyond_a_launch_is_refused():
+    big = 1 << 62
+    _refused("ygg_grouped_weight_grad_pauli_bf16", (P, P, 1 << 30, None, P, 1 << 30, 4, 4096, 4096, P, P, P, big, None), "launch")

@@ -133,6 +133,8 @@ int check_sizes(const char* who, int N, int d, int F, int E, int k, int act) {
   const char* why = pauli_size_limit(/*Pauli rows*/ 1, N, /*gathered*/ true, P, E, d, F, /*Pauli rows*/ 0, kBF16);
   if (!why) why = pauli_size_limit(1, P, false, P, E, F, d, /*blade*/ 1, kBF16);
   if (!why) why = pauli_size_limit(1, P, false, P, E, d, F, /*Pauli rows*/ 0, kBF16);
+  if (!why) why = weight_grad_bf16_limit(P, E, d, F, /*gathered*/ true, N);
+  if (!why) why = weight_grad_bf16_limit(P, E, F, d, false, P);
   YGG_CHECK_ARG(!why, "%s: %s (N=%d d=%d F=%d E=%d k=%d)", who, why, N, d, F, E, k);
   return 0;
 }

@@ -352,6 +352,16 @@ long long wb_planes(long long P, int E, int limit) {
 
 }  // namespace
 
+const char* weight_grad_bf16_limit(int P_max, int E, int d_in, int d_out, bool gathered, int a_rows) {
+  // offsets inside a chunk, past its end by the stages in flight, are 32 bits with one bit for "outside"
+  if ((long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 >= 1LL << 31)
+    return "the weight gradient's chunks of rows reach 2 GiB";
+  if ((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) >= 1LL << 24)
+    return "the weight gradient exceeds a launch";
+  if (gathered && (long long)a_rows * d_in * 16 >= 1LL << 31) return "gathered rows span 2 GiB or more";
+  return nullptr;
+}
+
 size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out) {
   return (size_t)wb_planes(P_max, E, chunk_rows(P_max, d_in, d_out)) * d_out * (d_in + 1) * 8 * sizeof(float);
 }
@@ -395,11 +405,9 @@ YGG_API int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void*
                 "d_out)", P_max, E, d_in, d_out);
   YGG_CHECK_ARG(a_rows >= 0 && (gather != nullptr || a_rows >= P_max),
                 "ygg_grouped_weight_grad_pauli_bf16: a has %d rows, %d are read without a gather", a_rows, P_max);
-  YGG_CHECK_ARG((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) < 1LL << 24 &&
-                    (long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 < 1LL << 31,
-                "ygg_grouped_weight_grad_pauli_bf16: P_max=%d d_in=%d d_out=%d exceed a launch", P_max, d_in, d_out);
-  YGG_CHECK_ARG(gather == nullptr || (long long)a_rows * d_in * 16 < 1LL << 31,
-                "ygg_grouped_weight_grad_pauli_bf16: gathered rows span 2 GiB or more (a_rows=%d d_in=%d)", a_rows, d_in);
+  const char* why = weight_grad_bf16_limit(P_max, E, d_in, d_out, gather != nullptr, a_rows);
+  YGG_CHECK_ARG(!why, "ygg_grouped_weight_grad_pauli_bf16: %s (P_max=%d d_in=%d d_out=%d a_rows=%d)", why, P_max, d_in, d_out,
+                a_rows);
   if (E == 0) return 0;
   YGG_CHECK_ARG(offsets && dW && (P_max == 0 || (dy_pauli && a_pauli)),
                 "ygg_grouped_weight_grad_pauli_bf16: null pointer argument");

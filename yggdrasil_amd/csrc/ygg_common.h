@@ -289,6 +289,7 @@ int dispatch_backward(const float* dxs, int N, int k, int d, const int32_t* slot
 int pauli_linear_save_pre(const void* x, int x_rows, const int32_t* gather, int P, const void* w, const float* bias,
                           const int32_t* offsets, int E, int d_in, int d_out, int act, void* h, void* h_pre,
                           hipStream_t stream);
+const char* weight_grad_bf16_limit(int P_max, int E, int d_in, int d_out, bool gathered, int a_rows);  // of the sizes, or nullptr
 size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out);
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream);
