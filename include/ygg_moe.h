@@ -352,7 +352,7 @@ int ygg_prepare_adjoint_weights_bf16(const float* W, int E, int d_out, int d_in,
  * output; h_pre: bf16 blade rows (P_max, d_in, 8), the activation's input (not read for
  * act 0).  dx_layout 0: Pauli half-rows (P_max, 2, d_in, 4) bf16 (d_in even); 1: blade
  * rows (P_max, d_in, 8) of dx_dtype.  Sums and slopes are fp32, dx is rounded once.  Rows
- * past offsets[E] are left as they were. */
+ * past offsets[E] are left as they were.  dx shares no memory with dy or h_pre. */
 int ygg_pauli_grouped_input_grad(const void* dy, int P_max, const void* w_adj, const int32_t* offsets, int E, int d_out,
                                  int d_in, int act, const void* h_pre, void* dx, int dx_layout, int dx_dtype,
                                  ygg_stream_t stream);
@@ -398,12 +398,14 @@ int ygg_moe_backward_bf16(int N, int d, int F, int E, int k, int act, const void
  * gradient of topk_w (ygg_moe_backward's output); E <= 64, k <= 8.
  *
  * dlogits (N, E) = topk_w (dtopk_w - sum_s topk_w dtopk_w) at the chosen experts, zero at
- * the others (and everywhere for k = 1, whose one weight is constant). */
+ * the others (and everywhere for k = 1, whose one weight is constant); it shares no memory
+ * with the inputs. */
 int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, int N, int E, int k,
                        float* dlogits, ygg_stream_t stream);
 
 /* The same through the grade-energy logits: dx (N, d, 8) of x's type (plus dx_add, of the
- * same type, when not NULL; dx may be dx_add), drouter_w (E, 4) and drouter_b (E), fp32. */
+ * same type, when not NULL; dx may be dx_add, not x), drouter_w (E, 4) and drouter_b (E),
+ * fp32.  Outputs that share memory with x or router_w are refused. */
 size_t ygg_route_energy_backward_workspace_bytes(int N, int d, int E, int k);
 int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const float* router_w, int E, int k,
                               const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, const void* dx_add,
@@ -437,7 +439,8 @@ int ygg_clifford_layer_norm(const void* x, int x_dtype, int N, int d, const floa
  *   dx = (gx - x_hat <gx, x_hat> / d) / rms with gx_i = ~gamma_i dy_i (plus residual_grad,
  *        of x's type, when not NULL), of x's type;
  *   dgamma_i = sum over the tokens of dy_i ~x_hat_i, dbeta_i = sum of dy_i, fp32 (d, 8),
- * sums in fp32 and in an order that the sizes alone fix.  dx may be residual_grad, not dy. */
+ * sums in fp32 and in an order that the sizes alone fix.  dx may be residual_grad; it may share no
+ * memory with x or dy, nor dgamma and dbeta with gamma (refused: other workgroups still read them). */
 size_t ygg_clifford_layer_norm_backward_workspace_bytes(int N, int d);
 int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const void* x, int x_dtype, int N, int d,
                                      const float* gamma, double eps, const void* residual_grad, void* dx, float* dgamma,

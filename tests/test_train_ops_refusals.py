@@ -277,3 +277,36 @@ def test_a_training_step_has_the_weight_gradients_limits(N, d, F):
 def test_a_weight_gradient_beyond_a_launch_is_refused():
     big = 1 << 62
     _refused("ygg_grouped_weight_grad_pauli_bf16", (P, P, 1 << 30, None, P, 1 << 30, 4, 4096, 4096, P, P, P, big, None), "launch")
+
+
+M = 1 << 20  # a megabyte apart
+
+
+@pytest.mark.parametrize("dx,residual,dgamma,dbeta,word", [
+    (1 * M, None, 9 * M, 10 * M, "dx is dy"), (1 * M + 480, None, 9 * M, 10 * M, "dx is dy"),
+    (2 * M, None, 9 * M, 10 * M, "dx is x"), (2 * M - 16, None, 9 * M, 10 * M, "dx is x"),
+    (2 * M + 1008, 2 * M + 4096, 9 * M, 10 * M, "dx is x"),
+    (4 * M, 4 * M + 16, 9 * M, 10 * M, "residual_grad"), (4 * M, None, 3 * M, 10 * M, "gamma"),
+    (4 * M, None, 9 * M, 3 * M + 96, "gamma"), (4 * M, 4 * M, 3 * M - 32, 10 * M, "gamma")])
+@pytest.mark.parametrize("N", [8, 4000])
+def test_norm_gradients_in_the_place_of_their_inputs(N, dx, residual, dgamma, dbeta, word):
+    """dy bf16 at 1 MiB, x fp32 at 2, gamma at 3: 8 or 4000 tokens of 4 multivectors."""
+    _refused("ygg_clifford_layer_norm_backward", (1 * M, 1, 2 * M, 0, N, 4, 3 * M, 1e-6, residual, dx, dgamma, dbeta,
+                                                  32 * M, 1 << 24, None), word)
+
+
+@pytest.mark.parametrize("dx,add,dw,db,word", [
+    (1 * M, None, 9 * M, 10 * M, "dx is x"), (1 * M + 1008, 4 * M, 9 * M, 10 * M, "dx is x"),
+    (4 * M, 4 * M - 16, 9 * M, 10 * M, "dx_add"), (4 * M, 4 * M, 2 * M, 10 * M, "router_w"),
+    (4 * M, None, 9 * M, 2 * M + 60, "router_w")])
+@pytest.mark.parametrize("N", [8, 4000])
+def test_router_gradients_in_the_place_of_their_inputs(N, dx, add, dw, db, word):
+    _refused("ygg_route_energy_backward", (1 * M, 0, N, 4, 2 * M, 4, 2, 5 * M, 6 * M, 7 * M, add, dx, dw, db, 32 * M, 1 << 24,
+                                           None), word)
+
+
+def test_other_gradients_in_the_place_of_their_inputs():
+    for at in (1 * M, 2 * M, 3 * M, 3 * M + 60):
+        _refused("ygg_route_backward", (1 * M, 2 * M, 3 * M, 8, 4, 2, at, None), "shares memory")
+    for act, at in ((0, 1 * M), (1, 1 * M + 64), (1, 4 * M), (1, 4 * M + 496), (1, 4 * M - 16)):
+        _refused("ygg_pauli_grouped_input_grad", (1 * M, 8, 2 * M, 3 * M, 2, 4, 4, act, 4 * M, at, 1, 1, None), "shares memory")

@@ -492,7 +492,15 @@ YGG_API int ygg_clifford_layer_norm_backward(const void* dy, int dy_dtype, const
   YGG_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                 "ygg_clifford_layer_norm_backward: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0,
                 need);
-  YGG_CHECK_ARG(N == 0 || dx != dy, "ygg_clifford_layer_norm_backward: dx is dy, which other workgroups read");
+  const size_t mv = (size_t)N * d * 8, bx = mv * dtype_size(x_dtype), bp = (size_t)d * 8 * sizeof(float);
+  YGG_CHECK_ARG(!overlap(dx, bx, dy, mv * dtype_size(dy_dtype)),
+                "ygg_clifford_layer_norm_backward: dx is dy, or shares memory with it: other workgroups read dy");
+  YGG_CHECK_ARG(!overlap(dx, bx, x, bx),
+                "ygg_clifford_layer_norm_backward: dx is x, or shares memory with it: other workgroups read x");
+  YGG_CHECK_ARG(dx == residual_grad || !overlap(dx, bx, residual_grad, bx),
+                "ygg_clifford_layer_norm_backward: dx shares a part of residual_grad's memory");
+  YGG_CHECK_ARG(!overlap(dgamma, bp, gamma, bp) && !overlap(dbeta, bp, gamma, bp),
+                "ygg_clifford_layer_norm_backward: dgamma or dbeta shares memory with gamma, which other workgroups read");
   const float two_eps = (float)(2.0 * eps);  // as the forward adds it
   if (x_dtype == kF32)
     return dy_dtype == kF32

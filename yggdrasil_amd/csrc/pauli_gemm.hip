@@ -1064,6 +1064,10 @@ YGG_API int ygg_pauli_grouped_input_grad(const void* dy, int P_max, const void* 
   YGG_CHECK_ARG(!why, "ygg_pauli_grouped_input_grad: %s (rows=%d d_out=%d d_in=%d)", why, P_max, d_out, d_in);
   if (P_max == 0) return 0;
   YGG_CHECK_ARG(dy && w_adj && offsets && dx && (act == kActNone || h_pre), "ygg_pauli_grouped_input_grad: null pointer");
+  const size_t b_dx = (size_t)P_max * d_in * (dx_layout == kOutPauliRows || dx_dtype == kBF16 ? 16 : 32);
+  YGG_CHECK_ARG(!overlap(dx, b_dx, dy, (size_t)P_max * d_out * 16) &&
+                    (act == kActNone || !overlap(dx, b_dx, h_pre, (size_t)P_max * d_in * 16)),
+                "ygg_pauli_grouped_input_grad: dx shares memory with dy or h_pre, which other workgroups read");
   const uint16_t* D = static_cast<const uint16_t*>(dy);
   const uint16_t* W = static_cast<const uint16_t*>(w_adj);
   const uint64_t bytes = (uint64_t)P_max * d_out * 16;

@@ -344,7 +344,10 @@ YGG_API int ygg_route_backward(const int32_t* topk_idx, const float* topk_w, con
                 "ygg_route_backward: bad sizes N=%d E=%d k=%d (E <= %d, k <= min(%d, E))", N, E, k, kRbMaxExperts, kRbMaxK);
   if (N == 0) return 0;
   YGG_CHECK_ARG(topk_idx && topk_w && dtopk_w && dlogits, "ygg_route_backward: null pointer argument");
-  const size_t n = (size_t)N * E;
+  const size_t n = (size_t)N * E, slots = (size_t)N * k * 4;
+  YGG_CHECK_ARG(!overlap(dlogits, n * 4, topk_idx, slots) && !overlap(dlogits, n * 4, topk_w, slots) &&
+                    !overlap(dlogits, n * 4, dtopk_w, slots),
+                "ygg_route_backward: dlogits shares memory with the routing, which other threads read");
   const unsigned groups = (unsigned)std::min<size_t>((n + 255) / 256, 1u << 23);  // a launch holds below 2^32 threads
   hipLaunchKernelGGL(route_backward_kernel, dim3(groups), dim3(256), 0, stream, topk_idx, topk_w, dtopk_w, N, E, k,
                      dlogits);
@@ -369,6 +372,12 @@ YGG_API int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, 
   const size_t need = ygg_route_energy_backward_workspace_bytes(N, d, E, k);
   YGG_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                 "ygg_route_energy_backward: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0, need);
+  const size_t bx = (size_t)N * d * 8 * dtype_size(x_dtype), bw = (size_t)E * 4 * sizeof(float);
+  YGG_CHECK_ARG(!overlap(dx, bx, x, bx), "ygg_route_energy_backward: dx is x, or shares memory with it: other workgroups read x");
+  YGG_CHECK_ARG(dx == dx_add || !overlap(dx, bx, dx_add, bx),
+                "ygg_route_energy_backward: dx shares a part of dx_add's memory");
+  YGG_CHECK_ARG(!overlap(drouter_w, bw, router_w, bw) && !overlap(drouter_b, bw / 4, router_w, bw),
+                "ygg_route_energy_backward: a gradient shares memory with router_w, which other workgroups read");
   if (few_rows(N, d, k)) {
     auto run = [&](auto* xt, auto nq) {
       using T = std::remove_const_t<std::remove_pointer_t<decltype(xt)>>;

@@ -294,6 +294,13 @@ size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out);
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream);
 
+// Whether n bytes at a and m bytes at b share any (nullptr: none).  Entries whose kernels write one tensor while other
+// workgroups still read another refuse such a pair.
+inline bool overlap(const void* a, size_t n, const void* b, size_t m) {
+  const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
+  return a != nullptr && b != nullptr && n != 0 && m != 0 && p < q + m && q < p + n;
+}
+
 inline int dtype_size(int dt) { return dt == kF32 ? 4 : dt == kBF16 ? 2 : dt == kI8 ? 1 : 0; }
 
 }  // namespace ygg
