@@ -88,24 +88,41 @@ __device__ inline float sigmoid_and_slope(float z2, float& slope) {  // z2 = z l
   slope = er * r;
   return z2 >= 0.f ? r : er;
 }
-// grades 1 and 2: out = (f(m) / m) g + (f'(m) - f(m) / m) (c . g) c / m^2, m the length of c
+// The same for z2 >= 0
+__device__ inline float sigmoid_and_slope_positive(float z2, float& slope) {
+  const float e = __builtin_amdgcn_exp2f(-z2), r = __builtin_amdgcn_rcpf(1.0f + e);
+  slope = e * r * r;
+  return r;
+}
+// v, and at most `most` (NaN stays NaN): squares are bounded far beyond where a slope is 0, so that no overflow meets it
+__device__ inline float at_most(float v, float most) { return __builtin_elementwise_minimum(v, most); }
+// grades 1 and 2, with m the length of h and u = h / m:  out = (f(m) / m) g + (f'(m) - f(m) / m) (u . g) u.  The sigmoid's
+// far lengths, where s is 1 and out = (g - (u . g) u) / m, are taken at 2^-70 of their size.
 template <int ACT>
-__device__ inline void gate_grad(const float* c, float* g) {
+__device__ inline void gate_grad(const float* h, float* g) {
   constexpr float kL = 1.4426950408889634f, k2 = 2.0f * 0.7978845608028654f;
-  const float m2 = __builtin_fmaf(c[2], c[2], __builtin_fmaf(c[1], c[1], __builtin_fmaf(c[0], c[0], 1e-12f)));
-  const float rm = __builtin_amdgcn_rsqf(m2), m = m2 * rm;
-  const float dot = __builtin_fmaf(c[2], g[2], __builtin_fmaf(c[1], g[1], c[0] * g[0]));
-  float a, b, slope;
+  const float near2 = __builtin_fmaf(h[2], h[2], __builtin_fmaf(h[1], h[1], __builtin_fmaf(h[0], h[0], 1e-12f)));
+  float slope;
   if constexpr (ACT == kActGelu) {  // f(m) / m = s(z), z = k2 (m + 0.044715 m^3): f' - f / m = m s' z'
-    a = sigmoid_and_slope(m * __builtin_fmaf(kL * k2 * 0.044715f, m2, kL * k2), slope);
-    b = slope * __builtin_fmaf(3.0f * 0.044715f * k2, m2, k2) * rm;
-  } else {  // f = s
-    a = sigmoid_and_slope(kL * m, slope) * rm;
-    b = (slope - a) * (rm * rm);
-  }
-  b *= dot;
+    const float m2 = at_most(near2, 3e38f), rm = __builtin_amdgcn_rsqf(m2);
+    const float u[3] = {rm * h[0], rm * h[1], rm * h[2]};
+    const float a = sigmoid_and_slope_positive(m2 * rm * __builtin_fmaf(kL * k2 * 0.044715f, m2, kL * k2), slope);
+    const float b = slope * __builtin_fmaf(3.0f * 0.044715f * k2, m2, k2) *
+                    __builtin_fmaf(u[2], g[2], __builtin_fmaf(u[1], g[1], u[0] * g[0]));
 #pragma unroll
-  for (int q = 0; q < 3; ++q) g[q] = __builtin_fmaf(a, g[q], b * c[q]);
+    for (int q = 0; q < 3; ++q) g[q] = __builtin_fmaf(a, g[q], b * h[q]);
+  } else {  // f = s
+    const bool far = near2 > 1e24f;
+    const float t = far ? 0x1p-70f : 1.0f;
+    const float c[3] = {t * h[0], t * h[1], t * h[2]};
+    const float m2 = far ? __builtin_fmaf(c[2], c[2], __builtin_fmaf(c[1], c[1], c[0] * c[0])) : near2;
+    const float rm = __builtin_amdgcn_rsqf(m2);
+    const float u[3] = {rm * c[0], rm * c[1], rm * c[2]};
+    const float a = sigmoid_and_slope_positive(far ? 1000.0f : kL * (m2 * rm), slope) * rm;
+    const float b = (slope - a) * __builtin_fmaf(u[2], g[2], __builtin_fmaf(u[1], g[1], u[0] * g[0]));
+#pragma unroll
+    for (int q = 0; q < 3; ++q) g[q] = t * __builtin_fmaf(a, g[q], b * u[q]);
+  }
 }
 template <int ACT>
 __device__ inline void activate_grad_blade(const float* h, float* g) {
@@ -114,11 +131,11 @@ __device__ inline void activate_grad_blade(const float* h, float* g) {
     g[7] = h[7] != 0.f ? g[7] : 0.f;
   } else if constexpr (ACT == kActGelu || ACT == kActSigmoid) {
     constexpr float kL = 1.4426950408889634f, k2 = 2.0f * 0.7978845608028654f;
-    const float v = h[0], v2 = v * v;
+    const float v = h[0], v2 = at_most(v * v, 1e12f);
     float slope;
     if constexpr (ACT == kActGelu) {  // (v s(z))' = s + v s' z'
       const float s = sigmoid_and_slope(v * __builtin_fmaf(kL * k2 * 0.044715f, v2, kL * k2), slope);
-      g[0] *= __builtin_fmaf(v * __builtin_fmaf(3.0f * 0.044715f * k2, v2, k2), slope, s);
+      g[0] *= __builtin_fmaf(v, slope * __builtin_fmaf(3.0f * 0.044715f * k2, v2, k2), s);
     } else {
       sigmoid_and_slope(kL * v, slope);
       g[0] *= slope;
