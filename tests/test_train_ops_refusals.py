@@ -310,3 +310,27 @@ def test_other_gradients_in_the_place_of_their_inputs():
         _refused("ygg_route_backward", (1 * M, 2 * M, 3 * M, 8, 4, 2, at, None), "shares memory")
     for act, at in ((0, 1 * M), (1, 1 * M + 64), (1, 4 * M), (1, 4 * M + 496), (1, 4 * M - 16)):
         _refused("ygg_pauli_grouped_input_grad", (1 * M, 8, 2 * M, 3 * M, 2, 4, 4, act, 4 * M, at, 1, 1, None), "shares memory")
+
+
+def test_weights_prepared_on_another_device_are_refused(monkeypatch):
+    class Tensor:
+        is_cuda = True
+
+        def __init__(self, n):
+            self.device = torch.device("cuda", n)
+
+        def get_device(self):
+            return self.device.index
+
+        def is_contiguous(self):
+            return True
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    a = Tensor(0)
+    here, there = (ops.PreparedWeights(Tensor(n), None, "pauli", 2, 4, 4) for n in (0, 1))
+    routing = dict(topk_w=a, offsets=a)
+    for f in (lambda: ops.pauli_grouped_input_grad(a, there, a),
+              lambda: ops.moe_forward_train_bf16(a, 2, here, there), lambda: ops.moe_forward_train_bf16(a, 2, there, here),
+              lambda: ops.moe_backward_bf16(a, a, routing, here, there), lambda: ops.moe_backward_bf16(a, a, routing, there, here)):
+        with pytest.raises(ValueError, match="one device"):
+            f()

@@ -882,7 +882,7 @@ def pauli_grouped_input_grad(dy_pauli: torch.Tensor, pw_adj: PreparedWeights, of
         raise ValueError(f"act must be one of {tuple(ACT_CODE)}")
     if y_layout not in Y_LAYOUT:
         raise ValueError("y_layout must be 'blade' or 'pauli'")
-    dev = _one_device(dy_pauli, offsets, h_pre)
+    dev = _one_device(dy_pauli, offsets, h_pre, pw_adj.data)
     dy_pauli = _half_rows("dy_pauli", dy_pauli)
     P, d_out, d_in, E = dy_pauli.shape[0], dy_pauli.shape[2], pw_adj.d_out, pw_adj.E
     if d_out != pw_adj.d_in:
@@ -1046,7 +1046,7 @@ def moe_forward_train_bf16(x: torch.Tensor, k: int, w_up: PreparedWeights, w_dow
                            router_bias: torch.Tensor | None = None, residual: torch.Tensor | None = None):
     """:func:`moe_forward` for a training step of a bf16 layer ('pauli' weights): ``(out, routing, saved)`` with the
     rows that :func:`moe_backward_bf16` reads in ``saved`` (uint8)."""
-    dev = _one_device(x, logits, residual, router_weight, router_bias, b_up, b_down)
+    dev = _one_device(x, logits, residual, router_weight, router_bias, b_up, b_down, w_up.data, w_down.data)
     if w_up.fmt != "pauli" or w_down.fmt != "pauli" or x.dtype != torch.bfloat16:
         raise ValueError("moe_forward_train_bf16: bf16 layers with 'pauli' weights")
     if x.dim() != 3 or x.shape[2] != 8:
@@ -1081,7 +1081,7 @@ def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_
     ``saved`` and ``routing`` as the forward returned them, the adjoint weights from
     ``prepare_adjoint_weights(w, "pauli")``; dout and dx (N, d, 8) bf16, the weights' gradients fp32."""
     topk_w, offsets = routing["topk_w"], routing["offsets"]
-    dev = _one_device(dout, saved, topk_w, offsets)
+    dev = _one_device(dout, saved, topk_w, offsets, w_up_adj.data, w_down_adj.data)
     if w_up_adj.fmt != "pauli" or w_down_adj.fmt != "pauli" or dout.dtype != torch.bfloat16:
         raise ValueError("moe_backward_bf16: bf16 dout and adjoint weights prepared as 'pauli'")
     E, d, F = w_up_adj.E, w_up_adj.d_out, w_up_adj.d_in
