@@ -210,3 +210,16 @@ def test_gradients_are_not_differentiated_again(capturing, monkeypatch, dtype):
     a = torch.tensor(3.0, requires_grad=True)
     dres, = torch.autograd.grad(out, [res], a * torch.ones_like(out), create_graph=True)
     assert torch.autograd.grad(dres.sum(), [a])[0] == dres.numel()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bf16_training_step_takes_no_inference_workspace(capturing, monkeypatch, dtype):
+    seen = []
+    monkeypatch.setattr(layers.ops, "moe_workspace_bytes", lambda *a: 1000)
+    monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
+                        seen.append(workspace) or (2 * flat, (torch.zeros(0),) * 4))
+    monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
+    layer = _layer(dtype)
+    layer.moe_forward(torch.ones(1, 5, 4, 8, dtype=dtype))
+    kept = layer.__dict__["_workspace"]
+    assert (kept is None and seen == [None]) if dtype == torch.bfloat16 else seen[0] is kept and kept.numel() == 1000

@@ -248,8 +248,10 @@ class CliffordMoELayer(nn.Module):
                 residual = residual.reshape(x.shape).contiguous()
             if residual.dtype != x.dtype:
                 raise ValueError("residual must have x's shape and dtype")
-        ws_bytes = ops.moe_workspace_bytes(N, d, cfg.d_ff, E, cfg.top_k, cfg.dtype, cfg.weight_format)
-        ws = _call_workspace(self, ws_bytes, x.device)
+        ws = None
+        if not graph or cfg.weight_format == "pauli_f32":  # (a bf16 training step keeps its rows elsewhere)
+            ws_bytes = ops.moe_workspace_bytes(N, d, cfg.d_ff, E, cfg.top_k, cfg.dtype, cfg.weight_format)
+            ws = _call_workspace(self, ws_bytes, x.device)
         if graph:
             flat = x.reshape(N, d, 8)
             res = residual.reshape(N, d, 8) if residual is not None else None
