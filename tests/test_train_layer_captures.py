@@ -65,7 +65,7 @@ def _autograd(monkeypatch):
     none = torch.zeros(0)
     monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
                         (2 * flat, (none, none, none, none)))
-    monkeypatch.setattr(layers, "_train_backward", lambda layer, prep, flat, logits, kept, dout, residual:
+    monkeypatch.setattr(layers, "_train_backward", lambda layer, prep, flat, logits, kept, dout, residual, experts=None:
                         (2 * dout, *(torch.zeros_like(getattr(layer, n)) for n in ("w_up", "b_up", "w_down", "b_down")),
                          None, None, None))
     monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
@@ -223,3 +223,26 @@ def test_a_bf16_training_step_takes_no_inference_workspace(capturing, monkeypatc
     layer.moe_forward(torch.ones(1, 5, 4, 8, dtype=dtype))
     kept = layer.__dict__["_workspace"]
     assert (kept is None and seen == [None]) if dtype == torch.bfloat16 else seen[0] is kept and kept.numel() == 1000
+
+
+@pytest.mark.parametrize("frozen", [("w_up", "b_up"), ("w_down", "b_down"), ("w_up", "b_up", "w_down", "b_down"), ("w_up",)])
+def test_frozen_experts_have_no_weight_products(capturing, monkeypatch, frozen):
+    seen = []
+    monkeypatch.setattr(layers, "_train_forward", lambda layer, flat, res, logits, prep, workspace=None:
+                        (2 * flat, (torch.zeros(0),) * 4))
+    monkeypatch.setattr(layers.ops, "stream_handle", lambda dev: 0)
+
+    def backward(dout, rows, routing, up, down, act, residual, routing_grad, up_grad, down_grad):
+        seen.append((up_grad, down_grad))
+        z = lambda n, want: torch.zeros_like(getattr(layer, n)) if want else None
+        return dout, z("w_up", up_grad), z("b_up", up_grad), z("w_down", down_grad), z("b_down", down_grad), None
+
+    monkeypatch.setattr(layers.ops, "moe_backward_bf16", backward)
+    layer = _layer()
+    for n in frozen:
+        getattr(layer, n).requires_grad_(False)
+    x = torch.ones(1, 5, 4, 8, dtype=torch.bfloat16, requires_grad=True)
+    layer.moe_forward(x).sum().backward()
+    assert seen == [(not {"w_up", "b_up"} <= set(frozen), not {"w_down", "b_down"} <= set(frozen))] and x.grad is not None
+    assert [n for n in ("w_up", "b_up", "w_down", "b_down") if getattr(layer, n).grad is None] == sorted(frozen, key=(
+        "w_up", "b_up", "w_down", "b_down").index)

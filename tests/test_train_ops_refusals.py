@@ -334,3 +334,10 @@ def test_weights_prepared_on_another_device_are_refused(monkeypatch):
               lambda: ops.moe_backward_bf16(a, a, routing, here, there), lambda: ops.moe_backward_bf16(a, a, routing, there, here)):
         with pytest.raises(ValueError, match="one device"):
             f()
+
+
+@pytest.mark.parametrize("at", [15, 16, 17, 18])
+def test_a_weights_gradient_without_its_biases(at):
+    args = list(_BWD)
+    args[at] = None
+    _refused("ygg_moe_backward_bf16", args, "together")

@@ -212,11 +212,12 @@ YGG_API int ygg_moe_backward_bf16(int N, int d, int F, int E, int k, int act, co
                                   float* dw_down, float* db_down, float* dtopk_w, void* workspace, size_t workspace_bytes,
                                   hipStream_t stream) {
   if (check_sizes("ygg_moe_backward_bf16", N, d, F, E, k, act)) return -1;
-  YGG_CHECK_ARG(dw_up && dw_down && db_up && db_down, "ygg_moe_backward_bf16: null pointer");
+  YGG_CHECK_ARG(!dw_up == !db_up && !dw_down == !db_down,
+                "ygg_moe_backward_bf16: null pointer (a weight's gradient and its bias's are given together or not at all)");
   if (N == 0) {  // no tokens: the weight and bias gradients are zero
     const size_t nw = (size_t)E * F * d * 8;
-    return fill_zero_f32(dw_up, nw, stream) || fill_zero_f32(dw_down, nw, stream) ||
-                   fill_zero_f32(db_up, (size_t)E * F * 8, stream) || fill_zero_f32(db_down, (size_t)E * d * 8, stream)
+    return (dw_up && (fill_zero_f32(dw_up, nw, stream) || fill_zero_f32(db_up, (size_t)E * F * 8, stream))) ||
+                   (dw_down && (fill_zero_f32(dw_down, nw, stream) || fill_zero_f32(db_down, (size_t)E * d * 8, stream)))
                ? -1 : 0;
   }
   YGG_CHECK_ARG(w_up_adj && w_down_adj && dout && saved && topk_w && offsets && dx && workspace,
@@ -240,9 +241,9 @@ YGG_API int ygg_moe_backward_bf16(int N, int d, int F, int E, int k, int act, co
   if (check_launch("combine backward (bf16)")) return -1;
   if (ygg_pauli_grouped_input_grad(dy, P, w_down_adj, offsets, E, d, F, act, keep + at.h_pre, dh, /*Pauli rows*/ 0, kBF16,
                                    stream) ||
-      weight_grad_bf16(dy, keep + at.h, P, nullptr, offsets, P, E, F, d, dw_down, db_down, wg, stream) ||
+      (dw_down && weight_grad_bf16(dy, keep + at.h, P, nullptr, offsets, P, E, F, d, dw_down, db_down, wg, stream)) ||
       ygg_pauli_grouped_input_grad(dh, P, w_up_adj, offsets, E, F, d, kActNone, nullptr, dxs, /*blade*/ 1, kBF16, stream) ||
-      weight_grad_bf16(dh, keep + at.x, N, perm, offsets, P, E, d, F, dw_up, db_up, wg, stream))
+      (dw_up && weight_grad_bf16(dh, keep + at.x, N, perm, offsets, P, E, d, F, dw_up, db_up, wg, stream)))
     return -1;
   hipLaunchKernelGGL(dispatch_backward_bf16_kernel, dim3((unsigned)N), dim3(d <= 64 ? 64 : d <= 128 ? 128 : 256), 0, stream,
                      reinterpret_cast<const uint16_t*>(dxs), N, k, d, slot_pos,

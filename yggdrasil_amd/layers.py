@@ -457,10 +457,11 @@ def _for_backward(layer, flat, logits):
             logits if fp32 and logits is not None else flat.new_empty(0))
 
 
-def _train_backward(layer, prep, flat, logits, kept, dout, residual: bool):
+def _train_backward(layer, prep, flat, logits, kept, dout, residual: bool, experts=(True,) * 4):
     """Gradients of :func:`_train_forward`: ``(dx, dW_up, db_up, dW_down, db_down, drouter_weight, drouter_bias,
     dlogits)``, the last three None where the router gets none.  prep: the forward's layouts (fp32 layers).
-    ``residual``: dx includes dout (bf16 layers)."""
+    ``residual``: dx includes dout (bf16 layers).  ``experts``: which of W_up, b_up, W_down and b_down need gradients
+    (a bf16 layer leaves out the products of a frozen pair)."""
     rows, idx, w, offsets = kept
     cfg = layer.cfg
     adj = layer._adjoint_layouts() if _capturing() else layer._get_adjoint()
@@ -473,7 +474,8 @@ def _train_backward(layer, prep, flat, logits, kept, dout, residual: bool):
             h_pre=rows, residual=residual)
     else:
         dx, *grads, dtw = ops.moe_backward_bf16(dout, rows, dict(topk_w=w, offsets=offsets), adj["w_up"], adj["w_down"],
-                                                cfg.activation, residual=residual, routing_grad=cfg.router_grad)
+                                                cfg.activation, residual=residual, routing_grad=cfg.router_grad,
+                                                up_grad=any(experts[:2]), down_grad=any(experts[2:]))
     drw = drb = dlogits = None
     if cfg.router_grad and logits is not None:
         dlogits = ops.route_backward(idx, w, dtw, cfg.n_experts)
@@ -511,7 +513,7 @@ class _MoEFunction(torch.autograd.Function):
             _refuse_beside_eager(ctx.layer)
         _check_versions(ctx.layer, ctx.versions, logits)
         dx, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
-            ctx.layer, ctx.prep, flat, logits, kept, dout, residual=False)
+            ctx.layer, ctx.prep, flat, logits, kept, dout, residual=False, experts=ctx.needs_input_grad[2:6])
         return dx, (dout if ctx.has_res else None), dWu, dbu, dWd, dbd, drw, drb, None, None, None, dlogits
 
 
@@ -705,7 +707,7 @@ class _BlockFunction(torch.autograd.Function):
         _check_versions(ctx.block.moe, ctx.versions, logits)
         dout = dout.contiguous()
         dxn, dWu, dbu, dWd, dbd, drw, drb, dlogits = _train_backward(
-            ctx.block.moe, ctx.prep, xn, logits, kept, dout, residual=False)
+            ctx.block.moe, ctx.prep, xn, logits, kept, dout, residual=False, experts=ctx.needs_input_grad[3:7])
         dx, dgamma, dbeta = ops.clifford_layer_norm_backward(dxn, x, gamma, ctx.eps, residual_grad=dout)
         return (dx, dgamma.to(gamma.dtype), dbeta.to(ctx.beta_dtype), dWu, dbu, dWd, dbd, drw, drb, None,
                 dlogits if ctx.from_caller else None)

@@ -1075,8 +1075,10 @@ def moe_forward_train_bf16(x: torch.Tensor, k: int, w_up: PreparedWeights, w_dow
 
 @_on_its_device
 def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_up_adj: PreparedWeights,
-                      w_down_adj: PreparedWeights, act: str = "gelu", residual: bool = False, routing_grad: bool = False):
-    """Backward of :func:`moe_forward_train_bf16`: ``(dx, dW_up, db_up, dW_down, db_down, dtopk_w or None)``.
+                      w_down_adj: PreparedWeights, act: str = "gelu", residual: bool = False, routing_grad: bool = False,
+                      up_grad: bool = True, down_grad: bool = True):
+    """Backward of :func:`moe_forward_train_bf16`: ``(dx, dW_up, db_up, dW_down, db_down, dtopk_w or None)``.  Without
+    ``up_grad`` dW_up and db_up are not computed and None, without ``down_grad`` dW_down and db_down.
 
     ``saved`` and ``routing`` as the forward returned them, the adjoint weights from
     ``prepare_adjoint_weights(w, "pauli")``; dout and dx (N, d, 8) bf16, the weights' gradients fp32."""
@@ -1099,8 +1101,11 @@ def moe_backward_bf16(dout: torch.Tensor, saved: torch.Tensor, routing: dict, w_
     ws = torch.empty((max(ws_bytes, 1),), device=dev, dtype=torch.uint8)
     f32 = dict(device=dev, dtype=torch.float32)
     dx = torch.empty_like(dout)
-    dWu, dbu = torch.empty((E, F, d, 8), **f32), torch.empty((E, F, 8), **f32)
-    dWd, dbd = torch.empty((E, d, F, 8), **f32), torch.empty((E, d, 8), **f32)
+    dWu = dbu = dWd = dbd = None
+    if up_grad:
+        dWu, dbu = torch.empty((E, F, d, 8), **f32), torch.empty((E, F, 8), **f32)
+    if down_grad:
+        dWd, dbd = torch.empty((E, d, F, 8), **f32), torch.empty((E, d, 8), **f32)
     dtw = torch.empty((Nt, k), **f32) if routing_grad else None
     check(L.ygg_moe_backward_bf16(Nt, d, F, E, k, ACT_CODE[act], ptr(w_up_adj.data), ptr(w_down_adj.data), int(residual),
                                   ptr(dout), ptr(saved), saved.numel(), ptr(topk_w), ptr(offsets), ptr(dx), ptr(dWu),
