@@ -220,8 +220,9 @@ __global__ __launch_bounds__(256, 2) void weight_grad_bf16_kernel(
   auto loop = [&](auto bias_tag) __attribute__((always_inline)) {
     constexpr bool BIAS = decltype(bias_tag)::value;
     for (int f = 0; f < nf; ++f) {
-      // the loads of the newer stage may stay outstanding
-      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kWbStages - 2) * 2 * kWbWaveRows) : "memory");
+      // the loads of the newer stage may stay outstanding; this wave's reads of the stage that is loaded over next have
+      // returned
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kWbStages - 2) * 2 * kWbWaveRows) : "memory");
       const unsigned char* st = smem + (f % kWbStages) * kWbStage;
       uint32_t d[kWbRows / 4][2][4], a[kWbRows / 4][2][4];  // [four rows][block][half-row]
 #pragma unroll
