@@ -341,3 +341,10 @@ def test_a_weights_gradient_without_its_biases(at):
     args = list(_BWD)
     args[at] = None
     _refused("ygg_moe_backward_bf16", args, "together")
+
+
+@pytest.mark.parametrize("E,few", [(1, 252), (2, 348), (3, 348), (4, 444), (8, 540), (15, 540), (16, 636), (32, 732), (64, 828)])
+def test_weight_gradients_of_few_rows_take_no_workspace(E, few):
+    """252 + 96 log2(E) rows and fewer are one chunk an expert; one row more has planes."""
+    need = lambda P: N.lib().ygg_grouped_weight_grad_pauli_bf16_workspace_bytes(P, E, 64, 256)
+    assert need(1) == need(few) == 0 and need(few + 1) > 0

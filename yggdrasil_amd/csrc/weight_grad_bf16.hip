@@ -25,7 +25,6 @@ constexpr int kWbRows = 12;      // rows of a stage
 constexpr int kWbStages = 3;    // stages in LDS: two in flight while one is read
 constexpr int kWbWaveRows = kWbRows / 4;  // rows that a wave loads per stage
 constexpr int kWbMaxChunk = 1024, kWbMinChunk = 256;  // rows of a workgroup at most, see chunk_rows
-constexpr int kWbMaxRows1 = 516;  // rows up to which every expert is one chunk
 constexpr int kWbHalf = kWbTile * 8;               // bytes of a half-row of a stage
 constexpr int kWbOperand = kWbRows * 2 * kWbHalf;  // bytes of one operand of a stage
 constexpr int kWbStage = 2 * kWbOperand;
@@ -337,10 +336,26 @@ long long wb_tiles(int d_in, int d_out) {
 // within limits.  More rows leave CUs idle at the end, fewer make more planes, which the reduction reads at the
 // rate of memory: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's law took 180 us with 512 rows, 170 with 768,
 // 161 with this rule's 1024 (and the longest chunks first), 276 with 2048; 1500 tokens, d = 100, F = 300, E = 12,
-// k = 3 took 35 us with 512, 28 with 256, 29 with 128.  Few rows take one chunk an expert, no planes and no second
-// launch (256 tokens, d = 64, F = 256, E = 8, k = 2: 16 us a call with planes, 11 without).
-int chunk_rows(int P, int d_in, int d_out) {
-  if (P <= kWbMaxRows1) return kWbMaxRows1;  // one chunk an expert: no planes and no second launch
+// k = 3 took 35 us with 512, 28 with 256, 29 with 128.
+//
+// Few rows take one chunk an expert, no planes and no second launch.  That pays while the largest expert has little
+// more than the 252 rows of the shortest chunks, which the host does not know: it is taken for Zipf's law over E experts
+// (exponent 1.2), whose crossover lies at or above 252 + 96 log2(E) rows at all widths measured.  One chunk and chunks of
+// 252, us by graph replay, d = 64, F = 256: E = 1, 256 rows 18.8 and 15.3, 516 rows 30.4 and 18.6; E = 4, 400 rows 16.6
+// and 18.2, 516 rows 19.4 and 15.7; E = 8, 516 rows 17.4 and 19.0, 640 rows 19.5 and 15.8; E = 16, 640 rows 18.4 and
+// 20.3, 768 rows 20.6 and 17.0; E = 32, 768 rows 20.0 and 22.4, 900 rows 22.1 and 18.9; E = 64, 768 rows 20.6 and 24.7,
+// 900 rows 22.2 and 21.6 (d = 256, F = 1024: E = 4, 400 rows 25.8 and 29.8, 516 rows 30.3 and 29.1; E = 32, 768 rows 82 and
+// 107).  Even experts gain at every such size (E = 8, 516 rows 10.3 and 11.9); all rows at one of eight experts lose
+// (516 rows 30.6 and 18.2).
+int rows_of_one_chunk(int E) {
+  int log2e = 0;
+  while (E >> (log2e + 1)) ++log2e;
+  return 252 + 96 * log2e;
+}
+int chunk_rows(int P, int E, int d_in, int d_out) {
+  const int few = rows_of_one_chunk(E);
+  static_assert((252 + 96 * 6) <= kWbMaxChunk && 252 % kWbRows == 0 && 96 % kWbRows == 0, "chunks are whole stages");
+  if (P <= few) return few;
   const long long even = (long long)P * wb_tiles(d_in, d_out) / 512;
   return (int)std::min<long long>(kWbMaxChunk, std::max<long long>(kWbMinChunk, even)) / kWbRows * kWbRows;
 }
@@ -357,20 +372,20 @@ const char* weight_grad_bf16_limit(int P_max, int E, int d_in, int d_out, bool g
   // offsets inside a chunk, past its end by the stages in flight, are 32 bits with one bit for "outside"
   if ((long long)(kWbMaxChunk + kWbRows * (kWbStages + 1)) * std::max(d_in, d_out) * 16 >= 1LL << 31)
     return "the weight gradient's chunks of rows reach 2 GiB";
-  if ((wb_chunks(P_max, E, chunk_rows(P_max, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) >= 1LL << 24)
+  if ((wb_chunks(P_max, E, chunk_rows(P_max, E, d_in, d_out)) + 8) * wb_tiles(d_in, d_out) >= 1LL << 24)
     return "the weight gradient exceeds a launch";
   if (gathered && (long long)a_rows * d_in * 16 >= 1LL << 31) return "gathered rows span 2 GiB or more";
   return nullptr;
 }
 
 size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out) {
-  return (size_t)wb_planes(P_max, E, chunk_rows(P_max, d_in, d_out)) * d_out * (d_in + 1) * 8 * sizeof(float);
+  return (size_t)wb_planes(P_max, E, chunk_rows(P_max, E, d_in, d_out)) * d_out * (d_in + 1) * 8 * sizeof(float);
 }
 
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream) {
   if (E == 0) return 0;
-  const int limit = chunk_rows(P_max, d_in, d_out);
+  const int limit = chunk_rows(P_max, E, d_in, d_out);
   const long long planes = wb_planes(P_max, E, limit), chunks = wb_chunks(P_max, E, limit);
   float* part = static_cast<float*>(workspace);
   float* dbpart = part + (size_t)planes * d_out * d_in * 8;
