@@ -153,29 +153,31 @@ def test_weights_first_laid_out_in_a_capture(graph_of):
         assert torch.equal(got, want) and torch.equal(run(m), want)
 
 
-@pytest.mark.parametrize("block,dtype", [(False, torch.float32), (True, torch.bfloat16)])
-def test_an_inference_graph_keeps_the_layouts_of_its_capture(block, dtype):
-    """New weights are laid out beside those that a graph reads."""
-    m = _layer(np.random.default_rng(30), 16, 24, 4, 2, dtype, block=block)
+@pytest.mark.parametrize("block,dtype,router", [(False, torch.float32, "energy"), (True, torch.bfloat16, "energy"),
+                                                (False, torch.float32, "clifford_head")])
+def test_an_inference_graph_follows_the_weights(block, dtype, router):
+    """New weights, once an eager call has laid them out, are those of the graph's next replays."""
+    m = _layer(np.random.default_rng(30), 16, 24, 4, 2, dtype, block=block, router=router)
     x = _tokens(np.random.default_rng(31), 1, 20, 16, dtype)
-    say(f"an inference graph beside new weights, block={block} {dtype}")
+    say(f"an inference graph beside new weights, block={block} {dtype} {router}")
     with torch.no_grad():
         _run(m, x, block)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             got = _run(m, x, block)
-        graph.replay()
-        torch.cuda.synchronize()
-        want = got.clone()
         moe = m.moe if block else m
         for _ in range(3):
             moe.w_up.mul_(1.5)
-            assert not torch.equal(_run(m, x, block), want)
+            moe.b_down.add_(0.25)
+            want = _run(m, x, block).clone()
             other = [torch.full((n,), 255, device="cuda", dtype=torch.uint8) for n in (4096, 65536, 1 << 20) for _ in range(8)]
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+            fresh = _layer(np.random.default_rng(30), 16, 24, 4, 2, dtype, block=block, router=router)
+            fresh.load_state_dict(m.state_dict())
+            assert torch.equal(_run(fresh, x, block), want)
             del other
 
 

@@ -3,7 +3,6 @@ the layouts are copies of the weights here, a capture is one that says so, and a
 version counters, as the replays of a graph do."""
 
 import copy
-import weakref
 
 import pytest
 import torch
@@ -107,21 +106,30 @@ def test_layouts_of_a_capture_are_found_by_nothing_else(capturing, dtype):
     assert step is not after and layer._get_prepared() is not step
 
 
-def test_layouts_that_a_capture_reads_stay(capturing):
-    """An inference graph reads the layouts that it found at every replay: new ones do not free them."""
+def test_layouts_that_a_capture_reads_are_written_over(capturing):
+    """An inference graph reads the layouts that it found at every replay: new ones take their place in memory."""
     layer = _layer(torch.float32)
     layer._get_prepared()
     capturing[0] = True
     read = layer._get_prepared()
     assert layer._get_prepared() is read
     capturing[0] = False
-    alive = weakref.ref(read["w_up"])
+    for _ in range(3):
+        with torch.no_grad():
+            layer.w_up.add_(1.0)
+            layer.b_down.sub_(2.0)
+        new = layer._get_prepared()
+        assert _fresh(layer) and new is layer._get_prepared()
+        for n in ("w_up", "w_down"):
+            assert new[n].data.data_ptr() == read[n].data.data_ptr() and torch.equal(read[n].data, getattr(layer, n))
+        assert new["b_down"].data_ptr() == read["b_down"].data_ptr() and torch.equal(read["b_down"], layer.b_down)
+    capturing[0] = True  # and without a capture they are not
+    layer = _layer(torch.float32)
+    capturing[0] = False
+    old = layer._get_prepared()
     with torch.no_grad():
         layer.w_up.add_(1.0)
-    new = layer._get_prepared()
-    del read
-    assert new["w_up"] is not alive() and alive() is not None
-    assert "_kept" in layer.__dict__ and "_kept" not in copy.deepcopy(layer).__dict__
+    assert layer._get_prepared()["w_up"].data.data_ptr() != old["w_up"].data.data_ptr()
 
 
 def test_a_captured_backward_reads_layouts_of_its_own(capturing, monkeypatch):
@@ -246,3 +254,23 @@ def test_frozen_experts_have_no_weight_products(capturing, monkeypatch, frozen):
     assert seen == [(not {"w_up", "b_up"} <= set(frozen), not {"w_down", "b_down"} <= set(frozen))] and x.grad is not None
     assert [n for n in ("w_up", "b_up", "w_down", "b_down") if getattr(layer, n).grad is None] == sorted(frozen, key=(
         "w_up", "b_up", "w_down", "b_down").index)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_a_router_head_that_a_capture_read(capturing, dtype):
+    """An fp32 head is the parameter itself, which no new layout writes; one of another type is a copy, which is."""
+    layer = layers.CliffordMoELayer(layers.MoEHLMConfig(d_model=4, d_ff=6, n_experts=3, router="clifford_head"))
+    layer.head_weight = torch.nn.Parameter(layer.head_weight.detach().to(dtype))
+    layer._get_prepared()
+    capturing[0] = True
+    read = layer._get_prepared()["head"]
+    capturing[0] = False
+    first = layer.head_weight
+    kept = first.detach().clone()
+    with torch.no_grad():
+        other = torch.nn.Parameter(2 * first)
+        other.add_(1.0)
+    layer.head_weight = other  # replaced, not changed in place
+    new = layer._get_prepared()["head"]
+    assert torch.equal(first, kept) and torch.equal(new, other.float())
+    assert (new is read) == (dtype == torch.float64)

@@ -179,15 +179,16 @@ class CliffordMoELayer(nn.Module):
     _replayed = False
 
     def __getstate__(self):
-        return {n: v for n, v in self.__dict__.items() if n not in ("_replayed", "_kept")}  # (no graph knows a copy)
+        return {n: v for n, v in self.__dict__.items() if n != "_replayed"}  # (no graph updates a copy's parameters)
 
     @torch.no_grad()
     def prepare(self):
         """Build the device weight layouts (done lazily; redone when parameters change).  In a capture they are the
-        graph's own, which lays the weights out anew at every replay: no other call finds them."""
+        graph's own, which lays the weights out anew at every replay: no other call finds them.  Layouts that a graph
+        reads are written over in place."""
         prep = self._layouts()
         if not _capturing():
-            self._prepared = prep
+            prep = self._prepared = _into_captured(self._prepared, prep)
         return prep
 
     def _layouts(self) -> dict:
@@ -204,16 +205,15 @@ class CliffordMoELayer(nn.Module):
                                 ("b_down", b_down.shape, (E, d, 8))):
             if got != want:
                 raise ValueError(f"{name} must be of shape {want}, got {tuple(got)}")
-        return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head)
+        return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head,
+                    head_copied=head is not None and head.data_ptr() != self.head_weight.data_ptr())
 
     def _get_prepared(self):
         prep = self._prepared
         if self._replayed or prep is None or prep["key"] != self._param_versions():
             return self.prepare()
-        if _capturing():  # the graph reads these layouts at every replay: they outlive the next ones
-            kept = self.__dict__.setdefault("_kept", [])
-            if not any(k is prep for k in kept):
-                kept.append(prep)
+        if _capturing():
+            prep["captured"] = True
         return prep
 
     # -- forward ---------------------------------------------------------------
@@ -338,6 +338,29 @@ class CliffordMoELayer(nn.Module):
 
 def _capturing() -> bool:
     return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _tensors(prep):
+    """What was laid out (an fp32 router head is the parameter itself)."""
+    for name, v in prep.items():
+        if isinstance(v, ops.PreparedWeights):
+            yield from (t for t in (v.data, v.scales) if t is not None)
+        elif isinstance(v, torch.Tensor) and (name != "head" or prep["head_copied"]):
+            yield v
+
+
+def _into_captured(old, new) -> dict:
+    """The layouts to keep in the place of `old`.  Where a graph reads those at every replay, the new values are written
+    into them: the graph follows the weights, as it follows the router's, and reads no memory that has been freed."""
+    if old is None or not old.get("captured"):
+        return new
+    pairs = list(zip(_tensors(old), _tensors(new)))
+    if len(pairs) != len(list(_tensors(old))) or any(a.shape != b.shape or a.dtype != b.dtype or a.device != b.device
+                                                     for a, b in pairs):
+        return new  # (moved or replaced by others: the parameters that such a graph reads are gone too)
+    for a, b in pairs:
+        a.copy_(b)
+    return dict(old, key=new["key"], **({} if new["head_copied"] else dict(head=new["head"])))
 
 
 def _call_workspace(module, need: int, dev) -> torch.Tensor:
