@@ -274,3 +274,22 @@ def test_a_router_head_that_a_capture_read(capturing, dtype):
     new = layer._get_prepared()["head"]
     assert torch.equal(first, kept) and torch.equal(new, other.float())
     assert (new is read) == (dtype == torch.float64)
+
+
+def test_layouts_of_a_single_product_in_captures(capturing):
+    """CliffordLinear: a capture's own layouts where its weights had changed, the module's written over where not."""
+    lin = layers.CliffordLinear(4, 6)
+    lin._prepared()
+    capturing[0] = True
+    read = lin._prepared()
+    capturing[0] = False
+    with torch.no_grad():
+        lin.weight.add_(1.0)
+    new = lin._prepared()
+    assert new["w"].data.data_ptr() == read["w"].data.data_ptr() and torch.equal(read["w"].data[0], lin.weight)
+    with torch.no_grad():
+        lin.weight.add_(1.0)
+    capturing[0] = True
+    own = lin._prepared()
+    capturing[0] = False
+    assert own["w"] is not lin._prepared()["w"] and torch.equal(lin._prepared()["w"].data[0], lin.weight)

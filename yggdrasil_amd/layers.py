@@ -360,7 +360,7 @@ def _into_captured(old, new) -> dict:
         return new  # (moved or replaced by others: the parameters that such a graph reads are gone too)
     for a, b in pairs:
         a.copy_(b)
-    return dict(old, key=new["key"], **({} if new["head_copied"] else dict(head=new["head"])))
+    return dict(old, key=new["key"], **({} if new.get("head_copied", True) else dict(head=new["head"])))
 
 
 def _call_workspace(module, need: int, dev) -> torch.Tensor:
@@ -554,16 +554,22 @@ class CliffordLinear(nn.Module):
 
     def _prepared(self):
         key = (self.weight._version, None if self.bias is None else self.bias._version, self.weight.device)
-        if self._prep is None or self._prep[0] != key:
+        prep, capturing = self._prep, _capturing()
+        if not isinstance(prep, dict) or prep["key"] != key:  # (a module saved with another kind of layout)
             fmt = "pauli_f32" if self.dtype == torch.float32 else "bf16"
-            self._prep = (key, ops.prepare_weights(self.weight.detach().unsqueeze(0), fmt),
-                          ops.prepare_bias(self.bias.detach().unsqueeze(0)) if self.bias is not None else None)
-        return self._prep
+            prep = dict(key=key, w=ops.prepare_weights(self.weight.detach().unsqueeze(0), fmt),
+                        b=ops.prepare_bias(self.bias.detach().unsqueeze(0)) if self.bias is not None else None)
+            if capturing:  # the graph's own
+                return prep
+            prep = self._prep = _into_captured(self._prep if isinstance(self._prep, dict) else None, prep)
+        if capturing:
+            prep["captured"] = True
+        return prep
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         batch = x.shape[:-2]
-        _, pw, pb = self._prepared()
-        y = ops.clifford_linear(x.reshape(-1, self.d_in, 8).to(self.dtype).contiguous(), pw, pb)
+        prep = self._prepared()
+        y = ops.clifford_linear(x.reshape(-1, self.d_in, 8).to(self.dtype).contiguous(), prep["w"], prep["b"])
         return y.reshape(*batch, self.d_out, 8)
 
 
