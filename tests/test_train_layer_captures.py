@@ -156,13 +156,14 @@ def test_a_captured_backward_reads_layouts_of_its_own(capturing, monkeypatch):
 def test_a_graph_has_a_workspace_of_its_own(capturing):
     """What a graph writes is no tensor that a later eager call may free."""
     layer, dev = _layer(torch.float32), torch.device("cpu")
-    ws = layers._call_workspace(layer, 100, dev)
-    assert ws.numel() == 100 and layers._call_workspace(layer, 50, dev) is ws
+    take = lambda need: layers._call_workspace(layer, need, dev, capturing[0])
+    ws = take(100)
+    assert ws.numel() == 100 and take(50) is ws
     capturing[0] = True
-    own = layers._call_workspace(layer, 50, dev), layers._call_workspace(layer, 500, dev)
+    own = take(50), take(500)
     assert own[0] is not ws and own[1].numel() == 500 and layer._workspace is ws
     capturing[0] = False
-    assert layers._call_workspace(layer, 100, dev) is ws and layers._call_workspace(layer, 101, dev) is not ws
+    assert take(100) is ws and take(101) is not ws
 
 
 def test_a_captured_fp32_backward_is_refused_while_an_eager_graph_lives(capturing, monkeypatch):

@@ -208,11 +208,11 @@ class CliffordMoELayer(nn.Module):
         return dict(key=self._param_versions(), w_up=w_up, w_down=w_down, b_up=b_up, b_down=b_down, head=head,
                     head_copied=head is not None and head.data_ptr() != self.head_weight.data_ptr())
 
-    def _get_prepared(self):
+    def _get_prepared(self, capturing: bool | None = None):
         prep = self._prepared
         if self._replayed or prep is None or prep["key"] != self._param_versions():
             return self.prepare()
-        if _capturing():
+        if _capturing() if capturing is None else capturing:
             prep["captured"] = True
         return prep
 
@@ -234,7 +234,8 @@ class CliffordMoELayer(nn.Module):
         if not x.is_contiguous():
             x = x.contiguous()
         graph = self._needs_grad(x, residual, logits)
-        prep = _step_layouts(self) if graph else self._get_prepared()
+        capturing = x.is_cuda and torch.cuda.is_current_stream_capturing()
+        prep = _step_layouts(self) if graph else self._get_prepared(capturing)
         if cfg.router == "logits":
             if logits is None:
                 raise ValueError("router='logits' needs logits")
@@ -251,7 +252,7 @@ class CliffordMoELayer(nn.Module):
         ws = None
         if not graph or cfg.weight_format == "pauli_f32":  # (a bf16 training step keeps its rows elsewhere)
             ws_bytes = ops.moe_workspace_bytes(N, d, cfg.d_ff, E, cfg.top_k, cfg.dtype, cfg.weight_format)
-            ws = _call_workspace(self, ws_bytes, x.device)
+            ws = _call_workspace(self, ws_bytes, x.device, capturing)
         if graph:
             flat = x.reshape(N, d, 8)
             res = residual.reshape(N, d, 8) if residual is not None else None
@@ -363,11 +364,11 @@ def _into_captured(old, new) -> dict:
     return dict(old, key=new["key"], **({} if new.get("head_copied", True) else dict(head=new["head"])))
 
 
-def _call_workspace(module, need: int, dev) -> torch.Tensor:
+def _call_workspace(module, need: int, dev, capturing: bool) -> torch.Tensor:
     """The workspace of a call: kept by the module for its next one, except in a capture.  A graph's is its own, since
     an eager call of more tokens would free the module's while the graph still writes it."""
     ws = module.__dict__["_workspace"]
-    if _capturing():
+    if capturing:
         return torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
     if ws is None or ws.numel() < need or ws.device != dev:
         ws = module.__dict__["_workspace"] = torch.empty((max(need, 1),), device=dev, dtype=torch.uint8)
@@ -683,7 +684,8 @@ class CliffordMoEBlockFFN(nn.Module):
             raise ValueError("router='logits' needs logits")
         B, T = x.shape[:2]
         flat = x.reshape(B * T, cfg.d_model, 8).contiguous()
-        prep = moe._get_prepared()
+        capturing = x.is_cuda and torch.cuda.is_current_stream_capturing()
+        prep = moe._get_prepared(capturing)
         if logits is not None:
             logits = logits.reshape(B * T, cfg.n_experts).float().contiguous()
         ws_bytes = ops.moe_block_ffn_workspace_bytes(B * T, cfg.d_model, cfg.d_ff, cfg.n_experts, cfg.top_k,
@@ -693,7 +695,7 @@ class CliffordMoEBlockFFN(nn.Module):
             prep["w_down"], prep["b_up"], prep["b_down"], cfg.activation, logits=logits,
             router_weight=moe.router_weight.detach() if logits is None else None,
             router_bias=moe.router_bias.detach() if logits is None else None, norm_eps=self.ffn_norm.eps,
-            workspace=_call_workspace(self, ws_bytes, x.device))
+            workspace=_call_workspace(self, ws_bytes, x.device, capturing))
         moe.last_routing = routing
         return out.reshape(B, T, cfg.d_model, 8)
 
