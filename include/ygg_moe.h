@@ -378,7 +378,8 @@ int ygg_grouped_weight_grad_pauli_bf16(const void* dy_pauli, const void* a_pauli
  * forward added x to its output), dw_up (E, F, d, 8), db_up (E, F, 8), dw_down (E, d, F, 8),
  * db_down (E, d, 8) fp32 -- dw_up and db_up, or dw_down and db_down, may be NULL: not
  * computed -- and dtopk_w (N, k) when not NULL.  Rows between two operators are
- * bf16, sums inside one fp32.  `saved` is only read by the backward. */
+ * bf16, sums inside one fp32.  `saved` is only read by the backward.  Both refuse sizes beyond
+ * the limits of the products and of the weight gradients. */
 size_t ygg_moe_train_bf16_saved_bytes(int N, int d, int F, int E, int k);
 size_t ygg_moe_forward_train_bf16_workspace_bytes(int N, int d, int F, int E, int k);
 int ygg_moe_forward_train_bf16(const void* x, int N, int d, int F, int E, int k, int act, const float* logits,

@@ -89,13 +89,13 @@ __device__ __forceinline__ void zero_tile(int jt, int it, int e, int d_in, int d
 // One workgroup: 64 (j) x 64 (i) of one chunk's sum, a wave 32 x 32 of it.
 //
 // Bound by the matrix units and the loads into LDS together: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's
-// law take 159 us in all, 140 here and 18 in the planes' sum: 137 GFLOP at 0.98 PFLOP/s here, where a large bf16
-// product reaches 1.37.  The matrix units are busy 48 % of the time: of the two waves that a SIMD holds 1.4 are there
-// on average, as the chunks of uneven experts do not end together.  Without the loads (data in LDS as it was) the
-// whole took 137 us, without the products 133.  Larger tiles did not pay: 128 x 64 with eight waves 160 us, with four
-// waves of 64 x 32, one a SIMD, 179; nor did eight waves on one tile, half of a chunk's rows each (157, and half the
-// planes, but one tile a CU: 1500 ragged tokens as below 26-30 us against 27), reading the next stage's operands
-// into registers ahead (160) or raising the waves' priority (174).
+// law take 153-157 us in all, 131-142 here and 15-16 in the planes' sum: 137 GFLOP at 1.0 PFLOP/s here, where a large
+// bf16 product reaches 1.37.  The matrix units are busy 47 % of the time: of the two waves that a SIMD holds 1.4 are there
+// on average, as the chunks of uneven experts do not end together.  (Variants, against 159 in all at their time:) without
+// the loads (data in LDS as it was) 137 us, without the products 133.  Larger tiles did not pay: 128 x 64 with eight waves
+// 160 us, with four waves of 64 x 32, one a SIMD, 179; nor did eight waves on one tile, half of a chunk's rows each (157,
+// and half the planes, but one tile a CU: 1500 ragged tokens as below 26-30 us against 27), reading the next stage's
+// operands into registers ahead (160) or raising the waves' priority (174).
 //
 // v_mfma_f32_32x32x16_bf16 with the operand rows (j, a) and columns (i, c), 16 of each index: the dword
 // (re, im) of entry a of column b of D_rj is one (r, b) term of the contraction, and four such dwords (two
@@ -334,9 +334,9 @@ long long wb_tiles(int d_in, int d_out) {
 }
 // The rows of a chunk at most: what each of the 512 workgroups that the chip holds would have of all rows' tiles,
 // within limits.  More rows leave CUs idle at the end, fewer make more planes, which the reduction reads at the
-// rate of memory: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's law took 180 us with 512 rows, 170 with 768,
-// 161 with this rule's 1024 (and the longest chunks first), 276 with 2048; 1500 tokens, d = 100, F = 300, E = 12,
-// k = 3 took 35 us with 512, 28 with 256, 29 with 128.
+// rate of memory: 8192 tokens, d = 128, F = 512, E = 32, k = 4, Zipf's law take 171 us with at most 512 rows, 158 with
+// 768, 153 with this rule's 1024; 1500 tokens, d = 100, F = 300, E = 12, k = 3 take 33 us with at least 512 rows, 27 with
+// 256, 29 with 128.
 //
 // Few rows take one chunk an expert, no planes and no second launch.  That pays while the largest expert has little
 // more than the 252 rows of the shortest chunks, which the host does not know: it is taken for Zipf's law over E experts
