@@ -294,3 +294,17 @@ def test_layouts_of_a_single_product_in_captures(capturing):
     own = lin._prepared()
     capturing[0] = False
     assert own["w"] is not lin._prepared()["w"] and torch.equal(lin._prepared()["w"].data[0], lin.weight)
+
+
+def test_layouts_of_inference_mode_that_a_capture_reads(capturing):
+    """Made and captured in inference mode, written over outside of it."""
+    layer = _layer(torch.float32)
+    with torch.inference_mode():
+        layer._get_prepared()
+        capturing[0] = True
+        read = layer._get_prepared()
+        capturing[0] = False
+    with torch.no_grad():
+        layer.w_up.add_(1.0)
+    new = layer._get_prepared()
+    assert new["w_up"].data.data_ptr() == read["w_up"].data.data_ptr() and torch.equal(new["w_up"].data, layer.w_up)

@@ -359,8 +359,9 @@ def _into_captured(old, new) -> dict:
     if len(pairs) != len(list(_tensors(old))) or any(a.shape != b.shape or a.dtype != b.dtype or a.device != b.device
                                                      for a, b in pairs):
         return new  # (moved or replaced by others: the parameters that such a graph reads are gone too)
-    for a, b in pairs:
-        a.copy_(b)
+    with torch.inference_mode():  # (they may have been made in it)
+        for a, b in pairs:
+            a.copy_(b)
     return dict(old, key=new["key"], **({} if new.get("head_copied", True) else dict(head=new["head"])))
 
 
