@@ -30,7 +30,8 @@
  *    3 = bf16 Pauli (the weights as 2x2 complex matrices; even d_in),
  *    4 = fp32 Pauli (fp32 layers; ygg_f32_layer_split says on which MFMA units),
  *    5 = int8 Pauli (the entries of each weight's 2x2 complex matrix, int8 per
- *        output channel; bf16 decode layers of at most 128 tokens, d <= 128).
+ *        output channel; bf16 decode layers of at most 128 tokens, d <= 128),
+ *    6 = the weights of 5, met by rows in int8 (bf16 layers of any size).
  *    activation codes: 0 none, 1 gelu, 2 relu, 3 sigmoid
  *    (holograph/models/hlm_block.py:28-32).
  */
@@ -153,7 +154,7 @@ size_t ygg_prepared_weight_bytes(int E, int d_out, int d_in, int format);
  * Format 5 applies the same conventions to the eight real entries of each
  * weight's 2x2 complex matrix, M00 = (s + v3) + i (t + b12), M01 = (v1 - b13) +
  * i (b23 - v2), M10 = (v1 + b13) + i (b23 + v2), M11 = (s - v3) + i (t - b12),
- * in float64. */
+ * in float64; format 6 is the same codes in the same layout. */
 int ygg_prepare_weights(const float* W, int E, int d_out, int d_in, int format, void* out, float* scales,
                         ygg_stream_t stream);
 
@@ -224,6 +225,30 @@ int ygg_clifford_linear(const void* x, int dtype, int rows, const void* w, const
 int ygg_f32_product_split(int rows, int d_in, int d_out);
 int ygg_f32_layer_split(int N, int d, int F, int E, int k);
 
+/* ---- products of int8 rows with int8 weights ------------------------------------
+ * No counterpart in the reference, whose quantizers keep weights only.
+ *
+ * Rows of multivectors x (rows, d, 8) of x_dtype, blade order, quantized by the entries of
+ * their 2x2 complex matrices X (ygg_prepare_weights has them): per row a = max(|entries of
+ * X / 2|, 2^-100), scale = a / 127, code = rint(entry (127 / a)), each operation rounded to
+ * fp32.  A row with an infinity or a NaN gets the scale NaN.  codes: ygg_int8_rows_bytes, on
+ * 16 bytes: per row, column b of X, and 32 inputs 128 bytes [re, im][g 4][m 8][c 2], the code
+ * of entry (c, b) of input 8 g + m; zero past input d.  scale: rows fp32.  The outputs share
+ * no memory with x. */
+size_t ygg_int8_rows_bytes(int rows, int d);
+int ygg_quantize_rows(const void* x, int x_dtype, int rows, int d, void* codes, float* scale, ygg_stream_t stream);
+
+/* For every expert e, rows r in [offsets[e], offsets[e+1]), P_max >= offsets[E]:
+ *   y[r, j] = act( s_w[e, j] s_x[src] (sum_i W_e[j, i] X[src, i]) + b_e[j] ),  src = gather[r] or r,
+ * the sums in 32-bit integers, exact, and the rest in fp32; y (P_max, d_out, 8) of y_dtype,
+ * blade order.  codes, x_scale: ygg_quantize_rows of x_rows rows (x_rows >= P_max without
+ * gather; a gather[r] outside [0, x_rows) stands for a row of zeros); w_prepared, w_scale: format 5 or 6;
+ * bias: prepared (mask order) or NULL.  E <= 64, d_in <= 32768. */
+int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows, const int32_t* gather, int P_max,
+                            const void* w_prepared, const float* w_scale, const float* bias_prepared,
+                            const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,
+                            ygg_stream_t stream);
+
 /* Blade-order fp32 rows (rows, d, 8) -> fp32 Pauli rows (rows, d, 2, 2, 2): element
  * [m][i][b][k][c] is the real (k = 0) or imaginary (k = 1) part of entry (c, b) of
  * multivector x[m][i] as a 2x2 complex matrix. */
@@ -236,10 +261,10 @@ size_t ygg_moe_workspace_bytes(int N, int d, int F, int E, int k, int dtype, int
 /* HLMBlock._moe_forward (hlm_block.py:154-183): x (N, d, 8) of dtype ->
  * out (N, d, 8) of dtype (+ residual if not NULL).  logits (N, E) or NULL
  * (then router_w/router_b give the grade-energy logits).  Expert weights
- * prepared with ygg_prepare_weights (format 0 or 4 for fp32, 1, 2, 3 or 5 for bf16;
+ * prepared with ygg_prepare_weights (format 0 or 4 for fp32, 1, 2, 3, 5 or 6 for bf16;
  * format 3 gathers the token rows inside the up projection; format 5 runs the
  * routing, both products and the activation in one launch and takes N <= 128,
- * d <= 128),
+ * d <= 128; format 6 quantizes the rows of both products, see ygg_quantize_rows),
  * biases prepared with ygg_prepare_bias or NULL.  topk_idx/topk_w/counts/
  * offsets as in ygg_route. */
 int ygg_moe_forward(const void* x, int dtype, int N, int d, int F, int E, int k, int act, const float* logits,
@@ -413,6 +438,24 @@ int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const fl
                               const int32_t* topk_idx, const float* topk_w, const float* dtopk_w, const void* dx_add,
                               void* dx, float* drouter_w, float* drouter_b, void* workspace, size_t workspace_bytes,
                               ygg_stream_t stream);
+
+/* ---- backward of the sort by expert and of the weighted way back -------------------------
+ * The gradients of ygg_combine and ygg_dispatch (hlm_block.py:178, 180-181; the reference's
+ * MoE has no backward, hlm_block.py:202-206).  slot_pos (N, k) as ygg_route wrote it, or a
+ * caller's, every row named by at most one slot; a slot outside [0, P) is left out.  k <= 8.
+ *
+ * From dout (N, d, 8) of dout_dtype:  dy[slot] = w dout_t, P rows of dy_dtype, blade order
+ * (dy_layout 0) or as the products' backward reads them (1: bf16 half-rows (P, 2, d, 4), fp32
+ * Pauli rows (P, d, 2, 2, 2)); rows that no slot names are not written.  dtopk_w (N, k) =
+ * <dout_t, y_sorted[slot]>, with y_sorted (P, d, 8) of dy_dtype; both NULL: not computed.
+ * Outputs share no memory with inputs. */
+int ygg_combine_backward(const void* dout, int dout_dtype, const void* y_sorted, int N, int k, int d, int P,
+                         const float* topk_w, const int32_t* slot_pos, void* dy, int dy_dtype, int dy_layout,
+                         float* dtopk_w, ygg_stream_t stream);
+/* dx_t (N, d, 8) = dx_add_t (or zero) + sum over the slots, in slot order, of dx_sorted[slot];
+ * dx_sorted (P, d, 8), dx_add (which dx may be) and dx of one dtype, summed in fp32. */
+int ygg_dispatch_backward(const void* dx_sorted, int dtype, int N, int k, int d, int P, const int32_t* slot_pos,
+                          const void* dx_add, void* dx, ygg_stream_t stream);
 
 /* ---- weight import: grade-aware quantization -----------------------------------
  * quantize_multivector / dequantize_multivector

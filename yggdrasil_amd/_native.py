@@ -90,6 +90,13 @@ SIGNATURES = {
     "ygg_clifford_layer_norm_backward_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "ygg_clifford_layer_norm_backward": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_double, _vp, _vp, _vp,
                                                   _vp, _vp, _c_size, _vp]),
+    "ygg_int8_rows_bytes": (_c_size, [_c_int, _c_int]),
+    "ygg_quantize_rows": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
+    "ygg_int8_grouped_linear": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
+                                         _vp, _c_int, _vp]),
+    "ygg_combine_backward": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp,
+                                      _vp]),
+    "ygg_dispatch_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "ygg_grade_quantize": (_c_int, [_vp, _c_int, _c_size, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),
     "ygg_clifford_layer_norm": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_double, _vp, _c_int, _vp]),
     "ygg_moe_block_ffn_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),

@@ -63,6 +63,9 @@ extern "C" int ygg_grouped_clifford_linear(const void*, int, const void*, int, c
                                            const int32_t*, int, int, int, int, void*, int, int, hipStream_t);
 extern "C" int ygg_pauli_grouped_linear(const void*, int, int, const int32_t*, int, const void*, const float*,
                                         const int32_t*, int, int, int, int, void*, int, int, hipStream_t);
+extern "C" int ygg_quantize_rows(const void*, int, int, int, void*, float*, hipStream_t);
+extern "C" int ygg_int8_grouped_linear(const void*, const float*, int, const int32_t*, int, const void*, const float*,
+                                       const float*, const int32_t*, int, int, int, int, void*, int, hipStream_t);
 extern "C" int ygg_pauli_rows_from_blade(const void*, int, int, void*, hipStream_t);
 extern "C" int ygg_pauli_rows_from_blade_f32(const float*, int, int, float*, hipStream_t);
 extern "C" int ygg_pauli_grouped_linear_f32(const float*, const int32_t*, int, const float*, const float*,
@@ -99,6 +102,9 @@ YGG_API size_t ygg_moe_workspace_bytes(int N, int d, int F, int E, int k, int dt
   b += align256((size_t)N * E * 4);       // logits
   b += align256(P * 4) * 2;               // perm, slot_pos
   b += align256(ygg_route_workspace_bytes(N, E, k));
+  if (w_format == kWI8Rows)  // the codes and scales of x's rows, h, those of h's rows, y_sorted
+    return b + align256(int8_rows_bytes((size_t)N, d)) + align256((size_t)N * 4) + align256(P * F * 16) +
+           align256(int8_rows_bytes(P, F)) + align256(P * 4) + align256(P * d * 16);
   b += align256(P * d * 8 * es);          // x_sorted (Pauli rows of x for formats 3 and 4)
   b += align256(P * F * 8 * es);          // h
   b += align256(ys_bytes(P, E, d, F, dtype, w_format));  // y_sorted
@@ -122,6 +128,11 @@ static int layer_size_check(const char* who, int N, int d, int F, int E, int k, 
       return -1;
     }
   }
+  if (w_format == kWI8Rows && N > 0) {
+    const char* why = int8_linear_limit(N, /*gathered*/ true, E, d, F);
+    if (!why) why = int8_linear_limit(N * k, false, E, F, d);
+    YGG_CHECK_ARG(!why, "%s: %s (N=%d d=%d F=%d E=%d k=%d)", who, why, N, d, F, E, k);
+  }
   return 0;
 }
 
@@ -140,12 +151,12 @@ static int moe_forward_impl(const void* x, int dtype, int N, int d, int F, int E
   YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_moe_forward: activation %d", act);
   YGG_CHECK_ARG(N == 0 || (x && out && w_up && w_down && topk_idx && topk_w && counts && offsets && workspace),
                 "ygg_moe_forward: null pointer");
-  YGG_CHECK_ARG((w_format != kWI8 && w_format != kWPauliI8) || N == 0 || (s_up && s_down),
+  YGG_CHECK_ARG((w_format != kWI8 && w_format != kWPauliI8 && w_format != kWI8Rows) || N == 0 || (s_up && s_down),
                 "ygg_moe_forward: int8 weights need their scales");
   YGG_CHECK_ARG(dtype == kF32 || dtype == kBF16, "ygg_moe_forward: dtype %d unsupported", dtype);
   YGG_CHECK_ARG(dtype == kF32 ? (w_format == kWF32 || w_format == kWPauliF32)
                              : (w_format == kWBF16 || w_format == kWI8 || w_format == kWPauli ||
-                                w_format == kWPauliI8),
+                                w_format == kWPauliI8 || w_format == kWI8Rows),
                 "ygg_moe_forward: weight format %d does not match dtype %d", w_format, dtype);
   YGG_CHECK_ARG(w_format != kWPauliI8 || N == 0 || decode_pauli_fusable(N, E, k, d, F),
                 "ygg_moe_forward: int8 Pauli weights (format 5) serve decode batches of at most 128 tokens with "
@@ -242,6 +253,28 @@ static int moe_forward_impl(const void* x, int dtype, int N, int d, int F, int E
   } else if (ygg::route_convert(logits, N, E, k, topk_idx, topk_w, counts, offsets, perm, slot_pos, rws, rws_bytes,
                                 cv, stream)) {
     return -1;
+  }
+  if (w_format == kWI8Rows) {
+    // x's rows in int8, gathered through perm by the up product; h's rows in int8, read in place by the down product
+    char* q = static_cast<char*>(xs);
+    auto take = [&](size_t bytes) {
+      char* r = q;
+      q += align256(bytes);
+      return r;
+    };
+    void* xq = take(int8_rows_bytes((size_t)N, d));
+    float* xq_scale = reinterpret_cast<float*>(take((size_t)N * 4));
+    void* hb = take(P * F * 16);
+    void* hq = take(int8_rows_bytes(P, F));
+    float* hq_scale = reinterpret_cast<float*>(take(P * 4));
+    void* yb = take(P * d * 16);
+    if (ygg_quantize_rows(x, kBF16, N, d, xq, xq_scale, stream) ||
+        ygg_int8_grouped_linear(xq, xq_scale, N, perm, (int)P, w_up, s_up, b_up, offsets, E, d, F, act, hb, kBF16, stream) ||
+        ygg_quantize_rows(hb, kBF16, (int)P, F, hq, hq_scale, stream) ||
+        ygg_int8_grouped_linear(hq, hq_scale, (int)P, nullptr, (int)P, w_down, s_down, b_down, offsets, E, F, d, kActNone,
+                                yb, kBF16, stream))
+      return -1;
+    return ygg_combine(yb, kBF16, /*y_mask=*/0, N, k, d, topk_idx, topk_w, slot_pos, residual, out, kBF16, stream);
   }
   if (split) {  // fp32 Pauli, enough rows
     if (pauli_split_linear(static_cast<const float*>(xs), N, perm, (int)P, static_cast<const float*>(w_up), b_up, offsets, E,

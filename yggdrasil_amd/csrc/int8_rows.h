@@ -1,0 +1,28 @@
+// int8_rows.h -- the layout of quantized rows and of the int8 Pauli weights that they meet.
+#pragma once
+
+#include "pauli_common.h"
+
+namespace ygg {
+
+// A multivector's halved Pauli matrix holds 8 reals: entries (c, b), real and imaginary parts.  A quantized row keeps them
+// as int8 codes with one scale a row (both columns b): for b = 0, 1 and every 32 inputs (a K step), 128 bytes
+//   [re, im][g 4][16 bytes]: byte 2 m + c holds the code of entry (c, b) of input 32 ks + 8 g + m,
+// zero past the row's last input.  One 16-byte run is a lane's operand of v_mfma_i32_32x32x32_i8 -- real and imaginary
+// parts lie in runs of their own, so the rotation by i exchanges two registers instead of bytes -- and a K step
+// of a half-row is one line of memory.
+constexpr int kI8Step = 32;         // inputs of a K step
+constexpr int kI8StepBytes = 128;   // a half-row's bytes of it
+__host__ __device__ inline int i8_steps(int d) { return (d + kI8Step - 1) / kI8Step; }
+__host__ __device__ inline size_t i8_row_bytes(int d) { return (size_t)i8_steps(d) * 2 * kI8StepBytes; }
+
+// The weights of format 5 (decode_pauli.hip): per expert [ceil(d_out / 8)][K steps][U, V][g 4][n 16][16 bytes],
+// n = 2 jj + a (channel 8 jb + jj, matrix row a), byte 2 m + c the code of entry (a, c), the inputs as above.
+constexpr int kI8BlockBytes = 2048;  // 8 channels of a K step
+__host__ __device__ inline size_t i8_expert_bytes(int d_out, int d_in) {
+  return (size_t)((d_out + 7) / 8) * i8_steps(d_in) * kI8BlockBytes;
+}
+// 4 d_in products of codes up to 127 and -128 stay below 2^31
+constexpr int kI8MaxInputs = 32768;
+
+}  // namespace ygg

@@ -13,7 +13,7 @@
 
 #include <algorithm>
 
-#include "rows.h"
+#include "pauli_common.h"
 #include "ygg_common.h"
 
 extern "C" int ygg_combine(const void*, int, int, int, int, int, const int32_t*, const float*, const int32_t*,
@@ -28,74 +28,6 @@ namespace ygg {
 namespace {
 
 constexpr int kMaxTopK = 8;
-
-// One wave per token: dy[slot] = w dout_t as Pauli half-rows and dtopk_w = <dout_t, y[slot]> (when y is not
-// NULL).  Bound by memory: dout and y are read once, dy is written once (8192 tokens, d = 128, k = 4: 25.7 us, 151 MB
-// at 5.9 TB/s).
-__global__ __launch_bounds__(256) void combine_backward_bf16_kernel(const uint16_t* __restrict__ dout,
-                                                                    const uint16_t* __restrict__ y, int N, int k, int d,
-                                                                    const float* __restrict__ topk_w,
-                                                                    const int32_t* __restrict__ slot_pos,
-                                                                    uint16_t* __restrict__ dy, float* __restrict__ dtopk_w) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (t >= N) return;
-  float dot[kMaxTopK] = {};
-  for (int i = lane; i < d; i += 64) {
-    float g[8];
-    load_mv(dout, (size_t)t * d + i, g);
-    float c0[4], c1[4];
-    blade_to_pauli(g, c0, c1);
-#pragma unroll
-    for (int s = 0; s < kMaxTopK; ++s) {
-      if (s >= k) break;
-      const size_t row = (size_t)slot_pos[(size_t)t * k + s];
-      const float w = topk_w[(size_t)t * k + s];
-      uint16_t* to = dy + (row * 2 * d + i) * 4;
-      *reinterpret_cast<uint2*>(to) = make_uint2(pack2_bf16(w * c0[0], w * c0[1]), pack2_bf16(w * c0[2], w * c0[3]));
-      *reinterpret_cast<uint2*>(to + (size_t)d * 4) =
-          make_uint2(pack2_bf16(w * c1[0], w * c1[1]), pack2_bf16(w * c1[2], w * c1[3]));
-      if (y != nullptr) {
-        float v[8];
-        load_mv(y, row * d + i, v);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) dot[s] = __builtin_fmaf(g[c], v[c], dot[s]);
-      }
-    }
-  }
-  if (y != nullptr) {
-    const float sum = wave_sums<kMaxTopK>(dot, lane);
-    const int s = wave_sums_of<kMaxTopK>(lane);
-    if ((lane & (64 / kMaxTopK - 1)) == 0 && s < k) dtopk_w[(size_t)t * k + s] = sum;
-  }
-}
-
-// dx_t = (dout_t) + sum over the slots, in slot order, of dxs[slot_pos]; a thread per multivector.  Bound by memory: the
-// rows read and dx written once (8192 tokens, d = 128, k = 4: 17.6 us, 84 MB at 4.8 TB/s).
-__global__ __launch_bounds__(256) void dispatch_backward_bf16_kernel(const uint16_t* __restrict__ dxs, int N, int k, int d,
-                                                                     const int32_t* __restrict__ slot_pos,
-                                                                     const uint16_t* __restrict__ dout,
-                                                                     uint16_t* __restrict__ dx) {
-  const int t = blockIdx.x;
-  const int32_t* sp = slot_pos + (size_t)t * k;  // (the same for every thread: scalar loads)
-  for (int i = threadIdx.x; i < d; i += blockDim.x) {
-    float o[8] = {};
-    if (dout != nullptr) load_mv(dout, (size_t)t * d + i, o);
-    RawMv<uint16_t> r[kMaxTopK];
-#pragma unroll
-    for (int s = 0; s < kMaxTopK; ++s)
-      if (s < k) r[s] = load_raw(dxs, (size_t)sp[s] * d + i);
-#pragma unroll
-    for (int s = 0; s < kMaxTopK; ++s)
-      if (s < k) {
-        float v[8];
-        unpack(r[s], v);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) o[c] += v[c];
-      }
-    store_mv(dx, (size_t)t * d + i, o);
-  }
-}
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -236,19 +168,12 @@ YGG_API int ygg_moe_backward_bf16(int N, int d, int F, int E, int k, int act, co
   char* const dxs = dy + align256((size_t)P * d * 16);
   char* const dh = dxs + align256((size_t)P * d * 16);
   void* const wg = dh + align256((size_t)P * F * 16);
-  hipLaunchKernelGGL(combine_backward_bf16_kernel, dim3((N + 3) / 4), dim3(256), 0, stream,
-                     static_cast<const uint16_t*>(dout),
-                     dtopk_w ? reinterpret_cast<const uint16_t*>(keep + at.y) : nullptr, N, k, d, topk_w, slot_pos,
-                     reinterpret_cast<uint16_t*>(dy), dtopk_w);
-  if (check_launch("combine backward (bf16)")) return -1;
+  if (combine_backward_bf16(dout, dtopk_w ? keep + at.y : nullptr, N, k, d, topk_w, slot_pos, dy, dtopk_w, stream)) return -1;
   if (ygg_pauli_grouped_input_grad(dy, P, w_down_adj, offsets, E, d, F, act, keep + at.h_pre, dh, /*Pauli rows*/ 0, kBF16,
                                    stream) ||
       (dw_down && weight_grad_bf16(dy, keep + at.h, P, nullptr, offsets, P, E, F, d, dw_down, db_down, wg, stream)) ||
       ygg_pauli_grouped_input_grad(dh, P, w_up_adj, offsets, E, F, d, kActNone, nullptr, dxs, /*blade*/ 1, kBF16, stream) ||
       (dw_up && weight_grad_bf16(dh, keep + at.x, N, perm, offsets, P, E, d, F, dw_up, db_up, wg, stream)))
     return -1;
-  hipLaunchKernelGGL(dispatch_backward_bf16_kernel, dim3((unsigned)N), dim3(d <= 64 ? 64 : d <= 128 ? 128 : 256), 0, stream,
-                     reinterpret_cast<const uint16_t*>(dxs), N, k, d, slot_pos,
-                     residual ? static_cast<const uint16_t*>(dout) : nullptr, static_cast<uint16_t*>(dx));
-  return check_launch("dispatch backward (bf16)");
+  return dispatch_backward_bf16(dxs, N, k, d, slot_pos, residual ? dout : nullptr, dx, stream);
 }

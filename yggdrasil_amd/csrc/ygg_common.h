@@ -104,7 +104,7 @@ int check_launch(const char* what);
 enum DType : int { kF32 = 0, kBF16 = 1, kI8 = 2 };
 enum Act : int { kActNone = 0, kActGelu = 1, kActRelu = 2, kActSigmoid = 3 };
 // prepared weight formats (ygg_prepare_weights)
-enum WFormat : int { kWF32 = 0, kWBF16 = 1, kWI8 = 2, kWPauli = 3, kWPauliF32 = 4, kWPauliI8 = 5 };
+enum WFormat : int { kWF32 = 0, kWBF16 = 1, kWI8 = 2, kWPauli = 3, kWPauliF32 = 4, kWPauliI8 = 5, kWI8Rows = 6 };
 
 // bf16 Pauli weight layout (pauli_gemm.hip)
 int pauli_prepare_weights(const float* W, int E, int d_out, int d_in, void* out, hipStream_t stream);
@@ -247,6 +247,11 @@ int decode_pauli_layer(const uint16_t* x, const float* logits, int N, int E, int
                        const float* s_dn, const float* b_dn, int32_t* topk_idx, float* topk_w, int32_t* counts,
                        int32_t* offsets, int32_t* perm, int32_t* slot_pos, float* planes, hipStream_t stream);
 
+// int8 rows (int8_rows.hip): bytes of the codes of rows of d multivectors, and why the product cannot take these sizes
+// (nullptr: it can)
+size_t int8_rows_bytes(size_t rows, int d);
+const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out);
+
 // combine of fp32 blade-order partial planes (dispatch.hip): the planes of a
 // row are added in plane order, then weighted and combined as ygg_combine does.
 // slot_rows: the planes hold slot (t, s) at row t k + s, not at slot_pos[t k + s]
@@ -293,6 +298,13 @@ const char* weight_grad_bf16_limit(int P_max, int E, int d_in, int d_out, bool g
 size_t weight_grad_bf16_workspace_bytes(int P_max, int E, int d_in, int d_out);
 int weight_grad_bf16(const void* dy, const void* a, int a_rows, const int32_t* gather, const int32_t* offsets, int P_max,
                      int E, int d_in, int d_out, float* dW, float* db, void* workspace, hipStream_t stream);
+
+// The bf16 layer's combine and dispatch backward (sort_backward.hip): dy as Pauli half-rows, dtopk_w when y is not NULL;
+// dx = add + the sum of a token's rows, in slot order.
+int combine_backward_bf16(const void* dout, const void* y, int N, int k, int d, const float* topk_w, const int32_t* slot_pos,
+                          void* dy, float* dtopk_w, hipStream_t stream);
+int dispatch_backward_bf16(const void* dxs, int N, int k, int d, const int32_t* slot_pos, const void* add, void* dx,
+                           hipStream_t stream);
 
 // Whether n bytes at a and m bytes at b share any (nullptr: none).  Entries whose kernels write one tensor while other
 // workgroups still read another refuse such a pair.

@@ -46,7 +46,9 @@ class MoEHLMConfig:
                 vector units, 64); bf16 layers: 'pauli' (the default when d_model and d_ff are
                 even), 'bf16' (8x8 L(w) blocks), 'int8' (per-output-channel int8, L(w) blocks) or
                 'int8_pauli' (per-output-channel int8 of the complex 2x2 weights: the one-launch
-                decode layer, batches of at most 128 tokens with d_model <= 128)
+                decode layer, batches of at most 128 tokens with d_model <= 128) or 'int8_rows' (the same
+                weights, for any batch and width: the rows of both products are quantized to int8 too, with a
+                scale each; forward only)
     router      'energy' -- CliffordRouter's grade-energy logits (default, the reference);
                 'clifford_head' -- CliffordLinear(d -> E) then the scalar part;
                 'logits' -- the caller passes logits to forward()
@@ -78,11 +80,12 @@ class MoEHLMConfig:
         even = self.d_model % 2 == 0 and self.d_ff % 2 == 0
         if self.weight_format is None:
             self.weight_format = "pauli_f32" if self.dtype == torch.float32 else ("pauli" if even else "bf16")
-        if self.weight_format not in ("f32", "pauli_f32", "bf16", "int8", "pauli", "int8_pauli"):
-            raise ValueError("weight_format must be 'f32', 'pauli_f32', 'bf16', 'int8', 'pauli' or 'int8_pauli'")
+        if self.weight_format not in ("f32", "pauli_f32", "bf16", "int8", "pauli", "int8_pauli", "int8_rows"):
+            raise ValueError("weight_format must be 'f32', 'pauli_f32', 'bf16', 'int8', 'pauli', 'int8_pauli' or "
+                             "'int8_rows'")
         if (self.dtype == torch.float32) != (self.weight_format in ("f32", "pauli_f32")):
             raise ValueError("fp32 layers use 'pauli_f32' or 'f32' weights; bf16 layers use 'pauli', 'bf16', "
-                             "'int8' or 'int8_pauli'")
+                             "'int8', 'int8_pauli' or 'int8_rows'")
         if self.weight_format == "int8_pauli" and self.d_model > 128:
             raise ValueError("the 'int8_pauli' weight format serves d_model <= 128")
         if self.weight_format == "pauli" and not even:

@@ -18,8 +18,8 @@ from ._native import check, lib, ptr, stream_handle
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 ACT_CODE = {"none": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
-WFORMAT_CODE = {"f32": 0, "bf16": 1, "int8": 2, "pauli": 3, "pauli_f32": 4, "int8_pauli": 5}
-INT8_FORMATS = ("int8", "int8_pauli")
+WFORMAT_CODE = {"f32": 0, "bf16": 1, "int8": 2, "pauli": 3, "pauli_f32": 4, "int8_pauli": 5, "int8_rows": 6}
+INT8_FORMATS = ("int8", "int8_pauli", "int8_rows")
 # activation row layouts of pauli_grouped_linear
 X_LAYOUT = {"blade": 0, "pauli": 1}
 Y_LAYOUT = {"pauli": 0, "blade": 1}
@@ -337,6 +337,78 @@ def combine(y_sorted: torch.Tensor, routing: Routing, residual: torch.Tensor | N
     return out
 
 
+def _check_routing(who: str, routing: Routing, dev) -> tuple:
+    """The slots of a caller's routing: ``(N, k)``."""
+    if routing.slot_pos.dim() != 2:
+        raise ValueError(f"{who}: slot_pos must be (N, k), got {tuple(routing.slot_pos.shape)}")
+    for name, t, dtype in (("slot_pos", routing.slot_pos, torch.int32), ("topk_w", routing.topk_w, torch.float32)):
+        if t.dtype != dtype or t.shape != routing.slot_pos.shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(routing.slot_pos.shape)} on {dev}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return routing.slot_pos.shape
+
+
+@_on_its_device
+def combine_backward(dout: torch.Tensor, y_sorted: torch.Tensor | None, routing: Routing, y_layout: str = "blade",
+                     out_dtype: torch.dtype | None = None, rows: int | None = None):
+    """Gradients of :func:`combine` (whose residual's gradient is dout): ``(dy_sorted, dtopk_w)``.
+
+    dout (N, d, 8): the gradient of its output, float32 or bfloat16.  y_sorted (P, d, 8): its input, or None where the
+    routing weights need no gradient (then dtopk_w is None, ``rows`` is P, N k if not given, and ``out_dtype`` the
+    type of dy, dout's if not given; else they are y_sorted's).  y_layout 'blade' returns dy as (P, d, 8), 'pauli' as the
+    products' backward reads it: half-rows (P, 2, d, 4) for bfloat16, Pauli rows (P, d, 2, 2, 2) for float32.
+    dtopk_w (N, k) fp32.  A slot outside the P rows has a weight gradient of zero; rows that no slot names are not
+    written.
+    """
+    dev = _one_device(dout, y_sorted)
+    if dout.dim() != 3 or dout.shape[2] != 8:
+        raise ValueError(f"combine_backward: dout must be (N, d, 8), got {tuple(dout.shape)}")
+    if y_layout not in Y_LAYOUT:
+        raise ValueError("y_layout must be 'blade' or 'pauli'")
+    Nt, k = _check_routing("combine_backward", routing, dev)
+    d = dout.shape[1]
+    if dout.shape[0] != Nt:
+        raise ValueError(f"combine_backward: {Nt} tokens' routing for {dout.shape[0]} tokens")
+    if y_sorted is not None:
+        if y_sorted.dim() != 3 or y_sorted.shape[1:] != (d, 8):
+            raise ValueError(f"combine_backward: y_sorted must be (P, {d}, 8), got {tuple(y_sorted.shape)}")
+        if out_dtype not in (None, y_sorted.dtype) or rows not in (None, y_sorted.shape[0]):
+            raise ValueError("combine_backward: dy has y_sorted's type and rows")
+        out_dtype, rows = y_sorted.dtype, y_sorted.shape[0]
+    out_dtype, P = out_dtype or dout.dtype, Nt * k if rows is None else rows
+    dout, y_sorted = _aligned(dout), _aligned(y_sorted)
+    pauli = (P, 2, d, 4) if out_dtype == torch.bfloat16 else (P, d, 2, 2, 2)
+    dy = torch.empty(pauli if y_layout == "pauli" else (P, d, 8), device=dev, dtype=out_dtype)
+    dtw = torch.empty((Nt, k), device=dev, dtype=torch.float32) if y_sorted is not None else None
+    check(lib().ygg_combine_backward(dout.data_ptr(), _dtype_code(dout), ptr(y_sorted), Nt, k, d, P,
+                                     routing.topk_w.data_ptr(), routing.slot_pos.data_ptr(), dy.data_ptr(),
+                                     _dtype_code(dy), int(y_layout == "pauli"), ptr(dtw), stream_handle(dev)),
+          "combine_backward")
+    return dy, dtw
+
+
+@_on_its_device
+def dispatch_backward(dx_sorted: torch.Tensor, routing: Routing, dx_add: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of :func:`dispatch`: dx (N, d, 8) = the sum of each token's rows of dx_sorted (P, d, 8), in slot order.
+
+    ``dx_add`` (N, d, 8), of dx_sorted's type, is added before dx is rounded: the gradient that reaches x past the
+    sort.  A slot outside the P rows adds nothing.
+    """
+    dev = _one_device(dx_sorted, dx_add)
+    if dx_sorted.dim() != 3 or dx_sorted.shape[2] != 8:
+        raise ValueError(f"dispatch_backward: dx_sorted must be (P, d, 8), got {tuple(dx_sorted.shape)}")
+    Nt, k = _check_routing("dispatch_backward", routing, dev)
+    P, d = dx_sorted.shape[:2]
+    if dx_add is not None and (dx_add.shape != (Nt, d, 8) or dx_add.dtype != dx_sorted.dtype):
+        raise ValueError(f"dispatch_backward: dx_add must be {dx_sorted.dtype} ({Nt}, {d}, 8)")
+    code = _dtype_code(dx_sorted)
+    dx_sorted, dx_add = _aligned(dx_sorted), _aligned(dx_add)
+    dx = torch.empty((Nt, d, 8), device=dev, dtype=dx_sorted.dtype)
+    check(lib().ygg_dispatch_backward(dx_sorted.data_ptr(), code, Nt, k, d, P, routing.slot_pos.data_ptr(), ptr(dx_add),
+                                      dx.data_ptr(), stream_handle(dev)), "dispatch_backward")
+    return dx
+
+
 # ---------------------------------------------------------------------------
 # expert products
 # ---------------------------------------------------------------------------
@@ -356,9 +428,9 @@ class PreparedWeights:
 
 def prepare_weights(w: torch.Tensor, fmt: str) -> PreparedWeights:
     """w: (E, d_out, d_in, 8) fp32 blade order -> prepared layout ('f32' | 'bf16' | 'int8' | 'pauli' |
-    'pauli_f32' | 'int8_pauli').  The int8 formats also hold one fp32 scale per (expert, output channel):
-    'int8' quantizes the blade components, 'int8_pauli' the entries of each weight's 2x2 complex matrix
-    (the decode layer's format)."""
+    'pauli_f32' | 'int8_pauli' | 'int8_rows').  The int8 formats also hold one fp32 scale per (expert, output
+    channel): 'int8' quantizes the blade components, 'int8_pauli' and 'int8_rows' the entries of each weight's 2x2
+    complex matrix (one layout: the decode layer's format, and that of products with rows in int8)."""
     dev = _dev(w)
     if w.dim() == 3:
         w = w.unsqueeze(0)
@@ -394,9 +466,9 @@ def grouped_clifford_linear(x_sorted: torch.Tensor, pw: PreparedWeights, offsets
                             bias_prepared: torch.Tensor | None = None, act: str = "none",
                             out_dtype: torch.dtype | None = None, out_blade_order: bool = True) -> torch.Tensor:
     """Per-expert CliffordLinear on expert-grouped rows. x_sorted: (P, d_in, 8) in mask order."""
-    if pw.fmt in ("pauli", "pauli_f32", "int8_pauli"):
+    if pw.fmt in ("pauli", "pauli_f32", "int8_pauli", "int8_rows"):
         raise ValueError("Pauli weights run through pauli_grouped_linear / pauli_grouped_linear_f32 / the decode "
-                         "layer (int8_pauli)")
+                         "layer (int8_pauli) / int8_grouped_linear (int8_rows)")
     dev = _dev(x_sorted, offsets, bias_prepared)
     P = x_sorted.shape[0]
     if x_sorted.shape[1] != pw.d_in:
@@ -518,6 +590,90 @@ def pauli_rows_from_blade(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+@dataclass
+class Int8Rows:
+    """Rows of multivectors in int8 (:func:`quantize_rows`): the codes of their halved 2x2 matrices' entries, in runs of
+    16 bytes as the products read them, and one fp32 scale a row."""
+
+    codes: torch.Tensor  # (rows, 2, ceil(d / 32), 2, 4, 16) int8: column b, K step, re / im, 8 inputs, (input, row c)
+    scale: torch.Tensor  # (rows,) fp32
+    d: int
+
+    def values(self) -> torch.Tensor:
+        """What the codes stand for, as fp32 multivectors (rows, d, 8)."""
+        q = self.codes.float().view(*self.codes.shape[:5], 8, 2)  # [row, b, ks, part, g, m, c]
+        q = q.permute(0, 2, 4, 5, 6, 1, 3).reshape(q.shape[0], 32 * q.shape[2], 2, 2, 2)[:, :self.d]  # [row, i, c, b, part]
+        e = q * self.scale[:, None, None, None, None]
+        (r00, i00), (r01, i01), (r10, i10), (r11, i11) = [e[:, :, c, b].unbind(-1) for c in (0, 1) for b in (0, 1)]
+        return torch.stack([r00 + r11, r10 + r01, i10 - i01, r00 - r11, i00 - i11, r10 - r01, i10 + i01, i00 + i11], -1)
+
+
+@_on_its_device
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """Token rows x (rows, d, 8), float32 or bfloat16, in int8 with a scale each.
+
+    Per row: a the largest of |entries of X / 2| over its multivectors' 2x2 complex matrices X, at least 2^-100;
+    scale = a / 127, codes = rint(entry (127 / a)), every operation rounded to fp32.  A row that holds an infinity
+    or a NaN gets the scale NaN: its products are NaN.
+    """
+    dev = _one_device(x)
+    if x.dim() != 3 or x.shape[2] != 8:
+        raise ValueError(f"quantize_rows: x must be (rows, d, 8), got {tuple(x.shape)}")
+    rows, d = x.shape[:2]
+    code = _dtype_code(x)
+    x = _aligned(x)
+    codes = torch.empty((rows, 2, (d + 31) // 32, 2, 4, 16), device=dev, dtype=torch.int8)
+    scale = torch.empty(rows, device=dev, dtype=torch.float32)
+    check(lib().ygg_quantize_rows(x.data_ptr(), code, rows, d, codes.data_ptr(), scale.data_ptr(), stream_handle(dev)),
+          "quantize_rows")
+    return Int8Rows(codes, scale, d)
+
+
+@_on_its_device
+def _int8_grouped_linear(codes, scale, d, pw, offsets, bias_prepared, act, gather, out_dtype):
+    dev = _one_device(codes, scale, pw.data, pw.scales, offsets, bias_prepared, gather)
+    x_rows = codes.shape[0]
+    if (codes.dtype != torch.int8 or codes.shape != (x_rows, 2, (d + 31) // 32, 2, 4, 16) or
+            scale.dtype != torch.float32 or scale.shape != (x_rows,)):
+        raise ValueError("int8_grouped_linear: rows are not those of quantize_rows")
+    if d != pw.d_in:
+        raise ValueError(f"rows have d_in={d}, weights expect {pw.d_in}")
+    _check_bounds(offsets, pw.E, dev)
+    if gather is not None and (gather.dtype != torch.int32 or gather.dim() != 1):
+        raise ValueError(f"gather must be int32 (rows,), got {gather.dtype} {tuple(gather.shape)}")
+    if bias_prepared is not None and (bias_prepared.dtype != torch.float32 or
+                                      bias_prepared.shape != (pw.E, pw.d_out, 8)):
+        raise ValueError(f"the bias must be a prepared float32 ({pw.E}, {pw.d_out}, 8)")
+    P = x_rows if gather is None else gather.shape[0]
+    codes, bias_prepared = _aligned(codes), _aligned(bias_prepared)
+    y = torch.empty((P, pw.d_out, 8), device=dev, dtype=out_dtype)
+    check(lib().ygg_int8_grouped_linear(codes.data_ptr(), scale.data_ptr(), x_rows, ptr(gather), P, pw.data.data_ptr(),
+                                        pw.scales.data_ptr(), ptr(bias_prepared), offsets.data_ptr(), pw.E, d, pw.d_out,
+                                        ACT_CODE[act], y.data_ptr(), DTYPE_CODE[out_dtype], stream_handle(dev)),
+          "int8_grouped_linear")
+    return y
+
+
+def int8_grouped_linear(rows: Int8Rows, pw: PreparedWeights, offsets: torch.Tensor,
+                        bias_prepared: torch.Tensor | None = None, act: str = "none",
+                        gather: torch.Tensor | None = None,
+                        out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Per-expert CliffordLinear of int8 rows (:func:`quantize_rows`) with int8 weights (``fmt='int8_rows'`` or
+    'int8_pauli'): exact sums in 32-bit integers, then the scales of the row and of the output channel, bias and
+    activation in fp32.
+
+    Output row r reads rows[gather[r]] (or rows[r]); returns (P, d_out, 8) of out_dtype, float32 or bfloat16.
+    Rows past ``offsets[E]`` are not written; a gathered row outside ``rows`` counts as zeros.
+    """
+    if pw.fmt not in ("int8_rows", "int8_pauli"):
+        raise ValueError("int8_grouped_linear needs weights prepared with fmt='int8_rows' or 'int8_pauli'")
+    if act not in ACT_CODE:
+        raise ValueError(f"act must be one of {tuple(ACT_CODE)}")
+    if out_dtype not in DTYPE_CODE:
+        raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
+    return _int8_grouped_linear(rows.codes, rows.scale, rows.d, pw, offsets, bias_prepared, act, gather, out_dtype)
+
+
 def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert_counts: torch.Tensor,
                     w_up: PreparedWeights, w_down: PreparedWeights, b_up: torch.Tensor | None = None,
                     b_down: torch.Tensor | None = None, act: str = "gelu", validate: bool = False) -> torch.Tensor:
@@ -533,7 +689,8 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     expert e are ``expert_offsets[e] .. + expert_counts[e]``, the experts' ranges
     contiguous and ascending from row 0 (as a sort by expert leaves them).  Weights
     and biases are prepared (:func:`prepare_weights`, :func:`prepare_bias`); the
-    weight format picks the products (bf16 / fp32 Pauli, or the L(w) blocks).
+    weight format picks the products (bf16 / fp32 Pauli, the L(w) blocks, or int8 with the
+    rows of both products in int8).
     ``validate`` checks the ranges on the host (one synchronisation).  Without it the
     ranges are clamped on the device (no synchronisation) into ascending bounds within
     ``[0, P]``, so malformed ranges give wrong rows, never accesses past x_sorted or y.
@@ -571,6 +728,11 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     elif fmt == "pauli_f32":
         h = pauli_grouped_linear_f32(pauli_rows_from_blade_f32(x), w_up, offs, b_up, act, y_layout="pauli")
         y = pauli_grouped_linear_f32(h, w_down, offs, b_down, "none", y_layout="blade")
+    elif fmt == "int8_rows":
+        if x.dtype != torch.bfloat16:
+            raise ValueError("int8_rows experts take bf16 rows")
+        h = int8_grouped_linear(quantize_rows(x), w_up, offs, b_up, act)
+        y = int8_grouped_linear(quantize_rows(h), w_down, offs, b_down)
     else:  # L(w) blocks read and write mask order between the products
         h = grouped_clifford_linear(to_mask_order(x), w_up, offs, b_up, act, out_blade_order=False)
         y = grouped_clifford_linear(h, w_down, offs, b_down, "none", out_dtype=x.dtype, out_blade_order=True)
