@@ -22,6 +22,13 @@ constexpr int kI8BlockBytes = 2048;  // 8 channels of a K step
 __host__ __device__ inline size_t i8_expert_bytes(int d_out, int d_in) {
   return (size_t)((d_out + 7) / 8) * i8_steps(d_in) * kI8BlockBytes;
 }
+// An integer sum as the value that it stands for: three roundings in every kernel, so a row's outputs are the same
+// bit for bit whichever takes its batch (not contracted into the additions that follow).
+__device__ __forceinline__ float i8_value(int sum, float sw, float sx) {
+#pragma clang fp contract(off)
+  return ((float)sum * sw) * sx;
+}
+
 // 4 d_in products of codes up to 127 and -128 stay below 2^31
 constexpr int kI8MaxInputs = 32768;
 

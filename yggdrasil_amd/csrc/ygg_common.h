@@ -250,6 +250,9 @@ int decode_pauli_layer(const uint16_t* x, const float* logits, int N, int E, int
 // int8 rows (int8_rows.hip): bytes of the codes of rows of d multivectors, and why the product cannot take these sizes
 // (nullptr: it can)
 size_t int8_rows_bytes(size_t rows, int d);
+int int8_tile_linear(const void* x, const float* xs, int x_rows, const int32_t* gather, int P, const void* w, const float* ws,
+                     const float* bias, const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,
+                     hipStream_t stream);  // int8_tile.hip: the product for enough rows
 const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out);
 
 // combine of fp32 blade-order partial planes (dispatch.hip): the planes of a
