@@ -243,7 +243,7 @@ int ygg_quantize_rows(const void* x, int x_dtype, int rows, int d, void* codes, 
  * the sums in 32-bit integers, exact, and the rest in fp32; y (P_max, d_out, 8) of y_dtype,
  * blade order.  codes, x_scale: ygg_quantize_rows of x_rows rows (x_rows >= P_max without
  * gather; a gather[r] outside [0, x_rows) stands for a row of zeros); w_prepared, w_scale: format 5 or 6;
- * bias: prepared (mask order) or NULL.  E <= 64, d_in <= 32768. */
+ * bias: prepared (mask order) or NULL.  E <= 64, d_in <= 16384. */
 int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows, const int32_t* gather, int P_max,
                             const void* w_prepared, const float* w_scale, const float* bias_prepared,
                             const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,

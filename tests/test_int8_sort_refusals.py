@@ -40,7 +40,7 @@ _LIN = [FAR[0], FAR[1], 8, None, 8, FAR[2], FAR[3], None, FAR[4], 2, 40, 24, 0, 
 @pytest.mark.parametrize("at,value,word", [
     (0, None, "null"), (1, None, "null"), (5, None, "null"), (6, None, "null"), (8, None, "null"), (13, None, "null"),
     (2, -1, "bad sizes"), (2, 7, "7 rows"), (4, -1, "bad sizes"), (9, 0, "bad sizes"), (9, 65, "bad sizes"),
-    (10, 0, "bad sizes"), (10, 32769, "bad sizes"), (11, 0, "bad sizes"), (12, 4, "activation"), (14, 2, "dtype")])
+    (10, 0, "bad sizes"), (10, 16385, "bad sizes"), (11, 0, "bad sizes"), (12, 4, "activation"), (14, 2, "dtype")])
 def test_product(at, value, word):
     args = list(_LIN)
     args[at] = value
@@ -88,7 +88,7 @@ _FWD = [P, 1, 4, 8, 8, 4, 2, 1, P, None, None, P, P, None, P, P, None, 6, None, 
 
 
 @pytest.mark.parametrize("at,value,word", [(1, 0, "does not match dtype"), (12, None, "scales"), (15, None, "scales"),
-                                           (25, 64, "workspace"), (4, 40000, "32768"), (3, 40000, "32768")])
+                                           (25, 64, "workspace"), (4, 40000, "16384"), (3, 40000, "16384")])
 def test_layer(at, value, word):
     args = list(_FWD)
     args[at] = value

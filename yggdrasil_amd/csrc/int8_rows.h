@@ -22,14 +22,18 @@ constexpr int kI8BlockBytes = 2048;  // 8 channels of a K step
 __host__ __device__ inline size_t i8_expert_bytes(int d_out, int d_in) {
   return (size_t)((d_out + 7) / 8) * i8_steps(d_in) * kI8BlockBytes;
 }
-// An integer sum as the value that it stands for: three roundings in every kernel, so a row's outputs are the same
-// bit for bit whichever takes its batch (not contracted into the additions that follow).
-__device__ __forceinline__ float i8_value(int sum, float sw, float sx) {
-#pragma clang fp contract(off)
-  return ((float)sum * sw) * sx;
+// The blades of an output multivector from the sums of its halved matrix (entry a b, re and im): sums and differences of
+// two of them, still whole numbers, then one rounding to fp32, the two scales' product and the bias in one multiply-add.
+// The same in every kernel, so a row's outputs do not depend on which takes its batch.
+__device__ __forceinline__ void i8_blades(int r00, int i00, int r01, int i01, int r10, int i10, int r11, int i11, float scale,
+                                          const float (&bias)[8], float (&y)[8]) {
+  const int t[8] = {r00 + r11, r10 + r01, i10 - i01, r00 - r11, i00 - i11, r10 - r01, i10 + i01, i00 + i11};
+#pragma unroll
+  for (int c = 0; c < 8; ++c) y[c] = __builtin_fmaf((float)t[c], scale, bias[c]);
 }
 
-// 4 d_in products of codes up to 127 and -128 stay below 2^31
-constexpr int kI8MaxInputs = 32768;
+// Sums and differences of two sums of 4 d_in products of codes (up to 127, and -128 where a code is complemented) stay
+// below 2^31
+constexpr int kI8MaxInputs = 16384;
 
 }  // namespace ygg

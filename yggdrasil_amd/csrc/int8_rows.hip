@@ -169,15 +169,13 @@ __global__ __launch_bounds__(256) void int8_linear_simple_kernel(const uint4* __
           im[a][b] = dot(U, xim, dot(V, xre, im[a][b]));
         }
       }
-  const float sw = ws[(size_t)e * d_out + j], sx = in ? xs[src] : 0.f;
-  auto val = [&](int q) { return i8_value(q, sw, sx); };
-  float o[8];
-  pauli_to_blade(val(re[0][0]), val(im[0][0]), val(re[0][1]), val(im[0][1]), val(re[1][0]), val(im[1][0]), val(re[1][1]),
-                 val(im[1][1]), o);
+  float o[8], bv[8] = {};
   if (bias) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) o[c] += bias[((size_t)e * d_out + j) * 8 + blade_to_mask(c)];
+    for (int c = 0; c < 8; ++c) bv[c] = bias[((size_t)e * d_out + j) * 8 + blade_to_mask(c)];
   }
+  i8_blades(re[0][0], im[0][0], re[0][1], im[0][1], re[1][0], im[1][0], re[1][1], im[1][1],
+            ws[(size_t)e * d_out + j] * (in ? xs[src] : 0.f), bv, o);
   activate_blade<ACT>(o);
   store_out(y, (size_t)r * d_out + j, o);
 }
@@ -196,7 +194,7 @@ int launch_linear(const void* x, const float* xs, int x_rows, const int32_t* gat
 size_t int8_rows_bytes(size_t rows, int d) { return rows * i8_row_bytes(d); }
 
 const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out) {
-  if (d_in > kI8MaxInputs) return "int8 products sum at most 32768 inputs in 32 bits";
+  if (d_in > kI8MaxInputs) return "int8 products sum at most 16384 inputs in 32 bits";
   if (d_out > 1 << 19) return "int8 products write at most 524288 channels";
   if (i8_expert_bytes(d_out, d_in) >= 0x7fffffffull) return "one expert's int8 weights exceed 2 GiB";
   if (gathered && (uint64_t)x_rows * i8_row_bytes(d_in) >= 0x7fffffffull) return "the gathered int8 rows exceed 2 GiB";

@@ -40,9 +40,26 @@ __device__ __forceinline__ void i8_dma(__amdgpu_buffer_rsrc_t r, uint32_t lds, u
     asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, %3 offen lds" ::"v"(off), "s"(m0), "s"(r), "s"(so)
                  : "m0", "memory");
 }
-// every direct load landed and every LDS read returned, in all waves
+// at most N of every wave's memory operations outstanding, every LDS read returned, in all waves
+template <int N>
 __device__ __forceinline__ void i8_sync() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+
+template <int YT>
+__device__ __forceinline__ void store_blades(const float (&y)[8], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+  if constexpr (YT == kBF16) {
+    const u32x4_t o = {pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]), pack2_bf16(y[6], y[7])};
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, 0);
+  } else {
+    u32x4_t lo, hi;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) lo[c] = __builtin_bit_cast(unsigned, y[c]), hi[c] = __builtin_bit_cast(unsigned, y[4 + c]);
+    __builtin_amdgcn_raw_buffer_store_b128(lo, r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(hi, r, off + 16, 0, 0);
+  }
 }
 
 struct I8Tile {
@@ -50,8 +67,9 @@ struct I8Tile {
   static constexpr int A_BYTES = 2 * T * kI8StepBytes;       // 16 KiB: 128 half-rows of a K step
   static constexpr int W_BYTES = BN / 8 * kI8BlockBytes;     // 16 KiB
   static constexpr int STAGE = A_BYTES + W_BYTES;
-  static constexpr int S_OFF = 2 * STAGE;                    // 2 x 64 row scales (tile parity)
-  static constexpr int LDS = S_OFF + 2 * 256;
+  // by tile parity: 64 channels' bias and scale, 64 rows' scale and (gathered) place
+  static constexpr int BIAS = 0, WS = 2048, XS = WS + 256, IDX = XS + 256, SIDE = IDX + 256;
+  static constexpr int SIDE_OFF = 2 * STAGE, LDS = SIDE_OFF + 2 * SIDE;
 };
 
 template <int ACT, int YT>
@@ -112,29 +130,45 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   // swizzle) and of W (load q: 8 channels' U or V, matrix row a in front of the channel).
   const uint32_t lds0 = i8_lds(smem);
   __amdgpu_buffer_rsrc_t x_rsrc = rsrc_from(X, 0, x_bytes), s_rsrc = rsrc_from(xs, 0, (uint64_t)x_rows * 4), w_rsrc = x_rsrc;
-  uint32_t a_off[4], w_off[4], s_off = 0;
+  const __amdgpu_buffer_rsrc_t b_rsrc = rsrc_from(bias, 0, bias ? (uint64_t)E * d_out * 32 : 0);
+  const __amdgpu_buffer_rsrc_t ws_rsrc = rsrc_from(ws, 0, (uint64_t)E * d_out * 4);
+  uint32_t a_off[4], w_off[4];
   const uint32_t w_lane = (uint32_t)(lane >> 4) * 256 + (2 * (lane & 7) + ((lane >> 3) & 1)) * 16;
-  auto point_at = [&](const Info& t) __attribute__((always_inline)) {
+  auto side = [&](int n) { return lds0 + C::SIDE_OFF + (n & 1) * C::SIDE; };
+  // the rows of tile n that a gather names, asked for before the tile's first loads need them (past the tile's end
+  // the last row again)
+  auto ask_rows = [&](const Info& t, int n) __attribute__((always_inline)) {
+    if (gather && wave == 3)
+      i8_dma<4>(rsrc_from(gather, (uint64_t)t.row0 * 4, (uint64_t)(t.row_end - t.row0) * 4), side(n) + C::IDX,
+                (uint32_t)min(lane, t.row_end - t.row0 - 1) * 4, 0);
+  };
+  auto point_at = [&](const Info& t, int n) __attribute__((always_inline)) {
     if (!gather) {  // the tile's rows in place
       const uint64_t first = (uint64_t)t.row0 * half_bytes * 2;
       x_rsrc = rsrc_from(X, first, x_bytes - first);
       s_rsrc = rsrc_from(xs, (uint64_t)t.row0 * 4, (uint64_t)(x_rows - t.row0) * 4);
     }
     w_rsrc = rsrc_from(W, (uint64_t)t.e * expert_bytes, expert_bytes);
-    auto source = [&](int tok) {  // the byte offset of a row of the tile; past its end the last row again
-      const int r = min(t.row0 + tok, t.row_end - 1);
-      return gather ? gather[r] : r - t.row0;
-    };
-    const int own = source(lane);
-    s_off = !gather || (unsigned)own < (unsigned)x_rows ? (uint32_t)own * 4 : kBufferOff;
+    const int* const idx = reinterpret_cast<const int*>(smem + C::SIDE_OFF + (n & 1) * C::SIDE + C::IDX);
+    auto source = [&](int tok) { return gather ? idx[tok] : min(tok, t.row_end - t.row0 - 1); };
+    // (a place outside x, or behind the last channel, reads zeros)
+    if (wave < 2) {
+      const int at = wave * 1024 + lane * 16;
+      i8_dma<16>(b_rsrc, side(n) + C::BIAS + wave * 1024,
+                 t.col0 + (at >> 5) < d_out ? (uint32_t)(t.e * d_out + t.col0) * 32 + at : kBufferOff, 0);
+    } else if (wave == 2) {
+      i8_dma<4>(ws_rsrc, side(n) + C::WS, t.col0 + lane < d_out ? (uint32_t)(t.e * d_out + t.col0 + lane) * 4 : kBufferOff, 0);
+    } else {
+      const int own = source(lane);
+      i8_dma<4>(s_rsrc, side(n) + C::XS, (unsigned)own < (unsigned)x_rows ? (uint32_t)own * 4 : kBufferOff, 0);
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int r = 8 * (4 * wave + u) + (lane >> 3);
+      const int q = 4 * wave + u, r = 8 * q + (lane >> 3);
       const int src = source(r >> 1);
-      a_off[u] = !gather || (unsigned)src < (unsigned)x_rows
+      a_off[u] = (unsigned)src < (unsigned)x_rows
                      ? (uint32_t)(2 * src + (r & 1)) * half_bytes + (((lane & 7) ^ (r & 7)) << 4)
                      : kBufferOff;
-      const int q = 4 * wave + u;
       w_off[u] = (uint32_t)(t.col0 / 8 + (q >> 1)) * steps * kI8BlockBytes + (q & 1) * 1024 + w_lane;
     }
   };
@@ -152,23 +186,33 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   i32x16_t acc[2][2][2];  // [row block][a][re, im]
   int vsum[2];
 
+  // The next tile's first step is asked for in the last step of this one, and the rows of the tile after it; the
+  // stores of the epilogue come behind them, so the wait for that step leaves them on their way.
+  constexpr int kStores = 16 * (YT == kBF16 ? 1 : 2);
   int n = 0, ks = 0, stage = 0;
-  Info now = decode(0);
-  point_at(now);
+  Info now = decode(0), next = now;
+  ask_rows(now, 0);
+  i8_sync<0>();
+  point_at(now, 0);
   issue(0, 0);
-  if (wave == 0) i8_dma<4>(s_rsrc, lds0 + C::S_OFF, s_off, 0);
-  Info next = now;
+  if (n_mine > 1) {
+    next = decode(1);
+    ask_rows(next, 1);
+  }
+  i8_sync<0>();
   for (;;) {
-    i8_sync();
     const bool last = ks == steps - 1;
     const bool more = n + 1 < n_mine;
+    Info after = next;
     if (!last) {
       issue(ks + 1, stage ^ 1);
     } else if (more) {
-      next = decode(n + 1);
-      point_at(next);
+      point_at(next, n + 1);
       issue(0, stage ^ 1);
-      if (wave == 0) i8_dma<4>(s_rsrc, lds0 + C::S_OFF + ((n + 1) & 1) * 256, s_off, 0);
+      if (n + 2 < n_mine) {
+        after = decode(n + 2);
+        ask_rows(after, n + 2);
+      }
     }
     if (ks == 0) {
 #pragma unroll
@@ -210,47 +254,45 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
     stage ^= 1;
     if (!last) {
       ++ks;
+      i8_sync<0>();
       continue;
     }
-    // the epilogue of tile n: sums to floats, scales, blades, bias, activation
-    const int j = now.col0 + wj * 32 + l32;
+    // the epilogue of tile n: sums to blades in whole numbers, scales and bias, activation
+    const int jl = wj * 32 + l32, j = now.col0 + jl;
+    const unsigned char* const sd = smem + C::SIDE_OFF + (n & 1) * C::SIDE;
+    const float sw = *reinterpret_cast<const float*>(sd + C::WS + jl * 4);
+    float bv[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) bv[c] = *reinterpret_cast<const float*>(sd + C::BIAS + jl * 32 + blade_to_mask(c) * 4);
+    int vs[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) vs[a] = vsum[a] + __shfl_xor(vsum[a], 32);
+    const float* const scale = reinterpret_cast<const float*>(sd + C::XS);
     constexpr int MV_BYTES = YT == kBF16 ? 16 : 32;
-    if (j < d_out) {
-      const float sw = ws[(size_t)now.e * d_out + j];
-      float bv[8] = {};
-      if (bias) {
+    const __amdgpu_buffer_rsrc_t y_rsrc = rsrc_from(Y, (uint64_t)now.row0 * d_out * MV_BYTES,
+                                                    (uint64_t)(now.row_end - now.row0) * d_out * MV_BYTES);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) bv[c] = bias[((size_t)now.e * d_out + j) * 8 + blade_to_mask(c)];
-      }
-      int vs[2];
+    for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-      for (int a = 0; a < 2; ++a) vs[a] = vsum[a] + __shfl_xor(vsum[a], 32);
-      const float* const scale = reinterpret_cast<const float*>(smem + C::S_OFF + (n & 1) * 256);
-      const uint64_t first = (uint64_t)now.row0 * d_out * MV_BYTES;
-      const __amdgpu_buffer_rsrc_t y_rsrc =
-          rsrc_from(Y, first, (uint64_t)(now.row_end - now.row0) * d_out * MV_BYTES);
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int tok = wt * 32 + rb * 16 + 4 * q + 2 * g + h;  // its halves b = 0, 1 are sums v, v + 1
-            if (now.row0 + tok >= now.row_end) continue;
-            const int v = 4 * q + 2 * h;
-            const float sx = scale[tok];
-            auto val = [&](int s) { return i8_value(s, sw, sx); };
-            const auto& s = acc[rb];
-            pauli_store_mv<ACT, kOutBlade, YT, false>(
-                val(s[0][0][v] + vs[0]), val(s[0][1][v]), val(s[0][0][v + 1] + vs[0]), val(s[0][1][v + 1]),
-                val(s[1][0][v] + vs[1]), val(s[1][1][v]), val(s[1][0][v + 1] + vs[1]), val(s[1][1][v + 1]), bv, y_rsrc,
-                (uint32_t)(tok * d_out + j) * MV_BYTES, 0, d_out, y_rsrc, 0, 0, uint4{});
-          }
-    }
+        for (int h = 0; h < 2; ++h) {
+          const int tok = wt * 32 + rb * 16 + 4 * q + 2 * g + h;  // its halves b = 0, 1 are sums v, v + 1
+          const int v = 4 * q + 2 * h;
+          const auto& s = acc[rb];
+          float y[8];
+          i8_blades(s[0][0][v] + vs[0], s[0][1][v], s[0][0][v + 1] + vs[0], s[0][1][v + 1], s[1][0][v] + vs[1], s[1][1][v],
+                    s[1][0][v + 1] + vs[1], s[1][1][v + 1], sw * scale[tok], bv, y);
+          activate_blade<ACT>(y);
+          // (a store behind the tile's last row or channel lies past the buffer: every wave stores as often)
+          store_blades<YT>(y, y_rsrc, j < d_out ? (uint32_t)(tok * d_out + j) * MV_BYTES : kBufferOff);
+        }
     if (!more) break;
     now = next;
+    next = after;
     ++n;
     ks = 0;
+    i8_sync<kStores>();
   }
 }
 
