@@ -9,12 +9,13 @@
 // multivectors, a channel a lane, so that the epilogue needs no exchange.
 //
 // Tile: 64 tokens x 64 channels, four waves of 32 x 32 (128 sums a lane), two workgroups a CU, so that one's epilogue
-// overlaps the other's products.  K steps of 32 inputs (a line of memory a half-row) go straight to LDS, two stages
-// of 32 KiB.  Persistent: a workgroup asks for its next tile's first step before the epilogue of this one.
-
+// overlaps the other's products.  A K step is 32 inputs, a line of memory a half-row; its operands go straight to LDS
+// (two stages of 32 KiB), and within it each group of products has its operands read during the group before.
+// Persistent, one stream of steps over a workgroup's tiles: the loads run on through the epilogues.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "int8_rows.h"
 #include "pauli_tile.h"
@@ -64,12 +65,21 @@ __device__ __forceinline__ void store_blades(const float (&y)[8], __amdgpu_buffe
 
 struct I8Tile {
   static constexpr int NT = 256, T = 64, BN = 64;
-  static constexpr int A_BYTES = 2 * T * kI8StepBytes;       // 16 KiB: 128 half-rows of a K step
-  static constexpr int W_BYTES = BN / 8 * kI8BlockBytes;     // 16 KiB
+  static constexpr int A_BYTES = 2 * T * kI8StepBytes;    // 16 KiB: 128 half-rows of a K step
+  static constexpr int W_BYTES = BN / 8 * kI8BlockBytes;  // 16 KiB
   static constexpr int STAGE = A_BYTES + W_BYTES;
-  // by tile parity: 64 channels' bias and scale, 64 rows' scale and (gathered) place
+  // by tile parity: bias and scale of 64 channels, scale and (gathered) place of 64 rows
   static constexpr int BIAS = 0, WS = 2048, XS = WS + 256, IDX = XS + 256, SIDE = IDX + 256;
   static constexpr int SIDE_OFF = 2 * STAGE, LDS = SIDE_OFF + 2 * SIDE;
+  static_assert(LDS <= 80 * 1024, "two workgroups a CU");
+};
+
+// A tile.  The sums of block `which` (tokens 16 which .. of a wave's 32) alone where `half`; `compact`: an expert's last
+// rows, at most 32, laid into the tokens of block 0.
+struct I8Item {
+  int e, row0, row_end, col0;
+  bool half, compact;
+  int which;
 };
 
 template <int ACT, int YT>
@@ -85,40 +95,49 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   const int wt = wave & 1, wj = wave >> 1;
   const int g = lane >> 5, l32 = lane & 31;
 
-  // lane e: expert e's rows and the tiles before its own
+  // lane e: expert e's rows, and the tiles up to its last: whole ones, and short last ones ("compact", half the products)
   const int v_beg = min(lane < E ? offsets[lane] : 0, P_max), v_end = min(lane < E ? offsets[lane + 1] : 0, P_max);
-  const int v_nt = (v_end - v_beg + C::T - 1) / C::T;
-  int v_incl = v_nt;
+  const int v_all = (v_end - v_beg + C::T - 1) / C::T;
+  const int v_short = v_all > 0 && v_end - v_beg - (v_all - 1) * C::T <= C::T / 2 ? 1 : 0;
+  const int v_nt = v_all - v_short;
+  int v_incl = v_nt, v_sincl = v_short;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(v_incl, o);
-    if (lane >= o) v_incl += v;
+    const int p = __shfl_up(v_incl, o), q = __shfl_up(v_sincl, o);
+    if (lane >= o) v_incl += p, v_sincl += q;
   }
+  // One contiguous range of each list an XCD, a row tile's columns next to each other: the whole tiles in rounds over
+  // the XCD's workgroups, then items of half the work -- the compact tiles, and the whole tiles of the last round cut
+  // in halves where these still fit in one --, from the first workgroup that has a whole tile less.
   const int CT = (d_out + C::BN - 1) / C::BN;
-  const int n_tiles = __builtin_amdgcn_readlane(v_incl, 63) * CT;
-  // one contiguous range of tiles an XCD, a row tile's columns next to each other
+  const int n_whole = __builtin_amdgcn_readlane(v_incl, 63) * CT, n_short = __builtin_amdgcn_readlane(v_sincl, 63) * CT;
   const int per_xcd = gridDim.x / n_xcd;
   const int xcd = blockIdx.x % n_xcd, slot = blockIdx.x / n_xcd;
-  const int lo = (int)((long long)n_tiles * xcd / n_xcd), hi = (int)((long long)n_tiles * (xcd + 1) / n_xcd);
-  const int n_mine = hi - lo > slot ? (hi - lo - slot + per_xcd - 1) / per_xcd : 0;
+  auto cut = [&](int n, int x) { return (int)((long long)n * x / n_xcd); };
+  const int lo = cut(n_whole, xcd), R = cut(n_whole, xcd + 1) - lo;
+  const int slo = cut(n_short, xcd), n_shorts = cut(n_short, xcd + 1) - slo;
+  const int rounds = R / per_xcd, rem = R - rounds * per_xcd;
+  const bool split = rem > 0 && 2 * rem <= per_xcd;
+  const int n_full = rounds + (!split && slot < rem ? 1 : 0);
+  const int n_items = n_shorts + (split ? 2 * rem : 0);
+  const int rank = split || slot >= rem ? slot - (split ? 0 : rem) : slot - rem + per_xcd;
+  const int n_mine = n_full + (n_items > rank ? (n_items - rank + per_xcd - 1) / per_xcd : 0);
   if (n_mine == 0) return;
 
-  const int steps = i8_steps(d_in);
-  const uint32_t half_bytes = (uint32_t)steps * kI8StepBytes;   // of a half-row
-  const size_t expert_bytes = i8_expert_bytes(d_out, d_in);
-  struct Info {
-    int e, row0, row_end, col0;
-  };
   auto decode = [&](int n) __attribute__((always_inline)) {
-    const int L = lo + slot + n * per_xcd;
+    const int item = n - n_full < 0 ? -1 : rank + (n - n_full) * per_xcd;
+    I8Item t;
+    t.half = item >= 0;
+    t.compact = item >= 0 && item < n_shorts;
+    const int L = t.compact ? slo + item : item >= 0 ? lo + rounds * per_xcd + ((item - n_shorts) >> 1) : lo + slot + n * per_xcd;
+    t.which = t.half && !t.compact ? (item - n_shorts) & 1 : 0;
     const int rt = L / CT;
-    const int e = (int)__builtin_ctzll(__ballot(v_incl > rt));
-    Info t;
-    t.e = e;
-    t.row_end = __builtin_amdgcn_readlane(v_end, e);
-    t.row0 = __builtin_amdgcn_readlane(v_beg, e) +
-             (rt - (__builtin_amdgcn_readlane(v_incl, e) - __builtin_amdgcn_readlane(v_nt, e))) * C::T;
     t.col0 = (L - rt * CT) * C::BN;
+    t.e = (int)__builtin_ctzll(__ballot((t.compact ? v_sincl : v_incl) > rt));
+    const int beg = __builtin_amdgcn_readlane(v_beg, t.e);
+    const int whole = __builtin_amdgcn_readlane(v_nt, t.e);
+    t.row_end = __builtin_amdgcn_readlane(v_end, t.e);
+    t.row0 = beg + (t.compact ? whole : rt - (__builtin_amdgcn_readlane(v_incl, t.e) - whole)) * C::T;
     return t;
   };
   auto rsrc_from = [](const void* base, uint64_t off, uint64_t bytes) __attribute__((always_inline)) {
@@ -126,50 +145,69 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
                                              (uint32_t)(bytes < 0x7fffffffull ? bytes : 0x7fffffffull), kBufferFlags);
   };
 
-  // What the loads of a tile need: this lane's pieces of A (half-rows 8 q + lane / 8 of load q = 4 wave + u, through the
-  // swizzle) and of W (load q: 8 channels' U or V, matrix row a in front of the channel).
+  const int steps = i8_steps(d_in);
+  const uint32_t half_bytes = (uint32_t)steps * kI8StepBytes;  // of a half-row
+  const size_t expert_bytes = i8_expert_bytes(d_out, d_in);
   const uint32_t lds0 = i8_lds(smem);
   __amdgpu_buffer_rsrc_t x_rsrc = rsrc_from(X, 0, x_bytes), s_rsrc = rsrc_from(xs, 0, (uint64_t)x_rows * 4), w_rsrc = x_rsrc;
   const __amdgpu_buffer_rsrc_t b_rsrc = rsrc_from(bias, 0, bias ? (uint64_t)E * d_out * 32 : 0);
   const __amdgpu_buffer_rsrc_t ws_rsrc = rsrc_from(ws, 0, (uint64_t)E * d_out * 4);
-  uint32_t a_off[4], w_off[4];
-  const uint32_t w_lane = (uint32_t)(lane >> 4) * 256 + (2 * (lane & 7) + ((lane >> 3) & 1)) * 16;
-  auto side = [&](int n) { return lds0 + C::SIDE_OFF + (n & 1) * C::SIDE; };
-  // the rows of tile n that a gather names, asked for before the tile's first loads need them (past the tile's end
-  // the last row again)
-  auto ask_rows = [&](const Info& t, int n) __attribute__((always_inline)) {
-    if (gather && wave == 3)
-      i8_dma<4>(rsrc_from(gather, (uint64_t)t.row0 * 4, (uint64_t)(t.row_end - t.row0) * 4), side(n) + C::IDX,
-                (uint32_t)min(lane, t.row_end - t.row0 - 1) * 4, 0);
+
+  // The rows that a gather names, asked for a tile before the tile's own loads need them (past the tile's end the last
+  // row again).  Token slot t of a tile is its row t, or of a compact one row 16 (t / 32) + t % 16.
+  auto ask_rows = [&](const I8Item& t, int n) __attribute__((always_inline)) {
+    if (gather && wave == 3) {
+      const int row = t.compact ? (lane >> 5) * 16 + (lane & 15) : lane;
+      i8_dma<4>(rsrc_from(gather, (uint64_t)t.row0 * 4, (uint64_t)(t.row_end - t.row0) * 4), lds0 + C::SIDE_OFF + (n & 1) * C::SIDE + C::IDX,
+                (uint32_t)min(row, t.row_end - t.row0 - 1) * 4, 0);
+    }
   };
-  auto point_at = [&](const Info& t, int n) __attribute__((always_inline)) {
+  // What the row loads of a tile need -- this lane's pieces are half-rows 8 q + lane / 8 of load q = 4 wave + u, through
+  // the swizzle --, and the loads of its side.  A place outside x, behind the last channel or in a block that is not
+  // computed reads zeros, without traffic.
+  uint32_t a_off[4];
+  auto point_rows = [&](const I8Item& t, int n) __attribute__((always_inline)) {
     if (!gather) {  // the tile's rows in place
       const uint64_t first = (uint64_t)t.row0 * half_bytes * 2;
       x_rsrc = rsrc_from(X, first, x_bytes - first);
       s_rsrc = rsrc_from(xs, (uint64_t)t.row0 * 4, (uint64_t)(x_rows - t.row0) * 4);
     }
-    w_rsrc = rsrc_from(W, (uint64_t)t.e * expert_bytes, expert_bytes);
     const int* const idx = reinterpret_cast<const int*>(smem + C::SIDE_OFF + (n & 1) * C::SIDE + C::IDX);
-    auto source = [&](int tok) { return gather ? idx[tok] : min(tok, t.row_end - t.row0 - 1); };
-    // (a place outside x, or behind the last channel, reads zeros)
+    auto source = [&](int tok) {
+      const int row = t.compact ? (tok >> 5) * 16 + (tok & 15) : tok;
+      const int src = gather ? idx[tok] : min(row, t.row_end - t.row0 - 1);
+      return t.half && ((tok >> 4) & 1) != t.which ? -1 : src;
+    };
+    const uint32_t side = lds0 + C::SIDE_OFF + (n & 1) * C::SIDE;
     if (wave < 2) {
       const int at = wave * 1024 + lane * 16;
-      i8_dma<16>(b_rsrc, side(n) + C::BIAS + wave * 1024,
+      i8_dma<16>(b_rsrc, side + C::BIAS + wave * 1024,
                  t.col0 + (at >> 5) < d_out ? (uint32_t)(t.e * d_out + t.col0) * 32 + at : kBufferOff, 0);
     } else if (wave == 2) {
-      i8_dma<4>(ws_rsrc, side(n) + C::WS, t.col0 + lane < d_out ? (uint32_t)(t.e * d_out + t.col0 + lane) * 4 : kBufferOff, 0);
+      i8_dma<4>(ws_rsrc, side + C::WS, t.col0 + lane < d_out ? (uint32_t)(t.e * d_out + t.col0 + lane) * 4 : kBufferOff, 0);
     } else {
       const int own = source(lane);
-      i8_dma<4>(s_rsrc, side(n) + C::XS, (unsigned)own < (unsigned)x_rows ? (uint32_t)own * 4 : kBufferOff, 0);
+      i8_dma<4>(s_rsrc, side + C::XS, (unsigned)own < (unsigned)x_rows ? (uint32_t)own * 4 : kBufferOff, 0);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int q = 4 * wave + u, r = 8 * q + (lane >> 3);
+      const int r = 8 * (4 * wave + u) + (lane >> 3);
       const int src = source(r >> 1);
       a_off[u] = (unsigned)src < (unsigned)x_rows
-                     ? (uint32_t)(2 * src + (r & 1)) * half_bytes + (((lane & 7) ^ (r & 7)) << 4)
+                     ? (uint32_t)(2 * src + (r & 1)) * half_bytes + (((lane & 7) ^ ((r >> 1) & 7)) << 4)
                      : kBufferOff;
-      w_off[u] = (uint32_t)(t.col0 / 8 + (q >> 1)) * steps * kI8BlockBytes + (q & 1) * 1024 + w_lane;
+    }
+  };
+  // Weights: load q = 4 wave + u of a K step is 8 channels' U or V, 16 bytes of matrix row a and channel jj from (g, n =
+  // 2 jj + a); an odd block of channels has its rows a exchanged, so that 16 lanes of a read meet all banks.
+  uint32_t w_off[4];
+  auto point_weights = [&](const I8Item& t) __attribute__((always_inline)) {
+    w_rsrc = rsrc_from(W, (uint64_t)t.e * expert_bytes, expert_bytes);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int q = 4 * wave + u, a = ((lane >> 3) ^ (q >> 1)) & 1;
+      w_off[u] = (uint32_t)(t.col0 / 8 + (q >> 1)) * steps * kI8BlockBytes + (q & 1) * 1024 + (lane >> 4) * 256 +
+                 (2 * (lane & 7) + a) * 16;
     }
   };
   auto issue = [&](int ks, int stage) __attribute__((always_inline)) {
@@ -181,118 +219,137 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   };
 
   // this lane's operands in a stage
-  const uint32_t a_rd = (uint32_t)(wt * 64 + l32) * 128;
-  const uint32_t w_rd = C::A_BYTES + (uint32_t)(wj * 4 + (l32 >> 3)) * kI8BlockBytes + (uint32_t)g * 256 + (l32 & 7) * 16;
+  uint32_t a_rd[2], w_rd[2];  // [h] (the imaginary parts at ^ 64), [a]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    a_rd[h] = (uint32_t)(wt * 64 + l32) * 128 + (((2 * h + g) ^ ((l32 >> 1) & 7)) << 4);
+    w_rd[h] = C::A_BYTES + (uint32_t)(wj * 4 + (l32 >> 3)) * kI8BlockBytes + (uint32_t)g * 256 + ((h ^ (l32 >> 3)) & 1) * 128 +
+              (l32 & 7) * 16;
+  }
   i32x16_t acc[2][2][2];  // [row block][a][re, im]
   int vsum[2];
+  // A K step, of one row block where `half`, the first of a tile starting the sums: four groups of products, (h, a) -- 16
+  // inputs, one matrix row of the weights --, each group's operands read during the one before.
+  auto k_step = [&](uint32_t at, bool half, int which, auto first_tag) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first_tag)::value;
+    const unsigned char* const st = smem + at;
+    const uint32_t block = half ? which * 4096 : 0;
+    i8x16_t xr[2][2], xi[2][2], u[2], v[2];  // [h][rb], [a]
+    auto read = [&](int grp) __attribute__((always_inline)) {
+      const int h = grp >> 1, a = grp & 1;
+      if (a == 0) {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          xr[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + a_rd[h] + rb * 4096);
+          xi[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + (a_rd[h] ^ 64) + rb * 4096);
+        }
+      }
+      u[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512);
+      v[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512 + 1024);
+    };
+    if constexpr (FIRST) vsum[0] = vsum[1] = 0;
+    read(0);
+#pragma unroll
+    for (int grp = 0; grp < 4; ++grp) {
+      const int h = grp >> 1, a = grp & 1;
+      if (grp < 3) read(grp + 1);
+      auto multiply = [&](int rb) __attribute__((always_inline)) {
+        const bool zero = FIRST && h == 0;
+        acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][0], 0, 0, 0);
+        acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xi[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][1], 0, 0, 0);
+        acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(~xi[h][rb], v[a], acc[rb][a][0], 0, 0, 0);
+        acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], v[a], acc[rb][a][1], 0, 0, 0);
+      };
+      multiply(0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vsum[a] = __builtin_amdgcn_sdot4(v[a][q], 0x01010101, vsum[a], false);
+      if (!half) multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
 
-  // The next tile's first step is asked for in the last step of this one, and the rows of the tile after it; the
-  // stores of the epilogue come behind them, so the wait for that step leaves them on their way.
+  // The stream of K steps: during one, the next one's operands are asked for, in a tile's last step those of the next
+  // tile's first and the rows of the tile after it.  The epilogue's stores come behind them, so the wait for that step
+  // leaves them on their way.
   constexpr int kStores = 16 * (YT == kBF16 ? 1 : 2);
-  int n = 0, ks = 0, stage = 0;
-  Info now = decode(0), next = now;
-  ask_rows(now, 0);
+  I8Item t = decode(0), next = t;
+  ask_rows(t, 0);
   i8_sync<0>();
-  point_at(now, 0);
+  point_rows(t, 0);
+  point_weights(t);
   issue(0, 0);
   if (n_mine > 1) {
     next = decode(1);
     ask_rows(next, 1);
   }
   i8_sync<0>();
-  for (;;) {
-    const bool last = ks == steps - 1;
-    const bool more = n + 1 < n_mine;
-    Info after = next;
-    if (!last) {
-      issue(ks + 1, stage ^ 1);
-    } else if (more) {
-      point_at(next, n + 1);
-      issue(0, stage ^ 1);
-      if (n + 2 < n_mine) {
-        after = decode(n + 2);
-        ask_rows(after, n + 2);
+  int stage = 0;
+  for (int n = 0;; ++n) {
+    I8Item after = next;
+    auto run = [&](int ks, auto first_tag) __attribute__((always_inline)) {
+      if (ks + 1 < steps) {
+        issue(ks + 1, stage ^ 1);
+      } else if (n + 1 < n_mine) {
+        point_rows(next, n + 1);
+        point_weights(next);
+        issue(0, stage ^ 1);
+        if (n + 2 < n_mine) {
+          after = decode(n + 2);
+          ask_rows(after, n + 2);
+        }
       }
+      __builtin_amdgcn_s_setprio(2);
+      k_step(stage * C::STAGE, t.half, t.which, first_tag);
+      __builtin_amdgcn_s_setprio(0);
+      stage ^= 1;
+    };
+    run(0, std::true_type{});
+#pragma unroll 1
+    for (int ks = 1; ks < steps; ++ks) {
+      i8_sync<0>();
+      run(ks, std::false_type{});
     }
-    if (ks == 0) {
+    {
+      // the epilogue: sums to blades in whole numbers, scales and bias, activation
+      const int jl = wj * 32 + l32, j = t.col0 + jl;
+      const unsigned char* const sd = smem + C::SIDE_OFF + (n & 1) * C::SIDE;
+      const float sw = *reinterpret_cast<const float*>(sd + C::WS + jl * 4);
+      float bv[8];
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
+      for (int c = 0; c < 8; ++c) bv[c] = *reinterpret_cast<const float*>(sd + C::BIAS + jl * 32 + blade_to_mask(c) * 4);
+      int vs[2];
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[rb][a][p][v] = 0;
-      vsum[0] = vsum[1] = 0;
-    }
-    const unsigned char* const st = smem + stage * C::STAGE;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i8x16_t xr[2], xi[2], xn[2];
+      for (int a = 0; a < 2; ++a) vs[a] = vsum[a] + __shfl_xor(vsum[a], 32);
+      constexpr int MV_BYTES = YT == kBF16 ? 16 : 32;
+      const __amdgpu_buffer_rsrc_t y_rsrc = rsrc_from(Y, (uint64_t)t.row0 * d_out * MV_BYTES,
+                                                      (uint64_t)(t.row_end - t.row0) * d_out * MV_BYTES);
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb) {
-        const unsigned char* p = st + a_rd + rb * 4096;
-        xr[rb] = *reinterpret_cast<const i8x16_t*>(p + (((2 * h + g) ^ (l32 & 7)) << 4));
-        xi[rb] = *reinterpret_cast<const i8x16_t*>(p + (((4 + 2 * h + g) ^ (l32 & 7)) << 4));
-        xn[rb] = ~xi[rb];
-      }
+        if (rb == 1 && t.half) break;
+        const int tok0 = wt * 32 + (t.half ? t.which : rb) * 16;             // token slot of the block's first row
+        const int row0 = (t.compact ? wt * 16 : tok0) + 2 * g;               // its row in the tile, this lane's first
+        const float* const scale = reinterpret_cast<const float*>(sd + C::XS) + tok0 + 2 * g;
+        const uint32_t at = j < d_out ? (uint32_t)(row0 * d_out + j) * MV_BYTES : kBufferOff;
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const i8x16_t u = *reinterpret_cast<const i8x16_t*>(st + w_rd + h * 512 + a * 128);
-        const i8x16_t v = *reinterpret_cast<const i8x16_t*>(st + w_rd + 1024 + h * 512 + a * 128);
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) vsum[a] = __builtin_amdgcn_sdot4(v[q], 0x01010101, vsum[a], false);
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[rb], u, acc[rb][a][0], 0, 0, 0);
-          acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xi[rb], u, acc[rb][a][1], 0, 0, 0);
-          acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xn[rb], v, acc[rb][a][0], 0, 0, 0);
-          acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[rb], v, acc[rb][a][1], 0, 0, 0);
-        }
+          for (int h = 0; h < 2; ++h) {
+            const int v = 4 * q + 2 * h;  // the halves b = 0, 1 of row 4 q + h are sums v, v + 1
+            const auto& s = acc[rb];
+            float y[8];
+            i8_blades(s[0][0][v] + vs[0], s[0][1][v], s[0][0][v + 1] + vs[0], s[0][1][v + 1], s[1][0][v] + vs[1], s[1][1][v],
+                      s[1][0][v + 1] + vs[1], s[1][1][v + 1], sw * scale[4 * q + h], bv, y);
+            activate_blade<ACT>(y);
+            // (behind the tile's last row or the last channel lies past the buffer: every wave stores as often)
+            store_blades<YT>(y, y_rsrc, at + (uint32_t)((4 * q + h) * d_out) * MV_BYTES);
+          }
       }
     }
-    stage ^= 1;
-    if (!last) {
-      ++ks;
-      i8_sync<0>();
-      continue;
-    }
-    // the epilogue of tile n: sums to blades in whole numbers, scales and bias, activation
-    const int jl = wj * 32 + l32, j = now.col0 + jl;
-    const unsigned char* const sd = smem + C::SIDE_OFF + (n & 1) * C::SIDE;
-    const float sw = *reinterpret_cast<const float*>(sd + C::WS + jl * 4);
-    float bv[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) bv[c] = *reinterpret_cast<const float*>(sd + C::BIAS + jl * 32 + blade_to_mask(c) * 4);
-    int vs[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) vs[a] = vsum[a] + __shfl_xor(vsum[a], 32);
-    const float* const scale = reinterpret_cast<const float*>(sd + C::XS);
-    constexpr int MV_BYTES = YT == kBF16 ? 16 : 32;
-    const __amdgpu_buffer_rsrc_t y_rsrc = rsrc_from(Y, (uint64_t)now.row0 * d_out * MV_BYTES,
-                                                    (uint64_t)(now.row_end - now.row0) * d_out * MV_BYTES);
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tok = wt * 32 + rb * 16 + 4 * q + 2 * g + h;  // its halves b = 0, 1 are sums v, v + 1
-          const int v = 4 * q + 2 * h;
-          const auto& s = acc[rb];
-          float y[8];
-          i8_blades(s[0][0][v] + vs[0], s[0][1][v], s[0][0][v + 1] + vs[0], s[0][1][v + 1], s[1][0][v] + vs[1], s[1][1][v],
-                    s[1][0][v + 1] + vs[1], s[1][1][v + 1], sw * scale[tok], bv, y);
-          activate_blade<ACT>(y);
-          // (a store behind the tile's last row or channel lies past the buffer: every wave stores as often)
-          store_blades<YT>(y, y_rsrc, j < d_out ? (uint32_t)(tok * d_out + j) * MV_BYTES : kBufferOff);
-        }
-    if (!more) break;
-    now = next;
+    if (n + 1 == n_mine) break;
+    if (t.half) i8_sync<0>();  // (its stores are fewer)
+    else i8_sync<kStores>();
+    t = next;
     next = after;
-    ++n;
-    ks = 0;
-    i8_sync<kStores>();
   }
 }
 
@@ -303,9 +360,10 @@ int launch_tile(const void* x, const float* xs, int x_rows, const int32_t* gathe
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     cus = 256;
-  const long long most = ((long long)P / I8Tile::T + std::min(E, P)) * ((d_out + I8Tile::BN - 1) / I8Tile::BN);
+  // never more workgroups than items can exist (a tile may be cut in two)
+  const long long tiles = ((long long)P / I8Tile::T + std::min(E, P)) * ((d_out + I8Tile::BN - 1) / I8Tile::BN);
   const int xcds = cus % 8 == 0 ? 8 : 1;
-  const long long grid = std::min<long long>(2 * cus, (most + xcds - 1) / xcds * xcds);
+  const long long grid = std::min<long long>(2 * cus, (2 * tiles + xcds - 1) / xcds * xcds);
   int8_tile_kernel<ACT, YT><<<(unsigned)grid, I8Tile::NT, 0, stream>>>(
       static_cast<const unsigned char*>(x), (uint64_t)x_rows * i8_row_bytes(d_in), xs, x_rows, gather,
       static_cast<const unsigned char*>(w), ws, bias, offsets, E, d_in, d_out, P, y, xcds);
