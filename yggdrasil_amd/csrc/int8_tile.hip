@@ -10,8 +10,10 @@
 //
 // Tile: 64 tokens x 64 channels, four waves of 32 x 32 (128 sums a lane), two workgroups a CU, so that one's epilogue
 // overlaps the other's products.  A K step is 32 inputs, a line of memory a half-row; its operands go straight to LDS
-// (two stages of 32 KiB), and within it each group of products has its operands read during the group before.
-// Persistent, one stream of steps over a workgroup's tiles: the loads run on through the epilogues.
+// (two stages of 32 KiB).  A step's products are four groups, and each group's operands are read from LDS during the
+// group before: the first group's during the last of the step before, so the one barrier of a step stands in front of
+// its last group, when the step's own operands are all in registers and its stage is free for the step after the next.
+// Persistent, one stream of steps over a workgroup's tiles: loads and reads run on through the epilogues.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -68,9 +70,9 @@ struct I8Tile {
   static constexpr int A_BYTES = 2 * T * kI8StepBytes;    // 16 KiB: 128 half-rows of a K step
   static constexpr int W_BYTES = BN / 8 * kI8BlockBytes;  // 16 KiB
   static constexpr int STAGE = A_BYTES + W_BYTES;
-  // by tile parity: bias and scale of 64 channels, scale and (gathered) place of 64 rows
-  static constexpr int BIAS = 0, WS = 2048, XS = WS + 256, IDX = XS + 256, SIDE = IDX + 256;
-  static constexpr int SIDE_OFF = 2 * STAGE, LDS = SIDE_OFF + 2 * SIDE;
+  // three tiles' bias and scale of 64 channels and scale of 64 rows, two tiles' (gathered) places of 64 rows
+  static constexpr int BIAS = 0, WS = 2048, XS = WS + 256, SIDE = XS + 256;
+  static constexpr int SIDE_OFF = 2 * STAGE, IDX_OFF = SIDE_OFF + 3 * SIDE, LDS = IDX_OFF + 2 * 256;
   static_assert(LDS <= 80 * 1024, "two workgroups a CU");
 };
 
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   auto ask_rows = [&](const I8Item& t, int n) __attribute__((always_inline)) {
     if (gather && wave == 3) {
       const int row = t.compact ? (lane >> 5) * 16 + (lane & 15) : lane;
-      i8_dma<4>(rsrc_from(gather, (uint64_t)t.row0 * 4, (uint64_t)(t.row_end - t.row0) * 4), lds0 + C::SIDE_OFF + (n & 1) * C::SIDE + C::IDX,
+      i8_dma<4>(rsrc_from(gather, (uint64_t)t.row0 * 4, (uint64_t)(t.row_end - t.row0) * 4), lds0 + C::IDX_OFF + (n & 1) * 256,
                 (uint32_t)min(row, t.row_end - t.row0 - 1) * 4, 0);
     }
   };
@@ -172,13 +174,13 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
       x_rsrc = rsrc_from(X, first, x_bytes - first);
       s_rsrc = rsrc_from(xs, (uint64_t)t.row0 * 4, (uint64_t)(x_rows - t.row0) * 4);
     }
-    const int* const idx = reinterpret_cast<const int*>(smem + C::SIDE_OFF + (n & 1) * C::SIDE + C::IDX);
+    const int* const idx = reinterpret_cast<const int*>(smem + C::IDX_OFF + (n & 1) * 256);
     auto source = [&](int tok) {
       const int row = t.compact ? (tok >> 5) * 16 + (tok & 15) : tok;
       const int src = gather ? idx[tok] : min(row, t.row_end - t.row0 - 1);
       return t.half && ((tok >> 4) & 1) != t.which ? -1 : src;
     };
-    const uint32_t side = lds0 + C::SIDE_OFF + (n & 1) * C::SIDE;
+    const uint32_t side = lds0 + C::SIDE_OFF + (n % 3) * C::SIDE;
     if (wave < 2) {
       const int at = wave * 1024 + lane * 16;
       i8_dma<16>(b_rsrc, side + C::BIAS + wave * 1024,
@@ -228,91 +230,98 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   }
   i32x16_t acc[2][2][2];  // [row block][a][re, im]
   int vsum[2];
-  // A K step, of one row block where `half`, the first of a tile starting the sums: four groups of products, (h, a) -- 16
-  // inputs, one matrix row of the weights --, each group's operands read during the one before.
-  auto k_step = [&](uint32_t at, bool half, int which, auto first_tag) __attribute__((always_inline)) {
-    constexpr bool FIRST = decltype(first_tag)::value;
+  // A K step's products: group (h, a) is 16 inputs, one matrix row of the weights.  Where `half`, one row block.
+  i8x16_t xr[2][2], xi[2][2], u[2], v[2];  // [h][rb], [a]
+  auto read = [&](uint32_t at, const I8Item& t, int grp) __attribute__((always_inline)) {
+    const int h = grp >> 1, a = grp & 1;
     const unsigned char* const st = smem + at;
-    const uint32_t block = half ? which * 4096 : 0;
-    i8x16_t xr[2][2], xi[2][2], u[2], v[2];  // [h][rb], [a]
-    auto read = [&](int grp) __attribute__((always_inline)) {
-      const int h = grp >> 1, a = grp & 1;
-      if (a == 0) {
+    if (a == 0) {
+      const uint32_t block = t.half ? t.which * 4096 : 0;
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-          xr[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + a_rd[h] + rb * 4096);
-          xi[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + (a_rd[h] ^ 64) + rb * 4096);
-        }
+      for (int rb = 0; rb < 2; ++rb) {
+        xr[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + a_rd[h] + rb * 4096);
+        xi[h][rb] = *reinterpret_cast<const i8x16_t*>(st + block + (a_rd[h] ^ 64) + rb * 4096);
       }
-      u[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512);
-      v[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512 + 1024);
-    };
-    if constexpr (FIRST) vsum[0] = vsum[1] = 0;
-    read(0);
-#pragma unroll
-    for (int grp = 0; grp < 4; ++grp) {
-      const int h = grp >> 1, a = grp & 1;
-      if (grp < 3) read(grp + 1);
-      auto multiply = [&](int rb) __attribute__((always_inline)) {
-        const bool zero = FIRST && h == 0;
-        acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][0], 0, 0, 0);
-        acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xi[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][1], 0, 0, 0);
-        acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(~xi[h][rb], v[a], acc[rb][a][0], 0, 0, 0);
-        acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], v[a], acc[rb][a][1], 0, 0, 0);
-      };
-      multiply(0);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) vsum[a] = __builtin_amdgcn_sdot4(v[a][q], 0x01010101, vsum[a], false);
-      if (!half) multiply(1);
-      __builtin_amdgcn_sched_barrier(0);
     }
+    u[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512);
+    v[a] = *reinterpret_cast<const i8x16_t*>(st + w_rd[a] + h * 512 + 1024);
+  };
+  auto multiply = [&](bool half, int grp, auto first_tag) __attribute__((always_inline)) {
+    const int h = grp >> 1, a = grp & 1;
+    const bool zero = decltype(first_tag)::value && h == 0;
+    auto block = [&](int rb) __attribute__((always_inline)) {
+      acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][0], 0, 0, 0);
+      acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xi[h][rb], u[a], zero ? i32x16_t{} : acc[rb][a][1], 0, 0, 0);
+      acc[rb][a][0] = __builtin_amdgcn_mfma_i32_32x32x32_i8(~xi[h][rb], v[a], acc[rb][a][0], 0, 0, 0);
+      acc[rb][a][1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xr[h][rb], v[a], acc[rb][a][1], 0, 0, 0);
+    };
+    block(0);
+    if (zero) vsum[a] = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) vsum[a] = __builtin_amdgcn_sdot4(v[a][q], 0x01010101, vsum[a], false);
+    if (!half) block(1);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  // The stream of K steps: during one, the next one's operands are asked for, in a tile's last step those of the next
-  // tile's first and the rows of the tile after it.  The epilogue's stores come behind them, so the wait for that step
-  // leaves them on their way.
+  // The stream of K steps: c is the next step to be asked for, two ahead of the products.
+  I8Item ct = decode(0);
+  int cn = 0, cks = 0;
+  auto ask = [&](int stage) __attribute__((always_inline)) {
+    if (cn >= n_mine) return;
+    if (cks == 0) {
+      point_rows(ct, cn);
+      point_weights(ct);
+    }
+    issue(cks, stage);
+    if (++cks == steps) {
+      cks = 0;
+      if (++cn < n_mine) {
+        ct = decode(cn);
+        ask_rows(ct, cn);
+      }
+    }
+  };
+  ask_rows(ct, 0);
+  i8_sync<0>();
+  ask(0);
+  i8_sync<0>();
+  ask(1);
+  // At a step's barrier the loads of the step after it have landed: behind them come only the stores of an epilogue in
+  // between, which stay on their way.
   constexpr int kStores = 16 * (YT == kBF16 ? 1 : 2);
   I8Item t = decode(0), next = t;
-  ask_rows(t, 0);
-  i8_sync<0>();
-  point_rows(t, 0);
-  point_weights(t);
-  issue(0, 0);
-  if (n_mine > 1) {
-    next = decode(1);
-    ask_rows(next, 1);
-  }
-  i8_sync<0>();
+  read(0, t, 0);
   int stage = 0;
+  bool stores = false;
   for (int n = 0;; ++n) {
-    I8Item after = next;
-    auto run = [&](int ks, auto first_tag) __attribute__((always_inline)) {
-      if (ks + 1 < steps) {
-        issue(ks + 1, stage ^ 1);
-      } else if (n + 1 < n_mine) {
-        point_rows(next, n + 1);
-        point_weights(next);
-        issue(0, stage ^ 1);
-        if (n + 2 < n_mine) {
-          after = decode(n + 2);
-          ask_rows(after, n + 2);
-        }
-      }
+    const bool more = n + 1 < n_mine;
+    if (more) next = decode(n + 1);
+    auto k_step = [&](bool last, auto first_tag) __attribute__((always_inline)) {
+      const uint32_t at = stage * C::STAGE;
       __builtin_amdgcn_s_setprio(2);
-      k_step(stage * C::STAGE, t.half, t.which, first_tag);
+#pragma unroll
+      for (int grp = 0; grp < 3; ++grp) {
+        read(at, t, grp + 1);
+        multiply(t.half, grp, first_tag);
+      }
+      if (!last || more) {
+        if (stores) i8_sync<kStores>();
+        else i8_sync<0>();
+        stores = false;
+        ask(stage);
+        stage ^= 1;
+        read(stage * C::STAGE, last ? next : t, 0);
+      }
+      multiply(t.half, 3, first_tag);
       __builtin_amdgcn_s_setprio(0);
-      stage ^= 1;
     };
-    run(0, std::true_type{});
+    k_step(steps == 1, std::true_type{});
 #pragma unroll 1
-    for (int ks = 1; ks < steps; ++ks) {
-      i8_sync<0>();
-      run(ks, std::false_type{});
-    }
+    for (int ks = 1; ks < steps; ++ks) k_step(ks == steps - 1, std::false_type{});
     {
       // the epilogue: sums to blades in whole numbers, scales and bias, activation
       const int jl = wj * 32 + l32, j = t.col0 + jl;
-      const unsigned char* const sd = smem + C::SIDE_OFF + (n & 1) * C::SIDE;
+      const unsigned char* const sd = smem + C::SIDE_OFF + (n % 3) * C::SIDE;
       const float sw = *reinterpret_cast<const float*>(sd + C::WS + jl * 4);
       float bv[8];
 #pragma unroll
@@ -345,11 +354,9 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
           }
       }
     }
-    if (n + 1 == n_mine) break;
-    if (t.half) i8_sync<0>();  // (its stores are fewer)
-    else i8_sync<kStores>();
+    if (!more) break;
+    stores = !t.half;  // (a half tile's are fewer: the next wait takes them in)
     t = next;
-    next = after;
   }
 }
 
