@@ -50,12 +50,16 @@ __device__ __forceinline__ void i8_sync() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
+// bf16 rows go past L2: a store of 32 lanes is whole lines (up product of 8192 tokens, d = 128, F = 512, k = 4: 119 us a
+// call with L2's usual policy, 109 so).  fp32 ones take two stores, each half of every line, which L2 joins (4096
+// rows, 128 -> 512: 30 us with the usual policy, 41 so).
+constexpr int kNonTemporal = 2;
 template <int YT>
 __device__ __forceinline__ void store_blades(const float (&y)[8], __amdgpu_buffer_rsrc_t r, uint32_t off) {
   typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
   if constexpr (YT == kBF16) {
     const u32x4_t o = {pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]), pack2_bf16(y[6], y[7])};
-    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, kNonTemporal);
   } else {
     u32x4_t lo, hi;
 #pragma unroll
