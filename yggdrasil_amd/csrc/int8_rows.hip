@@ -42,6 +42,23 @@ __device__ __forceinline__ void codes_of(const float v[8], float inv, uint32_t q
     }
 }
 
+// Lane exchanges within rows of 16 lanes, on the vector units (through LDS the sums and codes of a row of 128 multivectors
+// took a third longer).
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, dpp<kXor1>(v));
+  v = max(v, dpp<kXor2>(v));
+  v = max(v, dpp<kHalfMirror>(v));
+  v = max(v, dpp<kMirror>(v));
+  const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+  return max(max(a, b), max(c, d));
+}
+
 // WAVES waves a row, four waves a workgroup; a lane takes every 64 WAVES-th multivector, KEEP of them kept from the pass
 // that finds the largest entry to the one that writes the codes.
 template <typename T, int WAVES, int KEEP>
@@ -70,8 +87,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   for (int u = 0; u < KEEP; ++u)
     if (first + u * STRIDE < d) look(kept[u]);
   for (int i = first + KEEP * STRIDE; i < d; i += STRIDE) look(load_raw(x, (size_t)row * d + i));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  top = wave_max(top);
   if constexpr (WAVES > 1) {
     if (lane == 0) s_max[wave] = top;
     __syncthreads();
@@ -90,10 +106,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     codes_of(v, finite ? inv : 0.f, q);
     const uint32_t w0 = q[0] | q[1] << 16, w1 = q[2] | q[3] << 16;
     const bool odd = lane & 1, up = lane & 2;
-    const uint32_t o0 = __shfl_xor((int)w0, 1), o1 = __shfl_xor((int)w1, 1);
+    const uint32_t o0 = dpp<kXor1>(w0), o1 = dpp<kXor1>(w1);
     const uint32_t p0 = odd ? (o0 >> 16 | (w0 & 0xffff0000u)) : (w0 & 0xffffu) | o0 << 16;  // pairs 0 and 1 of two inputs
     const uint32_t p1 = odd ? (o1 >> 16 | (w1 & 0xffff0000u)) : (w1 & 0xffffu) | o1 << 16;  // pairs 2 and 3
-    const uint32_t r0 = __shfl_xor((int)p0, 2), r1 = __shfl_xor((int)p1, 2);
+    const uint32_t r0 = dpp<kXor2>(p0), r1 = dpp<kXor2>(p1);
     const uint2 eight = up ? make_uint2(r1, p1) : make_uint2(p0, r0);
     const int pair = lane & 3;  // 2 b + part
     const int ks = i >> 5, g = (i >> 3) & 3, half = (i >> 2) & 1;
