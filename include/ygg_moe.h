@@ -249,6 +249,22 @@ int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows,
                             const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,
                             ygg_stream_t stream);
 
+/* Every expert's CliffordFFN (hlm_block.py:55-61) on bf16 rows grouped by expert, both
+ * products in int8: the rows quantized, the up product with bias and activation, its bf16
+ * rows quantized, the down product with bias; y (P, d, 8) bf16, what the calls above give.
+ * workspace on 256 bytes. */
+size_t ygg_int8_grouped_experts_workspace_bytes(int P, int d, int F);
+int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_up, const float* s_up, const float* b_up,
+                             const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets, int E,
+                             int d, int F, int act, void* y, void* workspace, size_t workspace_bytes,
+                             ygg_stream_t stream);
+
+/* Row ranges as a caller of the grouped products has them -- (E,) offsets and counts of 4 or
+ * 8 bytes (index_bytes) -- as the E + 1 bounds that they take, brought into [0, P] and into
+ * ascending order.  E <= 64. */
+int ygg_expert_bounds(const void* offsets, const void* counts, int index_bytes, int E, int P, int32_t* bounds,
+                      ygg_stream_t stream);
+
 /* Blade-order fp32 rows (rows, d, 8) -> fp32 Pauli rows (rows, d, 2, 2, 2): element
  * [m][i][b][k][c] is the real (k = 0) or imaginary (k = 1) part of entry (c, b) of
  * multivector x[m][i] as a 2x2 complex matrix. */

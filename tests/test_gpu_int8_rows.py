@@ -377,6 +377,36 @@ def test_captured_layer_replays():
         assert torch.equal(out, layer.moe_forward(x, logits=logits))
 
 
+@pytest.mark.parametrize("fmt", ["int8_rows", "pauli"])
+def test_experts_of_any_bounds(fmt):
+    """Ranges as int32, int64 or another type, and malformed ones: brought into ascending order inside the rows, in every
+    format."""
+    ops = _ops()
+    torch.manual_seed(6)
+    E, d, F, P = 4, 16, 24, 50
+    wu = ops.prepare_weights(torch.randn(E, F, d, 8, device="cuda") / (8 * d) ** 0.5, fmt)
+    wd = ops.prepare_weights(torch.randn(E, d, F, 8, device="cuda") / (8 * F) ** 0.5, fmt)
+    x = torch.randn(P, d, 8, device="cuda").bfloat16()
+    off, cnt = torch.tensor([0, 20, 20, 35], device="cuda"), torch.tensor([20, 0, 15, 15], device="cuda")
+    say(f"experts of any bounds {fmt}")
+    want = ops.grouped_experts(x, off, cnt, wu, wd)
+    for dt in (torch.int32, torch.int16):
+        assert torch.equal(ops.grouped_experts(x, off.to(dt), cnt.to(dt), wu, wd), want)
+    bad_off = torch.tensor([-5, 30, 10, 35], device="cuda")
+    for dt in (torch.int32, torch.int64):
+        bounds = torch.empty(E + 1, device="cuda", dtype=torch.int32)
+        o, c = bad_off.to(dt), torch.tensor([3, 3, 3, 2 ** 31 - 40], device="cuda").to(dt)
+        ops.check(ops.lib().ygg_expert_bounds(o.data_ptr(), c.data_ptr(), o.element_size(), E, P, bounds.data_ptr(),
+                                              ops.stream_handle()))
+        assert bounds.tolist() == [0, 30, 30, 35, P]
+    y = ops.grouped_experts(x, bad_off, torch.tensor([3, 3, 3, 15], device="cuda"), wu, wd)
+    good = ops.grouped_experts(x, torch.tensor([0, 30, 30, 35], device="cuda"), torch.tensor([30, 0, 5, 15], device="cuda"),
+                               wu, wd)
+    assert torch.equal(y, good)
+    one = ops.grouped_experts(x, torch.tensor([0, 0, 0, 0], device="cuda"), torch.tensor([0, 0, 0, 50], device="cuda"), wu, wd)
+    assert torch.equal(one[35:], want[35:])  # the same expert's rows
+
+
 def test_empty_batch():
     g = np.random.default_rng(13)
     layer, _, _ = _layer(g, 4, 16, 24, 4, 2)

@@ -47,6 +47,36 @@ def test_product(at, value, word):
     _refused("ygg_int8_grouped_linear", args, word)
 
 
+@pytest.mark.parametrize("at,value", [(0, FAR[5] + 16), (1, FAR[5] + 8), (3, FAR[5] + 60), (5, FAR[5] - 8), (6, FAR[5] + 4),
+                                      (7, FAR[5] + 32), (8, FAR[5] + 100)])
+def test_product_in_place(at, value):
+    args = list(_LIN)
+    args[at] = value
+    _refused("ygg_int8_grouped_linear", args, "share")
+
+
+_EXP = [FAR[0], 8, FAR[1], FAR[2], None, FAR[3], FAR[4], None, FAR[5], 2, 40, 24, 1, FAR[6], FAR[7], 1 << 20, None]
+
+
+@pytest.mark.parametrize("at,value,word", [
+    (0, None, "null"), (2, None, "null"), (3, None, "null"), (5, None, "null"), (6, None, "null"), (8, None, "null"),
+    (13, None, "null"), (14, None, "null"), (1, -1, "bad sizes"), (9, 0, "bad sizes"), (9, 65, "bad sizes"),
+    (10, 0, "bad sizes"), (11, 0, "bad sizes"), (12, 4, "activation"), (10, 20000, "16384"), (11, 20000, "16384"),
+    (15, 100, "workspace"), (14, FAR[0], "share"), (14, FAR[6] + 16, "share")])
+def test_experts(at, value, word):
+    args = list(_EXP)
+    args[at] = value
+    _refused("ygg_int8_grouped_experts", args, word)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, P, 4, 0, 8, P, None), "bad sizes"), ((P, P, 4, 65, 8, P, None), "bad sizes"), ((P, P, 4, 2, -1, P, None), "bad sizes"),
+    ((P, P, 2, 2, 8, P, None), "bytes"), ((None, P, 4, 2, 8, P, None), "null"), ((P, None, 4, 2, 8, P, None), "null"),
+    ((P, P, 4, 2, 8, None, None), "null")])
+def test_bounds(args, word):
+    _refused("ygg_expert_bounds", args, word)
+
+
 _COMB = [FAR[0], 0, FAR[1], 8, 2, 4, 16, FAR[2], FAR[3], FAR[4], 0, 0, FAR[5], None]
 
 

@@ -20,7 +20,7 @@ OUT_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(OUT_DIR, "libygg_moe.so")
 SOURCES = ["capi.hip", "route.hip", "dispatch.hip", "clifford_gemm.hip", "decode.hip", "decode_pauli.hip", "pauli_gemm.hip", "pauli_f32.hip", "pauli_split.hip", "pauli_small.hip",
            "norm.hip", "quantize.hip", "backward.hip", "norm_backward.hip", "route_backward.hip", "weight_grad_bf16.hip",
-           "train_bf16.hip", "int8_rows.hip", "int8_tile.hip", "sort_backward.hip"]
+           "train_bf16.hip", "int8_rows.hip", "int8_tile.hip", "int8_small.hip", "sort_backward.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

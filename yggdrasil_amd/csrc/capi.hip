@@ -63,9 +63,6 @@ extern "C" int ygg_grouped_clifford_linear(const void*, int, const void*, int, c
                                            const int32_t*, int, int, int, int, void*, int, int, hipStream_t);
 extern "C" int ygg_pauli_grouped_linear(const void*, int, int, const int32_t*, int, const void*, const float*,
                                         const int32_t*, int, int, int, int, void*, int, int, hipStream_t);
-extern "C" int ygg_quantize_rows(const void*, int, int, int, void*, float*, hipStream_t);
-extern "C" int ygg_int8_grouped_linear(const void*, const float*, int, const int32_t*, int, const void*, const float*,
-                                       const float*, const int32_t*, int, int, int, int, void*, int, hipStream_t);
 extern "C" int ygg_pauli_rows_from_blade(const void*, int, int, void*, hipStream_t);
 extern "C" int ygg_pauli_rows_from_blade_f32(const float*, int, int, float*, hipStream_t);
 extern "C" int ygg_pauli_grouped_linear_f32(const float*, const int32_t*, int, const float*, const float*,
@@ -103,8 +100,7 @@ YGG_API size_t ygg_moe_workspace_bytes(int N, int d, int F, int E, int k, int dt
   b += align256(P * 4) * 2;               // perm, slot_pos
   b += align256(ygg_route_workspace_bytes(N, E, k));
   if (w_format == kWI8Rows)  // the codes and scales of x's rows, h, those of h's rows, y_sorted
-    return b + align256(int8_rows_bytes((size_t)N, d)) + align256((size_t)N * 4) + align256(P * F * 16) +
-           align256(int8_rows_bytes(P, F)) + align256(P * 4) + align256(P * d * 16);
+    return b + int8_experts_bytes((size_t)N, P, d, F) + align256(P * d * 16);
   b += align256(P * d * 8 * es);          // x_sorted (Pauli rows of x for formats 3 and 4)
   b += align256(P * F * 8 * es);          // h
   b += align256(ys_bytes(P, E, d, F, dtype, w_format));  // y_sorted
@@ -256,23 +252,8 @@ static int moe_forward_impl(const void* x, int dtype, int N, int d, int F, int E
   }
   if (w_format == kWI8Rows) {
     // x's rows in int8, gathered through perm by the up product; h's rows in int8, read in place by the down product
-    char* q = static_cast<char*>(xs);
-    auto take = [&](size_t bytes) {
-      char* r = q;
-      q += align256(bytes);
-      return r;
-    };
-    void* xq = take(int8_rows_bytes((size_t)N, d));
-    float* xq_scale = reinterpret_cast<float*>(take((size_t)N * 4));
-    void* hb = take(P * F * 16);
-    void* hq = take(int8_rows_bytes(P, F));
-    float* hq_scale = reinterpret_cast<float*>(take(P * 4));
-    void* yb = take(P * d * 16);
-    if (ygg_quantize_rows(x, kBF16, N, d, xq, xq_scale, stream) ||
-        ygg_int8_grouped_linear(xq, xq_scale, N, perm, (int)P, w_up, s_up, b_up, offsets, E, d, F, act, hb, kBF16, stream) ||
-        ygg_quantize_rows(hb, kBF16, (int)P, F, hq, hq_scale, stream) ||
-        ygg_int8_grouped_linear(hq, hq_scale, (int)P, nullptr, (int)P, w_down, s_down, b_down, offsets, E, F, d, kActNone,
-                                yb, kBF16, stream))
+    void* yb = static_cast<char*>(xs) + int8_experts_bytes((size_t)N, P, d, F);
+    if (int8_experts(x, N, perm, (int)P, w_up, s_up, b_up, w_down, s_down, b_down, offsets, E, d, F, act, yb, xs, stream))
       return -1;
     return ygg_combine(yb, kBF16, /*y_mask=*/0, N, k, d, topk_idx, topk_w, slot_pos, residual, out, kBF16, stream);
   }

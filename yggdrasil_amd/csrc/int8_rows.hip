@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "int8_rows.h"
 #include "rows.h"
@@ -145,67 +146,63 @@ void launch_quantize(const void* x, int rows, int d, void* codes, float* scale, 
     quantize_rows_kernel<T, 4, 4><<<(unsigned)rows, 256, 0, stream>>>(X, rows, d, C, scale);
 }
 
-// ---- the product -------------------------------------------------------------------
-
-// sums of four byte products
-__device__ __forceinline__ int dot4(uint32_t a, uint32_t b, int c) { return __builtin_amdgcn_sdot4((int)a, (int)b, c, false); }
-
-__device__ __forceinline__ void store_out(float* y, size_t n, const float v[8]) { store_mv(y, n, v); }
-__device__ __forceinline__ void store_out(uint16_t* y, size_t n, const float v[8]) { store_mv(y, n, v); }
-
-// A thread per output multivector, four-byte products on the vector units.
-template <int ACT, typename TY>
-__global__ __launch_bounds__(256) void int8_linear_simple_kernel(const uint4* __restrict__ X, const float* __restrict__ xs,
-                                                                 int x_rows, const int32_t* __restrict__ gather,
-                                                                 const uint4* __restrict__ W, const float* __restrict__ ws,
-                                                                 const float* __restrict__ bias,
-                                                                 const int32_t* __restrict__ offsets, int E, int d_in,
-                                                                 int d_out, int P_max, TY* __restrict__ y) {
-  const int r = blockIdx.x;
-  const int j = blockIdx.y * 256 + threadIdx.x;
-  if (r >= min(offsets[E], P_max) || j >= d_out) return;
-  int e = 0;
-  while (offsets[e + 1] <= r) ++e;
-  const int src = gather ? gather[r] : r;
-  const int steps = i8_steps(d_in);
-  const bool in = (unsigned)src < (unsigned)x_rows;  // (else a row of zeros)
-  const uint4* xr = X + (size_t)(in ? src : 0) * steps * 16;
-  const uint4* w = W + (size_t)e * (i8_expert_bytes(d_out, d_in) / 16) + (size_t)(j >> 3) * steps * 128 + 2 * (j & 7);
-  int re[2][2] = {}, im[2][2] = {};  // [a][b]
-  auto dot = [](const uint4& p, const uint4& q, int c) {
-    return dot4(p.x, q.x, dot4(p.y, q.y, dot4(p.z, q.z, dot4(p.w, q.w, c))));
-  };
-  for (int ks = 0; ks < steps; ++ks)
-    for (int g = 0; g < 4; ++g)
-      for (int a = 0; a < 2; ++a) {
-        const uint4 U = w[(size_t)ks * 128 + g * 16 + a], V = w[(size_t)ks * 128 + 64 + g * 16 + a];
-        for (int b = 0; b < 2; ++b) {
-          const uint4 xre = xr[(size_t)(b * steps + ks) * 8 + g], xim = xr[(size_t)(b * steps + ks) * 8 + 4 + g];
-          re[a][b] = dot(U, xre, re[a][b]) - dot(V, xim, 0);
-          im[a][b] = dot(U, xim, dot(V, xre, im[a][b]));
-        }
-      }
-  float o[8], bv[8] = {};
-  if (bias) {
+// Bounds of experts' ranges as a caller has them, 4 or 8 bytes each: brought into [0, P] and into ascending order.
+template <typename I>
+__global__ __launch_bounds__(64) void expert_bounds_kernel(const I* __restrict__ offsets, const I* __restrict__ counts, int E,
+                                                           int P, int32_t* __restrict__ bounds) {
+  const int lane = threadIdx.x;
+  typedef typename std::make_unsigned<I>::type U;  // (sums may wrap)
+  const I at = lane < E ? offsets[lane] : 0, end = lane < E ? (I)((U)at + (U)counts[lane]) : 0;
+  auto clip = [&](I v) { return min(max((int32_t)v, 0), P); };
+  int v = lane < E ? clip(at) : 0;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) bv[c] = bias[((size_t)e * d_out + j) * 8 + blade_to_mask(c)];
+  for (int o = 1; o < 64; o <<= 1) {
+    const int p = __shfl_up(v, o);
+    if (lane >= o) v = max(v, p);
   }
-  i8_blades(re[0][0], im[0][0], re[0][1], im[0][1], re[1][0], im[1][0], re[1][1], im[1][1],
-            ws[(size_t)e * d_out + j] * (in ? xs[src] : 0.f), bv, o);
-  activate_blade<ACT>(o);
-  store_out(y, (size_t)r * d_out + j, o);
+  if (lane < E) bounds[lane] = v;
+  if (lane == E - 1) bounds[E] = max(v, clip(end));
 }
 
-template <int ACT, typename TY>
-int launch_linear(const void* x, const float* xs, int x_rows, const int32_t* gather, int P, const void* w, const float* ws,
-                  const float* bias, const int32_t* offsets, int E, int d_in, int d_out, void* y, hipStream_t stream) {
-  int8_linear_simple_kernel<ACT, TY><<<dim3((unsigned)P, (unsigned)((d_out + 255) / 256)), 256, 0, stream>>>(
-      static_cast<const uint4*>(x), xs, x_rows, gather, static_cast<const uint4*>(w), ws, bias, offsets, E, d_in, d_out, P,
-      static_cast<TY*>(y));
-  return check_launch("int8_grouped_linear");
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// The codes and scales of x's rows, h, the codes and scales of its rows; each on 256 bytes
+struct ExpertsAt {
+  size_t xq, xs, h, hq, hs, total;
+};
+ExpertsAt experts_at(size_t x_rows, size_t P, int d, int F) {
+  ExpertsAt at;
+  at.xq = 0;
+  at.xs = at.xq + align256(x_rows * i8_row_bytes(d));
+  at.h = at.xs + align256(x_rows * 4);
+  at.hq = at.h + align256(P * F * 16);
+  at.hs = at.hq + align256(P * i8_row_bytes(F));
+  at.total = at.hs + align256(P * 4);
+  return at;
 }
 
 }  // namespace
+
+size_t int8_experts_bytes(size_t x_rows, size_t P, int d, int F) { return experts_at(x_rows, P, d, F).total; }
+
+int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
+                 const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
+                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream) {
+  const ExpertsAt at = experts_at((size_t)x_rows, (size_t)P, d, F);
+  char* const b = static_cast<char*>(workspace);
+  float *xs = reinterpret_cast<float*>(b + at.xs), *hs = reinterpret_cast<float*>(b + at.hs);
+  auto product = [&](const void* q, const float* s, int rows, const int32_t* from, const void* w, const float* sw,
+                     const float* bias, int d_in, int d_out, int a, void* to) {
+    return (int8_small_pays(P, d_out) ? int8_small_linear : int8_tile_linear)(q, s, rows, from, P, w, sw, bias, offsets, E,
+                                                                              d_in, d_out, a, to, kBF16, stream);
+  };
+  launch_quantize<uint16_t>(x, x_rows, d, b + at.xq, xs, stream);
+  if (check_launch("int8_experts")) return -1;
+  if (product(b + at.xq, xs, x_rows, gather, w_up, s_up, b_up, d, F, act, b + at.h)) return -1;
+  launch_quantize<uint16_t>(b + at.h, P, F, b + at.hq, hs, stream);
+  if (check_launch("int8_experts")) return -1;
+  return product(b + at.hq, hs, P, nullptr, w_down, s_down, b_down, F, d, kActNone, y);
+}
 
 size_t int8_rows_bytes(size_t rows, int d) { return rows * i8_row_bytes(d); }
 
@@ -250,21 +247,51 @@ YGG_API int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int
   if (P_max == 0) return 0;
   YGG_CHECK_ARG(codes && x_scale && w_prepared && w_scale && offsets && y, "ygg_int8_grouped_linear: null pointer");
   YGG_CHECK_ARG(gather || x_rows >= P_max, "ygg_int8_grouped_linear: %d rows of x for %d product rows", x_rows, P_max);
-  // few rows: the weights set the time (32 rows of 64 experts, 256 -> 1024: 18.7 us, 21.5 on the tiles; 4500 rows of 12,
-  // 100 -> 300: 77 us, 25 on the tiles)
-  if (P_max > 64)
-    return int8_tile_linear(codes, x_scale, x_rows, gather, P_max, w_prepared, w_scale, bias, offsets, E, d_in, d_out, act, y,
-                            y_dtype, stream);
-#define YGG_I8(A)                                                                                                           \
-  return y_dtype == kF32 ? launch_linear<A, float>(codes, x_scale, x_rows, gather, P_max, w_prepared, w_scale, bias,       \
-                                                   offsets, E, d_in, d_out, y, stream)                                     \
-                         : launch_linear<A, uint16_t>(codes, x_scale, x_rows, gather, P_max, w_prepared, w_scale, bias,    \
-                                                      offsets, E, d_in, d_out, y, stream)
-  switch (act) {
-    case kActNone: YGG_I8(kActNone);
-    case kActGelu: YGG_I8(kActGelu);
-    case kActRelu: YGG_I8(kActRelu);
-    default: YGG_I8(kActSigmoid);
-  }
-#undef YGG_I8
+  const size_t yb = (size_t)P_max * d_out * 8 * dtype_size(y_dtype);
+  YGG_CHECK_ARG(!overlap(y, yb, codes, int8_rows_bytes((size_t)x_rows, d_in)) && !overlap(y, yb, x_scale, (size_t)x_rows * 4) &&
+                    !overlap(y, yb, w_prepared, (size_t)E * i8_expert_bytes(d_out, d_in)) &&
+                    !overlap(y, yb, w_scale, (size_t)E * d_out * 4) && !overlap(y, yb, bias, (size_t)E * d_out * 32) &&
+                    !overlap(y, yb, gather, (size_t)P_max * 4) && !overlap(y, yb, offsets, (size_t)(E + 1) * 4),
+                "ygg_int8_grouped_linear: y must not share memory with an input");
+  return (int8_small_pays(P_max, d_out) ? int8_small_linear : int8_tile_linear)(
+      codes, x_scale, x_rows, gather, P_max, w_prepared, w_scale, bias, offsets, E, d_in, d_out, act, y, y_dtype, stream);
+}
+
+YGG_API int ygg_expert_bounds(const void* offsets, const void* counts, int index_bytes, int E, int P, int32_t* bounds,
+                              hipStream_t stream) {
+  YGG_CHECK_ARG(E >= 1 && E <= 64 && P >= 0, "ygg_expert_bounds: bad sizes E=%d P=%d (E <= 64)", E, P);
+  YGG_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "ygg_expert_bounds: indexes of %d bytes", index_bytes);
+  YGG_CHECK_ARG(offsets && counts && bounds, "ygg_expert_bounds: null pointer");
+  if (index_bytes == 8)
+    expert_bounds_kernel<long long><<<1, 64, 0, stream>>>(static_cast<const long long*>(offsets),
+                                                          static_cast<const long long*>(counts), E, P, bounds);
+  else
+    expert_bounds_kernel<int32_t><<<1, 64, 0, stream>>>(static_cast<const int32_t*>(offsets),
+                                                        static_cast<const int32_t*>(counts), E, P, bounds);
+  return check_launch("expert_bounds");
+}
+
+YGG_API size_t ygg_int8_grouped_experts_workspace_bytes(int P, int d, int F) {
+  return P < 0 || d < 1 || F < 1 ? 0 : int8_experts_bytes((size_t)P, (size_t)P, d, F);
+}
+
+YGG_API int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_up, const float* s_up, const float* b_up,
+                                     const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
+                                     int E, int d, int F, int act, void* y, void* workspace, size_t workspace_bytes,
+                                     hipStream_t stream) {
+  YGG_CHECK_ARG(P >= 0 && E >= 1 && E <= 64 && d >= 1 && F >= 1, "ygg_int8_grouped_experts: bad sizes P=%d E=%d d=%d F=%d (E <= 64)",
+                P, E, d, F);
+  YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_int8_grouped_experts: activation %d", act);
+  const char* why = int8_linear_limit(P, false, E, d, F);
+  if (!why) why = int8_linear_limit(P, false, E, F, d);
+  YGG_CHECK_ARG(!why, "ygg_int8_grouped_experts: %s (P=%d E=%d d=%d F=%d)", why, P, E, d, F);
+  if (P == 0) return 0;
+  YGG_CHECK_ARG(x_sorted && w_up && s_up && w_down && s_down && offsets && y && workspace,
+                "ygg_int8_grouped_experts: null pointer");
+  const size_t need = int8_experts_bytes((size_t)P, (size_t)P, d, F), yb = (size_t)P * d * 16;
+  YGG_CHECK_ARG(workspace_bytes >= need, "ygg_int8_grouped_experts: workspace of %zu bytes, need %zu", workspace_bytes, need);
+  YGG_CHECK_ARG(!overlap(workspace, need, x_sorted, yb) && !overlap(workspace, need, y, yb),
+                "ygg_int8_grouped_experts: the workspace must not share memory with x_sorted or y");
+  return int8_experts(x_sorted, P, nullptr, P, w_up, s_up, b_up, w_down, s_down, b_down, offsets, E, d, F, act, y, workspace,
+                      stream);
 }

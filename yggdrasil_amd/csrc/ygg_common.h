@@ -250,9 +250,21 @@ int decode_pauli_layer(const uint16_t* x, const float* logits, int N, int E, int
 // int8 rows (int8_rows.hip): bytes of the codes of rows of d multivectors, and why the product cannot take these sizes
 // (nullptr: it can)
 size_t int8_rows_bytes(size_t rows, int d);
+// Every expert's two products of bf16 rows in int8, x's (x_rows of them, gathered or in place) and h's quantized between:
+// y (P, d, 8) bf16; workspace: int8_experts_bytes, on 256 bytes
+size_t int8_experts_bytes(size_t x_rows, size_t P, int d, int F);
+int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
+                 const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
+                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream);
+// The product itself, for enough rows (int8_tile.hip) and for few (int8_small.hip), the same outputs bit for bit; and
+// whether a call has few
 int int8_tile_linear(const void* x, const float* xs, int x_rows, const int32_t* gather, int P, const void* w, const float* ws,
                      const float* bias, const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,
-                     hipStream_t stream);  // int8_tile.hip: the product for enough rows
+                     hipStream_t stream);
+int int8_small_linear(const void* x, const float* xs, int x_rows, const int32_t* gather, int P, const void* w,
+                      const float* ws, const float* bias, const int32_t* offsets, int E, int d_in, int d_out, int act,
+                      void* y, int y_dtype, hipStream_t stream);
+bool int8_small_pays(int P, int d_out);
 const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out);
 
 // combine of fp32 blade-order partial planes (dispatch.hip): the planes of a

@@ -674,6 +674,7 @@ def int8_grouped_linear(rows: Int8Rows, pw: PreparedWeights, offsets: torch.Tens
     return _int8_grouped_linear(rows.codes, rows.scale, rows.d, pw, offsets, bias_prepared, act, gather, out_dtype)
 
 
+@_on_its_device
 def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert_counts: torch.Tensor,
                     w_up: PreparedWeights, w_down: PreparedWeights, b_up: torch.Tensor | None = None,
                     b_down: torch.Tensor | None = None, act: str = "gelu", validate: bool = False) -> torch.Tensor:
@@ -708,7 +709,6 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
         raise ValueError(f"expert_offsets and expert_counts must have shape ({E},)")
     x = x.contiguous()
     P = x.shape[0]
-    offs = torch.cat([expert_offsets.reshape(E), (expert_offsets[-1:] + expert_counts[-1:])]).to(torch.int32)
     if validate:
         o, c = expert_offsets.long().cpu(), expert_counts.long().cpu()
         if int(o[0]) != 0 or bool((c < 0).any()) or bool((o[1:] != o[:-1] + c[:-1]).any()) or int(o[-1] + c[-1]) != P:
@@ -716,7 +716,13 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     if P == 0:
         return x_sorted.clone()
     # the products take every range from these bounds: ascending and inside the rows
-    offs = torch.cummax(offs.clamp(0, P), 0).values.to(torch.int32).contiguous()
+    if E <= 64 and expert_offsets.dtype == expert_counts.dtype and expert_offsets.dtype in (torch.int32, torch.int64):
+        offs = torch.empty(E + 1, device=dev, dtype=torch.int32)
+        check(lib().ygg_expert_bounds(ptr(expert_offsets), ptr(expert_counts), expert_offsets.element_size(), E, P,
+                                      ptr(offs), stream_handle(dev)), "grouped_experts")
+    else:
+        offs = torch.cat([expert_offsets.reshape(E), (expert_offsets[-1:] + expert_counts[-1:])]).to(torch.int32)
+        offs = torch.cummax(offs.clamp(0, P), 0).values.to(torch.int32).contiguous()
     fmt = w_up.fmt
     if fmt == "int8_pauli":
         raise ValueError("int8_pauli weights run inside the decode layer (moe_forward), which routes its own "
@@ -731,8 +737,16 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     elif fmt == "int8_rows":
         if x.dtype != torch.bfloat16:
             raise ValueError("int8_rows experts take bf16 rows")
-        h = int8_grouped_linear(quantize_rows(x), w_up, offs, b_up, act)
-        y = int8_grouped_linear(quantize_rows(h), w_down, offs, b_down)
+        for name, b, want in (("b_up", b_up, (E, F, 8)), ("b_down", b_down, (E, d, 8))):
+            if b is not None and (b.dtype != torch.float32 or tuple(b.shape) != want):
+                raise ValueError(f"{name} must be a prepared float32 bias {want}, got {b.dtype} {tuple(b.shape)}")
+        x = _aligned(x)
+        y = torch.empty_like(x)
+        need = lib().ygg_int8_grouped_experts_workspace_bytes(P, d, F)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        check(lib().ygg_int8_grouped_experts(ptr(x), P, ptr(w_up.data), ptr(w_up.scales), ptr(b_up), ptr(w_down.data),
+                                             ptr(w_down.scales), ptr(b_down), ptr(offs), E, d, F, ACT_CODE[act], ptr(y),
+                                             ptr(ws), need, stream_handle(dev)), "grouped_experts")
     else:  # L(w) blocks read and write mask order between the products
         h = grouped_clifford_linear(to_mask_order(x), w_up, offs, b_up, act, out_blade_order=False)
         y = grouped_clifford_linear(h, w_down, offs, b_down, "none", out_dtype=x.dtype, out_blade_order=True)
