@@ -251,6 +251,24 @@ def test_a_row_does_not_depend_on_its_batch():
         assert torch.equal(part, y[first:first + n]), (first, n)
 
 
+def test_large_fp32_outputs():
+    """More output than the caches hold (past L2): the rows of a small batch, bit for bit; channels no multiple of four."""
+    ops = _ops()
+    g = np.random.default_rng(14)
+    E, d_in, d_out, P = 2, 33, 511, 14000
+    w, b = _weights(g, E, d_out, d_in)
+    pw, pb = ops.prepare_weights(_dev(w), "int8_rows"), ops.prepare_bias(_dev(b))
+    x = _dev(_rows(g, P, d_in, False))
+    say("int8 product of 229 MB of fp32 outputs")
+    y = ops.int8_grouped_linear(ops.quantize_rows(x), pw, _dev(_bounds([6000, 8000])), pb, out_dtype=torch.float32)
+    for first, n, e in ((0, 700, 0), (5700, 300, 0), (6000, 100, 1), (13300, 700, 1)):
+        few = [0, 0]
+        few[e] = n
+        part = ops.int8_grouped_linear(ops.quantize_rows(x[first:first + n]), pw, _dev(_bounds(few)), pb,
+                                       out_dtype=torch.float32)
+        assert torch.equal(part, y[first:first + n]), (first, n)
+
+
 def test_on_another_stream():
     ops = _ops()
     g = np.random.default_rng(11)

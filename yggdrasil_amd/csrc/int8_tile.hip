@@ -50,22 +50,32 @@ __device__ __forceinline__ void i8_sync() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
-// bf16 rows go past L2: a store of 32 lanes is whole lines (up product of 8192 tokens, d = 128, F = 512, k = 4: 119 us a
-// call with L2's usual policy, 109 so).  fp32 ones take two stores, each half of every line, which L2 joins (4096
-// rows, 128 -> 512: 30 us with the usual policy, 41 so).
-constexpr int kNonTemporal = 2;
-template <int YT>
-__device__ __forceinline__ void store_blades(const float (&y)[8], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+// A multivector of y to element (row, j) of a tile's rows; a row past the tile's last or a channel j past the last lies
+// past the buffer, so every wave stores as often.  fp32 takes two stores: four lanes exchange theirs so that each is 64
+// bytes a quad instead of every second 16.
+template <int YT, bool STREAM>
+__device__ __forceinline__ void store_blades(const float (&y)[8], __amdgpu_buffer_rsrc_t r, int row, int j, int d_out) {
   typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+  constexpr int kPolicy = STREAM ? 2 : 0;
   if constexpr (YT == kBF16) {
     const u32x4_t o = {pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]), pack2_bf16(y[6], y[7])};
-    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, kNonTemporal);
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, j < d_out ? (uint32_t)(row * d_out + j) * 16 : kBufferOff, 0, kPolicy);
   } else {
-    u32x4_t lo, hi;
+    constexpr int kLow = 0x50, kHigh = 0xFA;  // lanes 0 0 1 1 and 2 2 3 3 of a quad
+    const bool odd = threadIdx.x & 1;
+    u32x4_t first, second;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) lo[c] = __builtin_bit_cast(unsigned, y[c]), hi[c] = __builtin_bit_cast(unsigned, y[4 + c]);
-    __builtin_amdgcn_raw_buffer_store_b128(lo, r, off, 0, 0);
-    __builtin_amdgcn_raw_buffer_store_b128(hi, r, off + 16, 0, 0);
+    for (int c = 0; c < 4; ++c) {
+      const int lo = __builtin_bit_cast(int, y[c]), hi = __builtin_bit_cast(int, y[4 + c]);
+      const int f0 = __builtin_amdgcn_mov_dpp(lo, kLow, 0xf, 0xf, true), f1 = __builtin_amdgcn_mov_dpp(hi, kLow, 0xf, 0xf, true);
+      const int s0 = __builtin_amdgcn_mov_dpp(lo, kHigh, 0xf, 0xf, true), s1 = __builtin_amdgcn_mov_dpp(hi, kHigh, 0xf, 0xf, true);
+      first[c] = (unsigned)(odd ? f1 : f0);
+      second[c] = (unsigned)(odd ? s1 : s0);
+    }
+    const int j0 = (j & ~3) + ((j >> 1) & 1);  // the multivectors that this lane stores a half of: j0 and j0 + 2
+    const uint32_t at = (uint32_t)(row * d_out + j0) * 32 + (odd ? 16 : 0);
+    __builtin_amdgcn_raw_buffer_store_b128(first, r, j0 < d_out ? at : kBufferOff, 0, kPolicy);
+    __builtin_amdgcn_raw_buffer_store_b128(second, r, j0 + 2 < d_out ? at + 64 : kBufferOff, 0, kPolicy);
   }
 }
 
@@ -88,7 +98,7 @@ struct I8Item {
   int which;
 };
 
-template <int ACT, int YT>
+template <int ACT, int YT, bool STREAM>
 __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2))) void int8_tile_kernel(
     const unsigned char* __restrict__ X, uint64_t x_bytes, const float* __restrict__ xs, int x_rows,
     const int32_t* __restrict__ gather, const unsigned char* __restrict__ W, const float* __restrict__ ws,
@@ -342,7 +352,6 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
         const int tok0 = wt * 32 + (t.half ? t.which : rb) * 16;             // token slot of the block's first row
         const int row0 = (t.compact ? wt * 16 : tok0) + 2 * g;               // its row in the tile, this lane's first
         const float* const scale = reinterpret_cast<const float*>(sd + C::XS) + tok0 + 2 * g;
-        const uint32_t at = j < d_out ? (uint32_t)(row0 * d_out + j) * MV_BYTES : kBufferOff;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -353,8 +362,7 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
             i8_blades(s[0][0][v] + vs[0], s[0][1][v], s[0][0][v + 1] + vs[0], s[0][1][v + 1], s[1][0][v] + vs[1], s[1][1][v],
                       s[1][0][v + 1] + vs[1], s[1][1][v + 1], sw * scale[4 * q + h], bv, y);
             activate_blade<ACT>(y);
-            // (behind the tile's last row or the last channel lies past the buffer: every wave stores as often)
-            store_blades<YT>(y, y_rsrc, at + (uint32_t)((4 * q + h) * d_out) * MV_BYTES);
+            store_blades<YT, STREAM>(y, y_rsrc, row0 + 4 * q + h, j, d_out);
           }
       }
     }
@@ -375,7 +383,12 @@ int launch_tile(const void* x, const float* xs, int x_rows, const int32_t* gathe
   const long long tiles = ((long long)P / I8Tile::T + std::min(E, P)) * ((d_out + I8Tile::BN - 1) / I8Tile::BN);
   const int xcds = cus % 8 == 0 ? 8 : 1;
   const long long grid = std::min<long long>(2 * cus, (2 * tiles + xcds - 1) / xcds * xcds);
-  int8_tile_kernel<ACT, YT><<<(unsigned)grid, I8Tile::NT, 0, stream>>>(
+  // bf16 outputs go past L2: their stores are whole lines (a product with L2's usual policy / so, us: 2048 rows, 128 ->
+  // 512: 13.7 / 12.6, 32768, E = 32: 126 / 108).  fp32 ones do where they are far more than the caches behind it hold (128 ->
+  // 512: 67 MB 21.6 / 24.8, 134 MB 40 / 46, 268 MB 81 / 75, 537 MB 170 / 144).
+  const bool stream_out = YT == kBF16 || (uint64_t)P * d_out * 32 > (uint64_t)192 << 20;
+  auto* const kernel = stream_out ? int8_tile_kernel<ACT, YT, true> : int8_tile_kernel<ACT, YT, YT == kBF16>;
+  kernel<<<(unsigned)grid, I8Tile::NT, 0, stream>>>(
       static_cast<const unsigned char*>(x), (uint64_t)x_rows * i8_row_bytes(d_in), xs, x_rows, gather,
       static_cast<const unsigned char*>(w), ws, bias, offsets, E, d_in, d_out, P, y, xcds);
   return check_launch("int8_tile");
