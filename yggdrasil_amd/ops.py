@@ -337,15 +337,15 @@ def combine(y_sorted: torch.Tensor, routing: Routing, residual: torch.Tensor | N
     return out
 
 
-def _check_routing(who: str, routing: Routing, dev) -> tuple:
-    """The slots of a caller's routing: ``(N, k)``."""
-    if routing.slot_pos.dim() != 2:
-        raise ValueError(f"{who}: slot_pos must be (N, k), got {tuple(routing.slot_pos.shape)}")
-    for name, t, dtype in (("slot_pos", routing.slot_pos, torch.int32), ("topk_w", routing.topk_w, torch.float32)):
-        if t.dtype != dtype or t.shape != routing.slot_pos.shape or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{who}: {name} must be contiguous {dtype} {tuple(routing.slot_pos.shape)} on {dev}, got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    return routing.slot_pos.shape
+def _check_routing(who: str, routing: Routing, at: int) -> tuple:
+    """The slots of a caller's routing on device ``at``: ``(slot_pos, topk_w, (N, k))``."""
+    slots, w = routing.slot_pos, routing.topk_w
+    shape = slots.shape
+    if not (slots.dtype == torch.int32 and w.dtype == torch.float32 and len(shape) == 2 and w.shape == shape and
+            slots.get_device() == at and w.get_device() == at and slots.is_contiguous() and w.is_contiguous()):
+        raise ValueError(f"{who}: slot_pos must be contiguous int32 (N, k) and topk_w float32 of its shape, on device "
+                         f"{at}; got {slots.dtype} {tuple(shape)} on {slots.device}, {w.dtype} {tuple(w.shape)} on {w.device}")
+    return slots, w, shape
 
 
 @_on_its_device
@@ -361,29 +361,34 @@ def combine_backward(dout: torch.Tensor, y_sorted: torch.Tensor | None, routing:
     written.
     """
     dev = _one_device(dout, y_sorted)
-    if dout.dim() != 3 or dout.shape[2] != 8:
-        raise ValueError(f"combine_backward: dout must be (N, d, 8), got {tuple(dout.shape)}")
-    if y_layout not in Y_LAYOUT:
-        raise ValueError("y_layout must be 'blade' or 'pauli'")
-    Nt, k = _check_routing("combine_backward", routing, dev)
-    d = dout.shape[1]
-    if dout.shape[0] != Nt:
-        raise ValueError(f"combine_backward: {Nt} tokens' routing for {dout.shape[0]} tokens")
+    shape = dout.shape
+    if len(shape) != 3 or shape[2] != 8:
+        raise ValueError(f"combine_backward: dout must be (N, d, 8), got {tuple(shape)}")
+    slots, w, (Nt, k) = _check_routing("combine_backward", routing, dev.index)
+    d = shape[1]
+    if shape[0] != Nt:
+        raise ValueError(f"combine_backward: {Nt} tokens' routing for {shape[0]} tokens")
     if y_sorted is not None:
-        if y_sorted.dim() != 3 or y_sorted.shape[1:] != (d, 8):
-            raise ValueError(f"combine_backward: y_sorted must be (P, {d}, 8), got {tuple(y_sorted.shape)}")
-        if out_dtype not in (None, y_sorted.dtype) or rows not in (None, y_sorted.shape[0]):
+        want = y_sorted.shape
+        if len(want) != 3 or want[1] != d or want[2] != 8:
+            raise ValueError(f"combine_backward: y_sorted must be (P, {d}, 8), got {tuple(want)}")
+        if out_dtype not in (None, y_sorted.dtype) or rows not in (None, want[0]):
             raise ValueError("combine_backward: dy has y_sorted's type and rows")
-        out_dtype, rows = y_sorted.dtype, y_sorted.shape[0]
-    out_dtype, P = out_dtype or dout.dtype, Nt * k if rows is None else rows
-    dout, y_sorted = _aligned(dout), _aligned(y_sorted)
-    pauli = (P, 2, d, 4) if out_dtype == torch.bfloat16 else (P, d, 2, 2, 2)
-    dy = torch.empty(pauli if y_layout == "pauli" else (P, d, 8), device=dev, dtype=out_dtype)
-    dtw = torch.empty((Nt, k), device=dev, dtype=torch.float32) if y_sorted is not None else None
-    check(lib().ygg_combine_backward(dout.data_ptr(), _dtype_code(dout), ptr(y_sorted), Nt, k, d, P,
-                                     routing.topk_w.data_ptr(), routing.slot_pos.data_ptr(), dy.data_ptr(),
-                                     _dtype_code(dy), int(y_layout == "pauli"), ptr(dtw), stream_handle(dev)),
-          "combine_backward")
+        out_dtype, P = y_sorted.dtype, want[0]
+        y_sorted = _aligned(y_sorted)
+    else:
+        out_dtype, P = out_dtype or dout.dtype, Nt * k if rows is None else rows
+    dout = _aligned(dout)
+    if y_layout == "pauli":
+        dy = torch.empty((P, 2, d, 4) if out_dtype == torch.bfloat16 else (P, d, 2, 2, 2), device=dev, dtype=out_dtype)
+    elif y_layout == "blade":
+        dy = torch.empty((P, d, 8), device=dev, dtype=out_dtype) if y_sorted is None else torch.empty_like(y_sorted)
+    else:
+        raise ValueError("y_layout must be 'blade' or 'pauli'")
+    dtw = torch.empty_like(w) if y_sorted is not None else None
+    check(lib().ygg_combine_backward(dout.data_ptr(), _dtype_code(dout), ptr(y_sorted), Nt, k, d, P, w.data_ptr(),
+                                     slots.data_ptr(), dy.data_ptr(), _dtype_code(dy), y_layout == "pauli", ptr(dtw),
+                                     stream_handle(dev)), "combine_backward")
     return dy, dtw
 
 
@@ -395,17 +400,22 @@ def dispatch_backward(dx_sorted: torch.Tensor, routing: Routing, dx_add: torch.T
     sort.  A slot outside the P rows adds nothing.
     """
     dev = _one_device(dx_sorted, dx_add)
-    if dx_sorted.dim() != 3 or dx_sorted.shape[2] != 8:
-        raise ValueError(f"dispatch_backward: dx_sorted must be (P, d, 8), got {tuple(dx_sorted.shape)}")
-    Nt, k = _check_routing("dispatch_backward", routing, dev)
-    P, d = dx_sorted.shape[:2]
-    if dx_add is not None and (dx_add.shape != (Nt, d, 8) or dx_add.dtype != dx_sorted.dtype):
-        raise ValueError(f"dispatch_backward: dx_add must be {dx_sorted.dtype} ({Nt}, {d}, 8)")
+    shape = dx_sorted.shape
+    if len(shape) != 3 or shape[2] != 8:
+        raise ValueError(f"dispatch_backward: dx_sorted must be (P, d, 8), got {tuple(shape)}")
+    slots, _, (Nt, k) = _check_routing("dispatch_backward", routing, dev.index)
+    P, d = shape[0], shape[1]
     code = _dtype_code(dx_sorted)
-    dx_sorted, dx_add = _aligned(dx_sorted), _aligned(dx_add)
-    dx = torch.empty((Nt, d, 8), device=dev, dtype=dx_sorted.dtype)
-    check(lib().ygg_dispatch_backward(dx_sorted.data_ptr(), code, Nt, k, d, P, routing.slot_pos.data_ptr(), ptr(dx_add),
-                                      dx.data_ptr(), stream_handle(dev)), "dispatch_backward")
+    dx_sorted = _aligned(dx_sorted)
+    if dx_add is None:
+        dx = torch.empty((Nt, d, 8), device=dev, dtype=dx_sorted.dtype)
+    elif dx_add.shape != (Nt, d, 8) or dx_add.dtype != dx_sorted.dtype:
+        raise ValueError(f"dispatch_backward: dx_add must be {dx_sorted.dtype} ({Nt}, {d}, 8)")
+    else:
+        dx_add = _aligned(dx_add)
+        dx = torch.empty_like(dx_add)
+    check(lib().ygg_dispatch_backward(dx_sorted.data_ptr(), code, Nt, k, d, P, slots.data_ptr(), ptr(dx_add), dx.data_ptr(),
+                                      stream_handle(dev)), "dispatch_backward")
     return dx
 
 
@@ -636,19 +646,24 @@ def _int8_grouped_linear(codes, scale, d, pw, offsets, bias_prepared, act, gathe
     if (codes.dtype != torch.int8 or codes.shape != (x_rows, 2, (d + 31) // 32, 2, 4, 16) or
             scale.dtype != torch.float32 or scale.shape != (x_rows,)):
         raise ValueError("int8_grouped_linear: rows are not those of quantize_rows")
+    E, d_out = pw.E, pw.d_out
     if d != pw.d_in:
         raise ValueError(f"rows have d_in={d}, weights expect {pw.d_in}")
-    _check_bounds(offsets, pw.E, dev)
-    if gather is not None and (gather.dtype != torch.int32 or gather.dim() != 1):
-        raise ValueError(f"gather must be int32 (rows,), got {gather.dtype} {tuple(gather.shape)}")
-    if bias_prepared is not None and (bias_prepared.dtype != torch.float32 or
-                                      bias_prepared.shape != (pw.E, pw.d_out, 8)):
-        raise ValueError(f"the bias must be a prepared float32 ({pw.E}, {pw.d_out}, 8)")
-    P = x_rows if gather is None else gather.shape[0]
-    codes, bias_prepared = _aligned(codes), _aligned(bias_prepared)
-    y = torch.empty((P, pw.d_out, 8), device=dev, dtype=out_dtype)
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,):
+        _check_bounds(offsets, E, dev)
+    P = x_rows
+    if gather is not None:
+        if gather.dtype != torch.int32 or gather.dim() != 1:
+            raise ValueError(f"gather must be int32 (rows,), got {gather.dtype} {tuple(gather.shape)}")
+        P = gather.shape[0]
+    if bias_prepared is not None:
+        if bias_prepared.dtype != torch.float32 or bias_prepared.shape != (E, d_out, 8):
+            raise ValueError(f"the bias must be a prepared float32 ({E}, {d_out}, 8)")
+        bias_prepared = _aligned(bias_prepared)
+    codes = _aligned(codes)
+    y = torch.empty((P, d_out, 8), device=dev, dtype=out_dtype)
     check(lib().ygg_int8_grouped_linear(codes.data_ptr(), scale.data_ptr(), x_rows, ptr(gather), P, pw.data.data_ptr(),
-                                        pw.scales.data_ptr(), ptr(bias_prepared), offsets.data_ptr(), pw.E, d, pw.d_out,
+                                        pw.scales.data_ptr(), ptr(bias_prepared), offsets.data_ptr(), E, d, d_out,
                                         ACT_CODE[act], y.data_ptr(), DTYPE_CODE[out_dtype], stream_handle(dev)),
           "int8_grouped_linear")
     return y
