@@ -197,7 +197,7 @@ def test_rows_that_are_not_finite_touch_no_other_row():
     bad[7, 3, 2], bad[55, 0, 0], bad[89, 47, 7] = np.nan, np.inf, -np.inf
     pw, pb, off = ops.prepare_weights(_dev(w), "int8_rows"), ops.prepare_bias(_dev(b)), _dev(_bounds(rows))
     say("int8 product of rows that are not finite")
-    for act in ("none", "gelu"):
+    for act in ("none", "gelu", "relu", "sigmoid"):
         y0 = ops.int8_grouped_linear(ops.quantize_rows(_dev(x)), pw, off, pb, act, out_dtype=torch.float32)
         y1 = ops.int8_grouped_linear(ops.quantize_rows(_dev(bad)), pw, off, pb, act, out_dtype=torch.float32)
         keep = torch.ones(90, dtype=torch.bool, device="cuda")
@@ -267,6 +267,37 @@ def test_large_fp32_outputs():
         part = ops.int8_grouped_linear(ops.quantize_rows(x[first:first + n]), pw, _dev(_bounds(few)), pb,
                                        out_dtype=torch.float32)
         assert torch.equal(part, y[first:first + n]), (first, n)
+
+
+def test_rows_past_2_gib():
+    """Codes of more than 2 GiB and outputs of more than 4, in place: 64-bit addresses, the rows of a small batch bit for
+    bit; gathered, such rows are refused."""
+    ops = _ops()
+    g = np.random.default_rng(15)
+    E, d_in, d_out, P = 3, 260, 256, 1_100_000
+    w, b = _weights(g, E, d_out, d_in)
+    pw, pb = ops.prepare_weights(_dev(w), "int8_rows"), ops.prepare_bias(_dev(b))
+    bounds = [0, 100, 1_050_000, P]
+    say("int8 product of codes past 2 GiB")
+    part = _dev(_rows(g, 1000, d_in, True), torch.bfloat16)
+    x = torch.zeros(P, d_in, 8, device="cuda", dtype=torch.bfloat16)
+    places = [0, 500_000, 1_049_500, P - 1000]
+    for at in places:
+        x[at:at + 1000] = part
+    rows = ops.quantize_rows(x)
+    assert rows.codes.numel() > 2 ** 31 and P * d_out * 16 > 2 ** 32
+    del x
+    y = ops.int8_grouped_linear(rows, pw, _dev(np.array(bounds, np.int32)), pb, "relu")
+    one = [ops.int8_grouped_linear(ops.quantize_rows(part), pw, _dev(_bounds([1000 if e == f else 0 for f in range(E)])), pb,
+                                   "relu") for e in range(E)]
+    for at in places:
+        for first, e in ((0, 0), (100, 1), (1_050_000, 2)):
+            lo, hi = max(at, first), min(at + 1000, bounds[e + 1])
+            if lo < hi:
+                assert torch.equal(y[lo:hi], one[e][lo - at:hi - at]), (at, e)
+    with pytest.raises(Exception, match="2 GiB"):
+        ops.int8_grouped_linear(rows, pw, _dev(np.array(bounds, np.int32)), pb,
+                                gather=torch.zeros(P, device="cuda", dtype=torch.int32))
 
 
 def test_on_another_stream():
@@ -388,11 +419,12 @@ def test_captured_layer_replays():
             assert torch.equal(out, want), f"replay {r}"
             assert torch.equal(layer.moe_forward(x, logits=logits), want)
             layer.moe_forward(torch.cat([x, x], 1), logits=torch.cat([logits, logits], 1))  # a larger eager call between
-        x2 = torch.randn_like(x.float()).bfloat16()
-        x.copy_(x2)
+        layer.w_up.mul_(0.5)  # an eager call lays the weights out anew, in the place that the graph reads
+        x.copy_(torch.randn_like(x.float()).bfloat16())
+        want = layer.moe_forward(x, logits=logits)
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(out, layer.moe_forward(x, logits=logits))
+        assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("fmt", ["int8_rows", "pauli"])

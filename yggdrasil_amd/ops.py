@@ -741,7 +741,7 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     fmt = w_up.fmt
     if fmt == "int8_pauli":
         raise ValueError("int8_pauli weights run inside the decode layer (moe_forward), which routes its own "
-                         "rows; use 'int8' for grouped experts")
+                         "rows; use 'int8' or 'int8_rows' for grouped experts")
     if fmt == "pauli":
         h = pauli_grouped_linear(x, w_up, offs, b_up, act, x_layout="blade", y_layout="pauli")
         y = pauli_grouped_linear(h, w_down, offs, b_down, "none", x_layout="pauli", y_layout="blade",
