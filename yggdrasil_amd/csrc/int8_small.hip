@@ -34,7 +34,8 @@ __global__ __launch_bounds__(64) void int8_small_kernel(const unsigned char* __r
   const int n_ct = (d_out + 15) / 16;
   const int ct = blockIdx.x % n_ct, rt = blockIdx.x / n_ct;
   // lane e: expert e's rows; a scan finds the one that holds row tile rt
-  const int v_beg = min(lane < E ? offsets[lane] : 0, P_max), v_end = min(lane < E ? offsets[lane + 1] : 0, P_max);
+  auto inside = [&](int at) { return lane < E ? min(max(offsets[lane + at], 0), P_max) : 0; };
+  const int v_beg = inside(0), v_end = max(inside(1), v_beg);
   const int v_nt = (v_end - v_beg + kTokens - 1) / kTokens;
   int incl = v_nt;
 #pragma unroll

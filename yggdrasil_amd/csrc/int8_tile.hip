@@ -112,7 +112,8 @@ __global__ __launch_bounds__(I8Tile::NT) __attribute__((amdgpu_waves_per_eu(2)))
   const int g = lane >> 5, l32 = lane & 31;
 
   // lane e: expert e's rows, and the tiles up to its last: whole ones, and short last ones ("compact", half the products)
-  const int v_beg = min(lane < E ? offsets[lane] : 0, P_max), v_end = min(lane < E ? offsets[lane + 1] : 0, P_max);
+  auto inside = [&](int at) { return lane < E ? min(max(offsets[lane + at], 0), P_max) : 0; };
+  const int v_beg = inside(0), v_end = max(inside(1), v_beg);
   const int v_all = (v_end - v_beg + C::T - 1) / C::T;
   const int v_short = v_all > 0 && v_end - v_beg - (v_all - 1) * C::T <= C::T / 2 ? 1 : 0;
   const int v_nt = v_all - v_short;
