@@ -120,6 +120,10 @@ def test_quantize_rows_of_nothing_and_off_16_bytes():
     assert x.data_ptr() % 16
     a, b = ops.quantize_rows(x), ops.quantize_rows(x.clone())
     assert torch.equal(a.codes, b.codes) and torch.equal(a.scale, b.scale)
+    pw, off = ops.prepare_weights(torch.randn(1, 24, 40, 8, device="cuda"), "int8_rows"), _dev(_bounds([6]))
+    off_16 = torch.empty(a.block.numel() + 4, device="cuda", dtype=torch.uint8)[4:].copy_(a.block)
+    assert off_16.data_ptr() % 16
+    assert torch.equal(ops.int8_grouped_linear(ops.Int8Rows(off_16, 6, 40), pw, off), ops.int8_grouped_linear(b, pw, off))
 
 
 # ---- the product -------------------------------------------------------------------------------
@@ -481,9 +485,9 @@ def test_refusals():
                    dict(gather=torch.zeros(6, device="cuda")), dict(bias_prepared=torch.zeros(2, 7, 8, device="cuda")),
                    dict(pw=ops.prepare_weights(torch.randn(2, 8, 40, 8, device="cuda"), "pauli")),
                    dict(pw=ops.prepare_weights(torch.randn(2, 8, 41, 8, device="cuda"), "int8_rows")),
-                   dict(rows=ops.Int8Rows(rows.codes[:, :, :1], rows.scale, 40)),
-                   dict(rows=ops.Int8Rows(rows.codes, rows.scale.double(), 40)),
-                   dict(rows=ops.Int8Rows(rows.codes, rows.scale[:5], 40)), dict(offsets=off.cpu())):
+                   dict(rows=ops.Int8Rows(rows.block[:-1], 6, 40)), dict(rows=ops.Int8Rows(rows.block, 7, 40)),
+                   dict(rows=ops.Int8Rows(rows.block, 6, 39)), dict(rows=ops.Int8Rows(rows.block.float(), 6, 40)),
+                   dict(rows=ops.Int8Rows(rows.block.cpu(), 6, 40)), dict(offsets=off.cpu())):
         with pytest.raises(ValueError):
             ops.int8_grouped_linear(**{**dict(rows=rows, pw=pw, offsets=off), **kwargs})
     with pytest.raises(ValueError):  # fp32 rows into bf16 experts

@@ -600,18 +600,38 @@ def pauli_rows_from_blade(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
-@dataclass
 class Int8Rows:
-    """Rows of multivectors in int8 (:func:`quantize_rows`): the codes of their halved 2x2 matrices' entries, in runs of
-    16 bytes as the products read them, and one fp32 scale a row."""
+    """Rows of multivectors in int8 (:func:`quantize_rows`), in one uint8 buffer ``block``: the codes of their halved 2x2
+    matrices' entries, in runs of 16 bytes as the products read them, then (on 256 bytes) one fp32 scale a row.
+    ``codes`` and ``scale`` are its tensors."""
 
-    codes: torch.Tensor  # (rows, 2, ceil(d / 32), 2, 4, 16) int8: column b, K step, re / im, 8 inputs, (input, row c)
-    scale: torch.Tensor  # (rows,) fp32
-    d: int
+    __slots__ = ("block", "rows", "d")
+
+    def __init__(self, block: torch.Tensor, rows: int, d: int):
+        self.block, self.rows, self.d = block, rows, d
+
+    @staticmethod
+    def sizes(rows: int, d: int) -> tuple:
+        """Bytes in front of the scales, and in all."""
+        at = rows * ((d + 31) // 32 * 256)  # (a multiple of 256)
+        return at, at + 4 * rows
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """(rows, 2, ceil(d / 32), 2, 4, 16) int8: column b, K step, re / im, 8 inputs, (input, row c)."""
+        at = self.sizes(self.rows, self.d)[0]
+        return self.block[:at].view(torch.int8).view(self.rows, 2, (self.d + 31) // 32, 2, 4, 16)
+
+    @property
+    def scale(self) -> torch.Tensor:
+        """(rows,) fp32."""
+        at, end = self.sizes(self.rows, self.d)
+        return self.block[at:end].view(torch.float32)
 
     def values(self) -> torch.Tensor:
         """What the codes stand for, as fp32 multivectors (rows, d, 8)."""
-        q = self.codes.float().view(*self.codes.shape[:5], 8, 2)  # [row, b, ks, part, g, m, c]
+        codes = self.codes
+        q = codes.float().view(*codes.shape[:5], 8, 2)  # [row, b, ks, part, g, m, c]
         q = q.permute(0, 2, 4, 5, 6, 1, 3).reshape(q.shape[0], 32 * q.shape[2], 2, 2, 2)[:, :self.d]  # [row, i, c, b, part]
         e = q * self.scale[:, None, None, None, None]
         (r00, i00), (r01, i01), (r10, i10), (r11, i11) = [e[:, :, c, b].unbind(-1) for c in (0, 1) for b in (0, 1)]
@@ -627,25 +647,25 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     or a NaN gets the scale NaN: its products are NaN.
     """
     dev = _one_device(x)
-    if x.dim() != 3 or x.shape[2] != 8:
-        raise ValueError(f"quantize_rows: x must be (rows, d, 8), got {tuple(x.shape)}")
-    rows, d = x.shape[:2]
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != 8:
+        raise ValueError(f"quantize_rows: x must be (rows, d, 8), got {tuple(shape)}")
+    rows, d = shape[0], shape[1]
     code = _dtype_code(x)
     x = _aligned(x)
-    codes = torch.empty((rows, 2, (d + 31) // 32, 2, 4, 16), device=dev, dtype=torch.int8)
-    scale = torch.empty(rows, device=dev, dtype=torch.float32)
-    check(lib().ygg_quantize_rows(x.data_ptr(), code, rows, d, codes.data_ptr(), scale.data_ptr(), stream_handle(dev)),
-          "quantize_rows")
-    return Int8Rows(codes, scale, d)
+    at, need = Int8Rows.sizes(rows, d)
+    block = torch.empty(need, device=dev, dtype=torch.uint8)
+    to = block.data_ptr()
+    check(lib().ygg_quantize_rows(x.data_ptr(), code, rows, d, to, to + at, stream_handle(dev)), "quantize_rows")
+    return Int8Rows(block, rows, d)
 
 
 @_on_its_device
-def _int8_grouped_linear(codes, scale, d, pw, offsets, bias_prepared, act, gather, out_dtype):
-    dev = _one_device(codes, scale, pw.data, pw.scales, offsets, bias_prepared, gather)
-    x_rows = codes.shape[0]
-    if (codes.dtype != torch.int8 or codes.shape != (x_rows, 2, (d + 31) // 32, 2, 4, 16) or
-            scale.dtype != torch.float32 or scale.shape != (x_rows,)):
-        raise ValueError("int8_grouped_linear: rows are not those of quantize_rows")
+def _int8_grouped_linear(block, x_rows, d, pw, offsets, bias_prepared, act, gather, out_dtype):
+    dev = _one_device(block, pw.data, pw.scales, offsets, bias_prepared, gather)
+    at, need = Int8Rows.sizes(x_rows, d)
+    if block.dtype != torch.uint8 or block.numel() < need:
+        raise ValueError(f"int8_grouped_linear: {x_rows} rows of {d} multivectors take {need} bytes of uint8")
     E, d_out = pw.E, pw.d_out
     if d != pw.d_in:
         raise ValueError(f"rows have d_in={d}, weights expect {pw.d_in}")
@@ -660,12 +680,12 @@ def _int8_grouped_linear(codes, scale, d, pw, offsets, bias_prepared, act, gathe
         if bias_prepared.dtype != torch.float32 or bias_prepared.shape != (E, d_out, 8):
             raise ValueError(f"the bias must be a prepared float32 ({E}, {d_out}, 8)")
         bias_prepared = _aligned(bias_prepared)
-    codes = _aligned(codes)
+    block = _aligned(block)
+    codes = block.data_ptr()
     y = torch.empty((P, d_out, 8), device=dev, dtype=out_dtype)
-    check(lib().ygg_int8_grouped_linear(codes.data_ptr(), scale.data_ptr(), x_rows, ptr(gather), P, pw.data.data_ptr(),
-                                        pw.scales.data_ptr(), ptr(bias_prepared), offsets.data_ptr(), E, d, d_out,
-                                        ACT_CODE[act], y.data_ptr(), DTYPE_CODE[out_dtype], stream_handle(dev)),
-          "int8_grouped_linear")
+    check(lib().ygg_int8_grouped_linear(codes, codes + at, x_rows, ptr(gather), P, pw.data.data_ptr(), pw.scales.data_ptr(),
+                                        ptr(bias_prepared), offsets.data_ptr(), E, d, d_out, ACT_CODE[act], y.data_ptr(),
+                                        DTYPE_CODE[out_dtype], stream_handle(dev)), "int8_grouped_linear")
     return y
 
 
@@ -686,7 +706,7 @@ def int8_grouped_linear(rows: Int8Rows, pw: PreparedWeights, offsets: torch.Tens
         raise ValueError(f"act must be one of {tuple(ACT_CODE)}")
     if out_dtype not in DTYPE_CODE:
         raise ValueError(f"out_dtype must be float32 or bfloat16, got {out_dtype}")
-    return _int8_grouped_linear(rows.codes, rows.scale, rows.d, pw, offsets, bias_prepared, act, gather, out_dtype)
+    return _int8_grouped_linear(rows.block, rows.rows, rows.d, pw, offsets, bias_prepared, act, gather, out_dtype)
 
 
 @_on_its_device
