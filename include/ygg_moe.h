@@ -252,12 +252,12 @@ int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows,
 /* Every expert's CliffordFFN (hlm_block.py:55-61) on bf16 rows grouped by expert, both
  * products in int8: the rows quantized, the up product with bias and activation, its bf16
  * rows quantized, the down product with bias; y (P, d, 8) bf16, what the calls above give.
- * workspace on 256 bytes. */
-size_t ygg_int8_grouped_experts_workspace_bytes(int P, int d, int F);
+ * offsets and counts (E,) as ygg_expert_bounds takes them; workspace on 256 bytes. */
+size_t ygg_int8_grouped_experts_workspace_bytes(int P, int E, int d, int F);
 int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_up, const float* s_up, const float* b_up,
-                             const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets, int E,
-                             int d, int F, int act, void* y, void* workspace, size_t workspace_bytes,
-                             ygg_stream_t stream);
+                             const void* w_down, const float* s_down, const float* b_down, const void* offsets,
+                             const void* counts, int index_bytes, int E, int d, int F, int act, void* y, void* workspace,
+                             size_t workspace_bytes, ygg_stream_t stream);
 
 /* Row ranges as a caller of the grouped products has them -- (E,) offsets and counts of 4 or
  * 8 bytes (index_bytes) -- as the E + 1 bounds that they take, brought into [0, P] and into

@@ -55,14 +55,16 @@ def test_product_in_place(at, value):
     _refused("ygg_int8_grouped_linear", args, "share")
 
 
-_EXP = [FAR[0], 8, FAR[1], FAR[2], None, FAR[3], FAR[4], None, FAR[5], 2, 40, 24, 1, FAR[6], FAR[7], 1 << 20, None]
+_EXP = [FAR[0], 8, FAR[1], FAR[2], None, FAR[3], FAR[4], None, FAR[5], FAR[5] + 1024, 4, 2, 40, 24, 1, FAR[6], FAR[7], 1 << 20,
+        None]
 
 
 @pytest.mark.parametrize("at,value,word", [
     (0, None, "null"), (2, None, "null"), (3, None, "null"), (5, None, "null"), (6, None, "null"), (8, None, "null"),
-    (13, None, "null"), (14, None, "null"), (1, -1, "bad sizes"), (9, 0, "bad sizes"), (9, 65, "bad sizes"),
-    (10, 0, "bad sizes"), (11, 0, "bad sizes"), (12, 4, "activation"), (10, 20000, "16384"), (11, 20000, "16384"),
-    (15, 100, "workspace"), (14, FAR[0], "share"), (14, FAR[6] + 16, "share")])
+    (9, None, "null"), (15, None, "null"), (16, None, "null"), (1, -1, "bad sizes"), (11, 0, "bad sizes"),
+    (11, 65, "bad sizes"), (12, 0, "bad sizes"), (13, 0, "bad sizes"), (14, 4, "activation"), (10, 2, "bytes"),
+    (12, 20000, "16384"), (13, 20000, "16384"), (17, 100, "workspace"), (16, FAR[0], "share"), (16, FAR[6] + 16, "share"),
+    (16, FAR[5], "share"), (16, FAR[5] + 1024, "share")])
 def test_experts(at, value, word):
     args = list(_EXP)
     args[at] = value

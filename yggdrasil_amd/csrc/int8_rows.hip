@@ -60,16 +60,50 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return max(max(a, b), max(c, d));
 }
 
+// Bounds of experts' ranges as a caller has them, indexes of 4 or 8 bytes: brought into [0, P] and into ascending order,
+// by one wave.
+struct Ranges {
+  const void *offsets = nullptr, *counts = nullptr;
+  int index_bytes = 4, E = 0, P = 0;
+  int32_t* bounds = nullptr;
+};
+template <typename I>
+__device__ __forceinline__ void write_bounds(const Ranges& r) {
+  typedef typename std::make_unsigned<I>::type U;  // (sums may wrap)
+  const int lane = threadIdx.x & 63;
+  const I at = lane < r.E ? static_cast<const I*>(r.offsets)[lane] : 0;
+  const I end = lane < r.E ? (I)((U)at + (U) static_cast<const I*>(r.counts)[lane]) : 0;
+  auto clip = [&](I v) { return min(max((int32_t)v, 0), r.P); };
+  int v = lane < r.E ? clip(at) : 0;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int p = __shfl_up(v, o);
+    if (lane >= o) v = max(v, p);
+  }
+  if (lane < r.E) r.bounds[lane] = v;
+  if (lane == r.E - 1) r.bounds[r.E] = max(v, clip(end));
+}
+__device__ __forceinline__ void write_ranges(const Ranges& r) {
+  if (r.index_bytes == 8) write_bounds<long long>(r);
+  else write_bounds<int32_t>(r);
+}
+__global__ __launch_bounds__(64) void expert_bounds_kernel(const Ranges r) { write_ranges(r); }
+
 // WAVES waves a row, four waves a workgroup; a lane takes every 64 WAVES-th multivector, KEEP of them kept from the pass
-// that finds the largest entry to the one that writes the codes.
+// that finds the largest entry to the one that writes the codes.  The workgroup behind the rows' writes the bounds of
+// `ranges` where there are any (a launch less in front of the products that read them).
 template <typename T, int WAVES, int KEEP>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int rows, int d,
-                                                            unsigned char* __restrict__ codes, float* __restrict__ scale) {
+                                                            unsigned char* __restrict__ codes, float* __restrict__ scale,
+                                                            const Ranges ranges) {
   constexpr int RPB = 4 / WAVES;
   __shared__ uint32_t s_max[4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = blockIdx.x * RPB + wave / WAVES;
-  if (WAVES == 1 && row >= rows) return;  // (with several waves a row, every workgroup has one)
+  if (row >= rows) {
+    if (ranges.bounds != nullptr && blockIdx.x + 1 == gridDim.x && threadIdx.x < 64) write_ranges(ranges);
+    return;
+  }
   const int first = (wave % WAVES) * 64 + lane;
   constexpr int STRIDE = 64 * WAVES;
   RawMv<T> kept[KEEP];
@@ -134,34 +168,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 }
 
 template <typename T>
-void launch_quantize(const void* x, int rows, int d, void* codes, float* scale, hipStream_t stream) {
+void launch_quantize(const void* x, int rows, int d, void* codes, float* scale, hipStream_t stream, const Ranges& ranges = {}) {
   const T* X = static_cast<const T*>(x);
   unsigned char* C = static_cast<unsigned char*>(codes);
-  const unsigned quarter = (unsigned)(((long long)rows + 3) / 4);
+  const unsigned more = ranges.bounds != nullptr, quarter = (unsigned)(((long long)rows + 3) / 4) + more;
   if (d <= 64)
-    quantize_rows_kernel<T, 1, 1><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale);
+    quantize_rows_kernel<T, 1, 1><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
   else if (d <= 256)
-    quantize_rows_kernel<T, 1, 4><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale);
+    quantize_rows_kernel<T, 1, 4><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
   else
-    quantize_rows_kernel<T, 4, 4><<<(unsigned)rows, 256, 0, stream>>>(X, rows, d, C, scale);
-}
-
-// Bounds of experts' ranges as a caller has them, 4 or 8 bytes each: brought into [0, P] and into ascending order.
-template <typename I>
-__global__ __launch_bounds__(64) void expert_bounds_kernel(const I* __restrict__ offsets, const I* __restrict__ counts, int E,
-                                                           int P, int32_t* __restrict__ bounds) {
-  const int lane = threadIdx.x;
-  typedef typename std::make_unsigned<I>::type U;  // (sums may wrap)
-  const I at = lane < E ? offsets[lane] : 0, end = lane < E ? (I)((U)at + (U)counts[lane]) : 0;
-  auto clip = [&](I v) { return min(max((int32_t)v, 0), P); };
-  int v = lane < E ? clip(at) : 0;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int p = __shfl_up(v, o);
-    if (lane >= o) v = max(v, p);
-  }
-  if (lane < E) bounds[lane] = v;
-  if (lane == E - 1) bounds[E] = max(v, clip(end));
+    quantize_rows_kernel<T, 4, 4><<<(unsigned)rows + more, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
 }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -185,9 +201,10 @@ ExpertsAt experts_at(size_t x_rows, size_t P, int d, int F) {
 
 size_t int8_experts_bytes(size_t x_rows, size_t P, int d, int F) { return experts_at(x_rows, P, d, F).total; }
 
-int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
+namespace {
+int run_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
                  const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
-                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream) {
+                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream, const Ranges& ranges) {
   const ExpertsAt at = experts_at((size_t)x_rows, (size_t)P, d, F);
   char* const b = static_cast<char*>(workspace);
   float *xs = reinterpret_cast<float*>(b + at.xs), *hs = reinterpret_cast<float*>(b + at.hs);
@@ -196,12 +213,20 @@ int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const 
     return (int8_small_pays(P, d_out) ? int8_small_linear : int8_tile_linear)(q, s, rows, from, P, w, sw, bias, offsets, E,
                                                                               d_in, d_out, a, to, kBF16, stream);
   };
-  launch_quantize<uint16_t>(x, x_rows, d, b + at.xq, xs, stream);
+  launch_quantize<uint16_t>(x, x_rows, d, b + at.xq, xs, stream, ranges);
   if (check_launch("int8_experts")) return -1;
   if (product(b + at.xq, xs, x_rows, gather, w_up, s_up, b_up, d, F, act, b + at.h)) return -1;
   launch_quantize<uint16_t>(b + at.h, P, F, b + at.hq, hs, stream);
   if (check_launch("int8_experts")) return -1;
   return product(b + at.hq, hs, P, nullptr, w_down, s_down, b_down, F, d, kActNone, y);
+}
+}  // namespace
+
+int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
+                 const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
+                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream) {
+  return run_experts(x, x_rows, gather, P, w_up, s_up, b_up, w_down, s_down, b_down, offsets, E, d, F, act, y, workspace,
+                     stream, Ranges{});
 }
 
 size_t int8_rows_bytes(size_t rows, int d) { return rows * i8_row_bytes(d); }
@@ -262,36 +287,36 @@ YGG_API int ygg_expert_bounds(const void* offsets, const void* counts, int index
   YGG_CHECK_ARG(E >= 1 && E <= 64 && P >= 0, "ygg_expert_bounds: bad sizes E=%d P=%d (E <= 64)", E, P);
   YGG_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "ygg_expert_bounds: indexes of %d bytes", index_bytes);
   YGG_CHECK_ARG(offsets && counts && bounds, "ygg_expert_bounds: null pointer");
-  if (index_bytes == 8)
-    expert_bounds_kernel<long long><<<1, 64, 0, stream>>>(static_cast<const long long*>(offsets),
-                                                          static_cast<const long long*>(counts), E, P, bounds);
-  else
-    expert_bounds_kernel<int32_t><<<1, 64, 0, stream>>>(static_cast<const int32_t*>(offsets),
-                                                        static_cast<const int32_t*>(counts), E, P, bounds);
+  expert_bounds_kernel<<<1, 64, 0, stream>>>(Ranges{offsets, counts, index_bytes, E, P, bounds});
   return check_launch("expert_bounds");
 }
 
-YGG_API size_t ygg_int8_grouped_experts_workspace_bytes(int P, int d, int F) {
-  return P < 0 || d < 1 || F < 1 ? 0 : int8_experts_bytes((size_t)P, (size_t)P, d, F);
+YGG_API size_t ygg_int8_grouped_experts_workspace_bytes(int P, int E, int d, int F) {
+  return P < 0 || E < 1 || d < 1 || F < 1 ? 0 : int8_experts_bytes((size_t)P, (size_t)P, d, F) + align256((size_t)(E + 1) * 4);
 }
 
 YGG_API int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_up, const float* s_up, const float* b_up,
-                                     const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
-                                     int E, int d, int F, int act, void* y, void* workspace, size_t workspace_bytes,
-                                     hipStream_t stream) {
+                                     const void* w_down, const float* s_down, const float* b_down, const void* offsets,
+                                     const void* counts, int index_bytes, int E, int d, int F, int act, void* y,
+                                     void* workspace, size_t workspace_bytes, hipStream_t stream) {
   YGG_CHECK_ARG(P >= 0 && E >= 1 && E <= 64 && d >= 1 && F >= 1, "ygg_int8_grouped_experts: bad sizes P=%d E=%d d=%d F=%d (E <= 64)",
                 P, E, d, F);
   YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_int8_grouped_experts: activation %d", act);
+  YGG_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "ygg_int8_grouped_experts: indexes of %d bytes", index_bytes);
   const char* why = int8_linear_limit(P, false, E, d, F);
   if (!why) why = int8_linear_limit(P, false, E, F, d);
   YGG_CHECK_ARG(!why, "ygg_int8_grouped_experts: %s (P=%d E=%d d=%d F=%d)", why, P, E, d, F);
   if (P == 0) return 0;
-  YGG_CHECK_ARG(x_sorted && w_up && s_up && w_down && s_down && offsets && y && workspace,
+  YGG_CHECK_ARG(x_sorted && w_up && s_up && w_down && s_down && offsets && counts && y && workspace,
                 "ygg_int8_grouped_experts: null pointer");
-  const size_t need = int8_experts_bytes((size_t)P, (size_t)P, d, F), yb = (size_t)P * d * 16;
+  const size_t need = ygg_int8_grouped_experts_workspace_bytes(P, E, d, F), yb = (size_t)P * d * 16;
   YGG_CHECK_ARG(workspace_bytes >= need, "ygg_int8_grouped_experts: workspace of %zu bytes, need %zu", workspace_bytes, need);
-  YGG_CHECK_ARG(!overlap(workspace, need, x_sorted, yb) && !overlap(workspace, need, y, yb),
-                "ygg_int8_grouped_experts: the workspace must not share memory with x_sorted or y");
-  return int8_experts(x_sorted, P, nullptr, P, w_up, s_up, b_up, w_down, s_down, b_down, offsets, E, d, F, act, y, workspace,
-                      stream);
+  YGG_CHECK_ARG(!overlap(workspace, need, x_sorted, yb) && !overlap(workspace, need, y, yb) &&
+                    !overlap(workspace, need, offsets, (size_t)E * index_bytes) &&
+                    !overlap(workspace, need, counts, (size_t)E * index_bytes),
+                "ygg_int8_grouped_experts: the workspace must not share memory with x_sorted, y or the ranges");
+  int32_t* const bounds =
+      reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + int8_experts_bytes((size_t)P, (size_t)P, d, F));
+  return run_experts(x_sorted, P, nullptr, P, w_up, s_up, b_up, w_down, s_down, b_down, bounds, E, d, F, act, y, workspace,
+                     stream, Ranges{offsets, counts, index_bytes, E, P, bounds});
 }

@@ -709,6 +709,28 @@ def int8_grouped_linear(rows: Int8Rows, pw: PreparedWeights, offsets: torch.Tens
     return _int8_grouped_linear(rows.block, rows.rows, rows.d, pw, offsets, bias_prepared, act, gather, out_dtype)
 
 
+def _int8_grouped_experts(dev, x, offsets, counts, w_up, w_down, b_up, b_down, act):
+    E, d, F, P = w_up.E, w_up.d_in, w_up.d_out, x.shape[0]
+    _one_device(x, offsets, counts, b_up, b_down, w_up.data, w_down.data)
+    if x.dtype != torch.bfloat16:
+        raise ValueError("int8_rows experts take bf16 rows")
+    for name, b, want in (("b_up", b_up, (E, F, 8)), ("b_down", b_down, (E, d, 8))):
+        if b is not None and (b.dtype != torch.float32 or b.shape != want):
+            raise ValueError(f"{name} must be a prepared float32 bias {want}, got {b.dtype} {tuple(b.shape)}")
+    if offsets.dtype != counts.dtype or offsets.dtype not in (torch.int32, torch.int64):
+        offsets, counts = offsets.long(), counts.long()
+    x = _aligned(x)
+    y = torch.empty_like(x)
+    L = lib()
+    need = L.ygg_int8_grouped_experts_workspace_bytes(P, E, d, F)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    check(L.ygg_int8_grouped_experts(x.data_ptr(), P, w_up.data.data_ptr(), w_up.scales.data_ptr(), ptr(b_up),
+                                     w_down.data.data_ptr(), w_down.scales.data_ptr(), ptr(b_down), offsets.data_ptr(),
+                                     counts.data_ptr(), offsets.element_size(), E, d, F, ACT_CODE[act], y.data_ptr(),
+                                     ws.data_ptr(), need, stream_handle(dev)), "grouped_experts")
+    return y
+
+
 @_on_its_device
 def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert_counts: torch.Tensor,
                     w_up: PreparedWeights, w_down: PreparedWeights, b_up: torch.Tensor | None = None,
@@ -750,6 +772,10 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
             raise ValueError("expert ranges must be contiguous, ascending and cover the rows from 0")
     if P == 0:
         return x_sorted.clone()
+    fmt = w_up.fmt
+    if fmt == "int8_rows":
+        return _int8_grouped_experts(dev, x, expert_offsets, expert_counts, w_up, w_down, b_up, b_down,
+                                     act).reshape(x_sorted.shape)
     # the products take every range from these bounds: ascending and inside the rows
     if E <= 64 and expert_offsets.dtype == expert_counts.dtype and expert_offsets.dtype in (torch.int32, torch.int64):
         offs = torch.empty(E + 1, device=dev, dtype=torch.int32)
@@ -758,7 +784,6 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     else:
         offs = torch.cat([expert_offsets.reshape(E), (expert_offsets[-1:] + expert_counts[-1:])]).to(torch.int32)
         offs = torch.cummax(offs.clamp(0, P), 0).values.to(torch.int32).contiguous()
-    fmt = w_up.fmt
     if fmt == "int8_pauli":
         raise ValueError("int8_pauli weights run inside the decode layer (moe_forward), which routes its own "
                          "rows; use 'int8' or 'int8_rows' for grouped experts")
@@ -769,19 +794,6 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     elif fmt == "pauli_f32":
         h = pauli_grouped_linear_f32(pauli_rows_from_blade_f32(x), w_up, offs, b_up, act, y_layout="pauli")
         y = pauli_grouped_linear_f32(h, w_down, offs, b_down, "none", y_layout="blade")
-    elif fmt == "int8_rows":
-        if x.dtype != torch.bfloat16:
-            raise ValueError("int8_rows experts take bf16 rows")
-        for name, b, want in (("b_up", b_up, (E, F, 8)), ("b_down", b_down, (E, d, 8))):
-            if b is not None and (b.dtype != torch.float32 or tuple(b.shape) != want):
-                raise ValueError(f"{name} must be a prepared float32 bias {want}, got {b.dtype} {tuple(b.shape)}")
-        x = _aligned(x)
-        y = torch.empty_like(x)
-        need = lib().ygg_int8_grouped_experts_workspace_bytes(P, d, F)
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-        check(lib().ygg_int8_grouped_experts(ptr(x), P, ptr(w_up.data), ptr(w_up.scales), ptr(b_up), ptr(w_down.data),
-                                             ptr(w_down.scales), ptr(b_down), ptr(offs), E, d, F, ACT_CODE[act], ptr(y),
-                                             ptr(ws), need, stream_handle(dev)), "grouped_experts")
     else:  # L(w) blocks read and write mask order between the products
         h = grouped_clifford_linear(to_mask_order(x), w_up, offs, b_up, act, out_blade_order=False)
         y = grouped_clifford_linear(h, w_down, offs, b_down, "none", out_dtype=x.dtype, out_blade_order=True)
