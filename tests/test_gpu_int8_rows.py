@@ -110,6 +110,26 @@ def test_quantize_rows_far_values(d, bf16):
     assert np.array_equal(got.codes.cpu().numpy(), io.codes_layout(q))
 
 
+@pytest.mark.parametrize("d,rows", [(1, (1 << 22) + 5), (257, (1 << 22) + 1)])
+def test_quantize_rows_of_more_than_one_launch(d, rows):
+    """More rows than a launch takes: those at the seam and at the end, as in a batch of their own."""
+    ops = _ops()
+    say(f"quantize_rows {rows} x {d}")
+    part = _dev(_rows(np.random.default_rng(16), 64, d, True), torch.bfloat16)
+    x = torch.zeros(rows, d, 8, device="cuda", dtype=torch.bfloat16)
+    places = [0, (1 << 22) - 64, rows - 64]
+    for at in places:
+        x[at:at + 64] = part
+    got = ops.quantize_rows(x)
+    one = ops.quantize_rows(part)
+    at = rows - 64  # (the last to be written: whole)
+    assert torch.equal(got.codes[at:], one.codes) and torch.equal(got.scale[at:], one.scale)
+    assert torch.equal(got.codes[:64], one.codes) and torch.equal(got.scale[:64], one.scale)
+    n = at - places[1]
+    assert torch.equal(got.codes[places[1]:at], one.codes[:n]) and torch.equal(got.scale[places[1]:at], one.scale[:n])
+    assert int(got.codes[64:places[1]].max()) == 0 and float(got.scale[64:places[1]].max()) == float(got.scale[64:65])
+
+
 def test_quantize_rows_of_nothing_and_off_16_bytes():
     ops = _ops()
     say("quantize_rows of no rows, and of a tensor off 16 bytes")

@@ -103,6 +103,24 @@ def test_dispatch_backward(N, d, E, k, dt, with_add):
     _within(dx, want, bound, "dx")
 
 
+def test_more_tokens_than_one_launch():
+    """Powers of two as weights, so every product is exact; the rows in reversed order."""
+    ops = _ops()
+    N, d, k = (1 << 22) + 7, 1, 2
+    P = N * k
+    say(f"sort gradients of {N} tokens")
+    slots = torch.arange(P - 1, -1, -1, device="cuda", dtype=torch.int32).view(N, k)
+    w = torch.exp2(-(slots % 3).float())
+    r = ops.Routing(slots, w, slots[0], slots[0], slots[0], slots)
+    dout = torch.randint(-8, 9, (N, d, 8), device="cuda").float()
+    y = torch.randint(-8, 9, (P, d, 8), device="cuda").float()
+    dy, dw = ops.combine_backward(dout, y, r)
+    back = y.flip(0).view(N, k, 8)
+    assert torch.equal(dy.flip(0).view(N, k, 8), w[..., None] * dout)
+    assert torch.equal(dw, (dout * back).sum(-1))
+    assert torch.equal(ops.dispatch_backward(y, r, dout), (dout[:, 0] + back[:, 0] + back[:, 1])[:, None])
+
+
 def test_slots_outside_the_rows():
     """A caller who drops slots (a full expert) names rows outside: nothing is read or written for them."""
     ops = _ops()

@@ -71,6 +71,14 @@ def test_experts(at, value, word):
     _refused("ygg_int8_grouped_experts", args, word)
 
 
+@pytest.mark.parametrize("at", [2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("on", [_EXP[14 + 1], _EXP[14 + 2]])
+def test_experts_over_their_weights(at, on):
+    args = list(_EXP)
+    args[at] = on + 16
+    _refused("ygg_int8_grouped_experts", args, "share")
+
+
 @pytest.mark.parametrize("args,word", [
     ((P, P, 4, 0, 8, P, None), "bad sizes"), ((P, P, 4, 65, 8, P, None), "bad sizes"), ((P, P, 4, 2, -1, P, None), "bad sizes"),
     ((P, P, 2, 2, 8, P, None), "bytes"), ((None, P, 4, 2, 8, P, None), "null"), ((P, None, 4, 2, 8, P, None), "null"),

@@ -89,14 +89,14 @@ __device__ __forceinline__ void write_ranges(const Ranges& r) {
 }
 __global__ __launch_bounds__(64) void expert_bounds_kernel(const Ranges r) { write_ranges(r); }
 
-// WAVES waves a row, four waves a workgroup; a lane takes every 64 WAVES-th multivector, KEEP of them kept from the pass
+// WAVES waves a row, four waves a workgroup; a lane takes every 64 WAVES-th multivector, four of them kept from the pass
 // that finds the largest entry to the one that writes the codes.  The workgroup behind the rows' writes the bounds of
 // `ranges` where there are any (a launch less in front of the products that read them).
-template <typename T, int WAVES, int KEEP>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int rows, int d,
                                                             unsigned char* __restrict__ codes, float* __restrict__ scale,
                                                             const Ranges ranges) {
-  constexpr int RPB = 4 / WAVES;
+  constexpr int RPB = 4 / WAVES, KEEP = 4;
   __shared__ uint32_t s_max[4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int row = blockIdx.x * RPB + wave / WAVES;
@@ -167,17 +167,27 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   }
 }
 
+// Four waves a row where a row is long, or longer than two loads a lane and rows are few (one wave / four a row, bf16, us: 128
+// rows of 128: 2.4 / 2.3, 256: 3.0 / 2.3, 512: 5.2 / 2.6; 2048 rows of 128: 3.4 / 3.7, 256: 5.1 / 4.8, 320: 6.1 / 5.7; 32768
+// rows of 128: 23 / 32, 256: 40 / 44, 320: 51 / 52, 512: 85 / 71).  32768 rows of 512 run at 5.7 TB/s (402 MB).
+// Rows of a launch: a grid holds fewer than 2^32 threads.
+constexpr int kLaunchRows = 1 << 22;
+
 template <typename T>
-void launch_quantize(const void* x, int rows, int d, void* codes, float* scale, hipStream_t stream, const Ranges& ranges = {}) {
-  const T* X = static_cast<const T*>(x);
-  unsigned char* C = static_cast<unsigned char*>(codes);
-  const unsigned more = ranges.bounds != nullptr, quarter = (unsigned)(((long long)rows + 3) / 4) + more;
-  if (d <= 64)
-    quantize_rows_kernel<T, 1, 1><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
-  else if (d <= 256)
-    quantize_rows_kernel<T, 1, 4><<<quarter, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
-  else
-    quantize_rows_kernel<T, 4, 4><<<(unsigned)rows + more, 256, 0, stream>>>(X, rows, d, C, scale, ranges);
+int launch_quantize(const void* x, int rows, int d, void* codes, float* scale, hipStream_t stream, const Ranges& ranges = {}) {
+  for (size_t r0 = 0; r0 < (size_t)rows; r0 += kLaunchRows) {
+    const int n = (int)std::min<size_t>(rows - r0, kLaunchRows);
+    const T* const X = static_cast<const T*>(x) + r0 * d * 8;
+    unsigned char* const C = static_cast<unsigned char*>(codes) + r0 * i8_row_bytes(d);
+    const Ranges& with = r0 + n == (size_t)rows ? ranges : Ranges{};
+    const unsigned more = with.bounds != nullptr, quarter = (unsigned)(n + 3) / 4 + more;
+    if (d > 256 || (d > 128 && n <= 2048))
+      quantize_rows_kernel<T, 4><<<(unsigned)n + more, 256, 0, stream>>>(X, n, d, C, scale + r0, with);
+    else
+      quantize_rows_kernel<T, 1><<<quarter, 256, 0, stream>>>(X, n, d, C, scale + r0, with);
+    if (check_launch("quantize_rows")) return -1;
+  }
+  return 0;
 }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -203,8 +213,8 @@ size_t int8_experts_bytes(size_t x_rows, size_t P, int d, int F) { return expert
 
 namespace {
 int run_experts(const void* x, int x_rows, const int32_t* gather, int P, const void* w_up, const float* s_up,
-                 const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
-                 int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream, const Ranges& ranges) {
+                const float* b_up, const void* w_down, const float* s_down, const float* b_down, const int32_t* offsets,
+                int E, int d, int F, int act, void* y, void* workspace, hipStream_t stream, const Ranges& ranges) {
   const ExpertsAt at = experts_at((size_t)x_rows, (size_t)P, d, F);
   char* const b = static_cast<char*>(workspace);
   float *xs = reinterpret_cast<float*>(b + at.xs), *hs = reinterpret_cast<float*>(b + at.hs);
@@ -213,11 +223,9 @@ int run_experts(const void* x, int x_rows, const int32_t* gather, int P, const v
     return (int8_small_pays(P, d_out) ? int8_small_linear : int8_tile_linear)(q, s, rows, from, P, w, sw, bias, offsets, E,
                                                                               d_in, d_out, a, to, kBF16, stream);
   };
-  launch_quantize<uint16_t>(x, x_rows, d, b + at.xq, xs, stream, ranges);
-  if (check_launch("int8_experts")) return -1;
+  if (launch_quantize<uint16_t>(x, x_rows, d, b + at.xq, xs, stream, ranges)) return -1;
   if (product(b + at.xq, xs, x_rows, gather, w_up, s_up, b_up, d, F, act, b + at.h)) return -1;
-  launch_quantize<uint16_t>(b + at.h, P, F, b + at.hq, hs, stream);
-  if (check_launch("int8_experts")) return -1;
+  if (launch_quantize<uint16_t>(b + at.h, P, F, b + at.hq, hs, stream)) return -1;
   return product(b + at.hq, hs, P, nullptr, w_down, s_down, b_down, F, d, kActNone, y);
 }
 }  // namespace
@@ -254,9 +262,8 @@ YGG_API int ygg_quantize_rows(const void* x, int x_dtype, int rows, int d, void*
   YGG_CHECK_ARG(!overlap(x, xb, codes, cb) && !overlap(x, xb, scale, (size_t)rows * 4) &&
                     !overlap(codes, cb, scale, (size_t)rows * 4),
                 "ygg_quantize_rows: x, codes and scale must not share memory");
-  if (x_dtype == kF32) launch_quantize<float>(x, rows, d, codes, scale, stream);
-  else launch_quantize<uint16_t>(x, rows, d, codes, scale, stream);
-  return check_launch("quantize_rows");
+  return x_dtype == kF32 ? launch_quantize<float>(x, rows, d, codes, scale, stream)
+                         : launch_quantize<uint16_t>(x, rows, d, codes, scale, stream);
 }
 
 YGG_API int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows, const int32_t* gather, int P_max,
@@ -315,6 +322,16 @@ YGG_API int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_
                     !overlap(workspace, need, offsets, (size_t)E * index_bytes) &&
                     !overlap(workspace, need, counts, (size_t)E * index_bytes),
                 "ygg_int8_grouped_experts: the workspace must not share memory with x_sorted, y or the ranges");
+  // (y may be x_sorted, which is read before y is written; nothing else that the products read, nor the workspace)
+  const size_t up = (size_t)E * i8_expert_bytes(F, d), down = (size_t)E * i8_expert_bytes(d, F);
+  const struct {
+    const void* p;
+    size_t bytes;
+  } kept[] = {{w_up, up},     {s_up, (size_t)E * F * 4},   {b_up, (size_t)E * F * 32},
+              {w_down, down}, {s_down, (size_t)E * d * 4}, {b_down, (size_t)E * d * 32}};
+  for (const auto& k : kept)
+    YGG_CHECK_ARG(!overlap(workspace, need, k.p, k.bytes) && !overlap(y, yb, k.p, k.bytes),
+                  "ygg_int8_grouped_experts: y and the workspace must not share memory with the weights, scales or biases");
   int32_t* const bounds =
       reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + int8_experts_bytes((size_t)P, (size_t)P, d, F));
   return run_experts(x_sorted, P, nullptr, P, w_up, s_up, b_up, w_down, s_down, b_down, bounds, E, d, F, act, y, workspace,

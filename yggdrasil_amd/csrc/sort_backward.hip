@@ -9,6 +9,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "rows.h"
 #include "ygg_common.h"
 
@@ -103,16 +105,42 @@ __global__ __launch_bounds__(256) void dispatch_backward_kernel(const T* __restr
   }
 }
 
+// tokens of a launch: a grid holds fewer than 2^32 threads
+constexpr int kLaunchTokens = 1 << 22;
+
 template <typename TD, typename TY>
 int launch_combine(const void* dout, const void* y, int N, int k, int d, int P, const float* w, const int32_t* slots, void* dy,
                    int layout, float* dw, hipStream_t stream) {
-  const unsigned grid = (unsigned)(((long long)N + 3) / 4);
-  const TD* D = static_cast<const TD*>(dout);
   const TY* Y = static_cast<const TY*>(y);
   TY* O = static_cast<TY*>(dy);
-  if (layout == kDyPauli) combine_backward_kernel<TD, TY, kDyPauli><<<grid, 256, 0, stream>>>(D, Y, N, k, d, P, w, slots, O, dw);
-  else combine_backward_kernel<TD, TY, kDyBlade><<<grid, 256, 0, stream>>>(D, Y, N, k, d, P, w, slots, O, dw);
-  return check_launch("combine_backward");
+  for (size_t t0 = 0; t0 < (size_t)N; t0 += kLaunchTokens) {
+    const int n = (int)std::min<size_t>(N - t0, kLaunchTokens);
+    const unsigned grid = (unsigned)(n + 3) / 4;
+    const TD* const D = static_cast<const TD*>(dout) + t0 * d * 8;
+    const float* const W = w + t0 * k;
+    const int32_t* const S = slots + t0 * k;
+    float* const DW = dw ? dw + t0 * k : nullptr;
+    if (layout == kDyPauli) combine_backward_kernel<TD, TY, kDyPauli><<<grid, 256, 0, stream>>>(D, Y, n, k, d, P, W, S, O, DW);
+    else combine_backward_kernel<TD, TY, kDyBlade><<<grid, 256, 0, stream>>>(D, Y, n, k, d, P, W, S, O, DW);
+    if (check_launch("combine_backward")) return -1;
+  }
+  return 0;
+}
+
+// Workgroups no wider than the row's whole waves.
+template <typename T>
+int launch_dispatch(const void* dxs, int N, int k, int d, int P, const int32_t* slots, const void* add, void* dx,
+                    hipStream_t stream) {
+  const unsigned threads = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  for (size_t t0 = 0; t0 < (size_t)N; t0 += kLaunchTokens) {
+    const unsigned n = (unsigned)std::min<size_t>(N - t0, kLaunchTokens);
+    const size_t at = t0 * d * 8;
+    dispatch_backward_kernel<T><<<n, threads, 0, stream>>>(static_cast<const T*>(dxs), k, d, P, slots + t0 * k,
+                                                           add ? static_cast<const T*>(add) + at : nullptr,
+                                                           static_cast<T*>(dx) + at);
+    if (check_launch("dispatch_backward")) return -1;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -124,9 +152,7 @@ int combine_backward_bf16(const void* dout, const void* y, int N, int k, int d, 
 
 int dispatch_backward_bf16(const void* dxs, int N, int k, int d, const int32_t* slot_pos, const void* add, void* dx,
                            hipStream_t stream) {
-  dispatch_backward_kernel<uint16_t><<<(unsigned)N, d <= 64 ? 64 : d <= 128 ? 128 : 256, 0, stream>>>(
-      static_cast<const uint16_t*>(dxs), k, d, N * k, slot_pos, static_cast<const uint16_t*>(add), static_cast<uint16_t*>(dx));
-  return check_launch("dispatch_backward");
+  return launch_dispatch<uint16_t>(dxs, N, k, d, N * k, slot_pos, add, dx, stream);
 }
 
 }  // namespace ygg
@@ -171,12 +197,5 @@ YGG_API int ygg_dispatch_backward(const void* dx_sorted, int dtype, int N, int k
   YGG_CHECK_ARG(!overlap(dx, nb, dx_sorted, pb) && !overlap(dx, nb, slot_pos, (size_t)N * k * 4) &&
                     (dx == dx_add || !overlap(dx, nb, dx_add, nb)),
                 "ygg_dispatch_backward: dx must not share memory with dx_sorted, slot_pos or a part of dx_add");
-  const unsigned threads = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  if (dtype == kF32)
-    dispatch_backward_kernel<float><<<(unsigned)N, threads, 0, stream>>>(static_cast<const float*>(dx_sorted), k, d, P, slot_pos,
-                                                                         static_cast<const float*>(dx_add), static_cast<float*>(dx));
-  else
-    dispatch_backward_kernel<uint16_t><<<(unsigned)N, threads, 0, stream>>>(
-        static_cast<const uint16_t*>(dx_sorted), k, d, P, slot_pos, static_cast<const uint16_t*>(dx_add), static_cast<uint16_t*>(dx));
-  return check_launch("dispatch_backward");
+  return (dtype == kF32 ? launch_dispatch<float> : launch_dispatch<uint16_t>)(dx_sorted, N, k, d, P, slot_pos, dx_add, dx, stream);
 }

@@ -357,8 +357,8 @@ def combine_backward(dout: torch.Tensor, y_sorted: torch.Tensor | None, routing:
     routing weights need no gradient (then dtopk_w is None, ``rows`` is P, N k if not given, and ``out_dtype`` the
     type of dy, dout's if not given; else they are y_sorted's).  y_layout 'blade' returns dy as (P, d, 8), 'pauli' as the
     products' backward reads it: half-rows (P, 2, d, 4) for bfloat16, Pauli rows (P, d, 2, 2, 2) for float32.
-    dtopk_w (N, k) fp32.  A slot outside the P rows has a weight gradient of zero; rows that no slot names are not
-    written.
+    dtopk_w (N, k) fp32.  Every row is named by at most one slot, as routing leaves them (dy has one gradient a row); a
+    slot outside the P rows has a weight gradient of zero; rows that no slot names are not written.
     """
     dev = _one_device(dout, y_sorted)
     shape = dout.shape
@@ -711,7 +711,7 @@ def int8_grouped_linear(rows: Int8Rows, pw: PreparedWeights, offsets: torch.Tens
 
 def _int8_grouped_experts(dev, x, offsets, counts, w_up, w_down, b_up, b_down, act):
     E, d, F, P = w_up.E, w_up.d_in, w_up.d_out, x.shape[0]
-    _one_device(x, offsets, counts, b_up, b_down, w_up.data, w_down.data)
+    _one_device(x, w_up.data, w_down.data)
     if x.dtype != torch.bfloat16:
         raise ValueError("int8_rows experts take bf16 rows")
     for name, b, want in (("b_up", b_up, (E, F, 8)), ("b_down", b_down, (E, d, 8))):
@@ -719,7 +719,7 @@ def _int8_grouped_experts(dev, x, offsets, counts, w_up, w_down, b_up, b_down, a
             raise ValueError(f"{name} must be a prepared float32 bias {want}, got {b.dtype} {tuple(b.shape)}")
     if offsets.dtype != counts.dtype or offsets.dtype not in (torch.int32, torch.int64):
         offsets, counts = offsets.long(), counts.long()
-    x = _aligned(x)
+    x, b_up, b_down = _aligned(x), _aligned(b_up), _aligned(b_down)
     y = torch.empty_like(x)
     L = lib()
     need = L.ygg_int8_grouped_experts_workspace_bytes(P, E, d, F)
@@ -754,7 +754,7 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
     ``[0, P]``, so malformed ranges give wrong rows, never accesses past x_sorted or y.
     Returns y_sorted in x_sorted's shape and dtype.
     """
-    dev = _dev(x_sorted, expert_offsets, expert_counts, b_up, b_down)
+    dev = _one_device(x_sorted, expert_offsets, expert_counts, b_up, b_down)
     E, d, F = w_up.E, w_up.d_in, w_up.d_out
     if (w_down.E, w_down.d_in, w_down.d_out, w_down.fmt) != (E, F, d, w_up.fmt):
         raise ValueError("w_down must be (E, d, F) in w_up's format")
