@@ -24,7 +24,8 @@ __host__ __device__ inline size_t i8_expert_bytes(int d_out, int d_in) {
 }
 // The blades of an output multivector from the sums of its halved matrix (entry a b, re and im): sums and differences of
 // two of them, still whole numbers, then one rounding to fp32, the two scales' product and the bias in one multiply-add.
-// The same in every kernel, so a row's outputs do not depend on which takes its batch.
+// The same in every kernel, so a row's outputs do not depend on which takes its batch.  (A product of scales below
+// 2^-126, which takes rows or weights near their own lower limits, loses bits; one past fp32's largest is infinite.)
 __device__ __forceinline__ void i8_blades(int r00, int i00, int r01, int i01, int r10, int i10, int r11, int i11, float scale,
                                           const float (&bias)[8], float (&y)[8]) {
   const int t[8] = {r00 + r11, r10 + r01, i10 - i01, r00 - r11, i00 - i11, r10 - r01, i10 + i01, i00 + i11};

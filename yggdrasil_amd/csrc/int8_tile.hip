@@ -14,6 +14,12 @@
 // group before: the first group's during the last of the step before, so the one barrier of a step stands in front of
 // its last group, when the step's own operands are all in registers and its stage is free for the step after the next.
 // Persistent, one stream of steps over a workgroup's tiles: loads and reads run on through the epilogues.
+//
+// Bound: with few K steps a tile by the epilogue's vector work (8192 tokens, k = 4, E = 32, 128 -> 512, gelu: 96 us,
+// 1.43 POP/s; vector units 56 % of the cycles, matrix units 33 %), with many by the way of the operands through L2
+// and LDS (32768 rows, 512 -> 128: 80 us, 1.7 POP/s, 37 %; without its loads 62, without its products 78).  No faster:
+// loads two steps ahead; eight waves of 16 x 32 (102 -> 121, 74 -> 81); 64 x 128, one workgroup a CU, three stages
+// (102 -> 108, 75 -> 84).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
