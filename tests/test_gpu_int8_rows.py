@@ -211,6 +211,27 @@ def test_largest_codes_are_summed_exactly():
     _check(y, want, size, "none", False, "largest codes")
 
 
+@pytest.mark.parametrize("P", [5, 4000])
+def test_most_inputs_with_every_code_at_its_limit(P):
+    """16384 inputs, X = 1 + i and W = 1 - i in every entry of their matrices: each product of entries adds 2 127^2 to a sum,
+    and the scalar and e1 are the sum of two, 8 16384 127^2 < 2^31; Y = 4 16384 (1 + e1), or less that."""
+    ops = _ops()
+    d_in, d_out = 16384, 64
+    x = torch.zeros(P, d_in, 8, device="cuda", dtype=torch.bfloat16)
+    x[..., [0, 1, 6, 7]] = 1.0
+    x[1::2] *= -1
+    w = torch.zeros(1, d_out, d_in, 8, device="cuda")
+    w[..., [0, 1]], w[..., [6, 7]] = 1.0, -1.0
+    w[:, 2::3] *= -1
+    say(f"int8 product of {P} rows of 16384 inputs")
+    y = ops.int8_grouped_linear(ops.quantize_rows(x), ops.prepare_weights(w, "int8_rows"), _dev(_bounds([P])),
+                                out_dtype=torch.float32).cpu()
+    sign = torch.where(torch.arange(P) % 2 == 1, -1.0, 1.0)[:, None] * torch.where(torch.arange(d_out) % 3 == 2, -1.0, 1.0)
+    assert (y[..., 2:] == 0).all()
+    # two scales and their product, the sum's conversion and the multiply-add: half a step each
+    assert float((y[..., :2] / (sign[..., None] * 4 * d_in) - 1).abs().max()) <= 5 * U32
+
+
 def test_rows_that_are_not_finite_touch_no_other_row():
     ops = _ops()
     g = np.random.default_rng(8)
