@@ -248,6 +248,8 @@ int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows,
                             const void* w_prepared, const float* w_scale, const float* bias_prepared,
                             const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,
                             ygg_stream_t stream);
+/* Whether such a product runs on the kernel for few outputs; its outputs are the same bit for bit. */
+int ygg_int8_product_small(int P_max, int d_out);
 
 /* Every expert's CliffordFFN (hlm_block.py:55-61) on bf16 rows grouped by expert, both
  * products in int8: the rows quantized, the up product with bias and activation, its bf16

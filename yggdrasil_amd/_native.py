@@ -94,6 +94,7 @@ SIGNATURES = {
     "ygg_quantize_rows": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
     "ygg_int8_grouped_linear": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,
                                          _vp, _c_int, _vp]),
+    "ygg_int8_product_small": (_c_int, [_c_int, _c_int]),
     "ygg_expert_bounds": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "ygg_int8_grouped_experts_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int]),
     "ygg_int8_grouped_experts": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int,

@@ -289,6 +289,8 @@ YGG_API int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int
       codes, x_scale, x_rows, gather, P_max, w_prepared, w_scale, bias, offsets, E, d_in, d_out, act, y, y_dtype, stream);
 }
 
+YGG_API int ygg_int8_product_small(int P_max, int d_out) { return int8_small_pays(P_max, d_out); }
+
 YGG_API int ygg_expert_bounds(const void* offsets, const void* counts, int index_bytes, int E, int P, int32_t* bounds,
                               hipStream_t stream) {
   YGG_CHECK_ARG(E >= 1 && E <= 64 && P >= 0, "ygg_expert_bounds: bad sizes E=%d P=%d (E <= 64)", E, P);
