@@ -127,20 +127,28 @@ int ygg_route_energy(const void* x, int x_dtype, int N, int d, const float* rout
 
 /* ---- dispatch / combine ----------------------------------------------------
  * x_sorted[slot_pos[t, s]] = x[t]  (rows of d multivectors, dtype 0/1);
- * to_mask_order != 0 stores the rows in mask order.
+ * to_mask_order != 0 stores the rows in mask order.  x_sorted has N k rows, or P
+ * (ygg_dispatch_rows); a slot outside them is left out, a row that no slot names is
+ * not written.
  * Replaces expert_input = flat_x[token_ids] (hlm_block.py:178). */
 int ygg_dispatch(const void* x, int dtype, int N, int k, int d, const int32_t* slot_pos, void* x_sorted,
                  int to_mask_order, ygg_stream_t stream);
+int ygg_dispatch_rows(const void* x, int dtype, int N, int k, int d, int P, const int32_t* slot_pos, void* x_sorted,
+                      int to_mask_order, ygg_stream_t stream);
 
 /* out[t] = (residual[t] +) sum over the token's slots in ascending expert
  * order of topk_w[t, s] * y_sorted[slot_pos[t, s]], each product rounded
  * before its add.  y_mask_order != 0: y rows are in mask order (out is
- * always blade order).  residual may be NULL.
+ * always blade order).  residual may be NULL.  y_sorted has N k rows, or P
+ * (ygg_combine_rows); a slot outside them adds nothing.
  * Replaces weighted = w * y; np.add.at(output, token_ids, weighted)
  * (hlm_block.py:180-181) and the residual add x + ffn_out (hlm_block.py:151). */
 int ygg_combine(const void* y_sorted, int y_dtype, int y_mask_order, int N, int k, int d, const int32_t* topk_idx,
                 const float* topk_w, const int32_t* slot_pos, const void* residual, void* out, int out_dtype,
                 ygg_stream_t stream);
+int ygg_combine_rows(const void* y_sorted, int y_dtype, int y_mask_order, int N, int k, int d, int P,
+                     const int32_t* topk_idx, const float* topk_w, const int32_t* slot_pos, const void* residual,
+                     void* out, int out_dtype, ygg_stream_t stream);
 
 /* ---- grouped CliffordLinear expert products --------------------------------
  * Bytes of the prepared weights for E experts of a CliffordLinear d_in -> d_out. */

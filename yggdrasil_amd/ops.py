@@ -302,41 +302,6 @@ def route_energy(x: torch.Tensor, router_weight: torch.Tensor, router_bias: torc
     return r
 
 
-def dispatch(x: torch.Tensor, routing: Routing, mask_order: bool = False,
-             out: torch.Tensor | None = None) -> torch.Tensor:
-    """Expert-grouped copy of the token rows: ``out[slot_pos[t, s]] = x[t]``. x: (N, d, 8)."""
-    dev = _dev(x)
-    Nt, d = x.shape[0], x.shape[1]
-    k = routing.k
-    if out is None:
-        out = torch.empty((Nt * k, d, 8), device=dev, dtype=x.dtype)
-    elif tuple(out.shape) != (Nt * k, d, 8) or out.dtype != x.dtype:
-        raise ValueError("out must be (N*k, d, 8) of x's dtype")
-    check(lib().ygg_dispatch(ptr(x), _dtype_code(x), Nt, k, d, ptr(routing.slot_pos), ptr(out), int(mask_order),
-                             stream_handle(dev)), "dispatch")
-    return out
-
-
-def combine(y_sorted: torch.Tensor, routing: Routing, residual: torch.Tensor | None = None,
-            y_mask_order: bool = False, out_dtype: torch.dtype | None = None,
-            out: torch.Tensor | None = None) -> torch.Tensor:
-    """Weighted combine in ascending expert order (+ residual). y_sorted: (N*k, d, 8)."""
-    dev = _dev(y_sorted, residual)
-    Nt, k = routing.topk_idx.shape
-    d = y_sorted.shape[1]
-    out_dtype = out_dtype or y_sorted.dtype
-    if residual is not None and residual.dtype != out_dtype:
-        raise ValueError("residual dtype must equal the output dtype")
-    if out is None:
-        out = torch.empty((Nt, d, 8), device=dev, dtype=out_dtype)
-    elif tuple(out.shape) != (Nt, d, 8) or out.dtype != out_dtype:
-        raise ValueError("out must be (N, d, 8) of the output dtype")
-    check(lib().ygg_combine(ptr(y_sorted), _dtype_code(y_sorted), int(y_mask_order), Nt, k, d,
-                            ptr(routing.topk_idx), ptr(routing.topk_w), ptr(routing.slot_pos), ptr(residual),
-                            ptr(out), DTYPE_CODE[out_dtype], stream_handle(dev)), "combine")
-    return out
-
-
 def _check_routing(who: str, routing: Routing, at: int) -> tuple:
     """The slots of a caller's routing on device ``at``: ``(slot_pos, topk_w, (N, k))``."""
     slots, w = routing.slot_pos, routing.topk_w
@@ -346,6 +311,66 @@ def _check_routing(who: str, routing: Routing, at: int) -> tuple:
         raise ValueError(f"{who}: slot_pos must be contiguous int32 (N, k) and topk_w float32 of its shape, on device "
                          f"{at}; got {slots.dtype} {tuple(shape)} on {slots.device}, {w.dtype} {tuple(w.shape)} on {w.device}")
     return slots, w, shape
+
+
+def dispatch(x: torch.Tensor, routing: Routing, mask_order: bool = False,
+             out: torch.Tensor | None = None, rows: int | None = None) -> torch.Tensor:
+    """Expert-grouped copy of the token rows: ``out[slot_pos[t, s]] = x[t]``. x: (N, d, 8), out: (N k, d, 8).
+
+    A caller who drops slots (places them outside the rows: a full expert) or pads the experts' ranges gives ``rows``, the
+    rows of out: those that no slot names are zero.  Without it every row is named by a slot, as routing leaves them.
+    """
+    dev = _one_device(x, out)
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != 8:
+        raise ValueError(f"dispatch: x must be (N, d, 8), got {tuple(shape)}")
+    slots, _, (Nt, k) = _check_routing("dispatch", routing, dev.index)
+    d = shape[1]
+    if shape[0] != Nt:
+        raise ValueError(f"dispatch: {Nt} tokens' routing for {shape[0]} tokens")
+    P = Nt * k if rows is None else rows
+    if out is None:
+        out = (torch.empty if rows is None else torch.zeros)((P, d, 8), device=dev, dtype=x.dtype)
+    elif out.shape != (P, d, 8) or out.dtype != x.dtype:
+        raise ValueError("out must be (N*k, d, 8) of x's dtype" if rows is None else
+                         f"out must be ({P}, {d}, 8) of x's dtype")
+    elif rows is not None:
+        out.zero_()
+    check(lib().ygg_dispatch_rows(x.data_ptr(), _dtype_code(x), Nt, k, d, P, slots.data_ptr(), out.data_ptr(),
+                                  int(mask_order), stream_handle(dev)), "dispatch")
+    return out
+
+
+def combine(y_sorted: torch.Tensor, routing: Routing, residual: torch.Tensor | None = None,
+            y_mask_order: bool = False, out_dtype: torch.dtype | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Weighted combine in ascending expert order (+ residual). y_sorted: (P, d, 8), N k rows or a caller's; a slot outside
+    the P rows adds nothing."""
+    dev = _one_device(y_sorted, residual, out)
+    shape = y_sorted.shape
+    if len(shape) != 3 or shape[2] != 8:
+        raise ValueError(f"combine: y_sorted must be (P, d, 8), got {tuple(shape)}")
+    P, d, _ = shape
+    slots, w, shape = _check_routing("combine", routing, dev.index)
+    Nt, k = shape
+    idx = routing.topk_idx
+    if idx.dtype != torch.int32 or idx.shape != shape or idx.get_device() != dev.index or not idx.is_contiguous():
+        raise ValueError(f"combine: topk_idx must be contiguous int32 ({Nt}, {k}) on {dev}, got {idx.dtype} "
+                         f"{tuple(idx.shape)} on {idx.device}")
+    y_code = _dtype_code(y_sorted)
+    out_dtype = out_dtype or y_sorted.dtype
+    if out_dtype not in DTYPE_CODE:
+        raise ValueError(f"combine: out_dtype must be float32 or bfloat16, got {out_dtype}")
+    if residual is not None and (residual.dtype != out_dtype or residual.shape != (Nt, d, 8)):
+        raise ValueError(f"combine: residual must be ({Nt}, {d}, 8) of the output dtype")
+    if out is None:
+        out = torch.empty((Nt, d, 8), device=dev, dtype=out_dtype)
+    elif out.shape != (Nt, d, 8) or out.dtype != out_dtype:
+        raise ValueError("out must be (N, d, 8) of the output dtype")
+    check(lib().ygg_combine_rows(y_sorted.data_ptr(), y_code, int(y_mask_order), Nt, k, d, P,
+                                 idx.data_ptr(), w.data_ptr(), slots.data_ptr(), ptr(residual), out.data_ptr(),
+                                 DTYPE_CODE[out_dtype], stream_handle(dev)), "combine")
+    return out
 
 
 @_on_its_device
