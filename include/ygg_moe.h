@@ -474,10 +474,16 @@ int ygg_route_energy_backward(const void* x, int x_dtype, int N, int d, const fl
  * (dy_layout 0) or as the products' backward reads them (1: bf16 half-rows (P, 2, d, 4), fp32
  * Pauli rows (P, d, 2, 2, 2)); rows that no slot names are not written.  dtopk_w (N, k) =
  * <dout_t, y_sorted[slot]>, with y_sorted (P, d, 8) of dy_dtype; both NULL: not computed.
- * Outputs share no memory with inputs. */
+ * Outputs share no memory with inputs.  ygg_combine_backward_rows writes rows that no slot names
+ * too, zeros: the whole gradient for a caller who drops slots or pads the experts' ranges
+ * (workspace: none is needed where its size is 0). */
 int ygg_combine_backward(const void* dout, int dout_dtype, const void* y_sorted, int N, int k, int d, int P,
                          const float* topk_w, const int32_t* slot_pos, void* dy, int dy_dtype, int dy_layout,
                          float* dtopk_w, ygg_stream_t stream);
+int ygg_combine_backward_rows(const void* dout, int dout_dtype, const void* y_sorted, int N, int k, int d, int P,
+                              const float* topk_w, const int32_t* slot_pos, void* dy, int dy_dtype, int dy_layout,
+                              float* dtopk_w, void* workspace, size_t workspace_bytes, ygg_stream_t stream);
+size_t ygg_combine_backward_rows_workspace_bytes(int N, int k, int P);
 /* dx_t (N, d, 8) = dx_add_t (or zero) + sum over the slots, in slot order, of dx_sorted[slot];
  * dx_sorted (P, d, 8), dx_add (which dx may be) and dx of one dtype, summed in fp32. */
 int ygg_dispatch_backward(const void* dx_sorted, int dtype, int N, int k, int d, int P, const int32_t* slot_pos,

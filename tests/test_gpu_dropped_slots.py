@@ -100,6 +100,112 @@ def test_dispatch(N, d, E, k, P, dt, mask):
     assert torch.equal(out[low[low >= 0].long()], x[torch.arange(N, device="cuda")[:, None].expand(N, k)[low >= 0]])
 
 
+@pytest.mark.parametrize("N,d,E,k,P", SIZES + [(0, 6, 4, 2, 90), (3000, 3, 16, 2, 9000), (5, 4, 4, 2, 0),
+                                               (9000, 3, 16, 4, 32000)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["blade", "pauli"])
+@pytest.mark.parametrize("with_y", [False, True])
+def test_combine_backward(N, d, E, k, P, dt, layout, with_y):
+    """Rows that no slot names have the gradient zero whatever the memory held, the others that of the entry that leaves
+    the rest unwritten."""
+    ops = _ops()
+    r, on = _dropped(N + d, N, E, k, P) if N else (ops.route(torch.empty(0, E, device="cuda"), k), None)
+    dout, y = torch.randn(N, d, 8, device="cuda").to(dt), torch.randn(P, d, 8, device="cuda").to(dt)
+    say(f"combine_backward with dropped slots N={N} d={d} k={k} P={P} {dt} {layout} y={with_y}")
+    shape = (P, d, 8) if layout == "blade" else (P, 2, d, 4) if dt == torch.bfloat16 else (P, d, 2, 2, 2)
+    want, dw = torch.zeros(shape, device="cuda", dtype=dt), torch.full((N, k), 5.0, device="cuda")
+    args = (dout.data_ptr(), ops.DTYPE_CODE[dt], y.data_ptr(), N, k, d, P, r.topk_w.data_ptr(), r.slot_pos.data_ptr())
+    if N and P:
+        ops.check(ops.lib().ygg_combine_backward(*args, want.data_ptr(), ops.DTYPE_CODE[dt], layout == "pauli", dw.data_ptr(),
+                                                 ops.stream_handle()))
+        named = torch.zeros(P, dtype=torch.bool, device="cuda")
+        named[r.slot_pos[on].long()] = True
+        assert (want[~named] == 0).all() and not (want[named].flatten(1) == 0).all(1).any()
+    need = ops.lib().ygg_combine_backward_rows_workspace_bytes(N, k, P)
+    assert need == (4 * P if N == 9000 else 0)  # (both ways to find the rows that no slot names)
+    for fill in (0, 1):  # scratch and rows as an allocator may leave them: the scratch names a token of every row
+        dirty = torch.full(shape, float("nan"), device="cuda", dtype=dt)
+        tokens = torch.arange(P, device="cuda", dtype=torch.int32) * fill
+        ops.check(ops.lib().ygg_combine_backward_rows(*args[:2], y.data_ptr() if with_y else None, *args[3:], dirty.data_ptr(),
+                                                      ops.DTYPE_CODE[dt], layout == "pauli", dw.data_ptr() if with_y else None,
+                                                      tokens.data_ptr(), need, ops.stream_handle()))
+        assert torch.equal(dirty, want)
+    dy, dw2 = ops.combine_backward(dout, y if with_y else None, r, y_layout=layout, rows=P)
+    assert torch.equal(dy, want) and (dw2 is None if not with_y else not N or not P or torch.equal(dw2, dw))
+
+
+def test_combine_backward_captured():
+    ops = _ops()
+    N, d, E, k, P = 300, 24, 8, 2, 700
+    r, _ = _dropped(5, N, E, k, P)
+    dout, y = torch.randn(N, d, 8, device="cuda"), torch.randn(P, d, 8, device="cuda")
+    say("combine_backward with dropped slots captured")
+    ops.combine_backward(dout, y, r)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.combine_backward(dout, y, r)
+    for n in range(4):
+        r.slot_pos.copy_(r.slot_pos.flip(0))  # other rows are named
+        want = ops.combine_backward(dout, y, r)
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), f"replay {n}"
+
+
+def test_chain_with_full_and_padded_experts():
+    """Experts of a fixed capacity: their ranges padded, the tokens past it dropped.  The operators from tokens to output and
+    back, against float64 autograd; the chain's rows are bf16, so each of its five roundings is 2^-8 of the largest value
+    that it meets."""
+    ops = _ops()
+    N, d, F, E, k, C = 200, 32, 48, 8, 2, 56
+    P = E * C
+    torch.manual_seed(7)
+    full = ops.route(torch.randn(N, E, device="cuda") + torch.linspace(1, -1, E, device="cuda"), k)
+    owner = torch.repeat_interleave(torch.arange(E, device="cuda"), full.counts.long())
+    at = full.slot_pos.long()
+    e, place = owner[at], at - full.offsets.long()[owner[at]]
+    on = place < C
+    assert not on.all() and int(full.counts.min()) < C
+    slots = torch.where(on, e * C + place, -1).to(torch.int32)
+    offsets = torch.arange(0, P + 1, C, device="cuda", dtype=torch.int32)
+    r = ops.Routing(full.topk_idx, full.topk_w, full.counts, offsets, full.perm, slots)
+    x = torch.randn(N, d, 8, device="cuda").bfloat16()
+    w = torch.randn(E, F, d, 8, device="cuda") / (8 * d) ** 0.5
+    dout = torch.randn(N, F, 8, device="cuda").bfloat16()
+    say("chain with full and padded experts")
+    junk = torch.full((64 << 20,), float("nan"), device="cuda")  # what the next allocations find
+    del junk
+    xs = ops.dispatch(x, r, rows=P)
+    y = ops.pauli_grouped_linear(xs, ops.prepare_weights(w, "pauli"), offsets)
+    out = ops.combine(y, r)
+    dy, dw = ops.combine_backward(dout, y, r, y_layout="pauli")
+    dxs = ops.pauli_grouped_input_grad(dy, ops.prepare_adjoint_weights(w, "pauli"), offsets)
+    dx = ops.dispatch_backward(dxs, r)
+    gw, _ = ops.grouped_weight_grad_pauli(dy, ops.pauli_rows_from_blade(xs), offsets, E)
+    import numpy as np
+    from oracle import cl3
+
+    table = torch.zeros(8, 8, 8, dtype=torch.float64, device="cuda")
+    for p in range(8):
+        for q in range(8):
+            a, b = np.zeros((1, 8)), np.zeros((1, 8))
+            a[0, p] = b[0, q] = 1
+            table[p, q] = torch.from_numpy(np.asarray(cl3.geom_prod(a, b))[0]).cuda()
+    X, W = x.double().requires_grad_(True), w.double().requires_grad_(True)
+    tw = r.topk_w.double().requires_grad_(True)
+    total = torch.zeros(N, F, 8, dtype=torch.float64, device="cuda")
+    for n in range(E):
+        dense = torch.einsum("jip,pqs->iqjs", W[n], table).reshape(d * 8, F * 8)
+        tok, slot = torch.nonzero(on & (full.topk_idx == n), as_tuple=True)
+        total = total.index_add(0, tok, tw[tok, slot][:, None, None] * (X[tok].reshape(-1, d * 8) @ dense).reshape(-1, F, 8))
+    gx, gW, gt = torch.autograd.grad(total, (X, W, tw), dout.double())
+    for name, got, want in (("out", out, total), ("dx", dx, gx), ("dw", dw, gt), ("dW", gw, gW)):
+        err = float((got.double() - want.detach()).abs().max() / want.detach().abs().max())
+        assert err <= 5 * 2.0 ** -8, (name, err)
+
+
 def test_refusals():
     ops = _ops()
     r, _ = _dropped(2, 30, 4, 2, 60)

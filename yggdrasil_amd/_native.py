@@ -103,6 +103,9 @@ SIGNATURES = {
                                           _c_int, _vp, _vp, _c_size, _vp]),
     "ygg_combine_backward": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp,
                                       _vp]),
+    "ygg_combine_backward_rows": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int,
+                                           _vp, _vp, _c_size, _vp]),
+    "ygg_combine_backward_rows_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "ygg_dispatch_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "ygg_grade_quantize": (_c_int, [_vp, _c_int, _c_size, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),
     "ygg_clifford_layer_norm": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_double, _vp, _c_int, _vp]),

@@ -383,7 +383,7 @@ def combine_backward(dout: torch.Tensor, y_sorted: torch.Tensor | None, routing:
     type of dy, dout's if not given; else they are y_sorted's).  y_layout 'blade' returns dy as (P, d, 8), 'pauli' as the
     products' backward reads it: half-rows (P, 2, d, 4) for bfloat16, Pauli rows (P, d, 2, 2, 2) for float32.
     dtopk_w (N, k) fp32.  Every row is named by at most one slot, as routing leaves them (dy has one gradient a row); a
-    slot outside the P rows has a weight gradient of zero; rows that no slot names are not written.
+    slot outside the P rows has a weight gradient of zero, and so has dy in rows that no slot names.
     """
     dev = _one_device(dout, y_sorted)
     shape = dout.shape
@@ -411,9 +411,12 @@ def combine_backward(dout: torch.Tensor, y_sorted: torch.Tensor | None, routing:
     else:
         raise ValueError("y_layout must be 'blade' or 'pauli'")
     dtw = torch.empty_like(w) if y_sorted is not None else None
-    check(lib().ygg_combine_backward(dout.data_ptr(), _dtype_code(dout), ptr(y_sorted), Nt, k, d, P, w.data_ptr(),
-                                     slots.data_ptr(), dy.data_ptr(), _dtype_code(dy), y_layout == "pauli", ptr(dtw),
-                                     stream_handle(dev)), "combine_backward")
+    L = lib()
+    need = L.ygg_combine_backward_rows_workspace_bytes(Nt, k, P)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    check(L.ygg_combine_backward_rows(dout.data_ptr(), _dtype_code(dout), ptr(y_sorted), Nt, k, d, P, w.data_ptr(),
+                                      slots.data_ptr(), dy.data_ptr(), _dtype_code(dy), y_layout == "pauli", ptr(dtw),
+                                      ptr(ws), need, stream_handle(dev)), "combine_backward")
     return dy, dtw
 
 
