@@ -162,7 +162,8 @@ size_t ygg_prepared_weight_bytes(int E, int d_out, int d_in, int format);
  * Format 5 applies the same conventions to the eight real entries of each
  * weight's 2x2 complex matrix, M00 = (s + v3) + i (t + b12), M01 = (v1 - b13) +
  * i (b23 - v2), M10 = (v1 + b13) + i (b23 + v2), M11 = (s - v3) + i (t - b12),
- * in float64; format 6 is the same codes in the same layout. */
+ * in float64; format 6 is the same codes in the same layout.  Formats 5 and 6: a channel with an
+ * infinity or a NaN among its weights has the scale NaN and the codes 0, and its outputs are NaN. */
 int ygg_prepare_weights(const float* W, int E, int d_out, int d_in, int format, void* out, float* scales,
                         ygg_stream_t stream);
 

@@ -94,7 +94,8 @@ __device__ inline void dp_pauli_f64(const float* w, double (&p)[8]) {
   p[7] = t - b12;   // V11
 }
 
-// scale of (expert, channel) blockIdx.x: max(|entries|, 1e-12) / 127 in float64, rounded to fp32
+// scale of (expert, channel) blockIdx.x: max(|entries|, 1e-12) / 127 in float64, rounded to fp32; NaN where a weight is
+// infinite or NaN, so that the channel's outputs are NaN (its codes are 0)
 __global__ __launch_bounds__(256) void dp_scale_kernel(const float* __restrict__ W, int d_in,
                                                        float* __restrict__ scales) {
   __shared__ double red[256];
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256) void dp_scale_kernel(const float* __restrict__
     double p[8];
     dp_pauli_f64(w, p);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) m = fmax(m, fabs(p[q]));
+    for (int q = 0; q < 8; ++q) m = fmax(m, p[q] == p[q] ? fabs(p[q]) : __builtin_inf());  // (sums of two floats: finite or not)
   }
   red[threadIdx.x] = m;
   __syncthreads();
@@ -115,7 +116,8 @@ __global__ __launch_bounds__(256) void dp_scale_kernel(const float* __restrict__
     if (threadIdx.x < s) red[threadIdx.x] = fmax(red[threadIdx.x], red[threadIdx.x + s]);
     __syncthreads();
   }
-  if (threadIdx.x == 0) scales[blockIdx.x] = (float)(fmax(red[0], 1e-12) / 127.0);
+  if (threadIdx.x == 0)
+    scales[blockIdx.x] = red[0] < __builtin_inf() ? (float)(fmax(red[0], 1e-12) / 127.0) : __builtin_nanf("");
 }
 
 // one thread per 16-byte unit (expert, jb, ks, U/V, g, n) of the layout
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(256) void dp_prep_kernel(const float* __restrict__ 
   const int e = (int)(rest / JB);
   const int j = jb * 8 + (n >> 1), a = n & 1;
   uint32_t word[4] = {0u, 0u, 0u, 0u};
-  if (j < d_out) {
+  if (j < d_out && scales[(size_t)e * d_out + j] == scales[(size_t)e * d_out + j]) {
     const double s = (double)scales[(size_t)e * d_out + j];
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
@@ -520,9 +522,9 @@ __global__ __launch_bounds__(kDpThreads) void decode_pauli_kernel(
       for (int q = 0; q < 4; ++q) {
         hc0[q] = ok ? hc0[q] : 0.f;
         hc1[q] = ok ? hc1[q] : 0.f;
-        m = fmaxf(m, fmaxf(fabsf(hc0[q]), fabsf(hc1[q])));
+        m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(fabsf(hc0[q]), fabsf(hc1[q])));  // (keeps NaN)
       }
-      m = dc_row_max(m);  // over the token's 8 channels x 2 rows in this wave
+      m = dc_row_max(dc_mag(m));  // over the token's 8 channels x 2 rows in this wave
       if (n == 0) s_hmax[rb][wave][g] = m;
       __syncthreads();
       float mx = 0.f;
@@ -530,8 +532,8 @@ __global__ __launch_bounds__(kDpThreads) void decode_pauli_kernel(
       for (int w = 0; w < kDpWaves; ++w) mx = fmaxf(mx, s_hmax[rb][w][g]);
       const int sh = dc_shift(mx);
       const float hs = ldexpf(1.0f, sh);
-      // a hidden row is non-finite through an infinite entry (its maximum) or through a
-      // non-finite input row (NaN inverse scale: its hidden row is NaN)
+      // a hidden row is non-finite through an entry of its own (its maximum: a channel's scale or bias
+      // may be NaN) or through a non-finite input row (NaN inverse scale: its hidden row is NaN)
       if (wave == 0 && n == 0) {
         const float xinv = s_xinv[tk];
         s_hinv[tk] = xinv == xinv ? dc_inv_scale(mx, sh) : xinv;
