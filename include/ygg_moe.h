@@ -31,7 +31,8 @@
  *    4 = fp32 Pauli (fp32 layers; ygg_f32_layer_split says on which MFMA units),
  *    5 = int8 Pauli (the entries of each weight's 2x2 complex matrix, int8 per
  *        output channel; bf16 decode layers of at most 128 tokens, d <= 128),
- *    6 = the weights of 5, met by rows in int8 (bf16 layers of any size).
+ *    6 = the weights of 5, met by rows in int8 (bf16 layers with d and F up to 16384 and
+ *        fewer than 2 GiB of x's rows in int8: 8 N d bytes, d rounded up to 32).
  *    activation codes: 0 none, 1 gelu, 2 relu, 3 sigmoid
  *    (holograph/models/hlm_block.py:28-32).
  */
@@ -252,7 +253,8 @@ int ygg_quantize_rows(const void* x, int x_dtype, int rows, int d, void* codes, 
  * the sums in 32-bit integers, exact, and the rest in fp32; y (P_max, d_out, 8) of y_dtype,
  * blade order.  codes, x_scale: ygg_quantize_rows of x_rows rows (x_rows >= P_max without
  * gather; a gather[r] outside [0, x_rows) stands for a row of zeros); w_prepared, w_scale: format 5 or 6;
- * bias: prepared (mask order) or NULL.  E <= 64, d_in <= 16384. */
+ * bias: prepared (mask order) or NULL.  E <= 64, d_in <= 16384, d_out <= 524288, an expert's weights
+ * below 2 GiB, and so gathered codes. */
 int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int x_rows, const int32_t* gather, int P_max,
                             const void* w_prepared, const float* w_scale, const float* bias_prepared,
                             const int32_t* offsets, int E, int d_in, int d_out, int act, void* y, int y_dtype,

@@ -95,3 +95,24 @@ def test_bits_of_finite_weights():
     q, s = moe.quantize_int8_pauli(w)
     assert np.array_equal(ops.prepare_weights(torch.from_numpy(w).cuda(), "int8_rows").scales.cpu().numpy().ravel(),
                           np.asarray(s).ravel())
+
+
+def test_more_channels_than_one_launch_prepares():
+    """The most channels a product takes, of 33 experts: 2^24 and more in all.  Every expert as it is prepared alone."""
+    ops = _ops()
+    E, d_out = 33, 524288
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    w = torch.randn(E, d_out, 1, 8, generator=g, device="cuda")
+    say(f"prepare {E * d_out} channels")
+    pw = ops.prepare_weights(w, "int8_rows")
+    data, scales = pw.data.view(E, -1), pw.scales.view(E, d_out)
+    x = torch.randn(3, 1, 8, device="cuda").bfloat16()
+    rows = ops.quantize_rows(x)
+    for e in (0, 1, 15, 31, 32):
+        one = ops.prepare_weights(w[e:e + 1].contiguous(), "int8_rows")
+        assert torch.equal(scales[e], one.scales.view(-1)) and torch.equal(data[e], one.data.view(-1)), e
+        bounds = torch.zeros(E + 1, device="cuda", dtype=torch.int32)
+        bounds[e + 1:] = 3
+        alone = torch.tensor([0, 3], device="cuda", dtype=torch.int32)
+        assert torch.equal(ops.int8_grouped_linear(rows, pw, bounds), ops.int8_grouped_linear(rows, one, alone)), e

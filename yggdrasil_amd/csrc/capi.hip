@@ -125,8 +125,8 @@ static int layer_size_check(const char* who, int N, int d, int F, int E, int k, 
     }
   }
   if (w_format == kWI8Rows && N > 0) {
-    const char* why = int8_linear_limit(N, /*gathered*/ true, E, d, F);
-    if (!why) why = int8_linear_limit(N * k, false, E, F, d);
+    const char* why = int8_linear_limit(N, /*gathered*/ true, d, F);
+    if (!why) why = int8_linear_limit(N * k, false, F, d);
     YGG_CHECK_ARG(!why, "%s: %s (N=%d d=%d F=%d E=%d k=%d)", who, why, N, d, F, E, k);
   }
   return 0;

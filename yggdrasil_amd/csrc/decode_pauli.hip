@@ -47,6 +47,8 @@
 // planes are added by the consumer in chunk order), so results do not depend
 // on scheduling.
 
+#include <algorithm>
+
 #include "decode_common.h"
 #include "pauli_common.h"
 #include "route_select.h"
@@ -120,12 +122,13 @@ __global__ __launch_bounds__(256) void dp_scale_kernel(const float* __restrict__
     scales[blockIdx.x] = red[0] < __builtin_inf() ? (float)(fmax(red[0], 1e-12) / 127.0) : __builtin_nanf("");
 }
 
-// one thread per 16-byte unit (expert, jb, ks, U/V, g, n) of the layout
+// one thread per 16-byte unit (expert, jb, ks, U/V, g, n) of the layout, from unit `first` on
 __global__ __launch_bounds__(256) void dp_prep_kernel(const float* __restrict__ W, int E, int d_out, int d_in,
-                                                      const float* __restrict__ scales, uint4* __restrict__ out) {
+                                                      const float* __restrict__ scales, uint4* __restrict__ out,
+                                                      size_t first) {
   const int JB = (d_out + 7) / 8, KS = (d_in + 31) / 32;
   const size_t total = (size_t)E * JB * KS * 128;
-  const size_t u = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t u = first + (size_t)blockIdx.x * 256 + threadIdx.x;
   if (u >= total) return;
   const int n = (int)(u & 15), g = (int)((u >> 4) & 3), uv = (int)((u >> 6) & 1);
   size_t rest = u >> 7;
@@ -611,12 +614,19 @@ int ygg::decode_pauli_prepare_weights(const float* W, int E, int d_out, int d_in
   YGG_CHECK_ARG(decode_pauli_weight_bytes(1, d_out, d_in) < 0x7fffffffULL,
                 "ygg_prepare_weights: one expert's int8 Pauli weights must stay below 2 GiB (d_out=%d d_in=%d)",
                 d_out, d_in);
-  dp_scale_kernel<<<E * d_out, 256, 0, stream>>>(W, d_in, scales);
-  if (check_launch("dp_scale")) return -1;
-  const size_t units = decode_pauli_weight_bytes(E, d_out, d_in) / 16;
-  dp_prep_kernel<<<(unsigned)((units + 255) / 256), 256, 0, stream>>>(W, E, d_out, d_in, scales,
-                                                                      static_cast<uint4*>(out));
-  return check_launch("dp_prep");
+  // (a launch holds fewer than 2^32 threads)
+  constexpr size_t kGroups = 1 << 20;
+  const size_t channels = (size_t)E * d_out, units = decode_pauli_weight_bytes(E, d_out, d_in) / 16;
+  for (size_t c = 0; c < channels; c += kGroups) {
+    dp_scale_kernel<<<(unsigned)std::min(channels - c, kGroups), 256, 0, stream>>>(W + c * d_in * 8, d_in, scales + c);
+    if (check_launch("dp_scale")) return -1;
+  }
+  for (size_t u = 0; u < units; u += kGroups * 256) {
+    const size_t n = std::min(units - u, kGroups * 256);
+    dp_prep_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(W, E, d_out, d_in, scales, static_cast<uint4*>(out), u);
+    if (check_launch("dp_prep")) return -1;
+  }
+  return 0;
 }
 
 bool ygg::decode_pauli_fusable(int N, int E, int k, int d, int F) {

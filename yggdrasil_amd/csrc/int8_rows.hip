@@ -239,7 +239,7 @@ int int8_experts(const void* x, int x_rows, const int32_t* gather, int P, const 
 
 size_t int8_rows_bytes(size_t rows, int d) { return rows * i8_row_bytes(d); }
 
-const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out) {
+const char* int8_linear_limit(int x_rows, bool gathered, int d_in, int d_out) {
   if (d_in > kI8MaxInputs) return "int8 products sum at most 16384 inputs in 32 bits";
   if (d_out > 1 << 19) return "int8 products write at most 524288 channels";
   if (i8_expert_bytes(d_out, d_in) >= 0x7fffffffull) return "one expert's int8 weights exceed 2 GiB";
@@ -274,7 +274,7 @@ YGG_API int ygg_int8_grouped_linear(const void* codes, const float* x_scale, int
                 P_max, E, d_in, d_out, kI8MaxInputs);
   YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_int8_grouped_linear: activation %d", act);
   YGG_CHECK_ARG(y_dtype == kF32 || y_dtype == kBF16, "ygg_int8_grouped_linear: output dtype %d unsupported", y_dtype);
-  const char* const why = int8_linear_limit(x_rows, gather != nullptr, E, d_in, d_out);
+  const char* const why = int8_linear_limit(x_rows, gather != nullptr, d_in, d_out);
   YGG_CHECK_ARG(!why, "ygg_int8_grouped_linear: %s (x_rows=%d E=%d d_in=%d d_out=%d)", why, x_rows, E, d_in, d_out);
   if (P_max == 0) return 0;
   YGG_CHECK_ARG(codes && x_scale && w_prepared && w_scale && offsets && y, "ygg_int8_grouped_linear: null pointer");
@@ -312,8 +312,8 @@ YGG_API int ygg_int8_grouped_experts(const void* x_sorted, int P, const void* w_
                 P, E, d, F);
   YGG_CHECK_ARG(act >= kActNone && act <= kActSigmoid, "ygg_int8_grouped_experts: activation %d", act);
   YGG_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "ygg_int8_grouped_experts: indexes of %d bytes", index_bytes);
-  const char* why = int8_linear_limit(P, false, E, d, F);
-  if (!why) why = int8_linear_limit(P, false, E, F, d);
+  const char* why = int8_linear_limit(P, false, d, F);
+  if (!why) why = int8_linear_limit(P, false, F, d);
   YGG_CHECK_ARG(!why, "ygg_int8_grouped_experts: %s (P=%d E=%d d=%d F=%d)", why, P, E, d, F);
   if (P == 0) return 0;
   YGG_CHECK_ARG(x_sorted && w_up && s_up && w_down && s_down && offsets && counts && y && workspace,

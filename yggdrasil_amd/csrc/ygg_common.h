@@ -265,7 +265,7 @@ int int8_small_linear(const void* x, const float* xs, int x_rows, const int32_t*
                       const float* ws, const float* bias, const int32_t* offsets, int E, int d_in, int d_out, int act,
                       void* y, int y_dtype, hipStream_t stream);
 bool int8_small_pays(int P, int d_out);
-const char* int8_linear_limit(int x_rows, bool gathered, int E, int d_in, int d_out);
+const char* int8_linear_limit(int x_rows, bool gathered, int d_in, int d_out);
 
 // combine of fp32 blade-order partial planes (dispatch.hip): the planes of a
 // row are added in plane order, then weighted and combined as ygg_combine does.

@@ -47,8 +47,9 @@ class MoEHLMConfig:
                 even), 'bf16' (8x8 L(w) blocks), 'int8' (per-output-channel int8, L(w) blocks) or
                 'int8_pauli' (per-output-channel int8 of the complex 2x2 weights: the one-launch
                 decode layer, batches of at most 128 tokens with d_model <= 128) or 'int8_rows' (the same
-                weights, for any batch and width: the rows of both products are quantized to int8 too, with a
-                scale each; forward only)
+                weights, for batches and widths of any size up to d_model and d_ff of 16384 and 2 GiB of
+                x's rows in int8 (8 bytes a multivector): the rows of both products are quantized to int8
+                too, with a scale each; forward only)
     router      'energy' -- CliffordRouter's grade-energy logits (default, the reference);
                 'clifford_head' -- CliffordLinear(d -> E) then the scalar part;
                 'logits' -- the caller passes logits to forward()
