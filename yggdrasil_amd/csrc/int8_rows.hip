@@ -13,7 +13,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "int8_rows.h"
 #include "rows.h"
@@ -69,11 +68,12 @@ struct Ranges {
 };
 template <typename I>
 __device__ __forceinline__ void write_bounds(const Ranges& r) {
-  typedef typename std::make_unsigned<I>::type U;  // (sums may wrap)
   const int lane = threadIdx.x & 63;
-  const I at = lane < r.E ? static_cast<const I*>(r.offsets)[lane] : 0;
-  const I end = lane < r.E ? (I)((U)at + (U) static_cast<const I*>(r.counts)[lane]) : 0;
-  auto clip = [&](I v) { return min(max((int32_t)v, 0), r.P); };
+  const long long at = lane < r.E ? static_cast<const I*>(r.offsets)[lane] : 0;
+  const long long count = lane < r.E ? static_cast<const I*>(r.counts)[lane] : 0;
+  long long end;  // (a sum past 64 bits has the sign of its terms)
+  if (__builtin_add_overflow(at, count, &end)) end = at < 0 ? at : r.P;
+  auto clip = [&](long long v) { return (int)min(max(v, 0LL), (long long)r.P); };
   int v = lane < r.E ? clip(at) : 0;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {

@@ -810,8 +810,9 @@ def grouped_experts(x_sorted: torch.Tensor, expert_offsets: torch.Tensor, expert
         check(lib().ygg_expert_bounds(ptr(expert_offsets), ptr(expert_counts), expert_offsets.element_size(), E, P,
                                       ptr(offs), stream_handle(dev)), "grouped_experts")
     else:
-        offs = torch.cat([expert_offsets.reshape(E), (expert_offsets[-1:] + expert_counts[-1:])]).to(torch.int32)
-        offs = torch.cummax(offs.clamp(0, P), 0).values.to(torch.int32).contiguous()
+        at = expert_offsets.long()
+        offs = torch.cat([at, at[-1:] + expert_counts[-1:].long()]).clamp(0, P)
+        offs = torch.cummax(offs, 0).values.to(torch.int32)
     if fmt == "int8_pauli":
         raise ValueError("int8_pauli weights run inside the decode layer (moe_forward), which routes its own "
                          "rows; use 'int8' or 'int8_rows' for grouped experts")
