@@ -27,6 +27,8 @@ CASES = [
     ([5] * 64, 66, 640, True, True),
     ([300, 0, 500], 33, 257, False, True),
     ([3200], 5, 65, True, False),
+    ([13000], 40, 1, True, True),
+    ([9000, 5000, 33], 20, 4, False, True),
 ]
 
 

@@ -157,11 +157,15 @@ int launch_small(const void* x, const float* xs, int x_rows, const int32_t* gath
 
 }  // namespace
 
-// Few outputs: the tiles, 64 x 64, leave most of the chip idle (a product, few rows / tiles, us: 8 rows, E = 32, 128 -> 512:
-// 4.1 / 8.6; 32, E = 64, 256 -> 1024: 12.7 / 16.9, 1024 -> 256: 13.6 / 26.1; 512, E = 8, 256 -> 64: 5.3 / 9.9; 1024, E = 32,
-// 512 -> 128: 13.1 / 15.9, 128 -> 512: 15.8 / 11.5; 2048, E = 8, 256 -> 64: 7.8 / 10.1, 64 -> 256: 11.8 / 8.8; 300, E = 4,
-// 256 -> 1024: 12.9 / 12.0; 2048, E = 32, 512 -> 128: 19.9 / 16.4).
-bool int8_small_pays(int P, int d_out) { return (long long)P * d_out <= 200000; }
+// Few outputs, counted as this kernel computes them (channels in groups of 16): the tiles, 64 x 64, leave most of the chip
+// idle.  A product, few rows / tiles, us: 8 rows, E = 32, 128 -> 512: 4.1 / 8.6; 32, E = 64, 256 -> 1024: 12.7 / 16.9,
+// 1024 -> 256: 13.6 / 26.1; 512, E = 8, 256 -> 64: 5.3 / 9.9; 1024, E = 32, 512 -> 128: 13.1 / 15.9, 128 -> 512: 15.8 / 11.5;
+// 2048, E = 8, 256 -> 64: 7.8 / 10.1, 64 -> 256: 11.8 / 8.8; 300, E = 4, 256 -> 1024: 12.9 / 12.0; 2048, E = 32, 512 -> 128:
+// 19.9 / 16.4.  One expert, where rows are most: 3125 rows, 512 -> 64: 15.0 / 18.0, 6250: 25.7 / 19.0.  Narrow outputs (the
+// call's host time hides what is below 8): 12500 rows to 1, 4 or 16 channels of 512 inputs 14.6 to 15 / 19; 25000 rows,
+// 32 inputs 8.8 to 9.5 / 8.3, 128: 10.5 / 11.2, 512: 25 / 27; 100000 rows to 1 or 4 channels, 32 inputs 24 / 16.4, 128: 29.7 / 28.7,
+// 512: 92 to 96 / 92 to 93.
+bool int8_small_pays(int P, int d_out) { return (long long)P * ((d_out + 15LL) / 16 * 16) <= 200000; }
 
 int int8_small_linear(const void* x, const float* xs, int x_rows, const int32_t* gather, int P, const void* w,
                       const float* ws, const float* bias, const int32_t* offsets, int E, int d_in, int d_out, int act,

@@ -15,11 +15,12 @@
 // its last group, when the step's own operands are all in registers and its stage is free for the step after the next.
 // Persistent, one stream of steps over a workgroup's tiles: loads and reads run on through the epilogues.
 //
-// Bound: with few K steps a tile by the epilogue's vector work (8192 tokens, k = 4, E = 32, 128 -> 512, gelu: 96 us,
-// 1.43 POP/s; vector units 56 % of the cycles, matrix units 33 %), with many by the way of the operands through L2
-// and LDS (32768 rows, 512 -> 128: 80 us, 1.7 POP/s, 37 %; without its loads 62, without its products 78).  No faster:
-// loads two steps ahead; eight waves of 16 x 32 (102 -> 121, 74 -> 81); 64 x 128, one workgroup a CU, three stages
-// (102 -> 108, 75 -> 84).
+// Bound: with few K steps a tile by the epilogue's vector work (8192 tokens, k = 4, E = 32, 128 -> 512, gelu: 98 us,
+// 1.40 POP/s; vector units 56 % of the cycles, matrix units 33 %), with many by the way of the operands through L2
+// and LDS (32768 rows, 512 -> 128: 70 us with its codes in the caches, 82 behind the pass that writes them, 1.7 POP/s, 37 %; in
+// copies of an earlier step at 81 us, without its loads 62, without its products 78).  No faster, each against the kernel of its own
+// step, codes in the caches (it / this one): rows two steps ahead, up 107 / 103; eight waves of 16 x 32, up 121 / 102, down 81 /
+// 74; 64 x 128, one workgroup a CU, three stages, 108 / 102 and 84 / 75.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -391,7 +392,9 @@ int launch_tile(const void* x, const float* xs, int x_rows, const int32_t* gathe
   const int xcds = cus % 8 == 0 ? 8 : 1;
   const long long grid = std::min<long long>(2 * cus, (2 * tiles + xcds - 1) / xcds * xcds);
   // bf16 outputs go past L2: their stores are whole lines (a product with L2's usual policy / so, us: 2048 rows, 128 ->
-  // 512: 13.7 / 12.6, 32768, E = 32: 126 / 108).  fp32 ones do where they are far more than the caches behind it hold (128 ->
+  // 512: 13.7 / 12.6, 32768, E = 32: 111 / 88; 512 -> 128 70.5 / 69.7, with the combine that reads its rows next 86.6 / 88;
+  // layers of 2048 tokens, 128-512, E = 32, k = 2 73.0 / 69.4, 8192, k = 4 298 / 289.5, 4096, 256-1024, E = 64, k = 2
+  // 255 / 253.5, 512-2048, E = 16 677 / 674.7).  fp32 ones do where they are far more than the caches behind it hold (128 ->
   // 512: 67 MB 21.6 / 24.8, 134 MB 40 / 46, 268 MB 81 / 75, 537 MB 170 / 144).
   const bool stream_out = YT == kBF16 || (uint64_t)P * d_out * 32 > (uint64_t)192 << 20;
   auto* const kernel = stream_out ? int8_tile_kernel<ACT, YT, true> : int8_tile_kernel<ACT, YT, YT == kBF16>;
