@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 
 // Four waves a row where a row is long, or longer than two loads a lane and rows are few (one wave / four a row, bf16, us: 128
 // rows of 128: 2.4 / 2.3, 256: 3.0 / 2.3, 512: 5.2 / 2.6; 2048 rows of 128: 3.4 / 3.7, 256: 5.1 / 4.8, 320: 6.1 / 5.7; 32768
-// rows of 128: 23 / 32, 256: 40 / 44, 320: 51 / 52, 512: 85 / 71).  32768 rows of 512 run at 5.7 TB/s (402 MB).
+// rows of 128: 23 / 32, 256: 40 / 44, 320: 51 / 52, 512: 85 / 71).  262144 rows of 512 run at 6.1 TB/s (3.2 GB).
 // Rows of a launch: a grid holds fewer than 2^32 threads.
 constexpr int kLaunchRows = 1 << 22;
 

@@ -18,8 +18,8 @@
 // Bound: with few K steps a tile by the epilogue's vector work (8192 tokens, k = 4, E = 32, 128 -> 512, gelu: 98 us,
 // 1.40 POP/s; vector units 56 % of the cycles, matrix units 33 %), with many by the way of the operands through L2
 // and LDS (32768 rows, 512 -> 128: 70 us with its codes in the caches, 82 behind the pass that writes them, 1.7 POP/s, 37 %; in
-// copies of an earlier step at 81 us, without its loads 62, without its products 78).  No faster, each against the kernel of its own
-// step, codes in the caches (it / this one): rows two steps ahead, up 107 / 103; eight waves of 16 x 32, up 121 / 102, down 81 /
+// copies of an earlier step at 81 us, without its loads 62, without its products 78).  No faster, each timed in turn with the kernel
+// of its own step (it / that one): rows two steps ahead, up 107 / 103; eight waves of 16 x 32, up 121 / 102, down 81 /
 // 74; 64 x 128, one workgroup a CU, three stages, 108 / 102 and 84 / 75.
 #include <hip/hip_runtime.h>
 

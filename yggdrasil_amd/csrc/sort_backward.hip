@@ -86,7 +86,8 @@ __device__ __forceinline__ void find_and_clear(const int32_t* __restrict__ slot_
   for (int r = wave * 64; r < kFindRows; r += 256) clear_rows(s_named[r + (threadIdx.x & 63)], (size_t)row0 + r, row_pieces, dy);
 }
 
-// One wave per token (bf16 half-rows, 8192 tokens, d = 128, k = 4: 25.7 us, 151 MB at 5.9 TB/s).
+// One wave per token (bf16 half-rows, 8192 tokens, d = 128, k = 4: 25.7 us, 151 MB that the last-level cache holds in part;
+// 131072 tokens: 474 us with the search above, 2.4 GB at 5.1 TB/s).
 template <typename TD, typename TY, int LAYOUT>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const TD* __restrict__ dout, const TY* __restrict__ y, int N,
                                                                int k, int d, int P, const float* __restrict__ topk_w,
@@ -145,7 +146,8 @@ __global__ __launch_bounds__(256) void clear_unnamed_kernel(const int32_t* __res
   clear_rows(named, first, row_pieces, dy);
 }
 
-// A thread per multivector of a token (bf16, 8192 tokens, d = 128, k = 4: 17.6 us, 84 MB at 4.8 TB/s).
+// A thread per multivector of a token (bf16, 8192 tokens, d = 128, k = 4: 17.6 us, 84 MB; 131072 tokens: 250 us, 1.3 GB at 5.4
+// TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void dispatch_backward_kernel(const T* __restrict__ dxs, int k, int d, int P,
                                                                 const int32_t* __restrict__ slot_pos,
